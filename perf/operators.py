@@ -220,8 +220,10 @@ def _quantize(x: torch.Tensor, fmt: str, weight: bool):
     if weight:
         scale = torch.clamp(amax * (1.0 / 127.0), min=1e-12)
         return torch.clamp(torch.round(x / scale), -127.0, 127.0).to(torch.int8), scale
-    inverse = torch.where(amax > 0, 127.0 / amax, 0.0)
-    return torch.clamp(torch.round(x * inverse), -128.0, 127.0).to(torch.int8), amax / 127.0
+    # tensors on both sides: torch divides by a number, and a number by a tensor, through a rounded reciprocal
+    limit = torch.full_like(amax, 127.0)
+    inverse = torch.where(amax > 0, limit / amax, 0.0)
+    return torch.clamp(torch.round(x * inverse), -128.0, 127.0).to(torch.int8), amax / limit
 
 
 def _product(a, a_scale, w, w_scale, swiglu: bool):
@@ -352,7 +354,8 @@ def _exact_codes(x: torch.Tensor, fmt: str, weight: bool):
     x = x.float()
     amax = x.abs().max(dim=1, keepdim=True).values
     if fmt == "int8" and not weight:
-        codes = torch.round(x * torch.nan_to_num(127.0 / amax, posinf=0.0)).clamp(-128, 127)
+        inverse = torch.div(torch.full_like(amax, 127.0), amax)  # one IEEE division, as the codes' definition has it
+        codes = torch.round(x * torch.nan_to_num(inverse, posinf=0.0)).clamp(-128, 127)
         return codes.double(), amax.double() / 127.0
     scale = torch.clamp(amax * (1.0 / _LIMIT[fmt]), min=1e-12)
     if fmt == "e4m3":
