@@ -326,6 +326,88 @@ int h3q_residual_gate_rms_norm_modulate_quant(const void* residual, int64_t ldr,
                                               void* out, int64_t ldo, int format, int rounding, void* codes,
                                               int64_t ldq, float* scales, void* stream);
 
+/*
+ * Routed experts: a mixture-of-experts FFN on the W8A8 formats above.  No
+ * counterpart in the reference, whose FFN is dense.
+ *
+ * Expert ids are int32; an id below 0 means no expert.  A plan covers `experts`
+ * consecutive ids from `first` on (the experts this GPU holds); pairs whose id
+ * lies outside add nothing to any result.  A pair is token * top_k + slot.
+ * experts <= 1024, top_k <= 64, tokens * top_k < 2^31.
+ */
+#define H3Q_SCORE_SOFTMAX 0
+#define H3Q_SCORE_SIGMOID 1
+
+/*
+ * Top-k routing: for each row of logits [tokens, experts] (dtype: H3Q_DTYPE_*,
+ * ldl elements between rows) the top_k largest logits, largest first, the
+ * lowest expert among equals (+0 and -0 are equal); NaN and -inf are never
+ * taken, and slots that find no expert get id -1 and weight 0.  Weights, binary32:
+ *   SOFTMAX: exp(l - max) / sum, over all experts, or over the taken ones (renormalize);
+ *            an infinite maximum counts 1, everything below it 0
+ *   SIGMOID: 1 / (1 + exp(-l)), divided by the sum of the taken ones (renormalize)
+ * times scale.  ids int32 and weights fp32 [tokens, top_k], contiguous.  top_k <= experts.
+ */
+int h3q_route_topk(const void* logits, int dtype, int64_t ldl, int64_t tokens, int64_t experts, int64_t top_k,
+                   int scoring, int renormalize, float scale, int32_t* ids, float* weights, void* stream);
+
+/*
+ * The plan of an expert layer: the pairs sorted by expert, in pair order within one.
+ *   order[i]        pair of sorted row i, -1 past the last placed row   int32 [tokens * top_k]
+ *   offsets[e]      first sorted row of expert first + e                int32 [experts + 1]
+ *   slots[t, j]     sorted row of pair (t, j), -1 without an expert here   int32 [tokens, top_k]
+ * Deterministic; one launch.
+ */
+int h3q_plan_experts(const int32_t* ids, int64_t tokens, int64_t top_k, int64_t first, int64_t experts, int32_t* order,
+                     int32_t* offsets, int32_t* slots, void* stream);
+
+/*
+ * Scaled product of rows grouped by expert: for row i in [offsets[e], offsets[e + 1])
+ *   y[n] = a_scale[r] * (b_scale[e, n] * sum_k a[r, k] * b[e, n, k])
+ * with r = order[i] / top_k (order given: rows gathered from a [a_rows, k]), or r = i
+ * (order NULL, a_rows >= rows).  swiglu 0: out[i, 0..n) = bf16(y), or y itself
+ * (binary32) when out_f32; swiglu 1: b's rows are [gate | up] and out[i, 0..n/2) =
+ * bf16(silu(y[c]) * y[n/2 + c]), gate and up in binary32.  Rows of out past
+ * offsets[experts] are left as they were, and so are rows whose order entry is out
+ * of range of a (those of a plan never are).  a: codes with lda bytes between rows;
+ * b: codes [experts, n, k], each expert's matrix row-major or tiled (k % 128 == 0);
+ * a_scale [a_rows], b_scale [experts, n].  rows: an upper bound of offsets[experts]
+ * (tokens * top_k).  k % 16 == 0, n % 16 == 0 (swiglu: n % 32 == 0), lda and the
+ * output stride (in elements) multiples of 16 bytes, 16-byte aligned a, b, b_scale and
+ * out; one expert's weights, and the gathered a, below 2 GiB.
+ */
+int h3q_grouped_mm(int format, const void* a, int64_t lda, int64_t a_rows, const float* a_scale, const int32_t* order,
+                   int64_t top_k, const void* b, int b_layout, const float* b_scale, const int32_t* offsets,
+                   int64_t experts, int64_t rows, int64_t n, int64_t k, int swiglu, int out_f32, void* out,
+                   int64_t ldo, void* stream);
+
+/*
+ * out[t] = bf16(sum_j weights[t, j] * y[slots[t, j]]), binary32 in slot order; slots
+ * outside [0, rows) add nothing (a token with none gets zeros).  y: bf16, or binary32
+ * (y_f32), [rows, cols], ldy elements; cols % 8 == 0, strides multiples of 8
+ * elements, 16-byte aligned y and out.
+ */
+int h3q_combine_experts(const void* y, int y_f32, int64_t ldy, int64_t rows, const int32_t* slots,
+                        const float* weights, int64_t tokens, int64_t top_k, int64_t cols, void* out, int64_t ldo,
+                        void* stream);
+
+/*
+ * The whole FFN of the layer, x and out bf16 [tokens, d]:
+ *   q, s = codes of x per token (INT8: RCP_MUL, E4M3FN: DIV)
+ *   h = bf16(silu(gate) * up) from q and w13 [experts, 2 f, d] (rows [gate | up]), s13 [experts, 2 f]
+ *   qh, sh = codes of h per pair;  y = sh * (s2 * (qh . w2)), w2 [experts, d, f], s2 [experts, d]
+ *   out[t] = bf16(sum_j weights[t, j] * y[t, j])
+ * d % 16 == 0, f % 16 == 0 (a tiled matrix: its columns a multiple of 128); strides
+ * multiples of 8 elements, 16-byte aligned buffers.  workspace:
+ * h3q_expert_ffn_workspace_bytes(...) bytes of the caller's, free to use again when
+ * the call's work on the stream is done.
+ */
+int64_t h3q_expert_ffn_workspace_bytes(int64_t tokens, int64_t top_k, int64_t experts, int64_t d, int64_t f);
+int h3q_expert_ffn(int format, const void* x, int64_t ldx, int64_t tokens, int64_t d, int64_t f, const int32_t* ids,
+                   const float* weights, int64_t top_k, int64_t first, int64_t experts, const void* w13,
+                   int w13_layout, const float* s13, const void* w2, int w2_layout, const float* s2, void* out,
+                   int64_t ldo, void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -532,4 +532,242 @@ __attribute__((visibility("default"))) int h3q_lora_down_ws(const void* x, int64
     return check_launch(h3q::launch_lora_down(g, workspace, workspace_bytes, (hipStream_t)stream), who);
 }
 
+// Shared checks of the expert entry points.
+static int check_experts(const char* who, int64_t tokens, int64_t top_k, int64_t experts) {
+    if (tokens < 0) return fail(H3Q_ERR_INVALID, "%s: negative token count %lld", who, (long long)tokens);
+    if (experts < 1 || experts > h3q::kMaxExperts)
+        return fail(H3Q_ERR_INVALID, "%s: %lld experts, 1 to %d", who, (long long)experts, h3q::kMaxExperts);
+    if (top_k < 1 || top_k > h3q::kMaxTopK)
+        return fail(H3Q_ERR_INVALID, "%s: top_k=%lld, 1 to %d", who, (long long)top_k, h3q::kMaxTopK);
+    if (tokens > 0x7FFFFFFF / top_k)
+        return fail(H3Q_ERR_UNSUPPORTED, "%s: %lld pairs do not fit 31 bits", who, (long long)(tokens * top_k));
+    return H3Q_OK;
+}
+
+static int check_code_layout(const char* who, int format, int layout, int64_t k) {
+    if (format != H3Q_FMT_E4M3FN && format != H3Q_FMT_INT8)
+        return fail(H3Q_ERR_INVALID, "%s: unknown format %d", who, format);
+    if (layout != H3Q_LAYOUT_ROWS && layout != H3Q_LAYOUT_TILED)
+        return fail(H3Q_ERR_INVALID, "%s: unknown layout %d", who, layout);
+    if (layout == H3Q_LAYOUT_TILED && k % 128)
+        return fail(H3Q_ERR_INVALID, "%s: a tiled weight needs k=%lld a multiple of 128", who, (long long)k);
+    return H3Q_OK;
+}
+
+__attribute__((visibility("default"))) int h3q_route_topk(const void* logits, int dtype, int64_t ldl, int64_t tokens,
+                                                          int64_t experts, int64_t top_k, int scoring,
+                                                          int renormalize, float scale, int32_t* ids, float* weights,
+                                                          void* stream) {
+    const char* who = "h3q_route_topk";
+    const int rc = check_experts(who, tokens, top_k, experts);
+    if (rc != H3Q_OK) return rc;
+    if (top_k > experts)
+        return fail(H3Q_ERR_INVALID, "%s: top_k=%lld of %lld experts", who, (long long)top_k, (long long)experts);
+    if (dtype != H3Q_DTYPE_BF16 && dtype != H3Q_DTYPE_F16 && dtype != H3Q_DTYPE_F32)
+        return fail(H3Q_ERR_INVALID, "%s: unknown dtype %d", who, dtype);
+    if (scoring != H3Q_SCORE_SOFTMAX && scoring != H3Q_SCORE_SIGMOID)
+        return fail(H3Q_ERR_INVALID, "%s: unknown scoring %d", who, scoring);
+    if (ldl < experts) return fail(H3Q_ERR_INVALID, "%s: leading dimension below the expert count", who);
+    if (tokens == 0) return ok();
+    if (!logits || !ids || !weights) return fail(H3Q_ERR_INVALID, "%s: null pointer", who);
+    h3q::RouteArgs a{};
+    a.logits = logits;
+    a.ldl = ldl;
+    a.tokens = tokens;
+    a.experts = (int)experts;
+    a.top_k = (int)top_k;
+    a.scoring = scoring;
+    a.renormalize = renormalize != 0;
+    a.scale = scale;
+    a.ids = ids;
+    a.weights = weights;
+    return check_launch(h3q::launch_route_topk(a, dtype, (hipStream_t)stream), who);
+}
+
+__attribute__((visibility("default"))) int h3q_plan_experts(const int32_t* ids, int64_t tokens, int64_t top_k,
+                                                            int64_t first, int64_t experts, int32_t* order,
+                                                            int32_t* offsets, int32_t* slots, void* stream) {
+    const char* who = "h3q_plan_experts";
+    const int rc = check_experts(who, tokens, top_k, experts);
+    if (rc != H3Q_OK) return rc;
+    if (first < 0 || first > 0x7FFFFFFF - experts)
+        return fail(H3Q_ERR_INVALID, "%s: first expert %lld", who, (long long)first);
+    if (!offsets || (tokens > 0 && (!ids || !order || !slots))) return fail(H3Q_ERR_INVALID, "%s: null pointer", who);
+    h3q::PlanArgs a{};
+    a.ids = ids;
+    a.pairs = tokens * top_k;
+    a.first = (int)first;
+    a.experts = (int)experts;
+    a.vec = aligned(ids, 16);
+    a.order = order;
+    a.offsets = offsets;
+    a.slots = slots;
+    return check_launch(h3q::launch_plan_experts(a, (hipStream_t)stream), who);
+}
+
+__attribute__((visibility("default"))) int h3q_grouped_mm(int format, const void* a, int64_t lda, int64_t a_rows,
+                                                          const float* a_scale, const int32_t* order, int64_t top_k,
+                                                          const void* b, int b_layout, const float* b_scale,
+                                                          const int32_t* offsets, int64_t experts, int64_t rows,
+                                                          int64_t n, int64_t k, int swiglu, int out_f32, void* out,
+                                                          int64_t ldo, void* stream) {
+    const char* who = "h3q_grouped_mm";
+    int rc = check_code_layout(who, format, b_layout, k);
+    if (rc != H3Q_OK) return rc;
+    if (rows < 0 || a_rows < 0 || n <= 0 || k <= 0)
+        return fail(H3Q_ERR_INVALID, "%s: bad shape (%lld rows, a %lld, n %lld, k %lld)", who, (long long)rows,
+                    (long long)a_rows, (long long)n, (long long)k);
+    rc = check_experts(who, rows, 1, experts);
+    if (rc != H3Q_OK) return rc;
+    if (order && top_k < 1) return fail(H3Q_ERR_INVALID, "%s: top_k=%lld", who, (long long)top_k);
+    if (k % 16 || n % (swiglu ? 32 : 16))
+        return fail(H3Q_ERR_INVALID, "%s: k=%lld must be a multiple of 16 and n=%lld of %d", who, (long long)k,
+                    (long long)n, swiglu ? 32 : 16);
+    if (swiglu && out_f32) return fail(H3Q_ERR_UNSUPPORTED, "%s: the SwiGLU output is bf16", who);
+    const int64_t cols = swiglu ? n / 2 : n;
+    if (lda < k || lda % 16) return fail(H3Q_ERR_INVALID, "%s: lda=%lld must be >= k and a multiple of 16", who, (long long)lda);
+    if (ldo < cols || ldo % (out_f32 ? 4 : 8))
+        return fail(H3Q_ERR_INVALID, "%s: ldo=%lld must hold %lld columns in 16-byte steps", who, (long long)ldo,
+                    (long long)cols);
+    if (!order && a_rows < rows)
+        return fail(H3Q_ERR_INVALID, "%s: a has %lld rows, %lld needed", who, (long long)a_rows, (long long)rows);
+    if (n * k >= (int64_t(1) << 31) || n >= (int64_t(1) << 24))
+        return fail(H3Q_ERR_UNSUPPORTED, "%s: one expert's weights (%lld x %lld) must stay below 2 GiB", who,
+                    (long long)n, (long long)k);
+    if (order && a_rows * lda >= (int64_t(1) << 31))
+        return fail(H3Q_ERR_UNSUPPORTED, "%s: gathered activations must stay below 2 GiB", who);
+    if (lda >= (int64_t(1) << 22) || ldo >= (int64_t(1) << 22))
+        return fail(H3Q_ERR_UNSUPPORTED, "%s: row stride above 2^22", who);
+    if (rows == 0) return ok();
+    if (!b || !b_scale || !offsets || !out || (a_rows > 0 && (!a || !a_scale)))
+        return fail(H3Q_ERR_INVALID, "%s: null pointer", who);
+    if (!aligned(a, 16) || !aligned(b, 16) || !aligned(b_scale, 16) || !aligned(out, 16))
+        return fail(H3Q_ERR_INVALID, "%s: a, b, b_scale and out must be 16-byte aligned", who);
+    h3q::GroupedArgs g{};
+    g.a = a;
+    g.lda = lda;
+    g.a_rows = a_rows;
+    g.a_scale = a_scale;
+    g.order = order;
+    g.top_k = (int)(order ? top_k : 1);
+    g.b = b;
+    g.b_tiled = b_layout == H3Q_LAYOUT_TILED;
+    g.b_scale = b_scale;
+    g.offsets = offsets;
+    g.experts = (int)experts;
+    g.rows = rows;
+    g.n = (int)n;
+    g.k = k;
+    g.swiglu = swiglu != 0;
+    g.f32 = out_f32 != 0;
+    g.out = out;
+    g.ldo = ldo;
+    if (!h3q::grouped_mm_fits(g))
+        return fail(H3Q_ERR_UNSUPPORTED, "%s: %lld rows x %lld columns need too many workgroups", who, (long long)rows,
+                    (long long)n);
+    return check_launch(h3q::launch_grouped_mm(format == H3Q_FMT_INT8 ? h3q::kOpInt8 : h3q::kOpE4M3, g,
+                                               (hipStream_t)stream),
+                        who);
+}
+
+__attribute__((visibility("default"))) int h3q_combine_experts(const void* y, int y_f32, int64_t ldy, int64_t rows,
+                                                               const int32_t* slots, const float* weights,
+                                                               int64_t tokens, int64_t top_k, int64_t cols, void* out,
+                                                               int64_t ldo, void* stream) {
+    const char* who = "h3q_combine_experts";
+    const int rc = check_experts(who, tokens, top_k, 1);
+    if (rc != H3Q_OK) return rc;
+    if (rows < 0 || rows > 0x7FFFFFFF || cols <= 0 || cols % 8)
+        return fail(H3Q_ERR_INVALID, "%s: %lld rows of %lld columns (a multiple of 8)", who, (long long)rows,
+                    (long long)cols);
+    if (ldy < cols || ldy % 8 || ldo < cols || ldo % 8)
+        return fail(H3Q_ERR_INVALID, "%s: strides must hold %lld columns and be multiples of 8", who, (long long)cols);
+    if (tokens >= (int64_t(1) << 34) / cols)
+        return fail(H3Q_ERR_UNSUPPORTED, "%s: too many elements", who);
+    if (tokens == 0) return ok();
+    if ((rows > 0 && !y) || !slots || !weights || !out) return fail(H3Q_ERR_INVALID, "%s: null pointer", who);
+    if (!aligned(y, 16) || !aligned(out, 16)) return fail(H3Q_ERR_INVALID, "%s: y and out must be 16-byte aligned", who);
+    h3q::CombineArgs a{};
+    a.y = y;
+    a.ldy = ldy;
+    a.rows = rows;
+    a.slots = slots;
+    a.weights = weights;
+    a.tokens = tokens;
+    a.top_k = (int)top_k;
+    a.cols = cols;
+    a.out = (uint16_t*)out;
+    a.ldo = ldo;
+    return check_launch(h3q::launch_combine_experts(a, y_f32 != 0, (hipStream_t)stream), who);
+}
+
+__attribute__((visibility("default"))) int64_t h3q_expert_ffn_workspace_bytes(int64_t tokens, int64_t top_k,
+                                                                              int64_t experts, int64_t d, int64_t f) {
+    if (tokens <= 0 || top_k <= 0 || experts <= 0 || d <= 0 || f <= 0) return 0;
+    h3q::ExpertFfnArgs a{};
+    a.tokens = tokens;
+    a.top_k = (int)top_k;
+    a.experts = (int)experts;
+    a.d = d;
+    a.f = f;
+    return h3q::expert_ffn_workspace_bytes(a);
+}
+
+__attribute__((visibility("default"))) int h3q_expert_ffn(int format, const void* x, int64_t ldx, int64_t tokens,
+                                                          int64_t d, int64_t f, const int32_t* ids,
+                                                          const float* weights, int64_t top_k, int64_t first,
+                                                          int64_t experts, const void* w13, int w13_layout,
+                                                          const float* s13, const void* w2, int w2_layout,
+                                                          const float* s2, void* out, int64_t ldo, void* workspace,
+                                                          int64_t workspace_bytes, void* stream) {
+    const char* who = "h3q_expert_ffn";
+    int rc = check_code_layout(who, format, w13_layout, d);
+    if (rc == H3Q_OK) rc = check_code_layout(who, format, w2_layout, f);
+    if (rc == H3Q_OK) rc = check_experts(who, tokens, top_k, experts);
+    if (rc != H3Q_OK) return rc;
+    if (first < 0 || first > 0x7FFFFFFF - experts)
+        return fail(H3Q_ERR_INVALID, "%s: first expert %lld", who, (long long)first);
+    if (d <= 0 || f <= 0 || d % 16 || f % 16)
+        return fail(H3Q_ERR_INVALID, "%s: d=%lld and f=%lld must be multiples of 16", who, (long long)d, (long long)f);
+    if (d >= (int64_t(1) << 22) || f >= (int64_t(1) << 22) || 2 * f * d >= (int64_t(1) << 31))
+        return fail(H3Q_ERR_UNSUPPORTED, "%s: one expert's weights (%lld x %lld) must stay below 2 GiB", who,
+                    (long long)(2 * f), (long long)d);
+    if (tokens >= (int64_t(1) << 31) / d)
+        return fail(H3Q_ERR_UNSUPPORTED, "%s: the activation codes must stay below 2 GiB", who);
+    if (ldx < d || ldx % 8 || ldo < d || ldo % 8)
+        return fail(H3Q_ERR_INVALID, "%s: strides must hold %lld columns and be multiples of 8", who, (long long)d);
+    if (tokens == 0) return ok();
+    if (!x || !ids || !weights || !w13 || !s13 || !w2 || !s2 || !out) return fail(H3Q_ERR_INVALID, "%s: null pointer", who);
+    if (!aligned(x, 16) || !aligned(w13, 16) || !aligned(s13, 16) || !aligned(w2, 16) || !aligned(s2, 16) ||
+        !aligned(out, 16))
+        return fail(H3Q_ERR_INVALID, "%s: x, weights, scales and out must be 16-byte aligned", who);
+    h3q::ExpertFfnArgs a{};
+    a.kind = format == H3Q_FMT_INT8 ? h3q::kOpInt8 : h3q::kOpE4M3;
+    a.x = (const uint16_t*)x;
+    a.ldx = ldx;
+    a.tokens = tokens;
+    a.d = d;
+    a.f = f;
+    a.ids = ids;
+    a.weights = weights;
+    a.top_k = (int)top_k;
+    a.first = (int)first;
+    a.experts = (int)experts;
+    a.w13 = w13;
+    a.w13_tiled = w13_layout == H3Q_LAYOUT_TILED;
+    a.s13 = s13;
+    a.w2 = w2;
+    a.w2_tiled = w2_layout == H3Q_LAYOUT_TILED;
+    a.s2 = s2;
+    a.out = (uint16_t*)out;
+    a.ldo = ldo;
+    const int64_t need = h3q::expert_ffn_workspace_bytes(a);
+    if (!workspace || !aligned(workspace, 16) || workspace_bytes < need)
+        return fail(H3Q_ERR_INVALID, "%s: workspace of %lld bytes, %lld needed (16-byte aligned)", who,
+                    (long long)workspace_bytes, (long long)need);
+    if (!h3q::expert_ffn_fits(a))
+        return fail(H3Q_ERR_UNSUPPORTED, "%s: %lld tokens need too many workgroups", who, (long long)tokens);
+    return check_launch(h3q::launch_expert_ffn(a, workspace, (hipStream_t)stream), who);
+}
+
 }  // extern "C"

@@ -1,0 +1,71 @@
+// What the grouped products share: the matrix instructions, the tile of a workgroup and
+// the SwiGLU of an epilogue.
+#pragma once
+
+#include "h3q_common.hpp"
+#include "h3q_kernels.hpp"
+
+namespace h3q {
+
+// 16 x 16 products of 128-byte fragments (row = lane % 16, bytes 32 (lane / 16) .. + 31
+// of each operand); the first operand's rows are accumulator rows 4 (lane / 16) + v.
+template <int OP>
+struct GroupedMfma;
+template <>
+struct GroupedMfma<kOpE4M3> {
+    using acc_t = v4f;
+    static __device__ __forceinline__ acc_t run(v8i a, v8i b, acc_t c) {
+        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, 0, 0, 0);
+    }
+};
+template <>
+struct GroupedMfma<kOpInt8> {
+    using acc_t = v4i;
+    static __device__ __forceinline__ acc_t run(v8i a, v8i b, acc_t c) {
+        const v4i alo = {a[0], a[1], a[2], a[3]}, ahi = {a[4], a[5], a[6], a[7]};
+        const v4i blo = {b[0], b[1], b[2], b[3]}, bhi = {b[4], b[5], b[6], b[7]};
+        c = __builtin_amdgcn_mfma_i32_16x16x64_i8(alo, blo, c, 0, 0, 0);
+        return __builtin_amdgcn_mfma_i32_16x16x64_i8(ahi, bhi, c, 0, 0, 0);
+    }
+};
+
+// silu(g) * u in binary32: exp(-g) by the hardware exp2, IEEE sum, quotient and product.
+// (g = -inf gives NaN, as -inf / inf does.)
+__device__ __forceinline__ float swiglu_f32(float g, float u) {
+    const float e = __builtin_amdgcn_exp2f(-g * 0x1.715476p+0f);
+    return g / (1.0f + e) * u;
+}
+
+// Rows of one expert that a workgroup's tile covers.
+struct GroupTile {
+    int expert;
+    int64_t row0;
+    int rows;  // 0: no tile
+};
+
+// Tile `tile` of a launch in tiles of BM rows.  Expert e owns the tiles from
+// e + offsets[e] / BM on: floor(hi / BM) - floor(lo / BM) + 1 of them, always enough for
+// its hi - lo rows, so experts + rows / BM tiles cover every split of the rows and a
+// workgroup finds its own from the offsets alone (one load a lane per 64 experts), without
+// a prefix sum over the experts' tile counts.  The bounds come from device memory and
+// are clamped to the rows that the call was given.
+__device__ __forceinline__ GroupTile group_tile(const int* offsets, int experts, int64_t rows, int bm, int tile) {
+    const int lane = threadIdx.x & 63;
+    int n = 0;
+    for (int i = 0; i < experts; i += 64) {
+        const int e = i + lane;
+        n += __popcll(__ballot(e < experts && e + (int64_t)offsets[e < experts ? e : 0] / bm <= tile));
+    }
+    GroupTile t;
+    t.expert = n > 0 ? n - 1 : 0;
+    int64_t lo = offsets[t.expert], hi = offsets[t.expert + 1];
+    const int64_t first = t.expert + lo / bm;
+    lo = lo < 0 ? 0 : (lo > rows ? rows : lo);
+    hi = hi < lo ? lo : (hi > rows ? rows : hi);
+    t.row0 = lo + (tile - first) * bm;
+    const int64_t left = t.row0 < lo ? 0 : hi - t.row0;
+    t.rows = (int)(left < 0 ? 0 : (left > bm ? bm : left));
+    return t;
+}
+
+}  // namespace h3q

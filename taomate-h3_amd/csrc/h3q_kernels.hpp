@@ -163,4 +163,87 @@ struct NormQuantArgs {
 constexpr int kNormQuantMaxCols = 8192;
 hipError_t launch_norm_modulate_quant(const NormQuantArgs& a, bool resid, int fmt, int rounding, hipStream_t st);
 
+// Routing of an expert layer (experts.hip).  Values mirrored by include/taomate_h3_amd.h.
+enum Score : int { kScoreSoftmax = 0, kScoreSigmoid = 1 };
+constexpr int kMaxExperts = 1024;
+constexpr int kMaxTopK = 64;
+struct RouteArgs {
+    const void* logits;  // [tokens, experts], ldl elements between rows
+    int64_t ldl, tokens;
+    int experts, top_k;
+    int scoring, renormalize;
+    float scale;
+    int* ids;        // [tokens, top_k]
+    float* weights;  // [tokens, top_k]
+};
+hipError_t launch_route_topk(const RouteArgs& a, int dtype, hipStream_t st);
+
+struct PlanArgs {
+    const int* ids;  // [pairs]
+    int64_t pairs;   // below 2^31
+    int first, experts;
+    int vec;         // ids 16-byte aligned
+    int* order;      // [pairs]
+    int* offsets;    // [experts + 1]
+    int* slots;      // [pairs]
+};
+hipError_t launch_plan_experts(const PlanArgs& a, hipStream_t st);
+
+struct CombineArgs {
+    const void* y;  // [rows, cols] bf16 or binary32, ldy elements
+    int64_t ldy, rows;
+    const int* slots;      // [tokens, top_k]
+    const float* weights;  // [tokens, top_k]
+    int64_t tokens;
+    int top_k;
+    int64_t cols;   // a multiple of 8
+    uint16_t* out;  // [tokens, cols] bf16, ldo elements
+    int64_t ldo;
+};
+hipError_t launch_combine_experts(const CombineArgs& a, bool f32, hipStream_t st);
+
+// Scaled product of rows grouped by expert (grouped_stream.hip).
+struct GroupedArgs {
+    const void* a;         // codes [a_rows, k], row-major, lda bytes (16-byte aligned rows)
+    int64_t lda, a_rows;
+    const float* a_scale;  // [a_rows]
+    const int* order;      // [rows] pair of each row (row of a: pair / top_k), or null: row i of a
+    int top_k;
+    const void* b;         // codes [experts, n, k], each expert's matrix row-major or tiled
+    int b_tiled;
+    const float* b_scale;  // [experts, n]
+    const int* offsets;    // [experts + 1]
+    int experts;
+    int64_t rows;          // upper bound of offsets[experts]
+    int n;                 // a multiple of 16 (SwiGLU: of 32, rows [gate | up])
+    int64_t k;             // a multiple of 16 (tiled: of 128)
+    int swiglu, f32;       // f32: binary32 output instead of bf16 (not with SwiGLU)
+    void* out;             // [rows, n or n / 2]
+    int64_t ldo;           // in elements
+};
+// Whether the call's grid stays within what a launch takes.
+bool grouped_mm_fits(const GroupedArgs& a);
+hipError_t launch_grouped_mm(int kind, const GroupedArgs& a, hipStream_t st);
+
+// The FFN of a routed-expert layer (expert_ffn.hip).
+struct ExpertFfnArgs {
+    int kind;           // kOpE4M3 or kOpInt8
+    const uint16_t* x;  // bf16 [tokens, d], ldx elements
+    int64_t ldx, tokens, d, f;
+    const int* ids;        // [tokens, top_k]
+    const float* weights;  // [tokens, top_k]
+    int top_k, first, experts;
+    const void* w13;  // codes [experts, 2 f, d]
+    int w13_tiled;
+    const float* s13;  // [experts, 2 f]
+    const void* w2;    // codes [experts, d, f]
+    int w2_tiled;
+    const float* s2;  // [experts, d]
+    uint16_t* out;    // bf16 [tokens, d], ldo elements
+    int64_t ldo;
+};
+int64_t expert_ffn_workspace_bytes(const ExpertFfnArgs& a);
+bool expert_ffn_fits(const ExpertFfnArgs& a);
+hipError_t launch_expert_ffn(const ExpertFfnArgs& a, void* workspace, hipStream_t st);
+
 }  // namespace h3q

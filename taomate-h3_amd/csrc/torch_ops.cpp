@@ -12,6 +12,7 @@
 // What it saves is the host's time per call, which bounds every call of a few
 // dozen rows (measured on an MI355X host, Python wrapper -> this: quantizer 11.1
 // -> 5.7 us, scaled GEMM 13.7 -> 5.5 us, of which the launch itself is about 3).
+#include <c10/core/DeviceGuard.h>
 #include <torch/extension.h>
 
 #include <optional>
@@ -250,6 +251,120 @@ std::optional<Pair> quant_tensor(const Tensor& x, const Opt& static_scale, bool 
     return Pair(codes, scale);
 }
 
+// Elements between rows; a single row has the width's, rounded up to 16.
+int64_t row_stride(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : (t.size(1) + 15) / 16 * 16; }
+
+// A contiguous tensor of the given type beside `first`.
+bool dense(const Tensor& t, const Tensor& first, at::ScalarType type) {
+    return on(t, first) && t.scalar_type() == type && t.is_contiguous();
+}
+
+int logit_type(at::ScalarType type) {
+    return type == at::kBFloat16 ? H3Q_DTYPE_BF16 : type == at::kHalf ? H3Q_DTYPE_F16 : type == at::kFloat ? H3Q_DTYPE_F32 : -1;
+}
+
+int32_t* ints(const Tensor& t) { return static_cast<int32_t*>(t.data_ptr()); }
+
+std::optional<Pair> route_experts(const Tensor& logits, int64_t top_k, int64_t scoring, bool renormalize, double scale,
+                                  int64_t stream) {
+    const int dtype = logit_type(logits.scalar_type());
+    if (!logits.is_cuda() || dtype < 0 || !rows_2d(logits, logits.scalar_type()) || logits.size(0) == 0) return std::nullopt;
+    const int64_t tokens = logits.size(0), experts = logits.size(1);
+    if (top_k < 1 || top_k > experts) return std::nullopt;
+    const c10::DeviceGuard guard(logits.device());
+    const Tensor ids = empty(logits, {tokens, top_k}, at::kInt), weights = empty(logits, {tokens, top_k}, at::kFloat);
+    if (h3q_route_topk(logits.data_ptr(), dtype, tokens > 1 ? logits.stride(0) : experts, tokens, experts, top_k,
+                       (int)scoring, renormalize, (float)scale, ints(ids), floats(weights), stream_of(stream)))
+        return std::nullopt;
+    return Pair(ids, weights);
+}
+
+std::optional<Three> plan_experts(const Tensor& experts, int64_t n_experts, int64_t first, int64_t stream) {
+    if (!experts.is_cuda() || !dense(experts, experts, at::kInt) || experts.dim() != 2 || experts.numel() == 0 ||
+        n_experts < 1)
+        return std::nullopt;
+    const int64_t tokens = experts.size(0), top_k = experts.size(1);
+    const c10::DeviceGuard guard(experts.device());
+    const Tensor order = empty(experts, {tokens * top_k}, at::kInt), offsets = empty(experts, {n_experts + 1}, at::kInt);
+    const Tensor slots = empty(experts, {tokens, top_k}, at::kInt);
+    if (h3q_plan_experts(ints(experts), tokens, top_k, first, n_experts, ints(order), ints(offsets), ints(slots),
+                         stream_of(stream)))
+        return std::nullopt;
+    return Three(order, offsets, slots);
+}
+
+Opt grouped_scaled_mm(const Tensor& a, const Tensor& b, const Tensor& a_scale, const Tensor& b_scale,
+                      const Tensor& offsets, const Opt& order, int64_t top_k, bool swiglu, bool b_tiled, Opt out, bool f32,
+                      int64_t stream) {
+    const at::ScalarType type = a.scalar_type();
+    if (!a.is_cuda() || (type != at::kChar && type != at::kFloat8_e4m3fn) || !rows_2d(a, type)) return std::nullopt;
+    if (!dense(b, a, type) || b.dim() != 3 || b.size(2) != a.size(1)) return std::nullopt;
+    const int64_t experts = b.size(0), n = b.size(1), k = b.size(2);
+    if (!scales_ok(a_scale, a, a.size(0)) || !scales_ok(b_scale, a, experts * n)) return std::nullopt;
+    if (!dense(offsets, a, at::kInt) || offsets.dim() != 1 || offsets.size(0) != experts + 1) return std::nullopt;
+    if (order && (!dense(*order, a, at::kInt) || order->dim() != 1)) return std::nullopt;
+    if (swiglu && f32) return std::nullopt;
+    const int64_t rows = order ? order->size(0) : a.size(0), cols = swiglu ? n / 2 : n;
+    const at::ScalarType out_type = f32 ? at::kFloat : at::kBFloat16;
+    if (out && !(on(*out, a) && rows_2d(*out, out_type) && out->size(0) == rows && out->size(1) == cols))
+        return std::nullopt;
+    const c10::DeviceGuard guard(a.device());
+    if (!out) out = empty(a, {rows, cols}, out_type);
+    if (h3q_grouped_mm(type == at::kChar ? H3Q_FMT_INT8 : H3Q_FMT_E4M3FN, a.data_ptr(), row_stride(a), a.size(0),
+                       floats(a_scale), order ? ints(*order) : nullptr, top_k, b.data_ptr(),
+                       b_tiled ? H3Q_LAYOUT_TILED : H3Q_LAYOUT_ROWS, floats(b_scale), ints(offsets), experts, rows, n, k,
+                       swiglu, f32, out->data_ptr(), row_stride(*out), stream_of(stream)))
+        return std::nullopt;
+    return out;
+}
+
+Opt combine_experts(const Tensor& y, const Tensor& slots, const Tensor& weights, Opt out, int64_t stream) {
+    const at::ScalarType type = y.scalar_type();
+    if (!y.is_cuda() || (type != at::kBFloat16 && type != at::kFloat) || !rows_2d(y, type)) return std::nullopt;
+    if (!dense(slots, y, at::kInt) || slots.dim() != 2 || !dense(weights, y, at::kFloat) ||
+        weights.sizes() != slots.sizes())
+        return std::nullopt;
+    const int64_t tokens = slots.size(0), top_k = slots.size(1), cols = y.size(1);
+    if (out && !(on(*out, y) && rows_2d(*out, at::kBFloat16) && out->size(0) == tokens && out->size(1) == cols))
+        return std::nullopt;
+    const c10::DeviceGuard guard(y.device());
+    if (!out) out = empty(y, {tokens, cols}, at::kBFloat16);
+    if (h3q_combine_experts(y.data_ptr(), type == at::kFloat, row_stride(y), y.size(0), ints(slots), floats(weights),
+                            tokens, top_k, cols, out->data_ptr(), row_stride(*out), stream_of(stream)))
+        return std::nullopt;
+    return out;
+}
+
+Opt expert_ffn(const Tensor& x, const Tensor& experts, const Tensor& weights, const Tensor& w13, const Tensor& w13_scale,
+               const Tensor& w2, const Tensor& w2_scale, int64_t first, bool w13_tiled, bool w2_tiled, Opt out,
+               int64_t stream) {
+    if (!x.is_cuda() || !rows_2d(x, at::kBFloat16) || x.size(0) == 0) return std::nullopt;
+    const int64_t tokens = x.size(0), d = x.size(1);
+    if (!dense(experts, x, at::kInt) || experts.dim() != 2 || experts.size(0) != tokens ||
+        !dense(weights, x, at::kFloat) || weights.sizes() != experts.sizes())
+        return std::nullopt;
+    const at::ScalarType type = w13.scalar_type();
+    if ((type != at::kChar && type != at::kFloat8_e4m3fn) || !dense(w13, x, type) || !dense(w2, x, type))
+        return std::nullopt;
+    if (w13.dim() != 3 || w13.size(1) % 2 || w13.size(2) != d || w2.dim() != 3) return std::nullopt;
+    const int64_t count = w13.size(0), f = w13.size(1) / 2, top_k = experts.size(1);
+    if (w2.size(0) != count || w2.size(1) != d || w2.size(2) != f) return std::nullopt;
+    if (!scales_ok(w13_scale, x, count * 2 * f) || !scales_ok(w2_scale, x, count * d)) return std::nullopt;
+    if (out && !(on(*out, x) && rows_2d(*out, at::kBFloat16) && out->size(0) == tokens && out->size(1) == d))
+        return std::nullopt;
+    const c10::DeviceGuard guard(x.device());
+    if (!out) out = empty(x, {tokens, d}, at::kBFloat16);
+    const int64_t bytes = h3q_expert_ffn_workspace_bytes(tokens, top_k, count, d, f);
+    const Tensor ws = empty(x, {bytes}, at::kByte);  // from torch's allocator, as in lora_down
+    if (h3q_expert_ffn(type == at::kChar ? H3Q_FMT_INT8 : H3Q_FMT_E4M3FN, x.data_ptr(), row_stride(x), tokens, d, f,
+                       ints(experts), floats(weights), top_k, first, count, w13.data_ptr(),
+                       w13_tiled ? H3Q_LAYOUT_TILED : H3Q_LAYOUT_ROWS, floats(w13_scale), w2.data_ptr(),
+                       w2_tiled ? H3Q_LAYOUT_TILED : H3Q_LAYOUT_ROWS, floats(w2_scale), out->data_ptr(),
+                       row_stride(*out), ws.data_ptr(), bytes, stream_of(stream)))
+        return std::nullopt;
+    return out;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -261,4 +376,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("swiglu_quant", torch::wrap_pybind_function_no_gil(&swiglu_quant));
     m.def("quant_per_head", torch::wrap_pybind_function_no_gil(&quant_per_head));
     m.def("quant_tensor", torch::wrap_pybind_function_no_gil(&quant_tensor));
+    m.def("route_experts", torch::wrap_pybind_function_no_gil(&route_experts));
+    m.def("plan_experts", torch::wrap_pybind_function_no_gil(&plan_experts));
+    m.def("grouped_scaled_mm", torch::wrap_pybind_function_no_gil(&grouped_scaled_mm));
+    m.def("combine_experts", torch::wrap_pybind_function_no_gil(&combine_experts));
+    m.def("expert_ffn", torch::wrap_pybind_function_no_gil(&expert_ffn));
 }

@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import weakref
+from typing import NamedTuple
 
 import torch
 
@@ -27,6 +28,10 @@ OUT_F16 = 0x100      # scaled_mm format flag: binary16 output and bias
 QUOTIENT_EAGER = 0   # per-tensor quotient forms of h3q_quant_tensor_e4m3_typed
 QUOTIENT_TRITON = 1
 SKINNY_MAX_M = 128   # rows up to which the weight-streaming GEMM runs
+MAX_EXPERTS = 1024   # experts of one routing / plan
+MAX_TOP_K = 64       # slots of a token
+SCORE_SOFTMAX = 0
+SCORE_SIGMOID = 1
 
 _CODE_DTYPES = {FMT_E4M3FN: torch.float8_e4m3fn, FMT_INT8: torch.int8}
 _OUT_F16 = {torch.bfloat16: False, torch.float16: True}
@@ -608,4 +613,219 @@ def lora_down(x: torch.Tensor, lora_a: torch.Tensor, *, out: torch.Tensor | None
     ws = torch.empty(ws_bytes, device=x.device, dtype=torch.uint8)
     _lib.call("h3q_lora_down_ws", _ptr(x), x.stride(0), _ptr(lora_a), lora_a.stride(0), _ptr(out), out.stride(0), m,
               k, rank, _ptr(ws), ws_bytes, _stream(x))
+    return out
+
+
+# ------------------------------------------------------------ routed experts
+
+_SCORES = {"softmax": SCORE_SOFTMAX, "sigmoid": SCORE_SIGMOID}
+
+
+class ExpertPlan(NamedTuple):
+    """The (token, slot) pairs of a routed batch sorted by expert (pair = token * top_k + slot)."""
+
+    order: torch.Tensor    # int32 [tokens * top_k]: pair of each sorted row, -1 past the last
+    offsets: torch.Tensor  # int32 [experts + 1]: first sorted row of each expert
+    slots: torch.Tensor    # int32 [tokens, top_k]: sorted row of each pair, -1 without an expert here
+
+
+def _contiguous(name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple[int, ...] | None = None) -> None:
+    if t.dtype != dtype:
+        raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
+    if not t.is_contiguous() or (shape is not None and tuple(t.shape) != shape):
+        raise ValueError(f"{name}: expected a contiguous tensor" + (f" of shape {shape}, got {tuple(t.shape)}"
+                                                                    if shape is not None else ""))
+
+
+def _call_on(t: torch.Tensor, name: str, *args) -> None:
+    """The entry point on t's device and its current stream (another device may be the current one)."""
+    with torch.cuda.device(t.device):
+        _lib.call(name, *args, _stream(t))
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    """Elements between rows; a single row has the width's (rounded up to 16: it has no next row)."""
+    return t.stride(0) if t.shape[0] > 1 else (t.shape[1] + 15) // 16 * 16
+
+
+def route_experts(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax", renormalize: bool = True,
+                  scale: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
+    """Top-k routing of ``logits [tokens, experts]`` (fp32, bf16 or fp16): (experts
+    int32 [tokens, top_k], weights fp32 [tokens, top_k]).
+
+    The largest logits, largest first, the lowest expert among equals; NaN and
+    -inf are never taken, and a slot that finds no expert gets id -1 and weight 0.
+    ``scoring`` "softmax": exp(l - max) over the sum of all experts, or of the
+    taken ones (``renormalize``); "sigmoid": 1 / (1 + exp(-l)), divided by the
+    taken ones' sum when renormalized.  Both times ``scale``."""
+    if logits.get_device() >= 0 and scoring in _SCORES:
+        got = _native_call("route_experts", logits, top_k, _SCORES[scoring], bool(renormalize), float(scale))
+        if got is not None:
+            return got
+    _require_gpu("route_experts", logits)
+    if logits.dtype not in _TENSOR_DTYPES:
+        raise TypeError(f"route_experts: expected float32, bfloat16 or float16 logits, got {logits.dtype}")
+    _rows_2d("route_experts logits", logits, logits.dtype)
+    if scoring not in _SCORES:
+        raise ValueError(f"route_experts: scoring must be one of {sorted(_SCORES)}, got {scoring!r}")
+    tokens, experts = logits.shape
+    if not 1 <= top_k <= min(experts, MAX_TOP_K) or experts > MAX_EXPERTS:
+        raise ValueError(f"route_experts: top_k={top_k} of {experts} experts (top_k up to {MAX_TOP_K}, experts up to "
+                         f"{MAX_EXPERTS})")
+    ids = torch.empty((tokens, top_k), device=logits.device, dtype=torch.int32)
+    weights = torch.empty((tokens, top_k), device=logits.device, dtype=torch.float32)
+    _call_on(logits, "h3q_route_topk", _ptr(logits), _TENSOR_DTYPES[logits.dtype],
+              logits.stride(0) if tokens > 1 else experts, tokens, experts, top_k, _SCORES[scoring],
+              int(bool(renormalize)), float(scale), _ptr(ids), _ptr(weights))
+    return ids, weights
+
+
+def plan_experts(experts: torch.Tensor, n_experts: int, *, first_expert: int = 0) -> ExpertPlan:
+    """The plan of routed ids ``experts`` (int32 [tokens, top_k], contiguous) over the
+    experts [first_expert, first_expert + n_experts); pairs of other ids (and of -1)
+    are left out.  Deterministic: pair order within an expert."""
+    got = _native_call("plan_experts", experts, n_experts, first_expert)
+    if got is not None:
+        return ExpertPlan(*got)
+    _require_gpu("plan_experts", experts)
+    _contiguous("plan_experts experts", experts, torch.int32)
+    if experts.ndim != 2 or not 1 <= experts.shape[1] <= MAX_TOP_K:
+        raise ValueError(f"plan_experts: expected [tokens, top_k <= {MAX_TOP_K}] ids, got {tuple(experts.shape)}")
+    tokens, top_k = experts.shape
+    order = torch.empty(tokens * top_k, device=experts.device, dtype=torch.int32)
+    offsets = torch.empty(max(int(n_experts), 0) + 1, device=experts.device, dtype=torch.int32)
+    slots = torch.empty((tokens, top_k), device=experts.device, dtype=torch.int32)
+    _call_on(experts, "h3q_plan_experts", _ptr(experts), tokens, top_k, int(first_expert), int(n_experts), _ptr(order),
+              _ptr(offsets), _ptr(slots))
+    return ExpertPlan(order, offsets, slots)
+
+
+def grouped_scaled_mm(a: torch.Tensor, b: torch.Tensor, a_scale: torch.Tensor, b_scale: torch.Tensor,
+                      offsets: torch.Tensor, *, order: torch.Tensor | None = None, top_k: int = 1,
+                      swiglu: bool = False, b_tiled: bool = False, out: torch.Tensor | None = None,
+                      out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """Scaled product of rows grouped by expert: row i of expert e (offsets[e] <= i <
+    offsets[e + 1]) is a_scale[r] * (b_scale[e] * (a[r] @ b[e]^T)), rounded once to
+    ``out_dtype`` (bf16 or float32).
+
+    ``a [R, k]`` and ``b [experts, n, k]`` are both e4m3fn or both int8 codes.  With
+    ``order`` (a plan's) the rows are gathered: r = order[i] // top_k; without, r = i.
+    ``swiglu``: b's rows are [gate | up] and the result is bf16(silu(gate) * up), n / 2
+    columns.  ``b_tiled``: every expert's matrix is in the tiled layout.  Rows of
+    ``out`` past offsets[-1] are left as they were (allocated here: undefined)."""
+    if b_tiled or not is_tiled(b):
+        got = _native_call("grouped_scaled_mm", a, b, a_scale, b_scale, offsets, order, top_k, swiglu, b_tiled, out,
+                           out_dtype == torch.float32) if out_dtype in (torch.bfloat16, torch.float32) else None
+        if got is not None:
+            return got
+    name = "grouped_scaled_mm"
+    _require_gpu(name, a, b, a_scale, b_scale, offsets, order, out)
+    if a.dtype not in _FORMATS or b.dtype != a.dtype:
+        raise TypeError(f"{name}: operands must both be e4m3fn or int8, got {a.dtype} and {b.dtype}")
+    _rows_2d(f"{name} a", a, a.dtype)
+    _contiguous(f"{name} b", b, a.dtype)
+    if b.ndim != 3 or b.shape[2] != a.shape[1]:
+        raise ValueError(f"{name}: b must be [experts, n, {a.shape[1]}], got {tuple(b.shape)}")
+    experts, n, k = b.shape
+    check_layout(f"{name} b", b, b_tiled)
+    for label, s, count in (("a_scale", a_scale, a.shape[0]), ("b_scale", b_scale, experts * n)):
+        if s.dtype != torch.float32 or s.numel() != count or not s.is_contiguous():
+            raise ValueError(f"{name}: {label} must be {count} contiguous fp32 values")
+    _contiguous(f"{name} offsets", offsets, torch.int32, (experts + 1,))
+    if order is not None:
+        _contiguous(f"{name} order", order, torch.int32)
+        if order.ndim != 1 or top_k < 1:
+            raise ValueError(f"{name}: order must be a vector of pairs, top_k at least 1")
+    rows = int(a.shape[0] if order is None else order.shape[0])
+    if out_dtype not in (torch.bfloat16, torch.float32) or (swiglu and out_dtype != torch.bfloat16):
+        raise TypeError(f"{name}: out_dtype must be bfloat16 (or float32 without swiglu), got {out_dtype}")
+    cols = n // 2 if swiglu else n
+    if out is None:
+        out = torch.empty((rows, cols), device=a.device, dtype=out_dtype)
+    _rows_2d(f"{name} out", out, out_dtype)
+    if tuple(out.shape) != (rows, cols):
+        raise ValueError(f"{name}: out shape {tuple(out.shape)} != {(rows, cols)}")
+    _call_on(a, "h3q_grouped_mm", _FORMATS[a.dtype], _ptr(a), _row_stride(a), a.shape[0], _ptr(a_scale), _ptr(order),
+              int(top_k), _ptr(b), LAYOUT_TILED if b_tiled else LAYOUT_ROWS, _ptr(b_scale), _ptr(offsets), experts,
+              rows, n, k, int(bool(swiglu)), int(out_dtype == torch.float32), _ptr(out), _row_stride(out))
+    return out
+
+
+def combine_experts(y: torch.Tensor, slots: torch.Tensor, weights: torch.Tensor, *,
+                    out: torch.Tensor | None = None) -> torch.Tensor:
+    """bf16 [tokens, cols]: sum over a token's slots of weights[t, j] * y[slots[t, j]]
+    (y bf16 or fp32 rows, sums in binary32, slots of -1 add nothing)."""
+    got = _native_call("combine_experts", y, slots, weights, out)
+    if got is not None:
+        return got
+    name = "combine_experts"
+    _require_gpu(name, y, slots, weights, out)
+    if y.dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"{name}: expected bfloat16 or float32 rows, got {y.dtype}")
+    _rows_2d(f"{name} y", y, y.dtype)
+    _contiguous(f"{name} slots", slots, torch.int32)
+    if slots.ndim != 2:
+        raise ValueError(f"{name}: slots must be [tokens, top_k], got {tuple(slots.shape)}")
+    _contiguous(f"{name} weights", weights, torch.float32, tuple(slots.shape))
+    tokens, top_k = slots.shape
+    cols = int(y.shape[1])
+    if out is None:
+        out = torch.empty((tokens, cols), device=y.device, dtype=torch.bfloat16)
+    _rows_2d(f"{name} out", out, torch.bfloat16)
+    if tuple(out.shape) != (tokens, cols):
+        raise ValueError(f"{name}: out shape {tuple(out.shape)} != {(tokens, cols)}")
+    _call_on(y, "h3q_combine_experts", _ptr(y), int(y.dtype == torch.float32), _row_stride(y), y.shape[0], _ptr(slots),
+              _ptr(weights), tokens, top_k, cols, _ptr(out), _row_stride(out))
+    return out
+
+
+def expert_ffn(x: torch.Tensor, experts: torch.Tensor, weights: torch.Tensor, w13: torch.Tensor,
+               w13_scale: torch.Tensor, w2: torch.Tensor, w2_scale: torch.Tensor, *, first_expert: int = 0,
+               w13_tiled: bool = False, w2_tiled: bool = False, out: torch.Tensor | None = None) -> torch.Tensor:
+    """The FFN of a routed-expert layer, bf16 ``x [tokens, d]`` -> bf16 [tokens, d].
+
+    ``experts`` int32 and ``weights`` fp32 [tokens, top_k] (see route_experts);
+    ``w13 [E, 2 f, d]`` (rows [gate | up]) and ``w2 [E, d, f]`` codes of the experts
+    [first_expert, first_expert + E) with fp32 scales [E, 2 f] and [E, d].  Per
+    token: codes of x; h = bf16(silu(gate) * up) of each expert; codes of h; the down
+    product; the weighted sum over the token's slots, rounded once.  Activations
+    are quantized as the dense linears' are (int8: ROUND_RCP_MUL; e4m3fn: ROUND_DIV).
+    A token without an expert here gets zeros."""
+    if (w13_tiled or not is_tiled(w13)) and (w2_tiled or not is_tiled(w2)):
+        got = _native_call("expert_ffn", x, experts, weights, w13, w13_scale, w2, w2_scale, first_expert, w13_tiled,
+                           w2_tiled, out)
+        if got is not None:
+            return got
+    name = "expert_ffn"
+    _require_gpu(name, x, experts, weights, w13, w13_scale, w2, w2_scale, out)
+    _rows_2d(f"{name} x", x, torch.bfloat16)
+    tokens, d = x.shape
+    _contiguous(f"{name} experts", experts, torch.int32)
+    if experts.ndim != 2 or experts.shape[0] != tokens:
+        raise ValueError(f"{name}: experts must be [{tokens}, top_k], got {tuple(experts.shape)}")
+    _contiguous(f"{name} weights", weights, torch.float32, tuple(experts.shape))
+    if w13.dtype not in _FORMATS or w2.dtype != w13.dtype:
+        raise TypeError(f"{name}: weights must both be e4m3fn or int8, got {w13.dtype} and {w2.dtype}")
+    _contiguous(f"{name} w13", w13, w13.dtype)
+    if w13.ndim != 3 or w13.shape[1] % 2 or w13.shape[2] != d:
+        raise ValueError(f"{name}: w13 must be [experts, 2 f, {d}], got {tuple(w13.shape)}")
+    count, f = int(w13.shape[0]), int(w13.shape[1]) // 2
+    _contiguous(f"{name} w2", w2, w13.dtype, (count, d, f))
+    check_layout(f"{name} w13", w13, w13_tiled)
+    check_layout(f"{name} w2", w2, w2_tiled)
+    for label, s, size in (("w13_scale", w13_scale, count * 2 * f), ("w2_scale", w2_scale, count * d)):
+        if s.dtype != torch.float32 or s.numel() != size or not s.is_contiguous():
+            raise ValueError(f"{name}: {label} must be {size} contiguous fp32 values")
+    if out is None:
+        out = torch.empty((tokens, d), device=x.device, dtype=torch.bfloat16)
+    _rows_2d(f"{name} out", out, torch.bfloat16)
+    if tuple(out.shape) != (tokens, d):
+        raise ValueError(f"{name}: out shape {tuple(out.shape)} != {(tokens, d)}")
+    top_k = int(experts.shape[1])
+    size = int(_lib.lib().h3q_expert_ffn_workspace_bytes(tokens, top_k, count, d, f))
+    ws = torch.empty(size, device=x.device, dtype=torch.uint8)
+    _call_on(x, "h3q_expert_ffn", _FORMATS[w13.dtype], _ptr(x), _row_stride(x), tokens, d, f, _ptr(experts),
+              _ptr(weights), top_k, int(first_expert), count, _ptr(w13), LAYOUT_TILED if w13_tiled else LAYOUT_ROWS,
+              _ptr(w13_scale), _ptr(w2), LAYOUT_TILED if w2_tiled else LAYOUT_ROWS, _ptr(w2_scale), _ptr(out),
+              _row_stride(out), _ptr(ws), size)
     return out
