@@ -215,6 +215,8 @@ namespace {
 // Row blocks of a tile, from the mean rows of an expert.
 int stream_row_blocks(const GroupedArgs& a) { return a.rows / a.experts <= 16 ? 1 : 4; }
 
+bool tile_kernel(const GroupedArgs& a) { return a.rows / a.experts > 64 && grouped_tile_supported(a); }
+
 int stream_slices(const GroupedArgs& a) { return a.swiglu ? a.n / 32 : (a.n + 31) / 32; }
 
 int64_t stream_grid(const GroupedArgs& a) {
@@ -244,9 +246,10 @@ hipError_t launch_stream_op(const GroupedArgs& a, hipStream_t st) {
 }  // namespace
 
 // A grid of n workgroups of 256 threads takes n * 256 < 2^32.
-bool grouped_mm_fits(const GroupedArgs& a) { return stream_grid(a) < (int64_t(1) << 24); }
+bool grouped_mm_fits(const GroupedArgs& a) { return tile_kernel(a) || stream_grid(a) < (int64_t(1) << 24); }
 
 hipError_t launch_grouped_mm(int kind, const GroupedArgs& a, hipStream_t st) {
+    if (tile_kernel(a)) return launch_grouped_tile(kind, a, st);
     return kind == kOpInt8 ? launch_stream_op<kOpInt8>(a, st) : launch_stream_op<kOpE4M3>(a, st);
 }
 

@@ -221,6 +221,9 @@ struct GroupedArgs {
     void* out;             // [rows, n or n / 2]
     int64_t ldo;           // in elements
 };
+// The same over 256 x 256 tiles (grouped_tile.hip), for groups of many rows.
+bool grouped_tile_supported(const GroupedArgs& a);
+hipError_t launch_grouped_tile(int kind, const GroupedArgs& a, hipStream_t st);
 // Whether the call's grid stays within what a launch takes.
 bool grouped_mm_fits(const GroupedArgs& a);
 hipError_t launch_grouped_mm(int kind, const GroupedArgs& a, hipStream_t st);

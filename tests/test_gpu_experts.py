@@ -154,6 +154,44 @@ def test_grouped(ops, device, oracle, fmt, counts, n, k, tiled, swiglu):
 
 
 @pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("tiled,k", [(True, 384), (False, 336)])
+@pytest.mark.parametrize("out", ["bf16", "f32", "swiglu"])
+def test_grouped_many_tiles(ops, device, oracle, fmt, tiled, k, out):
+    """More 256 x 256 tiles than the chip has workgroups for, whole and half ones, and a last
+    column tile that is not full: every row, a sample of the columns."""
+    counts = [1100, 0, 129, 2000, 128, 300, 1]
+    e, n = len(counts), 5216
+    rows = sum(counts)
+    x = activations(rows, k, seed=21, outlier_channels=2)
+    qa, sa = oracle.quant_rows(bits16(x), fmt, "rcp" if fmt == "int8" else "div")
+    qa, sa = qa.view(np.uint8), sa.ravel()
+    f = ops.FMT_INT8 if fmt == "int8" else ops.FMT_E4M3FN
+    gen = torch.Generator(device=device).manual_seed(5)
+    w = (torch.randn(e * n, k, generator=gen, device=device) * 0.05).to(torch.bfloat16)
+    qw, sw = ops.quant_rows(w, f)
+    stack = ops.quant_rows_tiled(w, f)[0] if tiled else qw
+    offsets = np.concatenate(([0], np.cumsum(counts))).astype(np.int32)
+    got = ops.grouped_scaled_mm(_device_codes(qa, fmt, device), stack.view(e, n, k), torch.from_numpy(sa).to(device),
+                                sw.view(e, n), torch.from_numpy(offsets).to(device), swiglu=out == "swiglu", b_tiled=tiled,
+                                out_dtype=torch.float32 if out == "f32" else torch.bfloat16).double().cpu().numpy()
+    half = n // 2
+    sample = np.unique(np.concatenate((np.arange(0, half, 97), [15, 16, 63, 64, 127, 128, 255, 256, half - 1])))
+    cols = np.concatenate((sample, half + sample))
+    qs = qw.view(e, n, k)[:, cols].contiguous().view(torch.uint8).cpu().numpy()
+    ss = sw.view(e, n)[:, cols].cpu().numpy()
+    for i in range(e):
+        lo, hi = offsets[i], offsets[i + 1]
+        if lo == hi:
+            continue
+        y, b = R.scaled(oracle, fmt, qa[lo:hi], sa[lo:hi], qs[i], ss[i])
+        mine = got[lo:hi][:, sample if out == "swiglu" else cols]
+        if out == "swiglu":
+            y, b = R.swiglu(y, b)
+        bound = b + (0.0 if out == "f32" else R.HALF_BF16) * (np.abs(y) + b) + 2.0 ** -133
+        assert (np.abs(mine - y) <= bound).all(), (i, np.max(np.abs(mine - y) / bound))
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
 @pytest.mark.parametrize("t,k_top,e", [(3, 2, 4), (90, 3, 5), (700, 2, 3)])
 def test_grouped_gathers_rows(ops, device, fmt, t, k_top, e):
     """A gathered call equals the call on rows copied into the plan's order, bit for bit,
