@@ -9,7 +9,7 @@
 // between two dense linears are; gate and up are not rounded before that, and y stays
 // binary32 up to the sum over the experts, which is rounded once.
 //
-// Here: plan, quantize, grouped gate-up product with SwiGLU (rows gathered from the
+// A few tokens take two kernels of their own (expert_few.hip).  The rest, here: plan, quantize, grouped gate-up product with SwiGLU (rows gathered from the
 // tokens' codes, so no copy of a token per expert is made), quantize, grouped down product,
 // weighted sum.
 #include "h3q_common.hpp"
@@ -118,6 +118,7 @@ hipError_t launch_expert_ffn(const ExpertFfnArgs& a, void* workspace, hipStream_
     const int rounding = a.kind == kOpInt8 ? kRoundRcpMul : kRoundDiv;
     Workspace w{(uint8_t*)workspace};
     const Parts p = carve(w, a);
+    if (expert_few_supported(a)) return launch_expert_few(a, FewBuffers{p.xq, p.xs, p.h, p.hq, p.hs}, st);
 
     PlanArgs plan{};
     plan.ids = a.ids;

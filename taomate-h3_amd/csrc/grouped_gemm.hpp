@@ -7,21 +7,65 @@
 
 namespace h3q {
 
+constexpr uint32_t kOob = 0x80000000u;  // beyond every descriptor's range: loads return 0
+
+__device__ __forceinline__ v8i join(v4u lo, v4u hi) {
+    return v8i{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
+}
+__device__ __forceinline__ v8i join(v4i lo, v4i hi) { return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7); }
+
 // 16 x 16 products of 128-byte fragments (row = lane % 16, bytes 32 (lane / 16) .. + 31
 // of each operand); the first operand's rows are accumulator rows 4 (lane / 16) + v.
-template <int OP>
+// WIDE (e4m3): the codes become bf16, exactly, and four bf16 instructions take the place of
+// the FP8 one.  The FP8 instruction drops the low bits of small products inside each group
+// of 8 (2^-13 of the largest): 1.5e-5 to 3e-5 of the result, which the rounding of an
+// output hides, but which moves one code in a thousand to its neighbour where the output is
+// quantized again; bf16 products leave 5e-8 to 1e-7 (K = 1024 to 5376, measured).  Where
+// weights are streamed the conversions and the slower instruction hide under the loads.
+template <int OP, bool WIDE = false>
 struct GroupedMfma;
 template <>
-struct GroupedMfma<kOpE4M3> {
+struct GroupedMfma<kOpE4M3, false> {
     using acc_t = v4f;
-    static __device__ __forceinline__ acc_t run(v8i a, v8i b, acc_t c) {
+    using frag_t = v8i;
+    static __device__ __forceinline__ frag_t frag(v8i codes) { return codes; }
+    static __device__ __forceinline__ acc_t run(frag_t a, frag_t b, acc_t c) {
         return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, 0, 0, 0);
     }
 };
 template <>
-struct GroupedMfma<kOpInt8> {
+struct GroupedMfma<kOpE4M3, true> {
+    using acc_t = v4f;
+    struct frag_t {
+        v8bf q[4];
+    };
+    static __device__ __forceinline__ frag_t frag(v8i codes) {
+        frag_t f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const v2bf lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)codes[2 * i + h], 1.0f, false);
+                const v2bf hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)codes[2 * i + h], 1.0f, true);
+                f.q[i][4 * h] = lo[0];
+                f.q[i][4 * h + 1] = lo[1];
+                f.q[i][4 * h + 2] = hi[0];
+                f.q[i][4 * h + 3] = hi[1];
+            }
+        return f;
+    }
+    static __device__ __forceinline__ acc_t run(const frag_t& a, const frag_t& b, acc_t c) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.q[i], b.q[i], c, 0, 0, 0);
+        return c;
+    }
+};
+template <bool WIDE>
+struct GroupedMfma<kOpInt8, WIDE> {
     using acc_t = v4i;
-    static __device__ __forceinline__ acc_t run(v8i a, v8i b, acc_t c) {
+    using frag_t = v8i;
+    static __device__ __forceinline__ frag_t frag(v8i codes) { return codes; }
+    static __device__ __forceinline__ acc_t run(frag_t a, frag_t b, acc_t c) {
         const v4i alo = {a[0], a[1], a[2], a[3]}, ahi = {a[4], a[5], a[6], a[7]};
         const v4i blo = {b[0], b[1], b[2], b[3]}, bhi = {b[4], b[5], b[6], b[7]};
         c = __builtin_amdgcn_mfma_i32_16x16x64_i8(alo, blo, c, 0, 0, 0);

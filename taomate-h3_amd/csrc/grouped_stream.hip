@@ -21,18 +21,14 @@ namespace h3q {
 
 namespace {
 
-constexpr uint32_t kOob = 0x80000000u;  // beyond every descriptor's range: loads return 0
 constexpr int kStreamWaves = 4;
-
-__device__ __forceinline__ v8i join(v4u lo, v4u hi) {
-    return v8i{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
-}
 
 }  // namespace
 
 template <int OP, int MT, int SPW, bool TB, bool SWIGLU, bool F32>
 __global__ __launch_bounds__(kStreamWaves * 64) void grouped_stream_kernel(GroupedArgs p, int slices) {
-    using acc_t = typename GroupedMfma<OP>::acc_t;
+    using Mfma = GroupedMfma<OP, SWIGLU>;  // what SwiGLU gives is quantized again: wide products
+    using acc_t = typename Mfma::acc_t;
     constexpr int WAVES = kStreamWaves, NBLK = 2, BM = 16 * MT;
     constexpr int ITEMS = SWIGLU ? MT : NBLK * MT;  // 16 x 16 output blocks of the workgroup
     constexpr int PER_WAVE = (ITEMS + WAVES - 1) / WAVES;
@@ -138,11 +134,17 @@ __global__ __launch_bounds__(kStreamWaves * 64) void grouped_stream_kernel(Group
     };
     auto mfma_chunk = [&](const v8i (&wf)[SPW][NBLK], const v8i (&xf)[SPW][MT]) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < SPW; ++i)
+        for (int i = 0; i < SPW; ++i) {
+            typename Mfma::frag_t w[NBLK];
 #pragma unroll
-            for (int j = 0; j < NBLK; ++j)
+            for (int j = 0; j < NBLK; ++j) w[j] = Mfma::frag(wf[i][j]);
 #pragma unroll
-                for (int t = 0; t < MT; ++t) acc[j][t] = GroupedMfma<OP>::run(wf[i][j], xf[i][t], acc[j][t]);
+            for (int t = 0; t < MT; ++t) {
+                const typename Mfma::frag_t x = Mfma::frag(xf[i][t]);
+#pragma unroll
+                for (int j = 0; j < NBLK; ++j) acc[j][t] = Mfma::run(w[j], x, acc[j][t]);
+            }
+        }
     };
     const int iters = (int)((steps + WAVES - 1) / WAVES);
     const int nc = (iters + SPW - 1) / SPW;

@@ -32,7 +32,6 @@ namespace {
 constexpr int kStages = 4;
 constexpr int kStageBytes = (256 + 256) * 64;  // A and B, 64 bytes of k each
 constexpr int kABytes = 256 * 64;
-constexpr uint32_t kOob = 0x80000000u;  // beyond every descriptor's range
 constexpr int64_t kStreamOutBytes = int64_t(64) << 20;  // outputs stored past the caches (see gemm_w4.hip)
 
 // Wave copies global -> LDS (see copy16 in h3q_common.hpp), with a scalar offset.  A scalar

@@ -245,6 +245,16 @@ struct ExpertFfnArgs {
     uint16_t* out;    // bf16 [tokens, d], ldo elements
     int64_t ldo;
 };
+// The same for a few tokens, in two kernels (expert_few.hip).
+struct FewBuffers {
+    uint8_t* xq;  // codes of x and of h, where the kernels do not make them themselves
+    float* xs;
+    uint16_t* h;  // bf16 [pairs, f], by pair
+    uint8_t* hq;
+    float* hs;
+};
+bool expert_few_supported(const ExpertFfnArgs& a);
+hipError_t launch_expert_few(const ExpertFfnArgs& a, const FewBuffers& w, hipStream_t st);
 int64_t expert_ffn_workspace_bytes(const ExpertFfnArgs& a);
 bool expert_ffn_fits(const ExpertFfnArgs& a);
 hipError_t launch_expert_ffn(const ExpertFfnArgs& a, void* workspace, hipStream_t st);

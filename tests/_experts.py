@@ -57,13 +57,18 @@ def plan(ids: np.ndarray, experts: int, first: int = 0):
 
 
 def products(O, fmt: str, qa: np.ndarray, qb: np.ndarray):
-    """(sum, bound) of code rows [m, k] x [n, k]: int8 exactly; e4m3 by the matrix
-    instruction's model, bound on its remaining binary32 rounding.  int8 sums above 2^24
-    round once when they become binary32."""
+    """(sum, bound) of code rows [m, k] x [n, k]: the exact sums.  int8 keeps them (sums
+    above 2^24 round once when they become binary32).  e4m3 products run through the FP8
+    instruction (its model's distance from the exact sum and the bound on the model's own
+    rounding) or as bf16 (exact products, k binary32 additions in some order: at most k
+    U32 of the sum of the magnitudes): the larger of the two."""
     if fmt == "int8":
         s = qa.view(np.int8).astype(np.float64) @ qb.view(np.int8).astype(np.float64).T
         return s, np.abs(s) * U32
-    return O.gemm_e4m3_mfma(qa, qb)
+    a, b = O.e4m3_to_f32(qa).astype(np.float64), O.e4m3_to_f32(qb).astype(np.float64)
+    s = a @ b.T  # products of 4-bit significands: binary64 keeps the sums to 2^-53
+    model, rest = O.gemm_e4m3_mfma(qa, qb)
+    return s, np.maximum(np.abs(s - model) + rest, qa.shape[1] * U32 * (np.abs(a) @ np.abs(b).T))
 
 
 def scaled(O, fmt, qa, sa, qb, sb):
