@@ -356,10 +356,12 @@ int h3q_route_topk(const void* logits, int dtype, int64_t ldl, int64_t tokens, i
  *   order[i]        pair of sorted row i, -1 past the last placed row   int32 [tokens * top_k]
  *   offsets[e]      first sorted row of expert first + e                int32 [experts + 1]
  *   slots[t, j]     sorted row of pair (t, j), -1 without an expert here   int32 [tokens, top_k]
- * Deterministic; one launch.
+ * Deterministic.  One launch for a few thousand pairs; more take two, and a
+ * workspace of h3q_plan_experts_workspace_bytes(...) bytes of the caller's (0: none needed).
  */
+int64_t h3q_plan_experts_workspace_bytes(int64_t tokens, int64_t top_k, int64_t experts);
 int h3q_plan_experts(const int32_t* ids, int64_t tokens, int64_t top_k, int64_t first, int64_t experts, int32_t* order,
-                     int32_t* offsets, int32_t* slots, void* stream);
+                     int32_t* offsets, int32_t* slots, void* workspace, int64_t workspace_bytes, void* stream);
 
 /*
  * Scaled product of rows grouped by expert: for row i in [offsets[e], offsets[e + 1])

@@ -44,7 +44,8 @@ SIGNATURES: dict[str, tuple[type | None, list]] = {
     "h3q_residual_gate_rms_norm_modulate_quant": (_I, [_P, _I64, _P, _I64, _P, _P, _P, _P, _I64, _P, _I64, _I64, _F,
                                                        _P, _I64, _P, _I64, _I, _I, _P, _I64, _P, _P]),
     "h3q_route_topk": (_I, [_P, _I, _I64, _I64, _I64, _I64, _I, _I, _F, _P, _P, _P]),
-    "h3q_plan_experts": (_I, [_P, _I64, _I64, _I64, _I64, _P, _P, _P, _P]),
+    "h3q_plan_experts_workspace_bytes": (_I64, [_I64, _I64, _I64]),
+    "h3q_plan_experts": (_I, [_P, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _I64, _P]),
     "h3q_grouped_mm": (_I, [_I, _P, _I64, _I64, _P, _P, _I64, _P, _I, _P, _P, _I64, _I64, _I64, _I64, _I, _I, _P,
                             _I64, _P]),
     "h3q_combine_experts": (_I, [_P, _I, _I64, _I64, _P, _P, _I64, _I64, _I64, _P, _I64, _P]),

@@ -584,9 +584,16 @@ __attribute__((visibility("default"))) int h3q_route_topk(const void* logits, in
     return check_launch(h3q::launch_route_topk(a, dtype, (hipStream_t)stream), who);
 }
 
+__attribute__((visibility("default"))) int64_t h3q_plan_experts_workspace_bytes(int64_t tokens, int64_t top_k,
+                                                                                int64_t experts) {
+    if (tokens <= 0 || top_k <= 0 || experts <= 0 || experts > h3q::kMaxExperts || tokens > 0x7FFFFFFF / top_k) return 0;
+    return h3q::plan_workspace_ints(tokens * top_k, (int)experts) * (int64_t)sizeof(int32_t);
+}
+
 __attribute__((visibility("default"))) int h3q_plan_experts(const int32_t* ids, int64_t tokens, int64_t top_k,
                                                             int64_t first, int64_t experts, int32_t* order,
-                                                            int32_t* offsets, int32_t* slots, void* stream) {
+                                                            int32_t* offsets, int32_t* slots, void* workspace,
+                                                            int64_t workspace_bytes, void* stream) {
     const char* who = "h3q_plan_experts";
     const int rc = check_experts(who, tokens, top_k, experts);
     if (rc != H3Q_OK) return rc;
@@ -598,10 +605,14 @@ __attribute__((visibility("default"))) int h3q_plan_experts(const int32_t* ids, 
     a.pairs = tokens * top_k;
     a.first = (int)first;
     a.experts = (int)experts;
-    a.vec = aligned(ids, 16);
     a.order = order;
     a.offsets = offsets;
     a.slots = slots;
+    a.workspace = (int*)workspace;
+    const int64_t need = h3q::plan_workspace_ints(a.pairs, a.experts) * (int64_t)sizeof(int32_t);
+    if (need > 0 && (!workspace || !aligned(workspace, 4) || workspace_bytes < need))
+        return fail(H3Q_ERR_INVALID, "%s: workspace of %lld bytes, %lld needed", who, (long long)workspace_bytes,
+                    (long long)need);
     return check_launch(h3q::launch_plan_experts(a, (hipStream_t)stream), who);
 }
 

@@ -31,7 +31,7 @@ struct Workspace {
 };
 
 struct Parts {
-    int *order, *offsets, *slots;
+    int *order, *offsets, *slots, *plan;
     uint8_t* xq;
     float* xs;
     uint16_t* h;
@@ -46,6 +46,7 @@ Parts carve(Workspace& w, const ExpertFfnArgs& a) {
     p.order = w.take<int>(pairs);
     p.offsets = w.take<int>(a.experts + 1);
     p.slots = w.take<int>(pairs);
+    p.plan = w.take<int>(plan_workspace_ints(pairs, a.experts));
     p.xq = w.take<uint8_t>(a.tokens * a.d);
     p.xs = w.take<float>(a.tokens);
     p.h = w.take<uint16_t>(pairs * a.f);
@@ -125,10 +126,10 @@ hipError_t launch_expert_ffn(const ExpertFfnArgs& a, void* workspace, hipStream_
     plan.pairs = pairs;
     plan.first = a.first;
     plan.experts = a.experts;
-    plan.vec = (uintptr_t)a.ids % 16 == 0;
     plan.order = p.order;
     plan.offsets = p.offsets;
     plan.slots = p.slots;
+    plan.workspace = p.plan;
     hipError_t e = launch_plan_experts(plan, st);
     if (e != hipSuccess) return e;
     e = launch_quant_rows(a.x, a.ldx, a.tokens, a.d, fmt, rounding, p.xq, a.d, p.xs, st);

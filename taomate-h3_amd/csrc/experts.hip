@@ -1,6 +1,8 @@
 // Routing of a mixture-of-experts layer, gfx950: the top-k of the router's logits, the
 // plan that sorts the (token, slot) pairs by expert, and the weighted sum that brings
 // the experts' rows back to their tokens.
+#include <type_traits>
+
 #include "h3q_common.hpp"
 #include "h3q_kernels.hpp"
 
@@ -162,100 +164,198 @@ hipError_t launch_route_topk(const RouteArgs& a, int dtype, hipStream_t st) {
 }
 
 // Plan of an expert layer: the pairs (token * top_k + slot) sorted by expert, in pair
-// order within an expert.  Workgroup e places expert e's pairs: its waves take
-// consecutive spans of the pairs, count the ones of lower experts and its own, and after
-// one exchange walk their spans again and write.  No atomics, so the order is the same
-// every time; no workspace, one launch.  Pairs whose expert is not in
-// [first, first + experts) get slot -1 (workgroup 0), and the rows past the last placed
-// one order -1 (workgroup e for rows total + e, total + e + experts, ...).
+// order within an expert (a stable counting sort).  A block of the plan is a chunk of
+// consecutive pairs; its 16 waves take consecutive spans of it, 64 pairs a trip.
 //
-// What bounds it: every workgroup reads all ids twice (from the L2 after the first), so
-// the latency of a span's loads for few pairs, experts * pairs * 8 bytes for many.
-__global__ __launch_bounds__(1024) void plan_experts_kernel(PlanArgs p) {
-    constexpr int kWaves = 16;
-    __shared__ int lower[kWaves], own[kWaves], valid[kWaves];
+//   count   every wave counts its span's experts in its own row of an LDS table: the lanes
+//           with the same expert find each other by one ballot per bit of the expert's number,
+//           and the first of them adds their count (no atomics).
+//   place   with the table summed over the waves below, and the counts of the blocks below
+//           and of the lower experts added, the span is walked again, and every pair's row
+//           is the table's entry plus its rank among its peers of the trip.
+//
+// Up to kPlanChunk pairs one workgroup does both; more take a counting launch, whose blocks
+// leave their counts in the workspace, and a placing one, whose blocks each sum all the
+// counts they need (blocks * experts integers, read once, by all threads).  Deterministic.
+// Pairs whose expert is not in [first, first + experts) get slot -1, and the rows past the
+// last placed one order -1.
+//
+// What bounds it: dependent round trips; the work is 2 * log2(experts) ballots a trip.  One
+// workgroup per expert over all pairs took 46 us for 131072 pairs of 128 experts.
+constexpr int kPlanWaves = 16;
+constexpr int kPlanChunk = 2048;
+
+namespace {
+
+// Lanes of the wave with the same value (of `bits` bits) as this one, among `valid`.
+__device__ __forceinline__ uint64_t match(int v, int bits, uint64_t valid) {
+    uint64_t peers = valid;
+    for (int i = 0; i < bits; ++i) {
+        const bool one = v >> i & 1;
+        const uint64_t b = __ballot(one);
+        peers &= one ? b : ~b;
+    }
+    return peers;
+}
+
+}  // namespace
+
+enum PlanPhase : int { kPlanWhole = 0, kPlanCount = 1, kPlanPlace = 2 };
+
+template <int PHASE>
+__global__ __launch_bounds__(kPlanWaves * 64) void plan_experts_kernel(PlanArgs p, int64_t chunk, int bits) {
+    // [wave][expert]: counts, then the next row of that expert in the wave's span
+    extern __shared__ int table[];
+    __shared__ int wave_sum[kPlanWaves];
+    __shared__ int rows_all[kMaxExperts], rows_below[kMaxExperts];  // of each expert, over the blocks
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int e = blockIdx.x;
-    // spans in whole 256-pair trips of a wave (4 consecutive pairs a lane)
-    const int64_t trips = (p.pairs + 255) / 256;
-    const int64_t t0 = trips * wave / kWaves, t1 = trips * (wave + 1) / kWaves;
-    auto load = [&](int64_t t, int (&id)[4]) __attribute__((always_inline)) {
-        const int64_t i = t * 256 + lane * 4;
-        if (p.vec && i + 4 <= p.pairs) {
-            const int4 v = *reinterpret_cast<const int4*>(p.ids + i);
-            id[0] = v.x, id[1] = v.y, id[2] = v.z, id[3] = v.w;
-        } else {
-#pragma unroll
-            for (int c = 0; c < 4; ++c) id[c] = i + c < p.pairs ? p.ids[i + c] : -1;
-        }
-        // expert of this plan, or `experts` for none (ids below 0 or outside the range;
-        // the difference is taken unsigned, so no id wraps into the range)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            const uint32_t r = (uint32_t)id[c] - (uint32_t)p.first;
-            id[c] = id[c] >= 0 && id[c] >= p.first && r < (uint32_t)p.experts ? (int)r : p.experts;
-        }
-    };
-    int n_lower = 0, n_own = 0, n_valid = 0;
-    for (int64_t t = t0; t < t1; ++t) {
-        int id[4];
-        load(t, id);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            n_lower += __popcll(__ballot(id[c] < e));
-            n_own += __popcll(__ballot(id[c] == e));
-            n_valid += __popcll(__ballot(id[c] < p.experts));
-        }
-    }
-    if (lane == 0) {
-        lower[wave] = n_lower;
-        own[wave] = n_own;
-        valid[wave] = n_valid;
-    }
+    const int n = p.experts, blocks = gridDim.x, block = blockIdx.x;
+    const int64_t begin = block * chunk, end = begin + chunk < p.pairs ? begin + chunk : p.pairs;
+    const int64_t trips = (end - begin + 63) / 64;
+    const int64_t t0 = trips * wave / kPlanWaves, t1 = trips * (wave + 1) / kPlanWaves;
+    int* const mine = table + wave * n;
+    for (int i = threadIdx.x; i < kPlanWaves * n; i += kPlanWaves * 64) table[i] = 0;
+    if (threadIdx.x < n) rows_all[threadIdx.x] = rows_below[threadIdx.x] = 0;
     __syncthreads();
-    int base = 0, before = 0, count = 0, total = 0;
+
+    // Expert of pair i relative to the plan's first, or n for none (ids below 0 or outside the
+    // range; the difference is taken unsigned, so no id wraps into it).
+    auto expert_of = [&](int64_t i) __attribute__((always_inline)) -> int {
+        if (i >= end) return n;
+        const int id = p.ids[i];
+        const uint32_t r = (uint32_t)id - (uint32_t)p.first;
+        return id >= p.first && r < (uint32_t)n ? (int)r : n;
+    };
+    auto walk = [&](auto place) __attribute__((always_inline)) {
+        constexpr bool PLACE = decltype(place)::value;
+        for (int64_t t = t0; t < t1; t += 4) {  // four trips' loads in flight
+            int e4[4];
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-        base += lower[w];
-        if (w < wave) before += own[w];
-        count += own[w];
-        total += valid[w];
-    }
-    if (threadIdx.x == 0) {
-        p.offsets[e] = base;
-        if (e == p.experts - 1) p.offsets[p.experts] = base + count;
-    }
-    int pos = base + before;
-    for (int64_t t = t0; t < t1; ++t) {
-        int id[4];
-        load(t, id);
-        uint64_t b[4];
-        int rank = 0;
+            for (int c = 0; c < 4; ++c) e4[c] = t + c < t1 ? expert_of(begin + (t + c) * 64 + lane) : n;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            b[c] = __ballot(id[c] == e);
-            rank += __popcll(b[c] & ((uint64_t(1) << lane) - 1));
-        }
-        const int64_t i = t * 256 + lane * 4;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            if (id[c] == e) {
-                p.order[pos + rank] = (int)(i + c);
-                p.slots[i + c] = pos + rank;
-                ++rank;
-            } else if (e == 0 && id[c] == p.experts && i + c < p.pairs) {
-                p.slots[i + c] = -1;
+            for (int c = 0; c < 4; ++c) {
+                if (t + c >= t1) break;
+                const int64_t i = begin + (t + c) * 64 + lane;
+                const int e = e4[c];
+                const uint64_t peers = match(e, bits, __ballot(e < n));
+                const int rank = __popcll(peers & ((uint64_t(1) << lane) - 1));
+                if (e < n) {
+                    const int row = mine[e] + rank;
+                    if constexpr (PLACE) {
+                        p.order[row] = (int)i;
+                        p.slots[i] = row;
+                    }
+                    // after every peer has read the entry: a wave's LDS operations are in order
+                    if (rank == 0) mine[e] = row + __popcll(peers);
+                } else if (PLACE && i < end) {
+                    p.slots[i] = -1;
+                }
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // other lanes read it in the next trip
             }
         }
+    };
+    walk(std::false_type());
+    __syncthreads();
+
+    if constexpr (PHASE == kPlanCount) {
+        for (int e = threadIdx.x; e < n; e += kPlanWaves * 64) {
+            int sum = 0;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) pos += __popcll(b[c]);
+            for (int w = 0; w < kPlanWaves; ++w) sum += table[w * n + e];
+            p.workspace[(int64_t)block * n + e] = sum;
+        }
+        return;
     }
-    for (int64_t i = total + e + (int64_t)threadIdx.x * p.experts; i < p.pairs; i += 1024 * (int64_t)p.experts)
+    // Rows of every expert in all blocks and in those below, each thread a share of the blocks
+    // (LDS additions of integers: their order changes nothing).
+    if constexpr (PHASE == kPlanPlace) {
+        const int shares = kPlanWaves * 64 / n, share = threadIdx.x / n, e = threadIdx.x - share * n;
+        if (share < shares) {
+            int all = 0, below = 0;
+#pragma unroll 8
+            for (int b = share; b < blocks; b += shares) {
+                const int c = p.workspace[(int64_t)b * n + e];
+                all += c;
+                if (b < block) below += c;
+            }
+            atomicAdd(&rows_all[e], all);
+            atomicAdd(&rows_below[e], below);
+        }
+        __syncthreads();
+    }
+    const int e = threadIdx.x;
+    int all = 0;
+    if (e < n) {
+        if constexpr (PHASE == kPlanPlace) {
+            all = rows_all[e];
+        } else {
+#pragma unroll
+            for (int w = 0; w < kPlanWaves; ++w) all += table[w * n + e];
+        }
+    }
+    // Rows of the lower experts: a prefix sum over the threads.
+    int sum = all;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int o = __shfl_up(sum, d, 64);
+        if (lane >= d) sum += o;
+    }
+    if (lane == 63) wave_sum[wave] = sum;
+    __syncthreads();
+    int lower = sum - all, total = 0;
+#pragma unroll
+    for (int w = 0; w < kPlanWaves; ++w) {
+        if (w < wave) lower += wave_sum[w];
+        total += wave_sum[w];
+    }
+    if (e < n) {
+        if (block == 0) {
+            p.offsets[e] = lower;
+            if (e == n - 1) p.offsets[n] = total;
+        }
+        int row = lower + rows_below[e];
+#pragma unroll
+        for (int w = 0; w < kPlanWaves; ++w) {
+            const int c = table[w * n + e];
+            table[w * n + e] = row;
+            row += c;
+        }
+    }
+    __syncthreads();
+    walk(std::true_type());
+    for (int64_t i = total + (int64_t)block * (kPlanWaves * 64) + threadIdx.x; i < p.pairs;
+         i += (int64_t)blocks * (kPlanWaves * 64))
         p.order[i] = -1;
 }
 
+namespace {
+
+// Pairs per block: at most 256 blocks, so a placing block's sum over them stays short.
+int64_t plan_chunk(int64_t pairs) {
+    const int64_t per = (pairs + 255) / 256;
+    return per <= kPlanChunk ? kPlanChunk : (per + 1023) / 1024 * 1024;
+}
+
+}  // namespace
+
+int64_t plan_workspace_ints(int64_t pairs, int experts) {
+    const int64_t chunk = plan_chunk(pairs);
+    return pairs <= chunk ? 0 : (pairs + chunk - 1) / chunk * experts;
+}
+
 hipError_t launch_plan_experts(const PlanArgs& a, hipStream_t st) {
-    hipLaunchKernelGGL(plan_experts_kernel, dim3((unsigned)a.experts), dim3(1024), 0, st, a);
+    const int64_t chunk = plan_chunk(a.pairs);
+    const unsigned blocks = a.pairs <= chunk ? 1u : (unsigned)((a.pairs + chunk - 1) / chunk);
+    const unsigned lds = (unsigned)(kPlanWaves * a.experts * sizeof(int));
+    int bits = 0;
+    while ((1 << bits) < a.experts) ++bits;
+    const dim3 threads(kPlanWaves * 64);
+    if (blocks == 1) {
+        hipLaunchKernelGGL((plan_experts_kernel<kPlanWhole>), dim3(1), threads, lds, st, a, chunk, bits);
+    } else {
+        hipLaunchKernelGGL((plan_experts_kernel<kPlanCount>), dim3(blocks), threads, lds, st, a, chunk, bits);
+        hipLaunchKernelGGL((plan_experts_kernel<kPlanPlace>), dim3(blocks), threads, lds, st, a, chunk, bits);
+    }
     return hipGetLastError();
 }
 

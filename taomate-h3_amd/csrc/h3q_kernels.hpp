@@ -182,11 +182,12 @@ struct PlanArgs {
     const int* ids;  // [pairs]
     int64_t pairs;   // below 2^31
     int first, experts;
-    int vec;         // ids 16-byte aligned
     int* order;      // [pairs]
     int* offsets;    // [experts + 1]
     int* slots;      // [pairs]
+    int* workspace;  // plan_workspace_ints(...) of them
 };
+int64_t plan_workspace_ints(int64_t pairs, int experts);
 hipError_t launch_plan_experts(const PlanArgs& a, hipStream_t st);
 
 struct CombineArgs {

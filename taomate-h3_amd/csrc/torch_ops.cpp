@@ -287,8 +287,11 @@ std::optional<Three> plan_experts(const Tensor& experts, int64_t n_experts, int6
     const c10::DeviceGuard guard(experts.device());
     const Tensor order = empty(experts, {tokens * top_k}, at::kInt), offsets = empty(experts, {n_experts + 1}, at::kInt);
     const Tensor slots = empty(experts, {tokens, top_k}, at::kInt);
+    const int64_t bytes = h3q_plan_experts_workspace_bytes(tokens, top_k, n_experts);
+    Opt ws;
+    if (bytes > 0) ws = empty(experts, {bytes}, at::kByte);
     if (h3q_plan_experts(ints(experts), tokens, top_k, first, n_experts, ints(order), ints(offsets), ints(slots),
-                         stream_of(stream)))
+                         ws ? ws->data_ptr() : nullptr, bytes, stream_of(stream)))
         return std::nullopt;
     return Three(order, offsets, slots);
 }

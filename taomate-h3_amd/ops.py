@@ -695,8 +695,10 @@ def plan_experts(experts: torch.Tensor, n_experts: int, *, first_expert: int = 0
     order = torch.empty(tokens * top_k, device=experts.device, dtype=torch.int32)
     offsets = torch.empty(max(int(n_experts), 0) + 1, device=experts.device, dtype=torch.int32)
     slots = torch.empty((tokens, top_k), device=experts.device, dtype=torch.int32)
+    size = int(_lib.lib().h3q_plan_experts_workspace_bytes(tokens, top_k, int(n_experts)))
+    ws = torch.empty(size, device=experts.device, dtype=torch.uint8) if size else None
     _call_on(experts, "h3q_plan_experts", _ptr(experts), tokens, top_k, int(first_expert), int(n_experts), _ptr(order),
-              _ptr(offsets), _ptr(slots))
+             _ptr(offsets), _ptr(slots), _ptr(ws), size)
     return ExpertPlan(order, offsets, slots)
 
 

@@ -78,8 +78,12 @@ def test_native_refusals_without_gpu():
     refused(1, b"null", "h3q_route_topk", None, *route()[1:])
     assert lib.h3q_route_topk(*route(t=0)) == 0
 
-    refused(1, b"first", "h3q_plan_experts", p, 4, 2, -1, 8, p, p, p, None)
-    refused(1, b"null", "h3q_plan_experts", p, 4, 2, 0, 8, p, None, p, None)
+    refused(1, b"first", "h3q_plan_experts", p, 4, 2, -1, 8, p, p, p, None, 0, None)
+    refused(1, b"null", "h3q_plan_experts", p, 4, 2, 0, 8, p, None, p, None, 0, None)
+    many = lib.h3q_plan_experts_workspace_bytes(1 << 15, 8, 64)
+    assert many > 0 and lib.h3q_plan_experts_workspace_bytes(100, 8, 64) == 0
+    refused(1, b"workspace", "h3q_plan_experts", p, 1 << 15, 8, 0, 64, p, p, p, None, 0, None)
+    refused(1, b"workspace", "h3q_plan_experts", p, 1 << 15, 8, 0, 64, p, p, p, p, many - 1, None)
 
     def grouped(**k):
         return [k.get("fmt", 1), p, k.get("lda", 128), k.get("a_rows", 8), p, k.get("order"), k.get("top_k", 1), k.get("b", p),

@@ -70,7 +70,9 @@ def test_route_strided_rows_and_no_tokens(ops, device):
 
 
 @pytest.mark.parametrize("t,k,total,e,first", [(1, 1, 1, 1, 0), (1, 8, 64, 64, 0), (5, 3, 8, 4, 2), (257, 6, 128, 128, 0),
-                                               (1000, 8, 64, 16, 48), (4099, 4, 256, 64, 64), (63, 64, 1000, 1000, 0)])
+                                               (1000, 8, 64, 16, 48), (4099, 4, 256, 64, 64), (63, 64, 1000, 1000, 0),
+                                               (2048, 1, 8, 8, 0), (2049, 1, 1024, 1024, 0), (70001, 8, 128, 128, 0),
+                                               (9000, 63, 24, 20, 3)])
 def test_plan(ops, device, t, k, total, e, first):
     gen = torch.Generator().manual_seed(t + e)
     ids = torch.randint(-1, total, (t, k), generator=gen, dtype=torch.int32)
