@@ -31,27 +31,36 @@ constexpr int kRowPad = 16;  // LDS rows of codes: 128-byte steps + 16, so 16 ro
 
 __device__ __host__ inline int lds_pitch(int64_t cols) { return (int)((cols + 127) / 128 * 128) + kRowPad; }
 
-// Codes of a bf16 row [cols] (cols % 8 == 0) into LDS by one wave, zeros up to the next
-// multiple of 128; returns the scale.  The row is read twice (the second time from the caches).
-template <int FMT, int ROUND>
-__device__ __forceinline__ float quantize_row(const uint16_t* row, int cols, H3Q_LDS uint8_t* dst, int lane) {
+// Codes of a bf16 row [cols] (cols % 8 == 0) into LDS, zeros up to the next multiple of 128,
+// by the THREADS of one wave or of the workgroup (thread t takes vectors t, t + THREADS, ...);
+// returns the scale.  The first four vectors a thread stay in registers between the maximum
+// and the codes, the rest of a long row is read again.  max_of: the maximum over the threads.
+template <int FMT, int ROUND, int THREADS, class F>
+__device__ __forceinline__ float quantize_row(const uint16_t* row, int cols, H3Q_LDS uint8_t* dst, int t, F max_of) {
+    constexpr int NV = 4;
     const uint4* src = reinterpret_cast<const uint4*>(row);
     const int nvec = cols >> 3, padded = (cols + 127) / 128 * 16;
+    uint4 kept[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int v = t + i * THREADS;
+        kept[i] = v < nvec ? src[v] : make_uint4(0, 0, 0, 0);
+    }
     uint32_t m = 0;
-    for (int v = lane; v < nvec; v += 64) {
-        const uint4 w = src[v];
+    auto up = [&](const uint4& w) __attribute__((always_inline)) {
         m = pk_abs_max(pk_abs_max(pk_abs_max(pk_abs_max(m, w.x), w.y), w.z), w.w);
-    }
+    };
+#pragma unroll
+    for (int i = 0; i < NV; ++i) up(kept[i]);
+    for (int v = t + NV * THREADS; v < nvec; v += THREADS) up(src[v]);
     RowQuant<FMT, ROUND> q;
-    q.init(wave_max(amax_from_packed(m)));
-    for (int v = lane; v < padded; v += 64) {
-        v2u c = {0u, 0u};
-        if (v < nvec) {
-            const uint4 w = src[v];
-            c = v2u{q.pack4(w.x, w.y), q.pack4(w.z, w.w)};
-        }
-        *(H3Q_LDS v2u*)(dst + 8 * v) = c;
-    }
+    q.init(max_of(wave_max(amax_from_packed(m))));
+    auto put = [&](int v, const uint4& w) __attribute__((always_inline)) {
+        if (v < padded) *(H3Q_LDS v2u*)(dst + 8 * v) = v < nvec ? v2u{q.pack4(w.x, w.y), q.pack4(w.z, w.w)} : v2u{0u, 0u};
+    };
+#pragma unroll
+    for (int i = 0; i < NV; ++i) put(t + i * THREADS, kept[i]);
+    for (int v = t + NV * THREADS; v < padded; v += THREADS) put(v, v < nvec ? src[v] : make_uint4(0, 0, 0, 0));
     return q.s;
 }
 
@@ -91,7 +100,7 @@ __global__ __launch_bounds__(256) void few_gate_up_kernel(ExpertFfnArgs p, FewBu
     constexpr int WAVES = 4, SPW = 2;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds_dyn[];  // FUSED: codes of the tokens
     __shared__ __attribute__((aligned(16))) acc_t red[WAVES * 2 * 64];
-    __shared__ float lds_scale[64];
+    __shared__ float lds_scale[64], lds_amax[WAVES];
     __shared__ int lds_pair[WAVES][16];
     H3Q_LDS uint8_t* const codes = (H3Q_LDS uint8_t*)lds_dyn;
 
@@ -161,13 +170,28 @@ __global__ __launch_bounds__(256) void few_gate_up_kernel(ExpertFfnArgs p, FewBu
         uint64_t tokens = 0, m = members;
         for (int i = 0; i < skip; ++i) m &= m - 1;
         for (int i = 0; i < count; ++i, m &= m - 1) tokens |= uint64_t(1) << (__builtin_ctzll(m) / p.top_k);
-        int n = 0;
-        while (tokens) {
+        if (__popcll(tokens) == 1) {  // one token: the whole workgroup quantizes it
             const int t = __builtin_ctzll(tokens);
-            tokens &= tokens - 1;
-            if (n++ % WAVES != wave) continue;
-            const float s = quantize_row<FMT, ROUND>(p.x + t * p.ldx, (int)p.d, codes + t * pitch, lane);
-            if (lane == 0) lds_scale[t] = s;
+            const float s = quantize_row<FMT, ROUND, WAVES * 64>(
+                p.x + t * p.ldx, (int)p.d, codes + t * pitch, threadIdx.x, [&](float wave_amax) {
+                    if (lane == 0) lds_amax[wave] = wave_amax;
+                    __syncthreads();
+                    float m = lds_amax[0];
+#pragma unroll
+                    for (int i = 1; i < WAVES; ++i) m = mag_max(m, lds_amax[i]);
+                    return m;
+                });
+            if (threadIdx.x == 0) lds_scale[t] = s;
+        } else {  // a wave per token
+            int n = 0;
+            while (tokens) {
+                const int t = __builtin_ctzll(tokens);
+                tokens &= tokens - 1;
+                if (n++ % WAVES != wave) continue;
+                const float s = quantize_row<FMT, ROUND, 64>(p.x + t * p.ldx, (int)p.d, codes + t * pitch, lane,
+                                                             [](float m) { return m; });
+                if (lane == 0) lds_scale[t] = s;
+            }
         }
         __syncthreads();
     }
@@ -197,12 +221,12 @@ __global__ __launch_bounds__(256) void few_gate_up_kernel(ExpertFfnArgs p, FewBu
     };
     const int iters = (int)((steps + WAVES - 1) / WAVES);
     const int nc = (iters + SPW - 1) / SPW;
-    for (int c = 0; c < nc; c += 2) {  // chunks past the last read zeros
+    for (int c = 0; c < nc; c += 2) {  // (an odd last chunk's partner was read as zeros)
         mfma_chunk(c, wa);
-        load_w(c + 2, wa);
+        if (c + 2 < nc) load_w(c + 2, wa);
         __builtin_amdgcn_sched_barrier(0);
         mfma_chunk(c + 1, wb);
-        load_w(c + 3, wb);
+        if (c + 2 < nc) load_w(c + 3, wb);
         __builtin_amdgcn_sched_barrier(0);
     }
     red[(wave * 2 + 0) * 64 + lane] = acc[0];
@@ -224,17 +248,18 @@ __global__ __launch_bounds__(256) void few_gate_up_kernel(ExpertFfnArgs p, FewBu
         v2u{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
 }
 
-// 16 columns of the output, over all tiles.
-template <int OP, bool TB, bool FUSED>
+// COLS columns of the output, over all tiles.  8 columns (half a weight block: the other
+// half's lanes load nothing) where 16 would leave CUs without a workgroup.
+template <int OP, bool TB, bool FUSED, int COLS>
 __global__ __launch_bounds__(512) void few_down_kernel(ExpertFfnArgs p, FewBuffers w, int max_tiles) {
     using Mfma = GroupedMfma<OP>;
     using acc_t = typename Mfma::acc_t;
     constexpr int FMT = OP == kOpInt8 ? kFmtInt8 : kFmtE4M3, ROUND = OP == kOpInt8 ? kRoundRcpMul : kRoundDiv;
-    constexpr int WAVES = 8, SPW = 4;
+    constexpr int WAVES = 8, SPW = FUSED ? 4 : 2;  // as many registers as two workgroups a CU leave
     // Segments (1 KB each: one tile's sum by one wave, tile t of wave w at t + w: both only
     // grow along the stream), then (FUSED) the codes of h.
     extern __shared__ __attribute__((aligned(16))) uint8_t lds_dyn[];
-    __shared__ float lds_scale[64], lds_weight[64], lds_y[64 * 16];
+    __shared__ float lds_scale[64], lds_weight[64], lds_y[64 * COLS];
     __shared__ int lds_pair[64 * 16];   // pair of [tile][row], 0 where there is none
     __shared__ int lds_at[64];          // tile * 16 + row of each pair, -1 without an expert
     __shared__ int lds_w0[64], lds_w1[64];  // waves that hold a tile's first and last steps
@@ -244,7 +269,7 @@ __global__ __launch_bounds__(512) void few_down_kernel(ExpertFfnArgs p, FewBuffe
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r16 = lane & 15, kq = lane >> 4;
-    const int n0 = blockIdx.x * 16;
+    const int n0 = blockIdx.x * COLS;
     const int pairs = (int)(p.tokens * p.top_k);
     const int mine = pair_expert(p, pairs, lane);
     int at = -1, tile_expert = 0;  // of pair `lane`; of tile `lane`
@@ -262,7 +287,9 @@ __global__ __launch_bounds__(512) void few_down_kernel(ExpertFfnArgs p, FewBuffe
     // Weight steps s0 .. s1 - 1 of the stream, SPW at a time.
     const int64_t w_bytes = p.d * p.f;
     const int64_t block = TB ? (int64_t)(n0 / 16) * steps * 2048 : (int64_t)n0 * p.f;
-    const uint32_t block_bytes = TB ? (uint32_t)steps * 2048u : (uint32_t)(16 * p.f);
+    const uint32_t block_bytes = TB ? (uint32_t)steps * 2048u : (uint32_t)(COLS * p.f);
+    const bool has_row = r16 < COLS;
+    const uint32_t lane_off = TB ? (uint32_t)(16 * ((n0 & 15) + r16 + 16 * kq)) : (uint32_t)(r16 * p.f + 32 * kq);
     int lt = s0 / steps, lk = s0 - lt * steps;  // tile and k-step of the next load
     auto load_w = [&](int c, v8i (&wf)[SPW]) __attribute__((always_inline)) {
 #pragma unroll
@@ -272,13 +299,13 @@ __global__ __launch_bounds__(512) void few_down_kernel(ExpertFfnArgs p, FewBuffe
             const __amdgpu_buffer_rsrc_t rw = make_rsrc((const uint8_t*)p.w2 + e * w_bytes + block, block_bytes);
             uint32_t lo, hi;
             if constexpr (TB) {
-                lo = in ? (uint32_t)(lk * 2048 + 16 * lane) : kOob;
-                hi = in ? lo + 1024 : kOob;
+                lo = in && has_row ? (uint32_t)(lk * 2048) + lane_off : kOob;
+                hi = in && has_row ? lo + 1024 : kOob;
             } else {
                 const int left = (int)(p.f - lk * 128) - 32 * kq;
-                const uint32_t o = (uint32_t)(r16 * p.f + lk * 128 + 32 * kq);
-                lo = in && left > 0 ? o : kOob;
-                hi = in && left > 16 ? o + 16 : kOob;
+                const uint32_t o = (uint32_t)(lk * 128) + lane_off;
+                lo = in && has_row && left > 0 ? o : kOob;
+                hi = in && has_row && left > 16 ? o + 16 : kOob;
             }
             constexpr int policy = TB ? 2 : 0;
             wf[i] = join(__builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(rw, lo, 0, policy)),
@@ -299,13 +326,13 @@ __global__ __launch_bounds__(512) void few_down_kernel(ExpertFfnArgs p, FewBuffe
     float s2[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
-        const int pair = (threadIdx.x + 512 * q) / 16;
+        const int item = threadIdx.x + 512 * q, pair = item / COLS;
         const int e = __shfl(mine, pair & 63, 64);
-        if (pair < pairs && e >= 0) s2[q] = p.s2[e * p.d + n0 + (threadIdx.x & 15)];
+        if (pair < pairs && e >= 0) s2[q] = p.s2[e * p.d + n0 + item % COLS];
     }
     if (wave == 0) {
         lds_at[lane] = at;
-        lds_weight[lane] = lane < pairs ? p.weights[lane] : 0.0f;
+        lds_weight[lane] = lane < pairs && mine >= 0 ? p.weights[lane] : 0.0f;
         for (int i = 0; i < tiles; i += 4) lds_pair[i * 16 + lane] = 0;
         if (at >= 0) lds_pair[at] = lane;
         if (!FUSED) lds_scale[lane] = lane < pairs ? w.hs[lane] : 0.0f;
@@ -314,13 +341,38 @@ __global__ __launch_bounds__(512) void few_down_kernel(ExpertFfnArgs p, FewBuffe
     if constexpr (FUSED) {
         for (int pair = wave; pair < pairs; pair += WAVES) {
             if (__builtin_amdgcn_readlane(mine, pair) < 0) continue;
-            const float s = quantize_row<FMT, ROUND>(w.h + (int64_t)pair * p.f, (int)p.f, codes + pair * pitch, lane);
+            const float s = quantize_row<FMT, ROUND, 64>(w.h + (int64_t)pair * p.f, (int)p.f, codes + pair * pitch, lane,
+                                                         [](float m) { return m; });
             if (lane == 0) lds_scale[pair] = s;
         }
     }
     __syncthreads();
 
-    const __amdgpu_buffer_rsrc_t rx = make_rsrc(w.hq, (uint32_t)((int64_t)pairs * p.f));  // FUSED: not read
+    // Not FUSED: the codes' fragments are asked for with the weights of the same steps.
+    const __amdgpu_buffer_rsrc_t rx = make_rsrc(w.hq, (uint32_t)((int64_t)pairs * p.f));
+    int xt = s0 / steps, xk = s0 - xt * steps, xrow = 0;
+    v8i xa[FUSED ? 1 : SPW], xb[FUSED ? 1 : SPW];
+    auto load_x = [&](int c, v8i (&xf)[FUSED ? 1 : SPW]) __attribute__((always_inline)) {
+        if constexpr (!FUSED) {
+#pragma unroll
+            for (int i = 0; i < SPW; ++i) {
+                const bool in = s0 + c * SPW + i < s1;
+                if (in && (xk == 0 || c + i == 0)) xrow = lds_pair[xt * 16 + r16];
+                const int left = (int)(p.f - xk * 128) - 32 * kq;
+                const uint32_t o = (uint32_t)(xrow * p.f + xk * 128 + 32 * kq);
+                xf[i] = join(
+                    __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(rx, in && left > 0 ? o : kOob, 0, 0)),
+                    __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(rx, in && left > 16 ? o + 16 : kOob, 0, 0)));
+                if (++xk == steps) {
+                    xk = 0;
+                    ++xt;
+                }
+            }
+        }
+    };
+    load_x(0, xa);
+    load_x(1, xb);
+    __builtin_amdgcn_sched_barrier(0);
     int ct = s0 / steps, ck = s0 - ct * steps;  // tile and k-step of the next product
     int row = 0;                                // pair of this lane's row in tile ct
     acc_t acc = acc_t{};
@@ -333,7 +385,7 @@ __global__ __launch_bounds__(512) void few_down_kernel(ExpertFfnArgs p, FewBuffe
         *(H3Q_LDS acc_t*)(seg + ((ct + wave) * 64 + lane) * 4) = acc;
         if (ck == steps - 1 && lane == 0) lds_w1[ct] = wave;
     };
-    auto mfma_chunk = [&](int c, const v8i (&wf)[SPW]) __attribute__((always_inline)) {
+    auto mfma_chunk = [&](int c, const v8i (&wf)[SPW], const v8i (&xf)[FUSED ? 1 : SPW]) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < SPW; ++i) {
             const int s = s0 + c * SPW + i;
@@ -343,10 +395,7 @@ __global__ __launch_bounds__(512) void few_down_kernel(ExpertFfnArgs p, FewBuffe
                 const H3Q_LDS uint8_t* q = codes + row * pitch + ck * 128 + 32 * kq;
                 x = join(*(const H3Q_LDS v4i*)q, *(const H3Q_LDS v4i*)(q + 16));
             } else {
-                const int left = (int)(p.f - ck * 128) - 32 * kq;
-                const uint32_t o = (uint32_t)(row * p.f + ck * 128 + 32 * kq);
-                x = join(__builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(rx, left > 0 ? o : kOob, 0, 0)),
-                         __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(rx, left > 16 ? o + 16 : kOob, 0, 0)));
+                x = xf[i];
             }
             acc = Mfma::run(wf[i], x, acc);
             if (ck == steps - 1 || s == s1 - 1) leave();
@@ -360,11 +409,17 @@ __global__ __launch_bounds__(512) void few_down_kernel(ExpertFfnArgs p, FewBuffe
     if (s0 < s1) enter();
     const int nc = (s1 - s0 + SPW - 1) / SPW;
     for (int c = 0; c < nc; c += 2) {
-        mfma_chunk(c, wa);
-        load_w(c + 2, wa);
+        mfma_chunk(c, wa, xa);
+        if (c + 2 < nc) {
+            load_w(c + 2, wa);
+            load_x(c + 2, xa);
+        }
         __builtin_amdgcn_sched_barrier(0);
-        mfma_chunk(c + 1, wb);
-        load_w(c + 3, wb);
+        mfma_chunk(c + 1, wb, xb);
+        if (c + 2 < nc) {
+            load_w(c + 3, wb);
+            load_x(c + 3, xb);
+        }
         __builtin_amdgcn_sched_barrier(0);
     }
     __syncthreads();
@@ -372,22 +427,27 @@ __global__ __launch_bounds__(512) void few_down_kernel(ExpertFfnArgs p, FewBuffe
     // y of each pair, its waves' sums in wave order; then the tokens' weighted sums.
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
-        const int item = threadIdx.x + 512 * q, pair = item / 16, col = item & 15;
-        if (pair >= pairs || lds_at[pair] < 0) continue;
-        const int tile = lds_at[pair] / 16, r = lds_at[pair] & 15;
-        const int last = lds_w1[tile];
-        acc_t sum = acc_t{};  // one element of it is used
-        for (int v = lds_w0[tile]; v <= last; ++v)
-            sum[0] += ((const H3Q_LDS decltype(sum[0] + 0)*)seg)[((tile + v) * 64 + r + 16 * (col >> 2)) * 4 + (col & 3)];
-        lds_y[item] = __fmul_rn(lds_scale[pair], __fmul_rn(s2[q], (float)sum[0]));
+        const int item = threadIdx.x + 512 * q, pair = item / COLS, col = item % COLS;
+        if (pair >= pairs) continue;
+        float y = 0.0f;
+        const int place = lds_at[pair];
+        if (place >= 0) {
+            const int tile = place / 16, r = place & 15, last = lds_w1[tile];
+            acc_t sum = acc_t{};  // one element of it is used
+            for (int v = lds_w0[tile]; v <= last; ++v)
+                sum[0] += ((const H3Q_LDS decltype(sum[0] + 0)*)seg)[((tile + v) * 64 + r + 16 * (col >> 2)) * 4 + (col & 3)];
+            y = __fmul_rn(lds_scale[pair], __fmul_rn(s2[q], (float)sum[0]));
+        }
+        lds_y[item] = y;
     }
     __syncthreads();
-    for (int item = threadIdx.x; item < (int)p.tokens * 16; item += 512) {
-        const int token = item / 16, col = item & 15;
+    for (int item = threadIdx.x; item < (int)p.tokens * COLS; item += 512) {
+        const int token = item / COLS, col = item % COLS;
         float out = 0.0f;
-        for (int j = 0; j < p.top_k; ++j) {
+#pragma unroll 8
+        for (int j = 0; j < p.top_k; ++j) {  // a pair without an expert: 0 * 0
             const int pair = token * p.top_k + j;
-            if (lds_at[pair] >= 0) out = __builtin_fmaf(lds_weight[pair], lds_y[pair * 16 + col], out);
+            out = __builtin_fmaf(lds_weight[pair], lds_y[pair * COLS + col], out);
         }
         p.out[token * p.ldo + n0 + col] = (uint16_t)f32_to_bf16_bits(out);
     }
@@ -418,16 +478,22 @@ void launch_up(const ExpertFfnArgs& a, const FewBuffers& w, hipStream_t st) {
         hipLaunchKernelGGL((few_gate_up_kernel<OP, TB, false>), grid, dim3(256), 0, st, a, w, slices);
 }
 
-template <int OP, bool TB>
-void launch_down(const ExpertFfnArgs& a, const FewBuffers& w, hipStream_t st) {
+template <int OP, bool TB, int COLS>
+void launch_down_cols(const ExpertFfnArgs& a, const FewBuffers& w, hipStream_t st) {
     const int tiles = few_tiles(a);
     const unsigned segments = (unsigned)(tiles + 8) * 1024;
-    const dim3 grid((unsigned)(a.d / 16));
+    const dim3 grid((unsigned)(a.d / COLS));
     if (fused_down(a))
-        hipLaunchKernelGGL((few_down_kernel<OP, TB, true>), grid, dim3(512),
+        hipLaunchKernelGGL((few_down_kernel<OP, TB, true, COLS>), grid, dim3(512),
                            segments + (unsigned)(a.tokens * a.top_k * lds_pitch(a.f)), st, a, w, tiles);
     else
-        hipLaunchKernelGGL((few_down_kernel<OP, TB, false>), grid, dim3(512), segments, st, a, w, tiles);
+        hipLaunchKernelGGL((few_down_kernel<OP, TB, false, COLS>), grid, dim3(512), segments, st, a, w, tiles);
+}
+
+template <int OP, bool TB>
+void launch_down(const ExpertFfnArgs& a, const FewBuffers& w, hipStream_t st) {
+    if (a.d / 16 < 256) launch_down_cols<OP, TB, 8>(a, w, st);
+    else launch_down_cols<OP, TB, 16>(a, w, st);
 }
 
 }  // namespace
