@@ -204,7 +204,7 @@ __global__ __launch_bounds__(256) void few_gate_up_kernel(ExpertFfnArgs p, FewBu
             const H3Q_LDS uint8_t* q = codes + token * pitch + st * 128 + 32 * kq;
             return join(*(const H3Q_LDS v4i*)q, *(const H3Q_LDS v4i*)(q + 16));
         } else {
-            const int left = (int)(p.d - st * 128) - 32 * kq;
+            const int left = r16 < count ? (int)(p.d - st * 128) - 32 * kq : 0;
             const uint32_t o = (uint32_t)(token * p.d + st * 128 + 32 * kq);
             return join(__builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(rx, left > 0 ? o : kOob, 0, 0)),
                         __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(rx, left > 16 ? o + 16 : kOob, 0, 0)));
@@ -260,7 +260,7 @@ __global__ __launch_bounds__(512) void few_down_kernel(ExpertFfnArgs p, FewBuffe
     // grow along the stream), then (FUSED) the codes of h.
     extern __shared__ __attribute__((aligned(16))) uint8_t lds_dyn[];
     __shared__ float lds_scale[64], lds_weight[64], lds_y[64 * COLS];
-    __shared__ int lds_pair[64 * 16];   // pair of [tile][row], 0 where there is none
+    __shared__ int lds_pair[64 * 16];   // pair of [tile][row], -1 where there is none
     __shared__ int lds_at[64];          // tile * 16 + row of each pair, -1 without an expert
     __shared__ int lds_w0[64], lds_w1[64];  // waves that hold a tile's first and last steps
     H3Q_LDS float* const seg = (H3Q_LDS float*)lds_dyn;
@@ -333,7 +333,7 @@ __global__ __launch_bounds__(512) void few_down_kernel(ExpertFfnArgs p, FewBuffe
     if (wave == 0) {
         lds_at[lane] = at;
         lds_weight[lane] = lane < pairs && mine >= 0 ? p.weights[lane] : 0.0f;
-        for (int i = 0; i < tiles; i += 4) lds_pair[i * 16 + lane] = 0;
+        for (int i = 0; i < tiles; i += 4) lds_pair[i * 16 + lane] = -1;
         if (at >= 0) lds_pair[at] = lane;
         if (!FUSED) lds_scale[lane] = lane < pairs ? w.hs[lane] : 0.0f;
     }
@@ -358,7 +358,7 @@ __global__ __launch_bounds__(512) void few_down_kernel(ExpertFfnArgs p, FewBuffe
             for (int i = 0; i < SPW; ++i) {
                 const bool in = s0 + c * SPW + i < s1;
                 if (in && (xk == 0 || c + i == 0)) xrow = lds_pair[xt * 16 + r16];
-                const int left = (int)(p.f - xk * 128) - 32 * kq;
+                const int left = xrow < 0 ? 0 : (int)(p.f - xk * 128) - 32 * kq;
                 const uint32_t o = (uint32_t)(xrow * p.f + xk * 128 + 32 * kq);
                 xf[i] = join(
                     __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(rx, in && left > 0 ? o : kOob, 0, 0)),
@@ -378,6 +378,7 @@ __global__ __launch_bounds__(512) void few_down_kernel(ExpertFfnArgs p, FewBuffe
     acc_t acc = acc_t{};
     auto enter = [&]() __attribute__((always_inline)) {  // before a step of tile ct
         row = lds_pair[ct * 16 + r16];
+        row = row < 0 ? 0 : row;  // a row without a pair: any codes, its sums are not used
         acc = acc_t{};
         if (ck == 0 && lane == 0) lds_w0[ct] = wave;
     };
@@ -464,7 +465,11 @@ int few_tiles(const ExpertFfnArgs& a) {  // at most
     return most < pairs ? most : pairs;
 }
 
-bool fused_up(const ExpertFfnArgs& a) { return a.tokens * lds_pitch(a.d) <= kFewLdsCodes; }
+// Quantizing inside the gate-up kernel pays while its workgroups are all resident at once; in
+// further rounds each would pay again what one launch of the row quantizer costs.
+bool fused_up(const ExpertFfnArgs& a) {
+    return a.tokens * lds_pitch(a.d) <= kFewLdsCodes && a.f / 16 * few_tiles(a) <= 1024;
+}
 bool fused_down(const ExpertFfnArgs& a) { return a.tokens * a.top_k * lds_pitch(a.f) <= kFewLdsCodes; }
 
 template <int OP, bool TB>
