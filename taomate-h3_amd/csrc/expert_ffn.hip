@@ -130,11 +130,14 @@ hipError_t launch_expert_ffn(const ExpertFfnArgs& a, void* workspace, hipStream_
     plan.offsets = p.offsets;
     plan.slots = p.slots;
     plan.workspace = p.plan;
-    hipError_t e = launch_plan_experts(plan, st);
+    hipError_t e;
+    if (plan_quant_supported(plan, a.tokens)) {
+        e = launch_plan_quant(plan, fmt, a.x, a.ldx, a.tokens, a.d, p.xq, p.xs, st);
+    } else {
+        e = launch_plan_experts(plan, st);
+        if (e == hipSuccess) e = launch_quant_rows(a.x, a.ldx, a.tokens, a.d, fmt, rounding, p.xq, a.d, p.xs, st);
+    }
     if (e != hipSuccess) return e;
-    e = launch_quant_rows(a.x, a.ldx, a.tokens, a.d, fmt, rounding, p.xq, a.d, p.xs, st);
-    if (e != hipSuccess) return e;
-
     e = launch_grouped_mm(a.kind, gate_up(a, p), st);
     if (e != hipSuccess) return e;
     // Rows past the last placed pair hold what the workspace held; their codes are never read.

@@ -5,6 +5,7 @@
 
 #include "h3q_common.hpp"
 #include "h3q_kernels.hpp"
+#include "row_quant.hpp"
 
 namespace h3q {
 
@@ -202,14 +203,14 @@ __device__ __forceinline__ uint64_t match(int v, int bits, uint64_t valid) {
 
 enum PlanPhase : int { kPlanWhole = 0, kPlanCount = 1, kPlanPlace = 2 };
 
+// Block `block` of `blocks` of a plan.  table: LDS of kPlanWaves * experts integers,
+// [wave][expert]: counts, then the next row of that expert in the wave's span.
 template <int PHASE>
-__global__ __launch_bounds__(kPlanWaves * 64) void plan_experts_kernel(PlanArgs p, int64_t chunk, int bits) {
-    // [wave][expert]: counts, then the next row of that expert in the wave's span
-    extern __shared__ int table[];
+__device__ __forceinline__ void plan_block(const PlanArgs& p, int64_t chunk, int bits, int block, int blocks, int* table) {
     __shared__ int wave_sum[kPlanWaves];
     __shared__ int rows_all[kMaxExperts], rows_below[kMaxExperts];  // of each expert, over the blocks
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int n = p.experts, blocks = gridDim.x, block = blockIdx.x;
+    const int n = p.experts;
     const int64_t begin = block * chunk, end = begin + chunk < p.pairs ? begin + chunk : p.pairs;
     const int64_t trips = (end - begin + 63) / 64;
     const int64_t t0 = trips * wave / kPlanWaves, t1 = trips * (wave + 1) / kPlanWaves;
@@ -328,7 +329,58 @@ __global__ __launch_bounds__(kPlanWaves * 64) void plan_experts_kernel(PlanArgs 
         p.order[i] = -1;
 }
 
+template <int PHASE>
+__global__ __launch_bounds__(kPlanWaves * 64) void plan_experts_kernel(PlanArgs p, int64_t chunk, int bits) {
+    extern __shared__ int table[];
+    plan_block<PHASE>(p, chunk, bits, blockIdx.x, gridDim.x, table);
+}
+
+// The plan of up to kPlanChunk pairs (workgroup 0) and the codes of the tokens (a workgroup
+// each of the others), in one launch: neither needs the other, and both are shorter than the
+// launch that this saves.
+template <int FMT, int ROUND>
+__global__ __launch_bounds__(kPlanWaves * 64) void plan_quant_kernel(PlanArgs p, int bits, const uint16_t* x, int64_t ldx,
+                                                                     int cols, uint8_t* codes, float* scales) {
+    extern __shared__ int table[];
+    if (blockIdx.x == 0) {
+        plan_block<kPlanWhole>(p, kPlanChunk, bits, 0, 1, table);
+        return;
+    }
+    __shared__ float wave_amax[kPlanWaves];
+    const int64_t row = blockIdx.x - 1;
+    const uint4* const src = reinterpret_cast<const uint4*>(x + row * ldx);
+    const int nvec = cols >> 3, t = threadIdx.x;
+    constexpr int THREADS = kPlanWaves * 64;
+    const uint4 first = t < nvec ? src[t] : make_uint4(0, 0, 0, 0);
+    uint32_t m = pk_abs_max(pk_abs_max(pk_abs_max(pk_abs_max(0, first.x), first.y), first.z), first.w);
+    for (int v = t + THREADS; v < nvec; v += THREADS) {
+        const uint4 w = src[v];
+        m = pk_abs_max(pk_abs_max(pk_abs_max(pk_abs_max(m, w.x), w.y), w.z), w.w);
+    }
+    const float amax = wave_max(amax_from_packed(m));
+    if ((t & 63) == 0) wave_amax[t >> 6] = amax;
+    __syncthreads();
+    float all = wave_amax[0];
+#pragma unroll
+    for (int w = 1; w < kPlanWaves; ++w) all = mag_max(all, wave_amax[w]);
+    RowQuant<FMT, ROUND> q;
+    q.init(all);
+    v2u* const dst = reinterpret_cast<v2u*>(codes + row * cols);
+    if (t < nvec) dst[t] = v2u{q.pack4(first.x, first.y), q.pack4(first.z, first.w)};
+    for (int v = t + THREADS; v < nvec; v += THREADS) {
+        const uint4 w = src[v];
+        dst[v] = v2u{q.pack4(w.x, w.y), q.pack4(w.z, w.w)};
+    }
+    if (t == 0) scales[row] = q.s;
+}
+
 namespace {
+
+int expert_bits(int experts) {
+    int bits = 0;
+    while ((1 << bits) < experts) ++bits;
+    return bits;
+}
 
 // Pairs per block: at most 256 blocks, so a placing block's sum over them stays short.
 int64_t plan_chunk(int64_t pairs) {
@@ -347,8 +399,7 @@ hipError_t launch_plan_experts(const PlanArgs& a, hipStream_t st) {
     const int64_t chunk = plan_chunk(a.pairs);
     const unsigned blocks = a.pairs <= chunk ? 1u : (unsigned)((a.pairs + chunk - 1) / chunk);
     const unsigned lds = (unsigned)(kPlanWaves * a.experts * sizeof(int));
-    int bits = 0;
-    while ((1 << bits) < a.experts) ++bits;
+    const int bits = expert_bits(a.experts);
     const dim3 threads(kPlanWaves * 64);
     if (blocks == 1) {
         hipLaunchKernelGGL((plan_experts_kernel<kPlanWhole>), dim3(1), threads, lds, st, a, chunk, bits);
@@ -356,6 +407,22 @@ hipError_t launch_plan_experts(const PlanArgs& a, hipStream_t st) {
         hipLaunchKernelGGL((plan_experts_kernel<kPlanCount>), dim3(blocks), threads, lds, st, a, chunk, bits);
         hipLaunchKernelGGL((plan_experts_kernel<kPlanPlace>), dim3(blocks), threads, lds, st, a, chunk, bits);
     }
+    return hipGetLastError();
+}
+
+bool plan_quant_supported(const PlanArgs& a, int64_t tokens) { return a.pairs <= kPlanChunk && tokens <= 512; }
+
+hipError_t launch_plan_quant(const PlanArgs& a, int fmt, const uint16_t* x, int64_t ldx, int64_t tokens, int64_t cols,
+                             uint8_t* codes, float* scales, hipStream_t st) {
+    const dim3 grid((unsigned)(tokens + 1)), threads(kPlanWaves * 64);
+    const unsigned lds = (unsigned)(kPlanWaves * a.experts * sizeof(int));
+    const int bits = expert_bits(a.experts);
+    if (fmt == kFmtInt8)
+        hipLaunchKernelGGL((plan_quant_kernel<kFmtInt8, kRoundRcpMul>), grid, threads, lds, st, a, bits, x, ldx, (int)cols,
+                           codes, scales);
+    else
+        hipLaunchKernelGGL((plan_quant_kernel<kFmtE4M3, kRoundDiv>), grid, threads, lds, st, a, bits, x, ldx, (int)cols,
+                           codes, scales);
     return hipGetLastError();
 }
 
@@ -377,7 +444,7 @@ __device__ __forceinline__ void load8(const void* p, int64_t i, float (&v)[8]) {
 }  // namespace
 
 // out[t] = bf16(sum_j weights[t, j] * rows[slots[t, j]]), binary32 products and sums in
-// slot order, one rounding.  A thread takes 8 columns of a token, four slots' loads in
+// slot order, one rounding.  A thread takes 8 columns of a token, eight slots' loads in
 // flight at a time; a slot outside [0, rows) adds nothing.  Bound by reading the rows.
 template <bool F32>
 __global__ __launch_bounds__(256) void combine_experts_kernel(CombineArgs p) {
@@ -386,20 +453,27 @@ __global__ __launch_bounds__(256) void combine_experts_kernel(CombineArgs p) {
     if (i >= total) return;
     const int64_t token = i / vecs, col = (i - token * vecs) * 8;
     float sum[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-    for (int j0 = 0; j0 < p.top_k; j0 += 4) {
-        float v[4][8], w[4];
+    for (int j0 = 0; j0 < p.top_k; j0 += 8) {
+        float v[8][8], w[8];
+        int slot[8];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < 8; ++c) {
             const int j = j0 + c;
-            const int slot = j < p.top_k ? p.slots[token * p.top_k + j] : -1;
-            const bool in = slot >= 0 && slot < p.rows;
-            w[c] = in ? p.weights[token * p.top_k + j] : 0.0f;
-            if (in) load8<F32>(p.y, slot * p.ldy + col, v[c]);
-            else
-                for (int x = 0; x < 8; ++x) v[c][x] = 0.0f;
+            slot[c] = j < p.top_k ? p.slots[token * p.top_k + j] : -1;
+            w[c] = j < p.top_k ? p.weights[token * p.top_k + j] : 0.0f;
         }
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+        for (int c = 0; c < 8; ++c) {
+            if (slot[c] >= 0 && slot[c] < p.rows) {
+                load8<F32>(p.y, slot[c] * p.ldy + col, v[c]);
+            } else {
+                w[c] = 0.0f;
+#pragma unroll
+                for (int x = 0; x < 8; ++x) v[c][x] = 0.0f;
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
 #pragma unroll
             for (int x = 0; x < 8; ++x) sum[x] = __builtin_fmaf(w[c], v[c][x], sum[x]);
     }

@@ -190,6 +190,12 @@ struct PlanArgs {
 int64_t plan_workspace_ints(int64_t pairs, int experts);
 hipError_t launch_plan_experts(const PlanArgs& a, hipStream_t st);
 
+// The plan and the tokens' codes (rows of cols bytes) in one launch, for few pairs; x 16-byte
+// aligned, cols and ldx multiples of 8, cols of 16; fmt as the activations' (int8: RCP_MUL).
+bool plan_quant_supported(const PlanArgs& a, int64_t tokens);
+hipError_t launch_plan_quant(const PlanArgs& a, int fmt, const uint16_t* x, int64_t ldx, int64_t tokens, int64_t cols,
+                             uint8_t* codes, float* scales, hipStream_t st);
+
 struct CombineArgs {
     const void* y;  // [rows, cols] bf16 or binary32, ldy elements
     int64_t ldy, rows;
