@@ -25,7 +25,7 @@ CEILINGS_SRC = "ceilings.hip"
 CEILINGS_LIB = PKG / "libh3q_ceilings.so"
 SOURCES = ["act_quant.hip", "head_quant.hip", "norm_quant.hip", "swiglu_quant.hip", "gemm.hip", "gemm_w4.hip", "gemm_skinny.hip",
            "gemm_stream.hip", "gemm_stream_e4m3_tiled.hip", "gemm_stream_e4m3_rows.hip", "gemm_stream_int8_tiled.hip",
-           "gemm_stream_int8_rows.hip", "experts.hip", "grouped_stream.hip", "grouped_tile.hip", "expert_few.hip", "expert_ffn.hip", "capi.hip"]
+           "gemm_stream_int8_rows.hip", "experts.hip", "grouped_gemm.hip", "grouped_stream.hip", "grouped_band.hip", "grouped_tile.hip", "expert_few.hip", "expert_ffn.hip", "capi.hip"]
 
 # Native tensor wrappers (host code against torch's C++ interface), linked to LIB.
 TORCH_SRC = "torch_ops.cpp"

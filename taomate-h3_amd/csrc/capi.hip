@@ -673,12 +673,11 @@ __attribute__((visibility("default"))) int h3q_grouped_mm(int format, const void
     g.f32 = out_f32 != 0;
     g.out = out;
     g.ldo = ldo;
-    if (!h3q::grouped_mm_fits(g))
+    const int kind = format == H3Q_FMT_INT8 ? h3q::kOpInt8 : h3q::kOpE4M3;
+    if (!h3q::grouped_mm_fits(kind, g))
         return fail(H3Q_ERR_UNSUPPORTED, "%s: %lld rows x %lld columns need too many workgroups", who, (long long)rows,
                     (long long)n);
-    return check_launch(h3q::launch_grouped_mm(format == H3Q_FMT_INT8 ? h3q::kOpInt8 : h3q::kOpE4M3, g,
-                                               (hipStream_t)stream),
-                        who);
+    return check_launch(h3q::launch_grouped_mm(kind, g, (hipStream_t)stream), who);
 }
 
 __attribute__((visibility("default"))) int h3q_combine_experts(const void* y, int y_f32, int64_t ldy, int64_t rows,

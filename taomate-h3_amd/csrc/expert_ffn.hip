@@ -74,6 +74,7 @@ GroupedArgs gate_up(const ExpertFfnArgs& a, const Parts& p) {
     g.n = (int)(2 * a.f);
     g.k = a.d;
     g.swiglu = 1;
+    g.wide = 1;  // h is quantized again
     g.out = p.h;
     g.ldo = a.f;
     return g;
@@ -104,7 +105,8 @@ GroupedArgs down(const ExpertFfnArgs& a, const Parts& p) {
 
 bool expert_ffn_fits(const ExpertFfnArgs& a) {
     const Parts none{};
-    return grouped_mm_fits(gate_up(a, none)) && grouped_mm_fits(down(a, none));
+    return expert_few_supported(a) ||
+           (grouped_mm_fits(a.kind, gate_up(a, none)) && grouped_mm_fits(a.kind, down(a, none)));
 }
 
 int64_t expert_ffn_workspace_bytes(const ExpertFfnArgs& a) {

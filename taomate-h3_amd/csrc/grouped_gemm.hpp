@@ -73,6 +73,9 @@ struct GroupedMfma<kOpInt8, WIDE> {
     }
 };
 
+// What a grouped product stores.  kOutWide: SwiGLU from wide products.
+enum GroupedOut : int { kOutBF16 = 0, kOutF32 = 1, kOutSwiglu = 2, kOutWide = 3 };
+
 // silu(g) * u in binary32: exp(-g) by the hardware exp2, IEEE sum, quotient and product.
 // (g = -inf gives NaN, as -inf / inf does.)
 __device__ __forceinline__ float swiglu_f32(float g, float u) {

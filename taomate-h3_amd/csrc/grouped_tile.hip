@@ -97,8 +97,6 @@ struct TileOp<kOpInt8> {
     static constexpr int kSteps = 2;
 };
 
-enum TileOut : int { kOutBF16 = 0, kOutF32 = 1, kOutSwiglu = 2 };
-
 }  // namespace
 
 template <int OP, bool TB, int OUT>

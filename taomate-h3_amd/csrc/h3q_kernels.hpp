@@ -209,7 +209,7 @@ struct CombineArgs {
 };
 hipError_t launch_combine_experts(const CombineArgs& a, bool f32, hipStream_t st);
 
-// Scaled product of rows grouped by expert (grouped_stream.hip).
+// Scaled product of rows grouped by expert.
 struct GroupedArgs {
     const void* a;         // codes [a_rows, k], row-major, lda bytes (16-byte aligned rows)
     int64_t lda, a_rows;
@@ -225,14 +225,22 @@ struct GroupedArgs {
     int n;                 // a multiple of 16 (SwiGLU: of 32, rows [gate | up])
     int64_t k;             // a multiple of 16 (tiled: of 128)
     int swiglu, f32;       // f32: binary32 output instead of bf16 (not with SwiGLU)
+    int wide;              // SwiGLU of e4m3: bf16 products, for an output that is quantized again
     void* out;             // [rows, n or n / 2]
     int64_t ldo;           // in elements
 };
-// The same over 256 x 256 tiles (grouped_tile.hip), for groups of many rows.
+// Weight streaming for up to 16 rows of an expert at a time (grouped_stream.hip).
+int64_t grouped_stream_grid(const GroupedArgs& a);
+hipError_t launch_grouped_stream(int kind, const GroupedArgs& a, hipStream_t st);
+// Bands of 16 * blocks (2, 4 or 8) rows (grouped_band.hip).
+int64_t grouped_band_grid(const GroupedArgs& a, int blocks);
+hipError_t launch_grouped_band(int kind, const GroupedArgs& a, int blocks, hipStream_t st);
+// 256 x 256 tiles (grouped_tile.hip); no wide products.
 bool grouped_tile_supported(const GroupedArgs& a);
 hipError_t launch_grouped_tile(int kind, const GroupedArgs& a, hipStream_t st);
-// Whether the call's grid stays within what a launch takes.
-bool grouped_mm_fits(const GroupedArgs& a);
+// The one of them that suits the call (grouped_gemm.hip); whether its grid stays within
+// what a launch takes.
+bool grouped_mm_fits(int kind, const GroupedArgs& a);
 hipError_t launch_grouped_mm(int kind, const GroupedArgs& a, hipStream_t st);
 
 // The FFN of a routed-expert layer (expert_ffn.hip).
