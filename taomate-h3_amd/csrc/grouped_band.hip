@@ -9,7 +9,11 @@
 // D k-steps of 128 bytes ahead, and the activation rows of a step come once into an LDS ring
 // that the four waves share (LDS-DMA, gathered rows as cheaply as dense ones).  One barrier a
 // step publishes the next stage and frees the last.  No split of K: the experts give
-// workgroups enough.
+// workgroups enough.  Items (band x column slice) go to the XCDs in contiguous runs, an
+// expert's bands of one slice side by side, so weights and rows pass through one L2 about
+// once: spread over the XCDs, two bands an expert moved 505 MB from beyond the L2s where
+// 197 MB were needed, and that was the bound (32 experts of 2816 x 2048 with 200 rows each:
+// 84 -> 70 us; 8 of 14336 x 5376: 197 -> 185 us).
 //
 // SwiGLU: a wave's two 16-row blocks are gate and up rows of the same columns, so both sit in
 // one lane.  The output tile is staged in LDS and stored as whole row pieces.
@@ -35,28 +39,34 @@ __device__ __forceinline__ void band_copy(const CopySrc& src, uint32_t lds_base,
 }  // namespace
 
 template <int OP, int MT, bool TB, int OUT>
-__global__ __launch_bounds__(kBandWaves * 64, 2) void grouped_band_kernel(GroupedArgs p, int slices) {
+__global__ __launch_bounds__(kBandWaves * 64, MT == 8 || OUT == kOutWide ? 2 : 3) void grouped_band_kernel(GroupedArgs p, int slices) {
     constexpr bool SWIGLU = OUT == kOutSwiglu || OUT == kOutWide;
     using Mfma = GroupedMfma<OP, OUT == kOutWide>;
     using acc_t = typename Mfma::acc_t;
     // Loads complete in order, so the wait for a stage of rows also waits for the weights asked
-    // for before it: the ring is about as deep as the weights run ahead (two workgroups a CU).
-    constexpr int BM = 16 * MT, SA = MT == 8 ? 5 : 8, D = MT == 8 ? 4 : 6;
+    // for before it: the ring is as deep as the weights run ahead, and as two or three
+    // workgroups a CU (64 rows) have LDS for.
+    constexpr int BM = 16 * MT, SA = MT == 8 ? 5 : 6, D = 4;
     constexpr int STAGE = MT * 2048;   // one k-step of the rows
     constexpr int CA = MT / 2;         // 1 KiB copies per wave and step
     // Loads a wave has issued after the copies of stage s + 1 when it waits for them in step s:
     // the weights of that step and all of the SA - 3 steps since.
     constexpr int WAIT = 4 + (SA - 3) * (CA + 4);
-    static_assert(MT % 2 == 0 && D * 4 + SA * CA < 63, "vmcnt range");
+    static_assert((MT == 4 || MT == 8) && D * 4 + SA * CA < 63, "vmcnt range");
     __shared__ __attribute__((aligned(1024))) uint8_t lds_ring[SA * STAGE];
+    __shared__ __attribute__((aligned(16))) float lds_scales[MT == 8 ? 4 : BM + 128];
     H3Q_LDS uint8_t* const ring = (H3Q_LDS uint8_t*)lds_ring;
+    // Row scales [BM], then the column scales of the waves' blocks; 128-row bands have no LDS
+    // beside the ring (two workgroups share a CU's) and take its end, past the output tile.
+    H3Q_LDS float* const lds_sa = MT == 8 ? (H3Q_LDS float*)(ring + BM * 512) : (H3Q_LDS float*)lds_scales;
+    H3Q_LDS float* const lds_sw = lds_sa + BM;
 
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r16 = lane & 15, kq = lane >> 4;
-    const int slice = blockIdx.x % slices;
-    const GroupTile tile = group_tile(p.offsets, p.experts, p.rows, BM, blockIdx.x / slices);
-    if (tile.rows <= 0) return;
+    GroupTile tile;
+    int slice;
+    if (!group_item(p.offsets, p.experts, p.rows, BM, slices, blockIdx.x, tile, slice)) return;
     const int expert = __builtin_amdgcn_readfirstlane(tile.expert);
     const int rows = __builtin_amdgcn_readfirstlane(tile.rows);
     const int half = p.n / 2;
@@ -138,19 +148,13 @@ __global__ __launch_bounds__(kBandWaves * 64, 2) void grouped_band_kernel(Groupe
         return join(*(const H3Q_LDS v4i*)(q + frag_lo), *(const H3Q_LDS v4i*)(q + frag_hi));
     };
 
-    // Scales of the epilogue: this lane's row of each block, its four columns of each weight block.
-    float sa[MT];
-#pragma unroll
-    for (int t = 0; t < MT; ++t) {
-        const int64_t r = source_row(16 * t + r16);
-        sa[t] = r >= 0 ? p.a_scale[r] : 0.0f;
-    }
-    v4f sw[2];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const int row = block_row(j);
-        sw[j] = row < p.n ? *reinterpret_cast<const v4f*>(p.b_scale + (int64_t)expert * p.n + row + 4 * kq)
-                          : v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    // Scales of the epilogue, one row's and one weight row's a thread until then.
+    float my_sa = 0.0f, my_sw = 0.0f;
+    {
+        const int64_t r = threadIdx.x < BM ? source_row(threadIdx.x) : -1;
+        if (r >= 0) my_sa = p.a_scale[r];
+        const int row = block_row(lane >> 4 & 1);
+        if (row < p.n) my_sw = p.b_scale[(int64_t)expert * p.n + row + r16];
     }
     __builtin_amdgcn_sched_barrier(0);
 
@@ -202,15 +206,22 @@ __global__ __launch_bounds__(kBandWaves * 64, 2) void grouped_band_kernel(Groupe
 
     // The tile in LDS (16-byte chunk c of row r at c ^ (r % 8)), then whole row pieces.
     constexpr int EL = OUT == kOutF32 ? 4 : 2, COLS = SWIGLU ? 64 : 128, PITCH = COLS * EL, CH = PITCH / 16;
-    static_assert(BM * PITCH <= SA * STAGE, "output tile");
+    static_assert(BM * PITCH + (MT == 8 ? 4 * (BM + 128) : 0) <= SA * STAGE, "output tile");
+    if (threadIdx.x < BM) lds_sa[threadIdx.x] = my_sa;
+    if (lane < 32) lds_sw[32 * wave + lane] = my_sw;
+    __syncthreads();
+    v4f sw[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) sw[j] = *(const H3Q_LDS v4f*)(lds_sw + 32 * wave + 16 * j + 4 * kq);
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
         const int m = 16 * t + r16;
+        const float sa = lds_sa[m];
         float y[2][4];
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
-            for (int v = 0; v < 4; ++v) y[j][v] = __fmul_rn(sa[t], __fmul_rn(sw[j][v], (float)acc[j][t][v]));
+            for (int v = 0; v < 4; ++v) y[j][v] = __fmul_rn(sa, __fmul_rn(sw[j][v], (float)acc[j][t][v]));
         if constexpr (SWIGLU) {
             float h[4];
 #pragma unroll
@@ -248,7 +259,7 @@ int band_slices(const GroupedArgs& a) { return a.swiglu ? (a.n / 2 + 63) / 64 : 
 template <int OP, int MT, bool TB>
 hipError_t launch_band_tb(const GroupedArgs& a, hipStream_t st) {
     const int slices = band_slices(a);
-    const dim3 grid((unsigned)((a.experts + a.rows / (16 * MT)) * slices)), block(kBandWaves * 64);
+    const dim3 grid((unsigned)grouped_band_grid(a, MT)), block(kBandWaves * 64);
     if (OP == kOpE4M3 && a.swiglu && a.wide)
         hipLaunchKernelGGL((grouped_band_kernel<kOpE4M3, MT, TB, kOutWide>), grid, block, 0, st, a, slices);
     else if (a.swiglu)
@@ -267,17 +278,13 @@ hipError_t launch_band_mt(const GroupedArgs& a, hipStream_t st) {
 
 template <int OP>
 hipError_t launch_band_op(const GroupedArgs& a, int blocks, hipStream_t st) {
-    switch (blocks) {
-        case 2: return launch_band_mt<OP, 2>(a, st);
-        case 4: return launch_band_mt<OP, 4>(a, st);
-        default: return launch_band_mt<OP, 8>(a, st);
-    }
+    return blocks == 4 ? launch_band_mt<OP, 4>(a, st) : launch_band_mt<OP, 8>(a, st);
 }
 
 }  // namespace
 
 int64_t grouped_band_grid(const GroupedArgs& a, int blocks) {
-    return (a.experts + a.rows / (16 * blocks)) * band_slices(a);
+    return ((a.experts + a.rows / (16 * blocks)) * band_slices(a) + 7) / 8 * 8;  // a run of each of 8 XCDs
 }
 
 hipError_t launch_grouped_band(int kind, const GroupedArgs& a, int blocks, hipStream_t st) {

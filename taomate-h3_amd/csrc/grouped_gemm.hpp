@@ -76,11 +76,12 @@ struct GroupedMfma<kOpInt8, WIDE> {
 // What a grouped product stores.  kOutWide: SwiGLU from wide products.
 enum GroupedOut : int { kOutBF16 = 0, kOutF32 = 1, kOutSwiglu = 2, kOutWide = 3 };
 
-// silu(g) * u in binary32: exp(-g) by the hardware exp2, IEEE sum, quotient and product.
-// (g = -inf gives NaN, as -inf / inf does.)
+// silu(g) * u in binary32: exp(-g) by the hardware exp2, the quotient by its reciprocal (one
+// unit in the last place; an IEEE division is ten instructions, which an epilogue without
+// another wave to hide it pays in full).  g = -inf gives NaN, as -inf / inf does.
 __device__ __forceinline__ float swiglu_f32(float g, float u) {
     const float e = __builtin_amdgcn_exp2f(-g * 0x1.715476p+0f);
-    return g / (1.0f + e) * u;
+    return g * __builtin_amdgcn_rcpf(1.0f + e) * u;
 }
 
 // Rows of one expert that a workgroup's tile covers.
@@ -90,29 +91,91 @@ struct GroupTile {
     int rows;  // 0: no tile
 };
 
-// Tile `tile` of a launch in tiles of BM rows.  Expert e owns the tiles from
-// e + offsets[e] / BM on: floor(hi / BM) - floor(lo / BM) + 1 of them, always enough for
-// its hi - lo rows, so experts + rows / BM tiles cover every split of the rows and a
-// workgroup finds its own from the offsets alone (one load a lane per 64 experts), without
-// a prefix sum over the experts' tile counts.  The bounds come from device memory and
-// are clamped to the rows that the call was given.
-__device__ __forceinline__ GroupTile group_tile(const int* offsets, int experts, int64_t rows, int bm, int tile) {
+// Tiles of BM rows.  Expert e owns the tile numbers from e + offsets[e] / BM on: floor(hi /
+// BM) - floor(lo / BM) + 1 of them, always enough for its hi - lo rows, so experts + rows /
+// BM numbers cover every split of the rows, and a workgroup finds its own from the offsets
+// alone (one load a lane per 64 experts), without a prefix sum over the experts' tile counts.
+// The bounds come from device memory and are clamped to the rows that the call was given.
+__device__ __forceinline__ int64_t tile_number(const int* offsets, int bm, int e) {
+    return e + (int64_t)offsets[e] / bm;
+}
+
+// The expert that owns a tile number.
+__device__ __forceinline__ int tile_expert(const int* offsets, int experts, int bm, int64_t tile) {
     const int lane = threadIdx.x & 63;
     int n = 0;
     for (int i = 0; i < experts; i += 64) {
         const int e = i + lane;
-        n += __popcll(__ballot(e < experts && e + (int64_t)offsets[e < experts ? e : 0] / bm <= tile));
+        n += __popcll(__ballot(e < experts && tile_number(offsets, bm, e < experts ? e : 0) <= tile));
     }
+    return __builtin_amdgcn_readfirstlane(n > 0 ? n - 1 : 0);
+}
+
+__device__ __forceinline__ GroupTile tile_rows(const int* offsets, int64_t rows, int bm, int expert, int64_t m) {
     GroupTile t;
-    t.expert = n > 0 ? n - 1 : 0;
-    int64_t lo = offsets[t.expert], hi = offsets[t.expert + 1];
-    const int64_t first = t.expert + lo / bm;
+    t.expert = expert;
+    int64_t lo = offsets[expert], hi = offsets[expert + 1];
     lo = lo < 0 ? 0 : (lo > rows ? rows : lo);
     hi = hi < lo ? lo : (hi > rows ? rows : hi);
-    t.row0 = lo + (tile - first) * bm;
-    const int64_t left = t.row0 < lo ? 0 : hi - t.row0;
+    t.row0 = lo + m * bm;
+    const int64_t left = m < 0 ? 0 : hi - t.row0;
     t.rows = (int)(left < 0 ? 0 : (left > bm ? bm : left));
     return t;
+}
+
+// Tile number `tile`.
+__device__ __forceinline__ GroupTile group_tile(const int* offsets, int experts, int64_t rows, int bm, int tile) {
+    const int e = tile_expert(offsets, experts, bm, tile);
+    return tile_rows(offsets, rows, bm, e, tile - tile_number(offsets, bm, e));
+}
+
+// Work item of workgroup bid among the experts' tiles (whole ones and a last, partial one, no
+// empty ones) x column slices: each XCD (bid % 8) gets a contiguous run of equal length, and in
+// an expert the tiles of one slice are neighbours, so an expert's weights and rows pass
+// through one L2, about once.  (Numbers of group_tile would leave gaps, uneven over the
+// XCDs.)  Every wave sums the experts' tile counts for itself.  False: no item.
+__device__ __forceinline__ bool group_item(const int* offsets, int experts, int64_t rows, int bm, int slices, int bid,
+                                           GroupTile& tile, int& slice) {
+    const int lane = threadIdx.x & 63;
+    // Tiles of expert i + lane, and (first) those of the experts below it in its 64.
+    auto tiles = [&](int i, int& own, int& upto) __attribute__((always_inline)) {
+        own = 0;
+        if (i + lane < experts) {
+            int64_t lo = offsets[i + lane], hi = offsets[i + lane + 1];
+            lo = lo < 0 ? 0 : (lo > rows ? rows : lo);
+            hi = hi < lo ? lo : (hi > rows ? rows : hi);
+            own = (int)((hi - lo + bm - 1) / bm);
+        }
+        upto = own;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int o = __shfl_up(upto, d, 64);
+            if (lane >= d) upto += o;
+        }
+    };
+    int own, upto;
+    int64_t total = 0;
+    for (int i = 0; i < experts; i += 64) {
+        tiles(i, own, upto);
+        total += __builtin_amdgcn_readlane(upto, 63);
+    }
+    const int64_t items = total * slices, per = (items + 7) / 8, item = (bid & 7) * per + (bid >> 3);
+    if ((bid >> 3) >= per || item >= items) return false;
+    int64_t below = 0;
+    for (int i = 0; i < experts; i += 64) {
+        if (experts > 64) tiles(i, own, upto);
+        const uint64_t past = __ballot((below + upto) * slices > item);  // the first of them holds the item
+        if (past) {
+            const int l = __builtin_ctzll(past);
+            const int count = __builtin_amdgcn_readlane(own, l);
+            const int rest = (int)(item - (below + __builtin_amdgcn_readlane(upto, l) - count) * slices);
+            slice = rest / count;
+            tile = tile_rows(offsets, rows, bm, i + l, rest % count);
+            return tile.rows > 0;
+        }
+        below += __builtin_amdgcn_readlane(upto, 63);
+    }
+    return false;
 }
 
 }  // namespace h3q

@@ -232,7 +232,7 @@ struct GroupedArgs {
 // Weight streaming for up to 16 rows of an expert at a time (grouped_stream.hip).
 int64_t grouped_stream_grid(const GroupedArgs& a);
 hipError_t launch_grouped_stream(int kind, const GroupedArgs& a, hipStream_t st);
-// Bands of 16 * blocks (2, 4 or 8) rows (grouped_band.hip).
+// Bands of 16 * blocks (4 or 8) rows (grouped_band.hip).
 int64_t grouped_band_grid(const GroupedArgs& a, int blocks);
 hipError_t launch_grouped_band(int kind, const GroupedArgs& a, int blocks, hipStream_t st);
 // 256 x 256 tiles (grouped_tile.hip); no wide products.

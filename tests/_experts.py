@@ -84,14 +84,14 @@ def swiglu(y: np.ndarray, bound: np.ndarray):
 
     silu'(g) = s (1 + g (1 - s)) lies in [-0.1, 1.1]; its own evaluation: exp(-g) by
     exp2 of a rounded product (relative error |g| (U32 of the product + U32 of the
-    constant) + 2 U32 of exp2), reaching silu with at most that factor, then a sum, a
-    division and a product (3 U32): (2 |g| + 5) U32, doubled for second-order terms.
-    The up factor: its own relative bound."""
+    constant) + 2 U32 of exp2), reaching silu with at most that factor, then a sum (U32), a
+    reciprocal to one unit in the last place (2 U32) and two products (2 U32): (2 |g| + 7)
+    U32, doubled for second-order terms.  The up factor: its own relative bound."""
     half = y.shape[1] // 2
     g, u, bg, bu = y[:, :half], y[:, half:], bound[:, :half], bound[:, half:]
     silu = g / (1.0 + np.exp(-g))
     h = silu * u
-    b = 1.1 * bg * np.abs(u) + (np.abs(silu) + 1.1 * bg) * bu + 2 * (2 * np.abs(g) + 5) * U32 * np.abs(h)
+    b = 1.1 * bg * np.abs(u) + (np.abs(silu) + 1.1 * bg) * bu + 2 * (2 * np.abs(g) + 7) * U32 * np.abs(h)
     return h, b
 
 
