@@ -30,33 +30,44 @@ __device__ __forceinline__ uint32_t row_ror(uint32_t v) {
     return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x120 + N, 0xF, 0xF, true);
 }
 
-// Reductions over the LPT lanes (16 or 64) of a token; every lane gets the result.
+// One step of a wave's reduction over its rows of 16: lane 15 (31) of the row before.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t row_bcast(uint32_t old, uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp((int)old, (int)v, CTRL, ROWS, 0xF, false);
+}
+
+// Reductions over the LPT lanes (16 or 64) of a token; every lane gets the result.  neutral:
+// what leaves the other operand of f as it is.
 template <int LPT, class F>
-__device__ __forceinline__ uint32_t group_reduce(uint32_t v, F f) {
+__device__ __forceinline__ uint32_t group_reduce(uint32_t v, uint32_t neutral, F f) {
     v = f(v, row_ror<8>(v));
     v = f(v, row_ror<4>(v));
     v = f(v, row_ror<2>(v));
     v = f(v, row_ror<1>(v));
     if constexpr (LPT == 64) {
-        v = f(v, (uint32_t)__shfl_xor((int)v, 16, 64));
-        v = f(v, (uint32_t)__shfl_xor((int)v, 32, 64));
+        v = f(v, row_bcast<0x142, 0xA>(neutral, v));
+        v = f(v, row_bcast<0x143, 0xC>(neutral, v));
+        v = (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
     }
     return v;
 }
 template <int LPT>
 __device__ __forceinline__ uint32_t group_max(uint32_t v) {
-    return group_reduce<LPT>(v, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
+    return group_reduce<LPT>(v, 0u, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
 }
 template <int LPT>
 __device__ __forceinline__ uint32_t group_min(uint32_t v) {
-    return group_reduce<LPT>(v, [](uint32_t a, uint32_t b) { return a < b ? a : b; });
+    return group_reduce<LPT>(v, 0xFFFFFFFFu, [](uint32_t a, uint32_t b) { return a < b ? a : b; });
 }
 template <int LPT>
 __device__ __forceinline__ float group_sum(float v) {
-    return __uint_as_float(group_reduce<LPT>(__float_as_uint(v), [](uint32_t a, uint32_t b) {
+    return __uint_as_float(group_reduce<LPT>(__float_as_uint(v), 0u, [](uint32_t a, uint32_t b) {
         return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
     }));
 }
+
+// exp(x) for x <= 0 or a logit: the hardware exp2 of x / ln 2, within (|x| + 2) 2^-23 of exp(x).
+__device__ __forceinline__ float fast_exp(float x) { return __builtin_amdgcn_exp2f(x * 0x1.715476p+0f); }
 
 template <int DT>
 __device__ __forceinline__ float load_logit(const void* p, int64_t i) {
@@ -77,9 +88,10 @@ __device__ __forceinline__ float load_logit(const void* p, int64_t i) {
 // sigmoid 1 / (1 + exp(-l)), divided by the taken ones' sum when renormalized.
 // A slot without an expert (fewer than k logits above -inf) gets -1 and weight 0.
 //
-// What bounds it: the logits are read once, in registers; the k rounds cost about
-// 5 NV + 20 instructions each.  Four tokens to a wave rather than one cut the cross-lane
-// steps per token by four and stay within a row of 16 lanes (register permutes).
+// What bounds it: instructions.  The logits are read once, into registers; the k rounds cost
+// about 5 NV + 20 instructions each.  Four tokens to a wave rather than one cut the
+// cross-lane steps per token by four and stay within a row of 16 lanes (register permutes):
+// 32768 tokens of 128 experts, top 4, take 9.9 us (16.8 MB of logits: 3 us at the HBM's rate).
 template <int DT, int LPT, int NV>
 __global__ __launch_bounds__(256) void route_topk_kernel(RouteArgs p) {
     constexpr int TPB = 256 / LPT;
@@ -102,7 +114,7 @@ __global__ __launch_bounds__(256) void route_topk_kernel(RouteArgs p) {
     if (p.scoring == kScoreSoftmax && !p.renormalize) {
 #pragma unroll
         for (int i = 0; i < NV; ++i)
-            if (key[i] != 0u) whole += key[i] == top ? 1.0f : expf(key_logit(key[i]) - best);
+            if (key[i] != 0u) whole += key[i] == top ? 1.0f : fast_exp(key_logit(key[i]) - best);
         whole = group_sum<LPT>(whole);
     }
     int mine = -1;
@@ -120,7 +132,7 @@ __global__ __launch_bounds__(256) void route_topk_kernel(RouteArgs p) {
         if (m != 0u && j == lane) {
             mine = (int)e;
             const float l = key_logit(m);
-            weight = p.scoring == kScoreSigmoid ? 1.0f / (1.0f + expf(-l)) : m == top ? 1.0f : expf(l - best);
+            weight = p.scoring == kScoreSigmoid ? 1.0f / (1.0f + fast_exp(-l)) : m == top ? 1.0f : fast_exp(l - best);
         }
 #pragma unroll
         for (int i = 0; i < NV; ++i)
@@ -138,13 +150,16 @@ namespace {
 
 template <int DT>
 hipError_t launch_route_dt(const RouteArgs& a, hipStream_t st) {
-    const bool wide = a.experts > 256 || a.top_k > 16;
+    // A wave per token also for few tokens: a quarter of the work per wave while there are SIMDs
+    // for all of them (4093 tokens of 256 experts: 7.2 -> 6.5 us; 32768 of 128: 9.9 -> 16.4).
+    const bool wide = a.experts > 256 || a.top_k > 16 || a.tokens <= 4096;
     const int lpt = wide ? 64 : 16;
     const dim3 grid((unsigned)((a.tokens + 256 / lpt - 1) / (256 / lpt)));
     const int nv = (int)((a.experts + lpt - 1) / lpt);
 #define H3Q_ROUTE(LPT, NV) hipLaunchKernelGGL((route_topk_kernel<DT, LPT, NV>), grid, dim3(256), 0, st, a)
     if (wide) {
-        if (nv <= 4) H3Q_ROUTE(64, 4);
+        if (nv <= 1) H3Q_ROUTE(64, 1);
+        else if (nv <= 4) H3Q_ROUTE(64, 4);
         else H3Q_ROUTE(64, 16);
     } else {
         if (nv <= 1) H3Q_ROUTE(16, 1);
@@ -175,16 +190,17 @@ hipError_t launch_route_topk(const RouteArgs& a, int dtype, hipStream_t st) {
 //           and of the lower experts added, the span is walked again, and every pair's row
 //           is the table's entry plus its rank among its peers of the trip.
 //
-// Up to kPlanChunk pairs one workgroup does both; more take a counting launch, whose blocks
-// leave their counts in the workspace, and a placing one, whose blocks each sum all the
-// counts they need (blocks * experts integers, read once, by all threads).  Deterministic.
+// Up to kPlanWholePairs pairs one workgroup does both; more take a counting launch, whose
+// blocks leave their counts in the workspace, and a placing one, whose blocks each sum all
+// the counts they need (blocks * experts integers, by all threads).  Deterministic.
 // Pairs whose expert is not in [first, first + experts) get slot -1, and the rows past the
 // last placed one order -1.
 //
-// What bounds it: dependent round trips; the work is 2 * log2(experts) ballots a trip.  One
-// workgroup per expert over all pairs took 46 us for 131072 pairs of 128 experts.
+// What bounds it: dependent round trips and two launches; the work is log2(experts) ballots a
+// trip.  131072 pairs of 128 experts: 3.6 + 7.5 us (one workgroup per expert over all pairs,
+// in one launch: 46 us); 8 pairs: 3.6 us.
 constexpr int kPlanWaves = 16;
-constexpr int kPlanChunk = 2048;
+constexpr int kPlanWholePairs = 2048;
 
 namespace {
 
@@ -335,7 +351,7 @@ __global__ __launch_bounds__(kPlanWaves * 64) void plan_experts_kernel(PlanArgs 
     plan_block<PHASE>(p, chunk, bits, blockIdx.x, gridDim.x, table);
 }
 
-// The plan of up to kPlanChunk pairs (workgroup 0) and the codes of the tokens (a workgroup
+// The plan of up to kPlanWholePairs pairs (workgroup 0) and the codes of the tokens (a workgroup
 // each of the others), in one launch: neither needs the other, and both are shorter than the
 // launch that this saves.
 template <int FMT, int ROUND>
@@ -343,7 +359,7 @@ __global__ __launch_bounds__(kPlanWaves * 64) void plan_quant_kernel(PlanArgs p,
                                                                      int cols, uint8_t* codes, float* scales) {
     extern __shared__ int table[];
     if (blockIdx.x == 0) {
-        plan_block<kPlanWhole>(p, kPlanChunk, bits, 0, 1, table);
+        plan_block<kPlanWhole>(p, kPlanWholePairs, bits, 0, 1, table);
         return;
     }
     __shared__ float wave_amax[kPlanWaves];
@@ -382,10 +398,11 @@ int expert_bits(int experts) {
     return bits;
 }
 
-// Pairs per block: at most 256 blocks, so a placing block's sum over them stays short.
+// Pairs per block: one block for few, else at least 1024 and at most 256 blocks, so that a
+// placing block's sum over them stays short.
 int64_t plan_chunk(int64_t pairs) {
-    const int64_t per = (pairs + 255) / 256;
-    return per <= kPlanChunk ? kPlanChunk : (per + 1023) / 1024 * 1024;
+    if (pairs <= kPlanWholePairs) return kPlanWholePairs;
+    return (pairs + 256 * 1024 - 1) / (256 * 1024) * 1024;
 }
 
 }  // namespace
@@ -410,7 +427,7 @@ hipError_t launch_plan_experts(const PlanArgs& a, hipStream_t st) {
     return hipGetLastError();
 }
 
-bool plan_quant_supported(const PlanArgs& a, int64_t tokens) { return a.pairs <= kPlanChunk && tokens <= 512; }
+bool plan_quant_supported(const PlanArgs& a, int64_t tokens) { return a.pairs <= kPlanWholePairs && tokens <= 512; }
 
 hipError_t launch_plan_quant(const PlanArgs& a, int fmt, const uint16_t* x, int64_t ldx, int64_t tokens, int64_t cols,
                              uint8_t* codes, float* scales, hipStream_t st) {
