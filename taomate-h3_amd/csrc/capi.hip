@@ -532,6 +532,9 @@ __attribute__((visibility("default"))) int h3q_lora_down_ws(const void* x, int64
     return check_launch(h3q::launch_lora_down(g, workspace, workspace_bytes, (hipStream_t)stream), who);
 }
 
+// 128 * 127 * k stays below 2^31.
+constexpr int64_t kInt8MaxK = 132096;
+
 // Shared checks of the expert entry points.
 static int check_experts(const char* who, int64_t tokens, int64_t top_k, int64_t experts) {
     if (tokens < 0) return fail(H3Q_ERR_INVALID, "%s: negative token count %lld", who, (long long)tokens);
@@ -547,6 +550,9 @@ static int check_experts(const char* who, int64_t tokens, int64_t top_k, int64_t
 static int check_code_layout(const char* who, int format, int layout, int64_t k) {
     if (format != H3Q_FMT_E4M3FN && format != H3Q_FMT_INT8)
         return fail(H3Q_ERR_INVALID, "%s: unknown format %d", who, format);
+    if (format == H3Q_FMT_INT8 && k > kInt8MaxK)
+        return fail(H3Q_ERR_UNSUPPORTED, "%s: int8 sums over k=%lld may pass 32 bits (k up to %lld)", who, (long long)k,
+                    (long long)kInt8MaxK);
     if (layout != H3Q_LAYOUT_ROWS && layout != H3Q_LAYOUT_TILED)
         return fail(H3Q_ERR_INVALID, "%s: unknown layout %d", who, layout);
     if (layout == H3Q_LAYOUT_TILED && k % 128)
@@ -630,7 +636,7 @@ __attribute__((visibility("default"))) int h3q_grouped_mm(int format, const void
                     (long long)a_rows, (long long)n, (long long)k);
     rc = check_experts(who, rows, 1, experts);
     if (rc != H3Q_OK) return rc;
-    if (order && top_k < 1) return fail(H3Q_ERR_INVALID, "%s: top_k=%lld", who, (long long)top_k);
+    if (order && (top_k < 1 || top_k > 0x7FFFFFFF)) return fail(H3Q_ERR_INVALID, "%s: top_k=%lld", who, (long long)top_k);
     if (k % 16 || n % (swiglu ? 32 : 16))
         return fail(H3Q_ERR_INVALID, "%s: k=%lld must be a multiple of 16 and n=%lld of %d", who, (long long)k,
                     (long long)n, swiglu ? 32 : 16);

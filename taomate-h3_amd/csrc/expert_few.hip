@@ -503,7 +503,9 @@ void launch_down(const ExpertFfnArgs& a, const FewBuffers& w, hipStream_t st) {
 
 }  // namespace
 
-bool expert_few_supported(const ExpertFfnArgs& a) { return a.tokens * a.top_k <= kFewPairs; }
+bool expert_few_supported(const ExpertFfnArgs& a) {
+    return a.tokens * a.top_k <= kFewPairs && a.f / 16 * few_tiles(a) < (int64_t(1) << 24);  // grid * 256 < 2^32
+}
 
 hipError_t launch_expert_few(const ExpertFfnArgs& a, const FewBuffers& w, hipStream_t st) {
     const int fmt = a.kind == kOpInt8 ? kFmtInt8 : kFmtE4M3, rounding = a.kind == kOpInt8 ? kRoundRcpMul : kRoundDiv;

@@ -101,6 +101,8 @@ def test_native_refusals_without_gpu():
     refused(1, b"8 rows, 9", "h3q_grouped_mm", *grouped(rows=9))
     refused(2, b"2 GiB", "h3q_grouped_mm", *grouped(n=1 << 20, k=2048, lda=2048, ldo=1 << 20))
     refused(2, b"gathered", "h3q_grouped_mm", *grouped(order=p, a_rows=1 << 24))
+    refused(2, b"32 bits", "h3q_grouped_mm", *grouped(k=1 << 18, lda=1 << 18))
+    refused(1, b"top_k", "h3q_grouped_mm", *grouped(order=p, top_k=1 << 32))
     refused(1, b"null", "h3q_grouped_mm", *grouped(b=None))
     refused(1, b"aligned", "h3q_grouped_mm", *grouped(out=ctypes.c_void_p(264)))
     assert lib.h3q_grouped_mm(*grouped(rows=0)) == 0

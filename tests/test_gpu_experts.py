@@ -288,7 +288,8 @@ def _routed(t, k, total, seed):
 @pytest.mark.parametrize("t,k,total,e,first,d,f", [
     (1, 1, 1, 1, 0, 128, 128), (1, 8, 16, 16, 0, 512, 256), (3, 2, 8, 8, 0, 640, 384), (7, 4, 12, 4, 4, 256, 128),
     (5, 2, 6, 6, 0, 144, 80), (21, 3, 8, 8, 0, 272, 208), (20, 8, 40, 40, 0, 256, 256), (150, 2, 4, 4, 0, 384, 128),
-    (400, 4, 8, 4, 2, 256, 256), (64, 1, 2, 2, 0, 128, 1024)])
+    (400, 4, 8, 4, 2, 256, 256), (64, 1, 2, 2, 0, 128, 1024), (8, 8, 64, 64, 0, 256, 512), (1, 64, 64, 64, 0, 384, 256),
+    (2, 32, 300, 300, 0, 256, 128), (16, 4, 40, 20, 20, 16, 16)])
 def test_expert_ffn(ops, experts_module, device, oracle, fmt, t, k, total, e, first, d, f):
     layer, packed = _layer(ops, experts_module, device, oracle, fmt, e, d, f, first)
     x = activations(t, d, seed=t + d, outlier_channels=2)
@@ -449,6 +450,53 @@ def test_two_calls_on_two_streams(ops, experts_module, device, oracle):
                 got.append(layer(x, ids, weights))
         torch.cuda.synchronize()
         assert all(torch.equal(g.view(torch.int16), w.view(torch.int16)) for g, w in zip(got, want))
+
+
+def test_native_wrappers_equal_the_python_bodies(ops, experts_module, device, oracle, monkeypatch):
+    """Every call once through the native wrapper and once with it declining: the same bits."""
+    layer, _ = _layer(ops, experts_module, device, oracle, "e4m3", 6, 256, 128)
+    x = activations(40, 256, seed=4).to(device)
+    logits = torch.randn(40, 6, device=device)
+    native, taken = ops._native_call, []
+
+    def calls():
+        ids, w = ops.route_experts(logits, 3, scoring="sigmoid")
+        plan = ops.plan_experts(ids, 6)
+        q, s = ops.quant_rows(x, ops.FMT_E4M3FN)
+        used = int(plan.offsets[-1])
+        h = ops.grouped_scaled_mm(q, layer.w13, s, layer.w13_scale, plan.offsets, order=plan.order, top_k=3, swiglu=True,
+                                  b_tiled=True)[:used]
+        y = torch.randn(120, 64, device=device, generator=torch.Generator(device=device).manual_seed(1))
+        return (ids, w, *plan, h, ops.combine_experts(y, plan.slots, w), layer(x, ids, w), layer(x[:2], ids[:2], w[:2]))
+
+    def hook(enabled):
+        def call(name, first, *args):
+            out = native(name, first, *args) if enabled else None
+            taken.append(out is not None)
+            return out
+        return call
+
+    results = []
+    for enabled in (True, False):
+        taken.clear()
+        monkeypatch.setattr(ops, "_native_call", hook(enabled))
+        results.append(calls())
+        assert all(taken) == enabled and any(taken) == enabled
+    for a, b in zip(*results):
+        assert torch.equal(a.contiguous().view(torch.uint8), b.contiguous().view(torch.uint8))
+
+
+def test_in_place_layer(ops, experts_module, device, oracle):
+    """The output may be the input: x is read before any of it is written."""
+    layer, _ = _layer(ops, experts_module, device, oracle, "int8", 4, 256, 128)
+    for t in (3, 50):
+        x = activations(t, 256, seed=t).to(device)
+        ids, weights = _routed(t, 2, 4, 1)
+        ids, weights = torch.from_numpy(ids).to(device), torch.from_numpy(weights).to(device)
+        want = layer(x, ids, weights)
+        ops.expert_ffn(x, ids, weights, layer.w13, layer.w13_scale, layer.w2, layer.w2_scale, w13_tiled=True, w2_tiled=True,
+                       out=x)
+        assert torch.equal(x.view(torch.int16), want.view(torch.int16))
 
 
 # --------------------------------------------------------------- refusals
