@@ -11,6 +11,8 @@ of ``libtaomate_h3_amd.so`` (include/taomate_h3_amd.h):
                               per-token x per-channel FP8 W8A8
 * ``inference.lora``          H3/inference/lora_checkpoint.py:172-205,261-303
                               (LoRA side branch, fused into the GEMM epilogue)
+* ``inference.experts``       routed-expert FFN on the same formats (no counterpart
+                              in the reference)
 * ``distributed.linear``      H3/distributed/linear.py:15-191 and
                               FL/distributed/linear.py:50-128 (dispatch + linears)
 
