@@ -33,7 +33,8 @@ def route(logits: torch.Tensor, k: int, scoring: str, renorm: bool, scale: float
             continue
         v = np.array(values)
         if scoring == "sigmoid":
-            w = 1.0 / (1.0 + np.exp(-v))
+            with np.errstate(over="ignore"):
+                w = 1.0 / (1.0 + np.exp(-v))
             whole = w.sum() if renorm else 1.0
         else:
             e_of = lambda a: np.where(a == v[0], 1.0, np.exp(np.where(a == v[0], 0.0, a) - np.where(a == v[0], 0.0, v[0])))  # noqa: E731
