@@ -52,6 +52,7 @@ __global__ __launch_bounds__(kBandWaves * 64, MT == 8 || OUT == kOutWide ? 2 : 3
     // Loads a wave has issued after the copies of stage s + 1 when it waits for them in step s:
     // the weights of that step and all of the SA - 3 steps since.
     constexpr int WAIT = 4 + (SA - 3) * (CA + 4);
+    constexpr int WAIT_TAIL = (SA - 3) * CA;  // the last steps ask for no more weights
     static_assert((MT == 4 || MT == 8) && D * 4 + SA * CA < 63, "vmcnt range");
     __shared__ __attribute__((aligned(1024))) uint8_t lds_ring[SA * STAGE];
     __shared__ __attribute__((aligned(16))) float lds_scales[MT == 8 ? 4 : BM + 128];
@@ -173,7 +174,8 @@ __global__ __launch_bounds__(kBandWaves * 64, MT == 8 || OUT == kOutWide ? 2 : 3
     asm volatile("s_barrier" ::: "memory");
 
     int slot = 0;
-    auto step = [&](int s, v8i (&ws)[2]) __attribute__((always_inline)) {
+    auto step = [&](int s, v8i (&ws)[2], auto tail) __attribute__((always_inline)) {
+        constexpr bool TAIL = decltype(tail)::value;
         const int next = slot + 1 == SA ? 0 : slot + 1, last = slot == 0 ? SA - 1 : slot - 1;
         const typename Mfma::frag_t w0 = Mfma::frag(ws[0]), w1 = Mfma::frag(ws[1]);
 #pragma unroll
@@ -186,21 +188,21 @@ __global__ __launch_bounds__(kBandWaves * 64, MT == 8 || OUT == kOutWide ? 2 : 3
         // This wave has read its fragments of stage s and stage s + 1 has landed; after the
         // barrier that holds for every wave, and the slot of stage s - 1 takes stage s - 1 + SA
         // (every wave read that one before the previous barrier).
-        wait_vmcnt<WAIT>();
+        wait_vmcnt<TAIL ? WAIT_TAIL : WAIT>();
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
         copy_a(s - 1 + SA, last);
-        load_w(s + D, ws);
+        if constexpr (!TAIL) load_w(s + D, ws);
         __builtin_amdgcn_sched_barrier(0);
         slot = next;
     };
     int s = 0;
     for (; s + D <= steps; s += D) {
 #pragma unroll
-        for (int d = 0; d < D; ++d) step(s + d, w[d]);
+        for (int d = 0; d < D; ++d) step(s + d, w[d], std::false_type());
     }
 #pragma unroll
     for (int d = 0; d < D - 1; ++d)
-        if (s + d < steps) step(s + d, w[d]);
+        if (s + d < steps) step(s + d, w[d], std::true_type());
     wait_vmcnt<0>();
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 
