@@ -281,7 +281,7 @@ std::optional<Pair> route_experts(const Tensor& logits, int64_t top_k, int64_t s
 
 std::optional<Three> plan_experts(const Tensor& experts, int64_t n_experts, int64_t first, int64_t stream) {
     if (!experts.is_cuda() || !dense(experts, experts, at::kInt) || experts.dim() != 2 || experts.numel() == 0 ||
-        n_experts < 1)
+        n_experts < 1 || n_experts > 1024)
         return std::nullopt;
     const int64_t tokens = experts.size(0), top_k = experts.size(1);
     const c10::DeviceGuard guard(experts.device());

@@ -693,7 +693,7 @@ def plan_experts(experts: torch.Tensor, n_experts: int, *, first_expert: int = 0
         raise ValueError(f"plan_experts: expected [tokens, top_k <= {MAX_TOP_K}] ids, got {tuple(experts.shape)}")
     tokens, top_k = experts.shape
     order = torch.empty(tokens * top_k, device=experts.device, dtype=torch.int32)
-    offsets = torch.empty(max(int(n_experts), 0) + 1, device=experts.device, dtype=torch.int32)
+    offsets = torch.empty(min(max(int(n_experts), 0), MAX_EXPERTS) + 1, device=experts.device, dtype=torch.int32)
     slots = torch.empty((tokens, top_k), device=experts.device, dtype=torch.int32)
     size = int(_lib.lib().h3q_plan_experts_workspace_bytes(tokens, top_k, int(n_experts)))
     ws = torch.empty(size, device=experts.device, dtype=torch.uint8) if size else None

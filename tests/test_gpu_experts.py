@@ -526,8 +526,9 @@ def test_refusals(ops, experts_module, device, oracle):
         ops.route_experts(torch.zeros(4, 8, device=device), 2, scoring="tanh")
     with pytest.raises(TypeError):
         ops.route_experts(torch.zeros(4, 8, device=device, dtype=torch.float64), 2)
-    with pytest.raises(RuntimeError, match="experts"):
-        ops.plan_experts(ids, 0)
+    for count in (0, -3, 1025, 2 ** 40):
+        with pytest.raises(RuntimeError, match="experts"):
+            ops.plan_experts(ids, count)
     q, s = ops.quant_rows(x, ops.FMT_INT8)
     offsets = torch.zeros(5, dtype=torch.int32, device=device)
     with pytest.raises(ValueError):
