@@ -233,6 +233,27 @@ def test_grouped_strided_operands(ops, device):
     assert (buffer[:, :32] == 0).all() and (buffer[:, 96:] == 0).all()
 
 
+@pytest.mark.parametrize("experts,rows", [(1024, 10000), (64, 10000), (2, 10000)])
+def test_grouped_offsets_past_32_bits(ops, device, experts, rows):
+    """Rows of codes and of outputs that lie past 4 GiB of their tensors, through every kernel (by the
+    mean rows of an expert: 9, 156 and 5000): the last rows equal a call on those rows alone."""
+    k, n, a_stride, o_stride = 384, 64, 1 << 19, 1 << 18  # 5 GB of codes, 5 GB of outputs
+    gen = torch.Generator(device=device).manual_seed(1)
+    a = torch.empty(rows, a_stride, device=device, dtype=torch.int8)[:, :k]
+    a.copy_(torch.randint(-127, 128, (rows, k), device=device, generator=gen))
+    s = torch.rand(rows, device=device, generator=gen)
+    w = torch.randint(-127, 128, (experts, n, k), device=device, generator=gen).to(torch.int8)
+    sw = torch.rand(experts, n, device=device, generator=gen)
+    out = torch.empty(rows, o_stride, device=device, dtype=torch.bfloat16)[:, :n]
+    offsets = torch.full((experts + 1,), rows, dtype=torch.int32, device=device)
+    offsets[0], offsets[1] = 0, rows - 300
+    ops.grouped_scaled_mm(a, w, s, sw, offsets, out=out)
+    tail = a[-300:].contiguous()
+    want = ops.grouped_scaled_mm(tail, w[1:2].contiguous(), s[-300:].contiguous(), sw[1:2].contiguous(),
+                                 torch.tensor([0, 300], dtype=torch.int32, device=device))
+    assert torch.equal(out[-300:].contiguous().view(torch.int16), want.view(torch.int16))
+
+
 def test_grouped_bounds_beyond_the_rows(ops, device):
     """Offsets that claim more rows than the call has, and order entries past the tokens,
     touch nothing beside the call's own rows."""
