@@ -440,7 +440,8 @@ __global__ __launch_bounds__(512) void few_down_kernel(ExpertFfnArgs p, FewBuffe
             const int tile = place / 16, r = place & 15, last = lds_w1[tile];
             acc_t sum = acc_t{};  // one element of it is used
             for (int v = lds_w0[tile]; v <= last; ++v)
-                sum[0] += ((const H3Q_LDS decltype(sum[0] + 0)*)seg)[((tile + v) * 64 + r + 16 * (col >> 2)) * 4 + (col & 3)];
+                if (total * v / WAVES < total * (v + 1) / WAVES)  // with few steps some waves have none
+                    sum[0] += ((const H3Q_LDS decltype(sum[0] + 0)*)seg)[((tile + v) * 64 + r + 16 * (col >> 2)) * 4 + (col & 3)];
             y = __fmul_rn(lds_scale[pair], __fmul_rn(s2[q], (float)sum[0]));
         }
         lds_y[item] = y;

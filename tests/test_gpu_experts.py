@@ -324,6 +324,26 @@ def test_expert_ffn(ops, experts_module, device, oracle, fmt, t, k, total, e, fi
 
 
 @pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("f", [128, 256, 384, 512, 640, 896, 1024, 1152])
+@pytest.mark.parametrize("hit", [0, 1, 2, 3])
+def test_few_pairs_of_few_experts(ops, experts_module, device, oracle, fmt, f, hit):
+    """Fewer k-steps than waves (some have none): 0 to 3 experts of a rank hit, after a call that
+    leaves other sums in the same LDS."""
+    layer, packed = _layer(ops, experts_module, device, oracle, fmt, 16, 128, f)
+    gen = torch.Generator().manual_seed(f)
+    full = torch.stack([torch.randperm(16, generator=gen)[:8] for _ in range(8)]).to(torch.int32).to(device)
+    layer(activations(8, 128, seed=3).to(device) * 1000.0, full, torch.ones(8, 8, device=device))
+    ids = np.full((2, 6), -1, np.int32)
+    for i in range(hit):
+        ids[i % 2, 2 * i] = 5 * i
+    weights = np.full((2, 6), 0.5, np.float32)
+    x = activations(2, 128, seed=f)
+    got = layer(x.to(device), torch.from_numpy(ids).to(device), torch.from_numpy(weights).to(device))
+    want, bound = R.ffn(oracle, fmt, x, ids, weights, *packed)
+    assert (np.abs(got.double().cpu().numpy() - want) <= bound).all()
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
 @pytest.mark.parametrize("t,k,e,d,f", [(1, 4, 8, 512, 384), (6, 8, 16, 256, 640), (40, 2, 8, 384, 256), (300, 4, 8, 256, 384)])
 def test_expert_ffn_is_the_chain(ops, experts_module, device, oracle, fmt, t, k, e, d, f):
     """The layer against the operators one by one: the same bits in int8 (its sums are exact); in
