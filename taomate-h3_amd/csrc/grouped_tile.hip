@@ -37,6 +37,7 @@ namespace {
 constexpr int kStages = 4;
 constexpr int kStageBytes = (256 + 256) * 64;  // A and B, 64 bytes of k each
 constexpr int kABytes = 256 * 64;
+constexpr int kVecBytes = 3 * 256 * 4;  // a tile's row scales, column scales and pairs, 4 bytes each
 constexpr int64_t kStreamOutBytes = int64_t(64) << 20;  // outputs stored past the caches (see gemm_w4.hip)
 
 // Wave copies global -> LDS (see copy16 in h3q_common.hpp), with a scalar offset.  A scalar
@@ -112,7 +113,7 @@ __global__ __launch_bounds__(256, 1) void grouped_tile_kernel(GroupedArgs p, int
     constexpr bool SWIGLU = OUT == kOutSwiglu;
     __shared__ __attribute__((aligned(1024))) uint8_t lds_ring[kStages * kStageBytes];
     // Per tile parity: row scales [256] f32 | column scales [256] f32 | order [256] i32.
-    __shared__ __attribute__((aligned(1024))) uint8_t lds_vec[2 * 3 * 1024];
+    __shared__ __attribute__((aligned(1024))) uint8_t lds_vec[2 * kVecBytes];
     __shared__ int lds_first[kMaxExperts];  // row blocks of the experts below, and each one's rows
     __shared__ int lds_lo[kMaxExperts], lds_hi[kMaxExperts];
     H3Q_LDS uint8_t* const ring = (H3Q_LDS uint8_t*)lds_ring;
@@ -206,13 +207,13 @@ __global__ __launch_bounds__(256, 1) void grouped_tile_kernel(GroupedArgs p, int
     auto issue_order = [&](const Tile& t, int par) __attribute__((always_inline)) {
         if (gather && wave == 3)
             copy16_soff(CopySrc(p.order + t.row0, (uint32_t)t.rows * 4u),
-                        (uint32_t)(uintptr_t)(vec + par * 3072 + 2048), 16u * lane, 0);
+                        (uint32_t)(uintptr_t)(vec + par * kVecBytes + 2048), 16u * lane, 0);
     };
     // Row of a behind row i of the copy tile, or -1.
     auto source_row = [&](int i) __attribute__((always_inline)) -> int64_t {
         if (i >= cp.rows) return -1;
         if (!gather) return cp.row0 + i;
-        const int pair = ((const H3Q_LDS int*)(vec + (cj & 1) * 3072 + 2048))[i];
+        const int pair = ((const H3Q_LDS int*)(vec + (cj & 1) * kVecBytes + 2048))[i];
         const int r = pair / p.top_k;
         return pair >= 0 && r < p.a_rows ? r : -1;
     };
@@ -247,7 +248,7 @@ __global__ __launch_bounds__(256, 1) void grouped_tile_kernel(GroupedArgs p, int
         if (!live) return;
         // Epilogue vectors of the tile: its row scales (a row per lane of the four waves) and
         // column scales, and the next tile's order.
-        H3Q_LDS uint8_t* const v = vec + (cj & 1) * 3072;
+        H3Q_LDS uint8_t* const v = vec + (cj & 1) * kVecBytes;
         const int64_t r = source_row(threadIdx.x);
         copy4(gather ? CopySrc(p.a_scale, (uint32_t)(p.a_rows * 4)) : CopySrc(p.a_scale + cp.row0, (uint32_t)cp.rows * 4u),
               (uint32_t)(uintptr_t)(v + wave * 256), r >= 0 ? (uint32_t)((gather ? r : r - cp.row0) * 4) : kOob);
@@ -364,7 +365,7 @@ __global__ __launch_bounds__(256, 1) void grouped_tile_kernel(GroupedArgs p, int
         const int wm0 = (wave >> 1) * 32 * MI;
         const int ln = opaque_lane();
         const int gg = ln >> 5, cc = ln & 31;
-        const H3Q_LDS uint8_t* e = vec + par * 3072;
+        const H3Q_LDS uint8_t* e = vec + par * kVecBytes;
         H3Q_LDS uint8_t* const scratch = ring + st * kStageBytes + wave * 8192;
         constexpr int EL = OUT == kOutF32 ? 4 : 2;
         const __amdgpu_buffer_rsrc_t ro =
