@@ -55,12 +55,14 @@ __global__ __launch_bounds__(kBandWaves * 64, MT == 8 || OUT == kOutWide ? 2 : 3
     constexpr int WAIT_TAIL = (SA - 3) * CA;  // the last steps ask for no more weights
     static_assert((MT == 4 || MT == 8) && D * 4 + SA * CA < 63, "vmcnt range");
     __shared__ __attribute__((aligned(1024))) uint8_t lds_ring[SA * STAGE];
-    __shared__ __attribute__((aligned(16))) float lds_scales[MT == 8 ? 4 : BM + 128];
+    __shared__ __attribute__((aligned(16))) float lds_scales[MT == 8 ? 4 : BM + 128 + BM / 32];
     H3Q_LDS uint8_t* const ring = (H3Q_LDS uint8_t*)lds_ring;
-    // Row scales [BM], then the column scales of the waves' blocks; 128-row bands have no LDS
+    // Row scales [BM], the column scales of the waves' blocks, a bit for each row of the band that
+    // has a row of a (the others keep what out held); 128-row bands have no LDS
     // beside the ring (two workgroups share a CU's) and take its end, past the output tile.
     H3Q_LDS float* const lds_sa = MT == 8 ? (H3Q_LDS float*)(ring + BM * 512) : (H3Q_LDS float*)lds_scales;
     H3Q_LDS float* const lds_sw = lds_sa + BM;
+    H3Q_LDS uint32_t* const lds_live = (H3Q_LDS uint32_t*)(lds_sw + 128);
 
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -151,9 +153,11 @@ __global__ __launch_bounds__(kBandWaves * 64, MT == 8 || OUT == kOutWide ? 2 : 3
 
     // Scales of the epilogue, one row's and one weight row's a thread until then.
     float my_sa = 0.0f, my_sw = 0.0f;
+    uint64_t live;  // rows 64 wave .. + 63
     {
         const int64_t r = threadIdx.x < BM ? source_row(threadIdx.x) : -1;
         if (r >= 0) my_sa = p.a_scale[r];
+        live = __ballot(r >= 0);
         const int row = block_row(lane >> 4 & 1);
         if (row < p.n) my_sw = p.b_scale[(int64_t)expert * p.n + row + r16];
     }
@@ -208,9 +212,10 @@ __global__ __launch_bounds__(kBandWaves * 64, MT == 8 || OUT == kOutWide ? 2 : 3
 
     // The tile in LDS (16-byte chunk c of row r at c ^ (r % 8)), then whole row pieces.
     constexpr int EL = OUT == kOutF32 ? 4 : 2, COLS = SWIGLU ? 64 : 128, PITCH = COLS * EL, CH = PITCH / 16;
-    static_assert(BM * PITCH + (MT == 8 ? 4 * (BM + 128) : 0) <= SA * STAGE, "output tile");
+    static_assert(BM * PITCH + (MT == 8 ? 4 * (BM + 128 + BM / 32) : 0) <= SA * STAGE, "output tile");
     if (threadIdx.x < BM) lds_sa[threadIdx.x] = my_sa;
     if (lane < 32) lds_sw[32 * wave + lane] = my_sw;
+    if (lane < 2 && wave < BM / 64) lds_live[2 * wave + lane] = (uint32_t)(live >> (32 * lane));
     __syncthreads();
     v4f sw[2];
 #pragma unroll
@@ -249,7 +254,7 @@ __global__ __launch_bounds__(kBandWaves * 64, MT == 8 || OUT == kOutWide ? 2 : 3
     for (int i = threadIdx.x; i < rows * CH; i += kBandWaves * 64) {
         const int r = i / CH, c = i % CH;
         const v4u v = *(const H3Q_LDS v4u*)(ring + r * PITCH + ((c ^ (r & 7)) << 4));
-        if (16 / EL * c < cols)
+        if (16 / EL * c < cols && (lds_live[r >> 5] >> (r & 31) & 1))
             *reinterpret_cast<v4u*>((uint8_t*)p.out + ((tile.row0 + r) * p.ldo + COLS * slice) * EL + 16 * c) = v;
     }
 }

@@ -179,7 +179,7 @@ __global__ __launch_bounds__(kStreamWaves * 64) void grouped_stream_kernel(Group
         for (int v = 0; v < 4; ++v)
             y[v] = swiglu_f32(y[v], __fmul_rn(sa, __fmul_rn(sw[SWIGLU ? 1 : 0][v], (float)s1[v])));
     }
-    if (r16 < rows && row < p.n) {
+    if (r >= 0 && row < p.n) {  // rows past the tile, or without a row of a, keep what out held
         const int64_t at = (tile.row0 + r16) * p.ldo + row + 4 * kq;
         if constexpr (F32) *reinterpret_cast<v4f*>((float*)p.out + at) = v4f{y[0], y[1], y[2], y[3]};
         else *reinterpret_cast<v2u*>((uint16_t*)p.out + at) = v2u{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};

@@ -114,6 +114,7 @@ __global__ __launch_bounds__(256, 1) void grouped_tile_kernel(GroupedArgs p, int
     __shared__ __attribute__((aligned(1024))) uint8_t lds_ring[kStages * kStageBytes];
     // Per tile parity: row scales [256] f32 | column scales [256] f32 | order [256] i32.
     __shared__ __attribute__((aligned(1024))) uint8_t lds_vec[2 * kVecBytes];
+    __shared__ uint32_t lds_live[2][8];  // a bit for each row of the tile that has a row of a
     __shared__ int lds_first[kMaxExperts];  // row blocks of the experts below, and each one's rows
     __shared__ int lds_lo[kMaxExperts], lds_hi[kMaxExperts];
     H3Q_LDS uint8_t* const ring = (H3Q_LDS uint8_t*)lds_ring;
@@ -250,6 +251,8 @@ __global__ __launch_bounds__(256, 1) void grouped_tile_kernel(GroupedArgs p, int
         // column scales, and the next tile's order.
         H3Q_LDS uint8_t* const v = vec + (cj & 1) * kVecBytes;
         const int64_t r = source_row(threadIdx.x);
+        const uint64_t rows_live = __ballot(r >= 0);
+        if (lane < 2) lds_live[cj & 1][2 * wave + lane] = (uint32_t)(rows_live >> (32 * lane));
         copy4(gather ? CopySrc(p.a_scale, (uint32_t)(p.a_rows * 4)) : CopySrc(p.a_scale + cp.row0, (uint32_t)cp.rows * 4u),
               (uint32_t)(uintptr_t)(v + wave * 256), r >= 0 ? (uint32_t)((gather ? r : r - cp.row0) * 4) : kOob);
         const float* const sw = p.b_scale + (int64_t)cp.expert * p.n;
@@ -383,14 +386,16 @@ __global__ __launch_bounds__(256, 1) void grouped_tile_kernel(GroupedArgs p, int
             else __builtin_amdgcn_raw_buffer_store_b128(v, ro, off, 0, 0);
         };
         // The wave's rows of a staged pass: `chunks` 16-byte chunks a row from byte column col0 of out.
+        // A row without a row of a keeps what out held, as those past the tile do.
         auto flush = [&](int i, int chunks, int pitch, int col0, int limit) __attribute__((always_inline)) {
+            const uint32_t live = lds_live[par][(wm0 >> 5) + i];
             const int per = 64 / chunks;  // rows a store covers
 #pragma unroll
             for (int r = 0; r < 32 / per; ++r) {
                 const int row = per * r + ln / chunks, c = ln % chunks;
                 const v4u v = *(const H3Q_LDS v4u*)(scratch + row * pitch + ((c ^ (row & (chunks - 1))) << 4));
                 const int m = wm0 + 32 * i + row;
-                store(v, 16 * c < limit && m < cur.rows ? (uint32_t)m * (uint32_t)p.ldo * EL + (uint32_t)(col0 + 16 * c)
+                store(v, 16 * c < limit && (live >> row & 1) ? (uint32_t)m * (uint32_t)p.ldo * EL + (uint32_t)(col0 + 16 * c)
                                                         : 0xFFFFFFF0u);
             }
         };

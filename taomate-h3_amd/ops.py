@@ -714,7 +714,8 @@ def grouped_scaled_mm(a: torch.Tensor, b: torch.Tensor, a_scale: torch.Tensor, b
     ``order`` (a plan's) the rows are gathered: r = order[i] // top_k; without, r = i.
     ``swiglu``: b's rows are [gate | up] and the result is bf16(silu(gate) * up), n / 2
     columns.  ``b_tiled``: every expert's matrix is in the tiled layout.  Rows of
-    ``out`` past offsets[-1] are left as they were (allocated here: undefined)."""
+    ``out`` past offsets[-1], and rows whose order entry names no row of a (a plan
+    has none), are left as they were (allocated here: undefined)."""
     if b_tiled or not is_tiled(b):
         got = _native_call("grouped_scaled_mm", a, b, a_scale, b_scale, offsets, order, top_k, swiglu, b_tiled, out,
                            out_dtype == torch.float32) if out_dtype in (torch.bfloat16, torch.float32) else None

@@ -1,0 +1,96 @@
+"""Routed-expert operators on the GPU: rows that are not the call's, through every kernel."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from _util import activations
+
+pytestmark = pytest.mark.gpu
+
+
+def _bits(t: torch.Tensor) -> torch.Tensor:
+    return t.contiguous().view(torch.int16 if t.element_size() == 2 else torch.int32)
+
+
+def _codes(ops, rows, k, fmt, device, seed):
+    return ops.quant_rows(activations(rows, k, seed=seed, outlier_channels=2).to(device),
+                          ops.FMT_INT8 if fmt == "int8" else ops.FMT_E4M3FN)
+
+
+def _stack(ops, e, n, k, fmt, device, tiled, seed=5):
+    gen = torch.Generator(device=device).manual_seed(seed)
+    w = (torch.randn(e * n, k, generator=gen, device=device) * 0.05).to(torch.bfloat16)
+    quantize = ops.quant_rows_tiled if tiled else ops.quant_rows
+    codes, scales = quantize(w, ops.FMT_INT8 if fmt == "int8" else ops.FMT_E4M3FN)
+    return codes.view(e, n, k), scales.view(e, n)
+
+
+def _offsets(counts, device):
+    return torch.from_numpy(np.concatenate(([0], np.cumsum(counts))).astype(np.int32)).to(device)
+
+
+# Counts of two experts whose mean takes each kernel: streams (to 10 rows), bands of 64 (to 64)
+# and of 128 rows (to 384 or 512), 256 x 256 tiles (above).
+_EVERY_KERNEL = [[5, 11], [37, 66], [130, 271], [300, 1001]]
+_KERNEL_IDS = ["stream", "band64", "band128", "tile"]
+
+
+# ------------------------------------------------- rows that are not the call's
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("counts", _EVERY_KERNEL, ids=_KERNEL_IDS)
+@pytest.mark.parametrize("form", ["bf16", "f32", "swiglu"])
+@pytest.mark.parametrize("tiled", [True, False])
+def test_rows_of_invalid_order_entries_stay(ops, device, fmt, counts, form, tiled):
+    """A row whose order entry names no row of a keeps what out held; so do the rows past the last
+    group and everything around out.  The other rows equal the call on sorted rows, bit for bit."""
+    k, n, top_k, spare = 384, 96, 2, 3
+    rows = sum(counts)
+    tokens = rows // 2 + 1
+    q, s = _codes(ops, tokens, k, fmt, device, rows)
+    w, sw = _stack(ops, 2, n, k, fmt, device, tiled)
+    gen = torch.Generator().manual_seed(rows)
+    order = torch.randint(0, tokens * top_k, (rows + spare,), generator=gen, dtype=torch.int32)
+    bad = torch.rand(rows + spare, generator=gen) < 0.2
+    bad[0] = bad[rows - 1] = True
+    wrong = torch.tensor([-1, tokens * top_k, 2 ** 31 - 1, -2 ** 31], dtype=torch.int32)
+    order[bad] = wrong[torch.randint(0, 4, (int(bad.sum()),), generator=gen)]
+    dtype = torch.float32 if form == "f32" else torch.bfloat16
+    cols = n // 2 if form == "swiglu" else n
+    buffer = torch.full((rows + spare + 20, cols + 32), 7.0, device=device, dtype=dtype)
+    out = buffer[10:10 + rows + spare, 16:16 + cols]
+    kwargs = {"swiglu": form == "swiglu", "b_tiled": tiled, "out_dtype": dtype}
+    ops.grouped_scaled_mm(q, w, s, sw, _offsets(counts, device), order=order.to(device), top_k=top_k, out=out, **kwargs)
+    source = (order.clamp(0, tokens * top_k - 1) // top_k).long().to(device)
+    want = ops.grouped_scaled_mm(q.view(torch.uint8)[source].view(q.dtype), w, s[source], sw, _offsets(counts, device),
+                                 **kwargs)
+    good = ~bad
+    good[rows:] = False
+    assert torch.equal(_bits(out[good.to(device)]), _bits(want[good.to(device)]))
+    out[good.to(device)] = 7.0
+    assert (buffer == 7.0).all()
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("counts", _EVERY_KERNEL, ids=_KERNEL_IDS)
+def test_bounds_that_are_no_partition_touch_only_out(ops, device, fmt, counts):
+    """Offsets beyond the rows, below zero or falling: nothing around out is written, and a following
+    good call is right."""
+    k, n = 384, 96
+    rows = sum(counts)
+    q, s = _codes(ops, rows, k, fmt, device, rows)
+    w, sw = _stack(ops, 2, n, k, fmt, device, False)
+    buffer = torch.full((rows + 600, n + 32), 7.0, device=device, dtype=torch.bfloat16)
+    out = buffer[300:300 + rows, 16:16 + n]
+    for bounds in ([0, rows // 2, 10 * rows], [-5, 3, rows], [0, rows, 2], [1 << 30, 0, rows], [rows, rows, rows],
+                   [-2 ** 31, 2 ** 31 - 1, 2 ** 31 - 1]):
+        ops.grouped_scaled_mm(q, w, s, sw, torch.tensor(bounds, dtype=torch.int32, device=device), out=out)
+        whole = buffer.clone()
+        whole[300:300 + rows, 16:16 + n] = 7.0
+        assert (whole == 7.0).all(), bounds
+    ops.grouped_scaled_mm(q, w, s, sw, _offsets(counts, device), out=out)
+    want = ops.grouped_scaled_mm(q, w, s, sw, _offsets(counts, device))
+    assert torch.equal(_bits(out), _bits(want))
