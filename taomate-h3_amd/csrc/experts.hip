@@ -85,7 +85,10 @@ __device__ __forceinline__ float load_logit(const void* p, int64_t i) {
 // maximum over the keys and one minimum over the experts that hold it.  Lane j keeps
 // slot j.  The weights are binary32: softmax exp(l - max) / sum over all experts (or over
 // the taken ones), with exp(0) = 1 for the maximum itself, an infinite one included;
-// sigmoid 1 / (1 + exp(-l)), divided by the taken ones' sum when renormalized.
+// sigmoid 1 / (1 + exp(-l)), divided by the taken ones' sum when renormalized.  Below -18,
+// 1 + exp(l) is 1 in binary32 and the score is exp(l); where the largest logit is below it,
+// renormalized scores are taken as exp(l - max), whose common factor exp(max) falls out of the
+// shares (the scores themselves underflow from -88 on, and their sum would be 0).
 // A slot without an expert (fewer than k logits above -inf) gets -1 and weight 0.
 //
 // What bounds it: instructions.  The logits are read once, into registers; the k rounds cost
@@ -117,6 +120,7 @@ __global__ __launch_bounds__(256) void route_topk_kernel(RouteArgs p) {
             if (key[i] != 0u) whole += key[i] == top ? 1.0f : fast_exp(key_logit(key[i]) - best);
         whole = group_sum<LPT>(whole);
     }
+    const bool logistic = p.scoring == kScoreSigmoid && !(p.renormalize && best < -18.0f);
     int mine = -1;
     float weight = 0.0f;
     for (int j = 0; j < p.top_k; ++j) {
@@ -132,7 +136,7 @@ __global__ __launch_bounds__(256) void route_topk_kernel(RouteArgs p) {
         if (m != 0u && j == lane) {
             mine = (int)e;
             const float l = key_logit(m);
-            weight = p.scoring == kScoreSigmoid ? 1.0f / (1.0f + fast_exp(-l)) : m == top ? 1.0f : fast_exp(l - best);
+            weight = logistic ? 1.0f / (1.0f + fast_exp(-l)) : m == top ? 1.0f : fast_exp(l - best);
         }
 #pragma unroll
         for (int i = 0; i < NV; ++i)

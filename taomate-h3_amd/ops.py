@@ -657,7 +657,8 @@ def route_experts(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax",
     -inf are never taken, and a slot that finds no expert gets id -1 and weight 0.
     ``scoring`` "softmax": exp(l - max) over the sum of all experts, or of the
     taken ones (``renormalize``); "sigmoid": 1 / (1 + exp(-l)), divided by the
-    taken ones' sum when renormalized.  Both times ``scale``."""
+    taken ones' sum when renormalized (also where binary32 holds none of the
+    scores).  Both times ``scale``."""
     if logits.get_device() >= 0 and scoring in _SCORES:
         got = _native_call("route_experts", logits, top_k, _SCORES[scoring], bool(renormalize), float(scale))
         if got is not None:

@@ -1,4 +1,5 @@
-"""Routed-expert operators on the GPU: rows that are not the call's, through every kernel."""
+"""Routed-expert operators on the GPU: rows that are not the call's, through every kernel, and router
+weights far below zero."""
 
 from __future__ import annotations
 
@@ -6,6 +7,7 @@ import numpy as np
 import pytest
 import torch
 
+import _experts as R
 from _util import activations
 
 pytestmark = pytest.mark.gpu
@@ -94,3 +96,33 @@ def test_bounds_that_are_no_partition_touch_only_out(ops, device, fmt, counts):
     ops.grouped_scaled_mm(q, w, s, sw, _offsets(counts, device), out=out)
     want = ops.grouped_scaled_mm(q, w, s, sw, _offsets(counts, device))
     assert torch.equal(_bits(out), _bits(want))
+
+
+# ------------------------------------------------------------ sigmoid shares
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("spare", [0, 4096])  # a wave or 16 lanes a token
+def test_renormalized_sigmoid_far_below_zero(ops, device, dtype, spare):
+    """Scores of logits below -88 underflow binary32; their shares do not."""
+    inf = torch.inf
+    rows = torch.tensor([[-100.0, -101.0, -102.5, -100.0], [-88.0, -89.0, -90.0, -95.0], [-1000.0, -1001.0, -1003.0, -inf],
+                         [-60000.0, -60000.0, -60032.0, -inf], [-inf, -200.0, -inf, -inf], [-19.0, -18.5, -40.0, -20.0],
+                         [-17.0, -17.5, -40.0, -60.0], [-18.0, -18.0, -18.0, -18.0], [0.0, -100.0, -120.0, -1.0]]).to(dtype)
+    logits = torch.cat((rows, torch.zeros(spare, 4, dtype=dtype)))
+    ids, weights = ops.route_experts(logits.to(device), 3, scoring="sigmoid", renormalize=True, scale=2.0)
+    got = weights[:len(rows)].double().cpu()
+    want_ids, _ = R.route(rows, 3, "sigmoid", False)
+    assert (ids[:len(rows)].cpu().numpy() == want_ids).all()
+    taken = torch.from_numpy(want_ids >= 0)
+    l = torch.where(taken, rows.double().gather(1, torch.from_numpy(want_ids).clamp(min=0).long()), -inf)
+    log_score = torch.where(taken, -torch.logaddexp(torch.zeros(()).double(), -l), -inf)
+    want = 2.0 * torch.softmax(log_score, 1)
+    # A score by the hardware exp of x: (|x| + 2) 2^-23 of it, x the logit, or its distance from the
+    # largest where that one is far below zero; the sum as a whole the same again; 3 additions, the
+    # quotient, the scale and 1 + exp(l): 8 half-steps.  Scores below 2^-126 may become zero: of a
+    # sum of at least 2^-26, doubled by the scale, 2^-99.
+    far = l[:, :1] < -18.0
+    x = torch.where(taken, torch.where(far, l[:, :1] - l, l.abs()), 0.0).amax(1, keepdim=True)
+    bound = want * (2 * 2 * (x + 2) + 8) * R.U32 + 2.0 ** -99
+    assert ((got - want).abs() <= bound).all(), (got, want)
+    assert (got[~taken] == 0).all()
