@@ -532,8 +532,8 @@ __attribute__((visibility("default"))) int h3q_lora_down_ws(const void* x, int64
     return check_launch(h3q::launch_lora_down(g, workspace, workspace_bytes, (hipStream_t)stream), who);
 }
 
-// 128 * 127 * k stays below 2^31.
-constexpr int64_t kInt8MaxK = 132096;
+// 128 * 128 * k stays below 2^31 (codes of -128 on both sides), in multiples of 16.
+constexpr int64_t kInt8MaxK = 131056;
 
 // Shared checks of the expert entry points.
 static int check_experts(const char* who, int64_t tokens, int64_t top_k, int64_t experts) {

@@ -154,3 +154,25 @@ def test_expert_module_checks_shapes():
     with pytest.raises(ValueError, match="expert weights"):
         experts.QuantizedExperts(torch.zeros(2, 64, 32), torch.zeros(2, 64), torch.zeros(2, 32, 16), torch.zeros(2, 32),
                                  w13_tiled=False, w2_tiled=False)
+
+
+def test_int8_sums_stay_below_32_bits():
+    """128 * 128 * k of codes that are all -128 reaches 2^31 at k = 131072: refused, the k below it taken."""
+    from taomate_h3_amd import _lib
+
+    if not _lib.LIB_PATH.exists():
+        pytest.skip("library not built")
+    lib = _lib.lib()
+    p = ctypes.c_void_p(256)
+
+    def grouped(fmt, k):  # no rows: checked, nothing launched
+        return lib.h3q_grouped_mm(fmt, p, k, 8, p, None, 1, p, 0, p, p, 4, 0, 16, k, 0, 0, p, 16, None)
+
+    def ffn(fmt, d, f):
+        return lib.h3q_expert_ffn(fmt, p, d, 0, d, f, p, p, 2, 0, 4, p, 0, p, p, 0, p, p, d, p, 1 << 30, None)
+
+    assert 128 * 128 * 131056 < 2 ** 31 <= 128 * 128 * 131072
+    for call in (lambda fmt, k: grouped(fmt, k), lambda fmt, k: ffn(fmt, k, 16), lambda fmt, k: ffn(fmt, 16, k)):
+        assert call(1, 131056) == 0
+        assert call(1, 131072) == 2 and b"32 bits" in lib.h3q_last_error()
+        assert call(0, 131072) == 0  # e4m3 sums are binary32
