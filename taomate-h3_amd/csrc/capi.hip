@@ -587,6 +587,8 @@ __attribute__((visibility("default"))) int h3q_route_topk(const void* logits, in
     a.scale = scale;
     a.ids = ids;
     a.weights = weights;
+    if (!h3q::route_topk_fits(a))
+        return fail(H3Q_ERR_UNSUPPORTED, "%s: %lld tokens need too many workgroups", who, (long long)tokens);
     return check_launch(h3q::launch_route_topk(a, dtype, (hipStream_t)stream), who);
 }
 

@@ -152,16 +152,17 @@ __global__ __launch_bounds__(256) void route_topk_kernel(RouteArgs p) {
 
 namespace {
 
+// Lanes of a token.  A wave per token also for few tokens: a quarter of the work per wave while there
+// are SIMDs for all of them (4093 tokens of 256 experts: 7.2 -> 6.5 us; 32768 of 128: 9.9 -> 16.4).
+int route_lanes(const RouteArgs& a) { return a.experts > 256 || a.top_k > 16 || a.tokens <= 4096 ? 64 : 16; }
+
 template <int DT>
 hipError_t launch_route_dt(const RouteArgs& a, hipStream_t st) {
-    // A wave per token also for few tokens: a quarter of the work per wave while there are SIMDs
-    // for all of them (4093 tokens of 256 experts: 7.2 -> 6.5 us; 32768 of 128: 9.9 -> 16.4).
-    const bool wide = a.experts > 256 || a.top_k > 16 || a.tokens <= 4096;
-    const int lpt = wide ? 64 : 16;
+    const int lpt = route_lanes(a);
     const dim3 grid((unsigned)((a.tokens + 256 / lpt - 1) / (256 / lpt)));
     const int nv = (int)((a.experts + lpt - 1) / lpt);
 #define H3Q_ROUTE(LPT, NV) hipLaunchKernelGGL((route_topk_kernel<DT, LPT, NV>), grid, dim3(256), 0, st, a)
-    if (wide) {
+    if (lpt == 64) {
         if (nv <= 1) H3Q_ROUTE(64, 1);
         else if (nv <= 4) H3Q_ROUTE(64, 4);
         else H3Q_ROUTE(64, 16);
@@ -176,6 +177,9 @@ hipError_t launch_route_dt(const RouteArgs& a, hipStream_t st) {
 }
 
 }  // namespace
+
+// A grid of n workgroups of 256 threads takes n * 256 < 2^32.
+bool route_topk_fits(const RouteArgs& a) { return (a.tokens + 15) / 16 * 16 * route_lanes(a) < (int64_t(1) << 32); }
 
 hipError_t launch_route_topk(const RouteArgs& a, int dtype, hipStream_t st) {
     if (dtype == kInF32) return launch_route_dt<kInF32>(a, st);

@@ -176,6 +176,7 @@ struct RouteArgs {
     int* ids;        // [tokens, top_k]
     float* weights;  // [tokens, top_k]
 };
+bool route_topk_fits(const RouteArgs& a);  // its grid stays within what a launch takes
 hipError_t launch_route_topk(const RouteArgs& a, int dtype, hipStream_t st);
 
 struct PlanArgs {

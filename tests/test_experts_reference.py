@@ -176,3 +176,16 @@ def test_int8_sums_stay_below_32_bits():
         assert call(1, 131056) == 0
         assert call(1, 131072) == 2 and b"32 bits" in lib.h3q_last_error()
         assert call(0, 131072) == 0  # e4m3 sums are binary32
+
+
+def test_router_refuses_more_tokens_than_a_launch_takes():
+    """16 lanes a token (64 above 256 experts or 16 slots) and a grid of fewer than 2^32 threads."""
+    from taomate_h3_amd import _lib
+
+    if not _lib.LIB_PATH.exists():
+        pytest.skip("library not built")
+    lib = _lib.lib()
+    p = ctypes.c_void_p(256)
+    for tokens, experts, top_k in ((1 << 28, 256, 1), (1 << 26, 257, 1), (1 << 26, 64, 17)):
+        assert lib.h3q_route_topk(p, 2, experts, tokens, experts, top_k, 0, 1, 1.0, p, p, None) == 2
+        assert b"workgroups" in lib.h3q_last_error()
