@@ -1,7 +1,10 @@
-"""Routed-expert operators on the GPU: rows that are not the call's, through every kernel, and router
-weights far below zero."""
+"""Routed-expert operators on the GPU: the contract of rows that are not the call's, router
+weights far below zero, and every kernel of the grouped products and of the layer by its own
+sizes (the sizes that choose it stand at each test)."""
 
 from __future__ import annotations
+
+import importlib
 
 import numpy as np
 import pytest
@@ -11,6 +14,11 @@ import _experts as R
 from _util import activations
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def experts_module():
+    return importlib.import_module("taomate_h3_amd.inference.experts")
 
 
 def _bits(t: torch.Tensor) -> torch.Tensor:
@@ -126,3 +134,93 @@ def test_renormalized_sigmoid_far_below_zero(ops, device, dtype, spare):
     bound = want * (2 * 2 * (x + 2) + 8) * R.U32 + 2.0 ** -99
     assert ((got - want).abs() <= bound).all(), (got, want)
     assert (got[~taken] == 0).all()
+
+
+# ------------------------------------------------------- grouped: every kernel
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("tiled,k", [(True, 384), (False, 336)])
+@pytest.mark.parametrize("form", ["bf16", "f32", "swiglu"])
+def test_gathered_rows_over_many_tiles(ops, device, fmt, tiled, k, form):
+    """More 256 x 256 tiles than the chip has workgroups for (mean 579 rows): a tile's order is fetched
+    while another runs.  Bit for bit the call on sorted rows."""
+    counts, n, top_k = [1100, 0, 129, 2000, 128, 700, 1], 5216, 3
+    rows, tokens = sum(counts), 1500
+    q, s = _codes(ops, tokens, k, fmt, device, 3)
+    w, sw = _stack(ops, len(counts), n, k, fmt, device, tiled)
+    gen = torch.Generator().manual_seed(k)
+    order = torch.randint(0, tokens * top_k, (rows,), generator=gen, dtype=torch.int32).to(device)
+    source = (order // top_k).long()
+    kwargs = {"swiglu": form == "swiglu", "b_tiled": tiled,
+              "out_dtype": torch.float32 if form == "f32" else torch.bfloat16}
+    got = ops.grouped_scaled_mm(q, w, s, sw, _offsets(counts, device), order=order, top_k=top_k, **kwargs)
+    want = ops.grouped_scaled_mm(q.view(torch.uint8)[source].view(q.dtype), w, s[source], sw, _offsets(counts, device),
+                                 **kwargs)
+    assert torch.equal(_bits(got), _bits(want))
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("e", [65, 130])
+@pytest.mark.parametrize("mean", [4, 30, 150, 600], ids=_KERNEL_IDS)
+@pytest.mark.parametrize("form", ["bf16", "swiglu"])
+def test_more_experts_than_lanes(ops, device, fmt, e, mean, form):
+    """65 and 130 experts, some empty, in one call equal the same experts in calls of at most 64, bit
+    for bit (each part's mean takes the same kernel as the whole's)."""
+    k, n = 384, 96
+    pattern = np.array([0, 2, 1, 0, 1, 2, 1, 1])  # mean 1; the counts of a part stay near the mean
+    counts = pattern[np.arange(e) % 8] * mean + np.array([0, 1, 0, 0, 1, 0, 0, 1])[np.arange(e) % 8]
+    rows = int(counts.sum())
+    q, s = _codes(ops, rows, k, fmt, device, e)
+    w, sw = _stack(ops, e, n, k, fmt, device, True)
+    kwargs = {"swiglu": form == "swiglu", "b_tiled": True}
+    got = ops.grouped_scaled_mm(q, w, s, sw, _offsets(counts, device), **kwargs)
+    starts = np.concatenate(([0], np.cumsum(counts)))
+    for lo in range(0, e, 40):
+        hi = min(lo + 40, e)
+        a, b = int(starts[lo]), int(starts[hi])
+        want = ops.grouped_scaled_mm(q[a:b], w[lo:hi].contiguous(), s[a:b], sw[lo:hi].contiguous(),
+                                     _offsets(counts[lo:hi], device), **kwargs)
+        assert torch.equal(_bits(got[a:b]), _bits(want)), lo
+
+
+# -------------------------------------------------------- layer: every kernel
+
+def _layer(ops, experts_module, device, oracle, fmt, e, d, f, first=0, seed=11):
+    gen = torch.Generator().manual_seed(seed)
+    w13 = (torch.randn(e, 2 * f, d, generator=gen) * d ** -0.5).to(torch.bfloat16)
+    w2 = (torch.randn(e, d, f, generator=gen) * f ** -0.5).to(torch.bfloat16)
+    layer = experts_module.QuantizedExperts.from_weights(
+        w13.to(device), w2.to(device), ops.FMT_INT8 if fmt == "int8" else ops.FMT_E4M3FN, first_expert=first)
+    return layer, (*R.quantize_weights(w13, oracle, fmt), *R.quantize_weights(w2, oracle, fmt))
+
+
+def _routed(t, k, total, seed):
+    gen = torch.Generator().manual_seed(seed)
+    ids, weights = R.route(torch.randn(t, total, generator=gen) * 2, k, "softmax", True)
+    if t > 2:
+        ids[1], weights[1] = -1, 0.0  # a padded token
+    return ids, weights.astype(np.float32)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("t,k,total,e,first,d,f", [
+    # few tokens, 16 output columns a workgroup (d >= 4096), rows longer than the registers of a wave
+    # (2048 columns) and of a workgroup (8192), codes made inside and by a launch of their own
+    (3, 2, 4, 4, 0, 4096, 128), (3, 2, 4, 4, 0, 4112, 144), (12, 2, 4, 4, 0, 4096, 128), (1, 2, 2, 2, 0, 8320, 16),
+    (3, 2, 4, 4, 0, 128, 2304), (10, 3, 4, 4, 0, 128, 2304), (2, 1, 1, 1, 0, 4096, 4096),
+    # row-major weights, more than 64 pairs: streams, bands of 64 and of 128 rows
+    (40, 2, 16, 16, 0, 272, 208), (100, 1, 4, 4, 0, 272, 144), (300, 1, 2, 2, 0, 144, 208),
+    # tiled weights in bands of 64 rows; more than 512 tokens; more than 2048 pairs; a rank's share of them
+    (100, 1, 4, 4, 0, 256, 128), (520, 1, 16, 16, 0, 256, 128), (1030, 2, 8, 8, 0, 256, 128),
+    (1030, 2, 16, 8, 8, 272, 80), (520, 1, 90, 90, 0, 128, 128),
+    # above 512 rows an expert: tiles (e4m3: for the down product)
+    (1100, 1, 2, 2, 0, 384, 384)])
+def test_layer_kernels(ops, experts_module, device, oracle, fmt, t, k, total, e, first, d, f):
+    layer, packed = _layer(ops, experts_module, device, oracle, fmt, e, d, f, first)
+    x = activations(t, d, seed=t + d, outlier_channels=2)
+    ids, weights = _routed(t, k, total, t + k)
+    got = layer(x.to(device), torch.from_numpy(ids).to(device), torch.from_numpy(weights).to(device))
+    want, bound = R.ffn(oracle, fmt, x, ids, weights, *packed, first=first)
+    err = np.abs(got.double().cpu().numpy() - want)
+    assert (err <= bound).all(), np.max(err / bound)
+    assert np.linalg.norm(err) <= 0.02 * np.linalg.norm(want)
