@@ -78,10 +78,13 @@ enum GroupedOut : int { kOutBF16 = 0, kOutF32 = 1, kOutSwiglu = 2, kOutWide = 3 
 
 // silu(g) * u in binary32: exp(-g) by the hardware exp2, the quotient by its reciprocal (one
 // unit in the last place; an IEEE division is ten instructions, which an epilogue without
-// another wave to hide it pays in full).  g = -inf gives NaN, as -inf / inf does.
+// another wave to hide it pays in full).  The reciprocal instruction makes 0 of results below
+// 2^-126, which 1 / (1 + e) is for g in (-88.7, -87.3): quotient and gate are taken at 8 times
+// and an eighth of their size, powers of two that change no other result.  Below -88.7 e is
+// infinite and the result 0, as the quotient's.  g = -inf gives NaN, as -inf / inf does.
 __device__ __forceinline__ float swiglu_f32(float g, float u) {
     const float e = __builtin_amdgcn_exp2f(-g * 0x1.715476p+0f);
-    return g * __builtin_amdgcn_rcpf(1.0f + e) * u;
+    return 0.125f * g * __builtin_amdgcn_rcpf(__builtin_fmaf(e, 0.125f, 0.125f)) * u;
 }
 
 // Rows of one expert that a workgroup's tile covers.

@@ -183,6 +183,27 @@ def test_more_experts_than_lanes(ops, device, fmt, e, mean, form):
         assert torch.equal(_bits(got[a:b]), _bits(want)), lo
 
 
+@pytest.mark.parametrize("counts", _EVERY_KERNEL, ids=_KERNEL_IDS)
+def test_swiglu_of_far_negative_gates(ops, device, counts):
+    """Gates down to -88.7, where exp(-g) still is a binary32 number and its reciprocal no normal one,
+    beside up values that bring the product back to size."""
+    k, rows = 272, sum(counts)
+    gates = torch.tensor([-88.7, -88.5, -88.0, -87.6, -87.4, -87.3, -86.0, -60.0, -1.0, 0.0, 1e-30, 3.0, 90.0])
+    g = gates[torch.arange(rows) % len(gates)]
+    q = torch.zeros(rows, k, dtype=torch.int8)
+    q[:, 0] = 1
+    w = torch.zeros(2, 96, k, dtype=torch.int8)
+    w[:, :, 0] = 1
+    sw = torch.cat((torch.ones(48), torch.full((24,), -1e30), torch.full((24,), 3.0))).expand(2, 96).contiguous()
+    got = ops.grouped_scaled_mm(q.to(device), w.to(device), g.to(device), sw.to(device), _offsets(counts, device),
+                                swiglu=True).double().cpu().numpy()
+    y = g.double().numpy()[:, None] * sw[0].double().numpy()[None, :]
+    y_bound = 2.5 * R.U32 * np.abs(y)
+    y_bound[:, :48] = 0.0  # gates: products with 1, exact
+    want, bound = R.swiglu(y, y_bound)
+    assert (np.abs(got - want) <= bound + R.HALF_BF16 * (np.abs(want) + bound) + 2.0 ** -133).all()
+
+
 # -------------------------------------------------------- layer: every kernel
 
 def _layer(ops, experts_module, device, oracle, fmt, e, d, f, first=0, seed=11):
