@@ -389,7 +389,7 @@ int h3q_grouped_mm(int format, const void* a, int64_t lda, int64_t a_rows, const
  * out[t] = bf16(sum_j weights[t, j] * y[slots[t, j]]), binary32 in slot order; slots
  * outside [0, rows) add nothing (a token with none gets zeros).  y: bf16, or binary32
  * (y_f32), [rows, cols], ldy elements; cols % 8 == 0, strides multiples of 8
- * elements, 16-byte aligned y and out.
+ * elements, 16-byte aligned y and out.  out holds no element of y.
  */
 int h3q_combine_experts(const void* y, int y_f32, int64_t ldy, int64_t rows, const int32_t* slots,
                         const float* weights, int64_t tokens, int64_t top_k, int64_t cols, void* out, int64_t ldo,

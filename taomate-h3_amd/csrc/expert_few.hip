@@ -16,9 +16,9 @@
 //                 meet in LDS, and the weighted sum over a token's experts is taken there
 //                 in slot order.  No atomics, no third kernel for the sum.
 //
-// Measured (int8, one token, 8 of 64 experts, f = 1024, d = 2048, weights out of HBM): 16.9 us
-// in all, 10.7 + 8.1 by themselves, of which about 9 are the weights; the chain of five
-// launches takes 32.
+// Measured (int8, one token, 8 of 64 experts, f = 1024, d = 2048, weights out of HBM): 13 to 17
+// us in all over runs, 9.6 + 8.8 by themselves (medians), of which about 9 are the weights; the
+// chain of five launches takes 32.
 //
 // With many or long rows the quantizing inside every workgroup costs more than a launch of
 // the row quantizer; then that runs first and the kernels read codes (FUSED false).

@@ -94,7 +94,7 @@ __device__ __forceinline__ float load_logit(const void* p, int64_t i) {
 // What bounds it: instructions.  The logits are read once, into registers; the k rounds cost
 // about 5 NV + 20 instructions each.  Four tokens to a wave rather than one cut the
 // cross-lane steps per token by four and stay within a row of 16 lanes (register permutes):
-// 32768 tokens of 128 experts, top 4, take 9.9 us (16.8 MB of logits: 3 us at the HBM's rate).
+// 32768 tokens of 128 experts, top 4, take 9.8 us (16.8 MB of logits: 3 us at the HBM's rate).
 template <int DT, int LPT, int NV>
 __global__ __launch_bounds__(256) void route_topk_kernel(RouteArgs p) {
     constexpr int TPB = 256 / LPT;
@@ -153,7 +153,7 @@ __global__ __launch_bounds__(256) void route_topk_kernel(RouteArgs p) {
 namespace {
 
 // Lanes of a token.  A wave per token also for few tokens: a quarter of the work per wave while there
-// are SIMDs for all of them (4093 tokens of 256 experts: 7.2 -> 6.5 us; 32768 of 128: 9.9 -> 16.4).
+// are SIMDs for all of them (4093 tokens of 256 experts: 7.2 -> 6.5 us; 32768 of 128: 9.8 -> 16.4).
 int route_lanes(const RouteArgs& a) { return a.experts > 256 || a.top_k > 16 || a.tokens <= 4096 ? 64 : 16; }
 
 template <int DT>
@@ -205,7 +205,7 @@ hipError_t launch_route_topk(const RouteArgs& a, int dtype, hipStream_t st) {
 // last placed one order -1.
 //
 // What bounds it: dependent round trips and two launches; the work is log2(experts) ballots a
-// trip.  131072 pairs of 128 experts: 3.6 + 7.5 us (one workgroup per expert over all pairs,
+// trip.  131072 pairs of 128 experts: 3.7 + 7.6 us (one workgroup per expert over all pairs,
 // in one launch: 46 us); 8 pairs: 3.6 us.
 constexpr int kPlanWaves = 16;
 constexpr int kPlanWholePairs = 2048;
@@ -471,7 +471,7 @@ __device__ __forceinline__ void load8(const void* p, int64_t i, float (&v)[8]) {
 // out[t] = bf16(sum_j weights[t, j] * rows[slots[t, j]]), binary32 products and sums in
 // slot order, one rounding.  A thread takes 8 columns of a token, eight slots' loads in
 // flight at a time; a slot outside [0, rows) adds nothing.  Bound by
-// reading the rows: 12288 of 2048 in binary32 (100 MB) 17.8 us, 5.7 TB/s.
+// reading the rows: 12288 of 2048 in binary32 (100 MB) 18.0 us, 5.6 TB/s.
 template <bool F32>
 __global__ __launch_bounds__(256) void combine_experts_kernel(CombineArgs p) {
     const int64_t vecs = p.cols / 8, total = p.tokens * vecs;

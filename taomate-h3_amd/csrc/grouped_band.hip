@@ -11,9 +11,10 @@
 // step publishes the next stage and frees the last.  No split of K: the experts give
 // workgroups enough.  Items (band x column slice) go to the XCDs in contiguous runs, an
 // expert's bands of one slice side by side, so weights and rows pass through one L2 about
-// once: spread over the XCDs, two bands an expert moved 505 MB from beyond the L2s where
-// 197 MB were needed, and that was the bound (32 experts of 2816 x 2048 with 200 rows each:
-// 84 -> 70 us; 8 of 14336 x 5376: 197 -> 185 us).
+// once: spread over the XCDs, two bands an expert missed the L2s for 525 MB where 197 MB were
+// needed, and that was the bound (32 experts of 2816 x 2048 with 200 rows each, int8: 84 -> 70 to
+// 72 us; 8 of 14336 x 5376: 197 -> 185 to 192 us).  In runs the first misses for 227 MB (3.2 TB/s),
+// with the matrix instructions busy 28% of the time: neither binds it now.
 //
 // SwiGLU: a wave's two 16-row blocks are gate and up rows of the same columns, so both sit in
 // one lane.  The output tile is staged in LDS and stored as whole row pieces.

@@ -22,9 +22,10 @@
 // stays in registers.
 //
 // What bounds it: as the dense kernel, the matrix instructions at their power-limited clock
-// (int8 16384 rows over 8 experts of 14336 x 5376 with SwiGLU and gathered rows: 1130 us, 2.24
-// POP/s; the dense kernel's 2.31), and with a short k the epilogue, which no other wave
-// hides (e4m3 32768 rows over 64 experts of 2816 x 2048: 217 us, 1.74 PFLOP/s).
+// (int8 16384 rows over 8 experts of 14336 x 5376 with SwiGLU and gathered rows: 1126 to 1168 us
+// over eight runs on four cards, 2.16 to 2.24 POP/s; the dense kernel's 2.31), and with a short k the
+// epilogue, which no other wave hides (e4m3 32768 rows over 64 experts of 2816 x 2048: 215 to 224
+// us, 1.68 to 1.75 PFLOP/s).
 #include <type_traits>
 
 #include "gemm_tiles.hpp"

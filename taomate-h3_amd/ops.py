@@ -758,7 +758,8 @@ def grouped_scaled_mm(a: torch.Tensor, b: torch.Tensor, a_scale: torch.Tensor, b
 def combine_experts(y: torch.Tensor, slots: torch.Tensor, weights: torch.Tensor, *,
                     out: torch.Tensor | None = None) -> torch.Tensor:
     """bf16 [tokens, cols]: sum over a token's slots of weights[t, j] * y[slots[t, j]]
-    (y bf16 or fp32 rows, sums in binary32, slots of -1 add nothing)."""
+    (y bf16 or fp32 rows, sums in binary32, slots of -1 add nothing).  ``out`` holds no
+    element of y."""
     got = _native_call("combine_experts", y, slots, weights, out)
     if got is not None:
         return got
