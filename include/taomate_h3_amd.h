@@ -348,7 +348,7 @@ int h3q_residual_gate_rms_norm_modulate_quant(const void* residual, int64_t ldr,
  *   SIGMOID: 1 / (1 + exp(-l)), divided by the sum of the taken ones (renormalize: shares
  *            of the sum also where every score is too small for binary32)
  * times scale.  ids int32 and weights fp32 [tokens, top_k], contiguous.  top_k <= experts;
- * tokens below 2^28, or 2^26 with more than 256 experts or 16 slots.
+ * tokens at most 2^28 - 16, or 2^26 - 16 with more than 256 experts or 16 slots.
  */
 int h3q_route_topk(const void* logits, int dtype, int64_t ldl, int64_t tokens, int64_t experts, int64_t top_k,
                    int scoring, int renormalize, float scale, int32_t* ids, float* weights, void* stream);
