@@ -412,6 +412,96 @@ int h3q_expert_ffn(int format, const void* x, int64_t ldx, int64_t tokens, int64
                    int w13_layout, const float* s13, const void* w2, int w2_layout, const float* s2, void* out,
                    int64_t ldo, void* workspace, int64_t workspace_bytes, void* stream);
 
+/*
+ * What stands between the qkv product and the attention: rotary positions, the RMS
+ * norm of each query and key head, and keys and values appended to a paged cache.
+ * Beyond the reference's quantized linears (its Triton norm and rotation kernels have
+ * their own rounding points; here a row is rounded once, where it is stored).
+ *
+ * Rows [tokens, heads, head_dim] in bf16, binary16 or binary32 (dtype: H3Q_DTYPE_*)
+ * with unit stride along head_dim and any other strides, in elements: the packed rows
+ * of a product can be used as they are.  head_dim even, at most 512; at most 16384 heads.  A row is read
+ * whole before it is stored, so out may be x; otherwise they may not overlap.
+ * Sums and rotations are binary32.
+ */
+typedef struct {
+    const void* x;
+    int64_t token_stride, head_stride, heads;
+    const void* weight;     /* of the norm, weight_dtype: [head_dim] (weight_stride 0) or [heads, head_dim]; NULL: no norm */
+    int64_t weight_stride;
+    void* out;              /* rows of x's dtype; not used where the rows go into a cache */
+    int64_t out_token_stride, out_head_stride;
+} h3q_heads;
+
+/* cos and sin: fp32 [rows, rot_dim / 2], contiguous.  Channels [0, rot_dim) are rotated, the rest goes through. */
+typedef struct {
+    const float *cos, *sin;
+    int64_t rows, rot_dim;
+    const void* positions;  /* row of the tables for each token (NULL: its own number, rows >= tokens) */
+    int positions_i64;      /* int64, else int32 */
+    int interleaved;        /* pairs (2 i, 2 i + 1), else (i, rot_dim / 2 + i) */
+    int inverse;            /* by the negative angle: the rotation's inverse, and its gradient (without the magnitude) */
+} h3q_rotation;
+
+/* Pages [pages, page_size, heads, head_dim], strides in elements, pages * page_size < 2^31. */
+#define H3Q_PAGES_ROWS 0    /* rows of the call's dtype */
+#define H3Q_PAGES_STATIC 1  /* e4m3fn codes, scale [heads] (its head stride may be 0), read */
+#define H3Q_PAGES_BY_ROW 2  /* e4m3fn codes, scale [pages, page_size, heads], written */
+typedef struct {
+    void* pages;
+    int64_t n_pages, page_size, page_stride, slot_stride, head_stride;
+    int kind;
+    float* scale;
+    int64_t scale_page_stride, scale_slot_stride, scale_head_stride;
+} h3q_pages;
+
+/* Types of positions in h3q_rotary_tables. */
+#define H3Q_POSITIONS_I32 0
+#define H3Q_POSITIONS_I64 1
+#define H3Q_POSITIONS_F32 2
+#define H3Q_POSITIONS_F64 3
+
+/*
+ * cos and sin [n, half] (fp32) of positions[i] * frequencies[j] (radians, binary64),
+ * times magnitude.  The angle is a binary64 product, reduced there; n * half < 2^31.
+ */
+int h3q_rotary_tables(const void* positions, int type, int64_t n, const double* frequencies, int64_t half,
+                      double magnitude, float* cos_out, float* sin_out, void* stream);
+
+/*
+ * Rotation of rows (x->weight NULL), or the norm of query and key heads and their rotation in one
+ * pass (k may have 0 heads; a NULL weight leaves out its norm):
+ *   n = x / sqrt(sum(x * x) / head_dim + eps) * weight;  (a, b) -> (a cos - b sin, a sin + b cos)
+ * A token with a position below 0 is padding: its rows of out are left as they were.  One
+ * with a position past the tables gets NaN in its rotated channels.
+ */
+int h3q_rotary(int dtype, const h3q_heads* x, int64_t tokens, int64_t head_dim, const h3q_rotation* rotation,
+               void* stream);
+int h3q_qk_norm_rotary(int dtype, int weight_dtype, const h3q_heads* q, const h3q_heads* k, int64_t tokens,
+                       int64_t head_dim, float eps, const h3q_rotation* rotation, void* stream);
+
+/*
+ * Where the tokens of a step go: token t of sequence s (cu[s] <= t < cu[s + 1], cu int32 [seqs + 1])
+ * has position lengths[s] + t - cu[s] and slot table[s, position / page_size] * page_size + position %
+ * page_size.  Position and slot -1: a token of no sequence; slot -1: no page for it (a page id below
+ * 0, a position past the table's columns, a slot of 2^31 or more).
+ */
+int h3q_plan_append(const int32_t* table, int64_t table_stride, int64_t seqs, int64_t columns, const int32_t* lengths,
+                    const int32_t* cu, int64_t tokens, int64_t page_size, int32_t* positions, int32_t* slots,
+                    void* stream);
+
+/*
+ * One layer's append: k (norm and rotation as above, each if asked for) and v (as it is) of token t into slot
+ * slots[t] of k_pages and v_pages, and q (may be NULL) normed and rotated into its out.  e4m3fn pages
+ * hold e4m3(clamp(y * RN(1 / s), +-448)), s of the head, or max(max|y| * RN(1/448), 1e-12) of the
+ * row, which goes into the scale pages; NaN and infinities as in h3q_quant_rows.  Slots outside
+ * [0, n_pages * page_size) are not stored; padding (position below 0) stores neither k, v nor q.
+ * Slots of one call that are stored are distinct.  rotation NULL: no rotation, no positions.
+ */
+int h3q_append_kv(int dtype, int weight_dtype, const h3q_heads* q, const h3q_heads* k, const h3q_heads* v,
+                  const h3q_pages* k_pages, const h3q_pages* v_pages, const int32_t* slots, int64_t tokens,
+                  int64_t head_dim, float eps, const h3q_rotation* rotation, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -18,6 +18,31 @@ _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _I = ctypes.c_int
 _F = ctypes.c_float
+
+
+class Heads(ctypes.Structure):
+    """h3q_heads"""
+
+    _fields_ = [("x", _P), ("token_stride", _I64), ("head_stride", _I64), ("heads", _I64), ("weight", _P),
+                ("weight_stride", _I64), ("out", _P), ("out_token_stride", _I64), ("out_head_stride", _I64)]
+
+
+class Rotation(ctypes.Structure):
+    """h3q_rotation"""
+
+    _fields_ = [("cos", _P), ("sin", _P), ("rows", _I64), ("rot_dim", _I64), ("positions", _P), ("positions_i64", _I),
+                ("interleaved", _I), ("inverse", _I)]
+
+
+class Pages(ctypes.Structure):
+    """h3q_pages"""
+
+    _fields_ = [("pages", _P), ("n_pages", _I64), ("page_size", _I64), ("page_stride", _I64), ("slot_stride", _I64),
+                ("head_stride", _I64), ("kind", _I), ("scale", _P), ("scale_page_stride", _I64),
+                ("scale_slot_stride", _I64), ("scale_head_stride", _I64)]
+
+
+_HEADS, _ROTATION, _PAGES = (ctypes.POINTER(t) for t in (Heads, Rotation, Pages))
 SIGNATURES: dict[str, tuple[type | None, list]] = {
     "h3q_version": (_I, []),
     "h3q_last_error": (ctypes.c_char_p, []),
@@ -52,6 +77,11 @@ SIGNATURES: dict[str, tuple[type | None, list]] = {
     "h3q_expert_ffn_workspace_bytes": (_I64, [_I64, _I64, _I64, _I64, _I64]),
     "h3q_expert_ffn": (_I, [_I, _P, _I64, _I64, _I64, _I64, _P, _P, _I64, _I64, _I64, _P, _I, _P, _P, _I, _P, _P,
                             _I64, _P, _I64, _P]),
+    "h3q_rotary_tables": (_I, [_P, _I, _I64, _P, _I64, ctypes.c_double, _P, _P, _P]),
+    "h3q_rotary": (_I, [_I, _HEADS, _I64, _I64, _ROTATION, _P]),
+    "h3q_qk_norm_rotary": (_I, [_I, _I, _HEADS, _HEADS, _I64, _I64, _F, _ROTATION, _P]),
+    "h3q_plan_append": (_I, [_P, _I64, _I64, _I64, _P, _P, _I64, _I64, _P, _P, _P]),
+    "h3q_append_kv": (_I, [_I, _I, _HEADS, _HEADS, _HEADS, _PAGES, _PAGES, _P, _I64, _I64, _F, _ROTATION, _P]),
 }
 
 _lock = threading.Lock()

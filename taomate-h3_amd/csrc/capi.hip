@@ -788,4 +788,218 @@ __attribute__((visibility("default"))) int h3q_expert_ffn(int format, const void
     return check_launch(h3q::launch_expert_ffn(a, workspace, (hipStream_t)stream), who);
 }
 
+// Rows [tokens, heads, head_dim] of a call: 0, or the error.
+static int check_heads(const char* who, const char* what, const h3q_heads& h, int64_t tokens, int64_t size,
+                       bool has_out) {
+    if (h.heads < 0 || h.heads > h3q::kHeadMaxHeads) return fail(H3Q_ERR_INVALID, "%s: %lld %s heads", who, (long long)h.heads, what);
+    if (tokens == 0 || h.heads == 0) return H3Q_OK;
+    if (!h.x || (has_out && !h.out)) return fail(H3Q_ERR_INVALID, "%s: null %s pointer", who, what);
+    if (!aligned(h.x, size) || (has_out && !aligned(h.out, size)))
+        return fail(H3Q_ERR_INVALID, "%s: %s rows are not aligned to their type", who, what);
+    return H3Q_OK;
+}
+
+static int check_rotation(const char* who, const h3q_rotation& r, int64_t tokens, int64_t head_dim) {
+    if (r.rot_dim <= 0 || r.rot_dim % 2 || r.rot_dim > head_dim)
+        return fail(H3Q_ERR_INVALID, "%s: %lld rotated channels of %lld", who, (long long)r.rot_dim, (long long)head_dim);
+    if (r.rows < 0 || (!r.positions && r.rows < tokens))
+        return fail(H3Q_ERR_INVALID, "%s: tables of %lld rows for %lld tokens without positions", who,
+                    (long long)r.rows, (long long)tokens);
+    if (tokens > 0 && (!r.cos || !r.sin)) return fail(H3Q_ERR_INVALID, "%s: null table", who);
+    if (tokens > 0 && r.rows == 0) return fail(H3Q_ERR_INVALID, "%s: tables without rows", who);
+    if (!aligned(r.cos, 4) || !aligned(r.sin, 4) || !aligned(r.positions, r.positions_i64 ? 8 : 4))
+        return fail(H3Q_ERR_INVALID, "%s: misaligned tables or positions", who);
+    return H3Q_OK;
+}
+
+static int check_head_call(const char* who, int dtype, int weight_dtype, int64_t tokens, int64_t head_dim) {
+    if (dtype != H3Q_DTYPE_BF16 && dtype != H3Q_DTYPE_F16 && dtype != H3Q_DTYPE_F32)
+        return fail(H3Q_ERR_INVALID, "%s: unknown dtype %d", who, dtype);
+    if (weight_dtype != dtype && weight_dtype != H3Q_DTYPE_F32)
+        return fail(H3Q_ERR_INVALID, "%s: the norm's weights are of the rows' dtype or binary32", who);
+    if (tokens < 0 || tokens >= (int64_t(1) << 31))
+        return fail(H3Q_ERR_INVALID, "%s: %lld tokens", who, (long long)tokens);
+    if (head_dim <= 0 || head_dim % 2 || head_dim > h3q::kHeadMaxDim)
+        return fail(H3Q_ERR_UNSUPPORTED, "%s: head_dim=%lld must be even and at most %d", who, (long long)head_dim,
+                    h3q::kHeadMaxDim);
+    return H3Q_OK;
+}
+
+static h3q::HeadSegment head_segment(const h3q_heads& h, int dest, bool rotate) {
+    h3q::HeadSegment s{};
+    s.x = h.x;
+    s.token_stride = h.token_stride;
+    s.head_stride = h.head_stride;
+    s.weight = h.weight;
+    s.weight_stride = h.weight_stride;
+    s.out = h.out;
+    s.out_token_stride = h.out_token_stride;
+    s.out_head_stride = h.out_head_stride;
+    s.heads = (int)h.heads;
+    s.dest = dest;
+    s.rotate = rotate;
+    return s;
+}
+
+static h3q::HeadArgs head_args(int dtype, int weight_dtype, int64_t tokens, int64_t head_dim, float eps,
+                               const h3q_rotation* r) {
+    h3q::HeadArgs a{};
+    a.d = (int)head_dim;
+    a.tokens = tokens;
+    a.eps = eps;
+    a.weight_f32 = weight_dtype == H3Q_DTYPE_F32;
+    if (r) {
+        a.half = (int)(r->rot_dim / 2);
+        a.interleaved = r->interleaved != 0;
+        a.inverse = r->inverse != 0;
+        a.cos = r->cos;
+        a.sin = r->sin;
+        a.table_rows = r->rows;
+        a.positions = r->positions;
+        a.positions_i64 = r->positions_i64 != 0;
+    }
+    return a;
+}
+
+__attribute__((visibility("default"))) int h3q_rotary_tables(const void* positions, int type, int64_t n,
+                                                             const double* frequencies, int64_t half, double magnitude,
+                                                             float* cos_out, float* sin_out, void* stream) {
+    const char* who = "h3q_rotary_tables";
+    if (type < H3Q_POSITIONS_I32 || type > H3Q_POSITIONS_F64)
+        return fail(H3Q_ERR_INVALID, "%s: unknown type of positions %d", who, type);
+    if (n < 0 || half <= 0 || half > h3q::kHeadMaxDim / 2)
+        return fail(H3Q_ERR_INVALID, "%s: tables [%lld, %lld]", who, (long long)n, (long long)half);
+    if (n >= (int64_t(1) << 31) / half)
+        return fail(H3Q_ERR_UNSUPPORTED, "%s: tables [%lld, %lld] of 2^31 values or more", who, (long long)n,
+                    (long long)half);
+    if (n == 0) return ok();
+    if (!positions || !frequencies || !cos_out || !sin_out) return fail(H3Q_ERR_INVALID, "%s: null pointer", who);
+    const int size = type == H3Q_POSITIONS_I32 || type == H3Q_POSITIONS_F32 ? 4 : 8;
+    if (!aligned(positions, size) || !aligned(frequencies, 8) || !aligned(cos_out, 4) || !aligned(sin_out, 4))
+        return fail(H3Q_ERR_INVALID, "%s: misaligned pointer", who);
+    return check_launch(h3q::launch_rotary_tables(positions, type, n, frequencies, (int)half, magnitude, cos_out,
+                                                  sin_out, (hipStream_t)stream),
+                        who);
+}
+
+__attribute__((visibility("default"))) int h3q_rotary(int dtype, const h3q_heads* x, int64_t tokens, int64_t head_dim,
+                                                      const h3q_rotation* rotation, void* stream) {
+    const char* who = "h3q_rotary";
+    if (!x || !rotation) return fail(H3Q_ERR_INVALID, "%s: null argument", who);
+    int rc = check_head_call(who, dtype, dtype, tokens, head_dim);
+    if (rc == H3Q_OK) rc = check_heads(who, "x", *x, tokens, dtype == H3Q_DTYPE_F32 ? 4 : 2, true);
+    if (rc == H3Q_OK) rc = check_rotation(who, *rotation, tokens, head_dim);
+    if (rc != H3Q_OK) return rc;
+    if (x->weight) return fail(H3Q_ERR_INVALID, "%s: a weight without a norm", who);
+    if (tokens == 0 || x->heads == 0) return ok();
+    h3q::HeadArgs a = head_args(dtype, dtype, tokens, head_dim, 0.0f, rotation);
+    a.seg[a.segments++] = head_segment(*x, h3q::kDestRows, true);
+    return check_launch(h3q::launch_head_rotary(dtype, a, (hipStream_t)stream), who);
+}
+
+__attribute__((visibility("default"))) int h3q_qk_norm_rotary(int dtype, int weight_dtype, const h3q_heads* q,
+                                                              const h3q_heads* k, int64_t tokens, int64_t head_dim,
+                                                              float eps, const h3q_rotation* rotation, void* stream) {
+    const char* who = "h3q_qk_norm_rotary";
+    if (!q || !k || !rotation) return fail(H3Q_ERR_INVALID, "%s: null argument", who);
+    const int size = dtype == H3Q_DTYPE_F32 ? 4 : 2;
+    int rc = check_head_call(who, dtype, weight_dtype, tokens, head_dim);
+    if (rc == H3Q_OK) rc = check_heads(who, "q", *q, tokens, size, true);
+    if (rc == H3Q_OK) rc = check_heads(who, "k", *k, tokens, size, true);
+    if (rc == H3Q_OK) rc = check_rotation(who, *rotation, tokens, head_dim);
+    if (rc != H3Q_OK) return rc;
+    h3q::HeadArgs a = head_args(dtype, weight_dtype, tokens, head_dim, eps, rotation);
+    for (const h3q_heads* h : {q, k})
+        if (h->heads > 0) a.seg[a.segments++] = head_segment(*h, h3q::kDestRows, true);
+    if (tokens == 0 || a.segments == 0) return ok();
+    return check_launch(h3q::launch_head_rotary(dtype, a, (hipStream_t)stream), who);
+}
+
+__attribute__((visibility("default"))) int h3q_plan_append(const int32_t* table, int64_t table_stride, int64_t seqs,
+                                                           int64_t columns, const int32_t* lengths, const int32_t* cu,
+                                                           int64_t tokens, int64_t page_size, int32_t* positions,
+                                                           int32_t* slots, void* stream) {
+    const char* who = "h3q_plan_append";
+    if (seqs < 0 || columns < 0 || columns > 0x7FFFFFFF || table_stride < columns || tokens < 0 ||
+        tokens >= (int64_t(1) << 31))
+        return fail(H3Q_ERR_INVALID, "%s: %lld tokens, table [%lld, %lld] with %lld between rows", who,
+                    (long long)tokens, (long long)seqs, (long long)columns, (long long)table_stride);
+    if (page_size < 1 || page_size >= (int64_t(1) << 31))
+        return fail(H3Q_ERR_INVALID, "%s: page_size=%lld", who, (long long)page_size);
+    if (tokens == 0) return ok();
+    if ((seqs > 0 && (!lengths || (columns > 0 && !table))) || !cu || !positions || !slots)
+        return fail(H3Q_ERR_INVALID, "%s: null pointer", who);
+    h3q::PlanAppendArgs a{};
+    a.table = table;
+    a.lengths = lengths;
+    a.cu = cu;
+    a.table_stride = table_stride;
+    a.seqs = seqs;
+    a.tokens = tokens;
+    a.columns = (int)columns;
+    a.page_size = (int)page_size;
+    a.positions = positions;
+    a.slots = slots;
+    return check_launch(h3q::launch_plan_append(a, (hipStream_t)stream), who);
+}
+
+static int check_pages(const char* who, const char* what, const h3q_pages& p, int64_t size) {
+    if (p.kind < H3Q_PAGES_ROWS || p.kind > H3Q_PAGES_BY_ROW)
+        return fail(H3Q_ERR_INVALID, "%s: unknown kind of %s pages %d", who, what, p.kind);
+    if (p.n_pages < 0 || p.page_size < 1 || p.n_pages >= (int64_t(1) << 31) ||
+        p.page_size >= (int64_t(1) << 31) || p.n_pages * p.page_size >= (int64_t(1) << 31))
+        return fail(H3Q_ERR_UNSUPPORTED, "%s: %lld %s pages of %lld tokens (below 2^31 tokens in all)", who,
+                    (long long)p.n_pages, what, (long long)p.page_size);
+    if (p.n_pages > 0 && !p.pages) return fail(H3Q_ERR_INVALID, "%s: null %s pages", who, what);
+    if (!aligned(p.pages, p.kind == H3Q_PAGES_ROWS ? size : 1) || !aligned(p.scale, 4))
+        return fail(H3Q_ERR_INVALID, "%s: misaligned %s pages or scales", who, what);
+    if (p.kind != H3Q_PAGES_ROWS && p.n_pages > 0 && !p.scale)
+        return fail(H3Q_ERR_INVALID, "%s: e4m3fn %s pages need scales", who, what);
+    return H3Q_OK;
+}
+
+__attribute__((visibility("default"))) int h3q_append_kv(int dtype, int weight_dtype, const h3q_heads* q,
+                                                         const h3q_heads* k, const h3q_heads* v,
+                                                         const h3q_pages* k_pages, const h3q_pages* v_pages,
+                                                         const int32_t* slots, int64_t tokens, int64_t head_dim,
+                                                         float eps, const h3q_rotation* rotation, void* stream) {
+    const char* who = "h3q_append_kv";
+    if (!k || !v || !k_pages || !v_pages) return fail(H3Q_ERR_INVALID, "%s: null argument", who);
+    const int size = dtype == H3Q_DTYPE_F32 ? 4 : 2;
+    int rc = check_head_call(who, dtype, weight_dtype, tokens, head_dim);
+    if (rc == H3Q_OK && q) rc = check_heads(who, "q", *q, tokens, size, true);
+    if (rc == H3Q_OK) rc = check_heads(who, "k", *k, tokens, size, false);
+    if (rc == H3Q_OK) rc = check_heads(who, "v", *v, tokens, size, false);
+    if (rc == H3Q_OK) rc = check_pages(who, "k", *k_pages, size);
+    if (rc == H3Q_OK) rc = check_pages(who, "v", *v_pages, size);
+    if (rc == H3Q_OK && rotation) rc = check_rotation(who, *rotation, tokens, head_dim);
+    if (rc != H3Q_OK) return rc;
+    if (k->heads != v->heads)
+        return fail(H3Q_ERR_INVALID, "%s: %lld k heads and %lld v heads", who, (long long)k->heads, (long long)v->heads);
+    if (v->weight) return fail(H3Q_ERR_INVALID, "%s: values have no norm", who);
+    if (tokens == 0) return ok();
+    if (!slots || !aligned(slots, 4)) return fail(H3Q_ERR_INVALID, "%s: null or misaligned slots", who);
+    h3q::HeadArgs a = head_args(dtype, weight_dtype, tokens, head_dim, eps, rotation);
+    a.slots = slots;
+    if (q && q->heads > 0) a.seg[a.segments++] = head_segment(*q, h3q::kDestRows, rotation != nullptr);
+    for (int i = 0; i < 2 && k->heads > 0; ++i) {
+        const h3q_pages& p = i ? *v_pages : *k_pages;
+        h3q::HeadSegment s = head_segment(i ? *v : *k, h3q::kDestPages + p.kind, i == 0 && rotation != nullptr);
+        s.out = nullptr;
+        s.cache.pages = p.pages;
+        s.cache.page_stride = p.page_stride;
+        s.cache.slot_stride = p.slot_stride;
+        s.cache.head_stride = p.head_stride;
+        s.cache.slots = (int)(p.n_pages * p.page_size);
+        s.cache.page_size = (int)p.page_size;
+        s.cache.scale = p.scale;
+        s.cache.scale_page_stride = p.scale_page_stride;
+        s.cache.scale_slot_stride = p.scale_slot_stride;
+        s.cache.scale_head_stride = p.scale_head_stride;
+        a.seg[a.segments++] = s;
+    }
+    if (a.segments == 0) return ok();
+    return check_launch(h3q::launch_head_rotary(dtype, a, (hipStream_t)stream), who);
+}
+
 }  // extern "C"

@@ -275,4 +275,51 @@ int64_t expert_ffn_workspace_bytes(const ExpertFfnArgs& a);
 bool expert_ffn_fits(const ExpertFfnArgs& a);
 hipError_t launch_expert_ffn(const ExpertFfnArgs& a, void* workspace, hipStream_t st);
 
+// Rotary positions, head norms and the append to a paged cache (head_rotary.hip).
+enum HeadDest : int { kDestRows = 0, kDestPages = 1, kDestStatic = 2, kDestRowScale = 3 };
+enum PositionType : int { kPositionsI32 = 0, kPositionsI64 = 1, kPositionsF32 = 2, kPositionsF64 = 3 };
+struct HeadCache {
+    void* pages;
+    int64_t page_stride, slot_stride, head_stride;  // elements of a page's type
+    int slots, page_size;                           // pages * page_size
+    float* scale;  // e4m3 pages: [heads] (kDestStatic) or [pages, page_size, heads] (kDestRowScale)
+    int64_t scale_page_stride, scale_slot_stride, scale_head_stride;
+};
+struct HeadSegment {  // rows [tokens, heads, d] and where they go
+    const void* x;
+    int64_t token_stride, head_stride;
+    const void* weight;  // of the norm, [d] (weight_stride 0) or [heads, d]; null: no norm
+    int64_t weight_stride;
+    void* out;  // kDestRows
+    int64_t out_token_stride, out_head_stride;
+    HeadCache cache;  // the others
+    int heads, dest, rotate;
+    int units;  // waves a token (set by the launch)
+};
+struct HeadArgs {
+    HeadSegment seg[3];
+    int segments, d, half;  // half: pairs that are rotated (0: none)
+    int64_t tokens;
+    float eps;
+    int weight_f32, interleaved, inverse;
+    const float *cos, *sin;  // [table_rows, half]
+    int64_t table_rows;
+    const void* positions;  // row of the tables for each token (null: its own number), below 0: padding
+    int positions_i64;
+    const int* slots;
+    int lanes;  // of a row (set by the launch)
+};
+constexpr int kHeadMaxDim = 512;
+constexpr int kHeadMaxHeads = 16384;  // three segments of one row a wave stay within a grid's 65535
+hipError_t launch_head_rotary(int dtype, const HeadArgs& a, hipStream_t st);
+hipError_t launch_rotary_tables(const void* positions, int type, int64_t n, const double* frequencies, int half,
+                                double magnitude, float* cos_out, float* sin_out, hipStream_t st);
+struct PlanAppendArgs {
+    const int *table, *lengths, *cu;  // [seqs, columns], [seqs], [seqs + 1]
+    int64_t table_stride, seqs, tokens;
+    int columns, page_size;
+    int *positions, *slots;
+};
+hipError_t launch_plan_append(const PlanAppendArgs& a, hipStream_t st);
+
 }  // namespace h3q

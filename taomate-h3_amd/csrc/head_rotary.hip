@@ -1,0 +1,422 @@
+// What stands between the qkv product and the attention, gfx950: rotary positions, the RMS norm of
+// each query and key head, and the append of keys and values to a paged cache.
+//
+//   n  = x * (1 / sqrt(sum(x * x) / d + eps)) * weight            (rows with a norm)
+//   (a, b) -> (a cos - b sin, a sin + b cos)                      (the first 2 * half channels, pair by pair)
+//   q  = e4m3(clamp(y * (1 / s), +-448)), s a head's own or max(max|y| / 448, 1e-12) of the row   (e4m3 pages)
+//
+// All of it in binary32 on the values as they are, rounded once where the row is stored.
+//
+// Bound by the rows' bytes, so one pass: a row of d channels belongs to G lanes (the power of two that
+// holds d / (2 V)), each with V pairs of one 16-byte vector per side, and a wave takes 64 / G heads of one
+// token at a time.  The token's cosines and sines (fp32: as many bytes as two bf16 rows) and the norm's
+// weights stay in registers over the HEADS * 64 / G heads of the wave; its HEADS vectors are asked for
+// together, ahead of the first use.  The lanes that own a row read all of it before they store any of it,
+// so a call may run in place.
+//
+// Pairs: (i, half + i), where a lane's two vectors are those at c V and half + c V, or (2 i, 2 i + 1), where
+// they are neighbours.  Channels from 2 * half on go through as they are (a select, not a rotation by zero:
+// 0 * inf would be a NaN).
+#include "h3q_common.hpp"
+#include "h3q_kernels.hpp"
+
+namespace h3q {
+
+namespace {
+
+template <int DT>
+struct Elem;
+template <>
+struct Elem<kInBF16> {
+    using T = uint16_t;
+    static __device__ __forceinline__ float up(T v) { return __uint_as_float((uint32_t)v << 16); }
+    static __device__ __forceinline__ T down(float v) { return (T)pack_bf16x2(v, 0.0f); }
+};
+template <>
+struct Elem<kInF16> {
+    using T = uint16_t;
+    static __device__ __forceinline__ float up(T v) { return (float)__builtin_bit_cast(_Float16, v); }
+    static __device__ __forceinline__ T down(float v) { return __builtin_bit_cast(uint16_t, (_Float16)v); }
+};
+template <>
+struct Elem<kInF32> {
+    using T = float;
+    static __device__ __forceinline__ float up(T v) { return v; }
+    static __device__ __forceinline__ T down(float v) { return v; }
+};
+
+template <typename T, int V>
+struct Vec {
+    typedef T type __attribute__((ext_vector_type(V)));
+};
+template <typename T>
+struct Vec<T, 1> {
+    typedef T type;
+};
+template <typename T, int V>
+__device__ __forceinline__ T at(const typename Vec<T, V>::type& v, int i) {
+    if constexpr (V == 1) return v;
+    else return v[i];
+}
+
+// Sum, and largest magnitude (bits; a NaN above all), over the G lanes of a row.
+__device__ __forceinline__ float row_sum(float v, int lanes) {
+    for (int off = lanes >> 1; off >= 1; off >>= 1) v += __shfl_xor(v, off, 64);
+    return v;
+}
+__device__ __forceinline__ float row_max(float v, int lanes) {
+    for (int off = lanes >> 1; off >= 1; off >>= 1) v = mag_max(v, __shfl_xor(v, off, 64));
+    return v;
+}
+
+// V binary32 values -> V e4m3 codes at p.
+template <int V>
+__device__ __forceinline__ void store_codes(uint8_t* p, const float (&y)[V]) {
+    if constexpr (V == 1) {
+        *p = (uint8_t)cvt_e4m3x2(y[0], 0.0f);
+    } else {
+        uint32_t w[V / 4];
+#pragma unroll
+        for (int i = 0; i < V / 4; ++i)
+            w[i] = cvt_e4m3x2(y[4 * i], y[4 * i + 1]) | (cvt_e4m3x2(y[4 * i + 2], y[4 * i + 3]) << 16);
+        if constexpr (V == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+        else *reinterpret_cast<uint32_t*>(p) = w[0];
+    }
+}
+
+// DT: the rows' type.  V: channels a vector.  NC: chunks of 2 V channels a lane (1, or 4 at V = 1).
+// HEADS: rows a lane group takes.  INTER: interleaved pairs.
+template <int DT, int V, int NC, int HEADS, bool INTER>
+__global__ __launch_bounds__(256) void head_rotary_kernel(HeadArgs p) {
+    using E = Elem<DT>;
+    using T = typename E::T;
+    using VT = typename Vec<T, V>::type;
+    using VF = typename Vec<float, V>::type;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t token = (int64_t)blockIdx.x * 4 + wave;
+    if (token >= p.tokens) return;
+    int unit = blockIdx.y, which = 0;
+    while (which + 1 < p.segments && unit >= p.seg[which].units) unit -= p.seg[which++].units;
+    const HeadSegment& s = p.seg[which];
+
+    int64_t pos = token;
+    if (p.positions) pos = p.positions_i64 ? ((const int64_t*)p.positions)[token] : ((const int32_t*)p.positions)[token];
+    if (pos < 0) return;  // padding: its rows are left as they were
+    int64_t page = 0;
+    int place = 0;
+    if (s.dest != kDestRows) {
+        const int slot = p.slots[token];
+        if (slot < 0 || slot >= s.cache.slots) return;  // no page for it
+        page = slot / s.cache.page_size;
+        place = slot - (int)page * s.cache.page_size;
+    }
+
+    const int g = lane & (p.lanes - 1), rows = 64 / p.lanes;  // this lane of a row; rows of a wave at a time
+    const int head0 = unit * rows * HEADS + lane / p.lanes;
+    const int turned = s.rotate ? p.half / V : 0;  // chunks that are rotated; the others lie behind 2 * half
+    const int chunks = p.d / (2 * V);
+    int off[NC][2];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        const int chunk = g + c * 64;
+        const bool apart = !INTER && chunk < turned;
+        off[c][0] = apart ? chunk * V : chunk * 2 * V;
+        // a head without rotation is read as one run, whatever the pairs
+        off[c][1] = apart ? p.half + chunk * V : chunk * 2 * V + V;
+    }
+
+    VT raw[HEADS][NC][2];
+    const T* const x = (const T*)s.x + token * s.token_stride;
+#pragma unroll
+    for (int h = 0; h < HEADS; ++h) {
+        const int head = head0 + h * rows;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const bool in = head < s.heads && g + c * 64 < chunks;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                raw[h][c][i] = in ? *reinterpret_cast<const VT*>(x + head * s.head_stride + off[c][i]) : VT{};
+        }
+    }
+
+    VF cs[NC], sn[NC];
+    if (s.rotate) {
+        const bool known = pos < p.table_rows;  // a position past the table gives NaN, never another one's angle
+        const int64_t row = (known ? pos : 0) * p.half;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int chunk = g + c * 64;
+            cs[c] = VF{};
+            sn[c] = VF{};
+            if (chunk < turned) {
+                cs[c] = *reinterpret_cast<const VF*>(p.cos + row + chunk * V);
+                sn[c] = *reinterpret_cast<const VF*>(p.sin + row + chunk * V);
+                if (!known) cs[c] = sn[c] = VF{} + __builtin_nanf("");
+                if (p.inverse) sn[c] = -sn[c];
+            }
+        }
+    }
+
+    float w[NC][2][V];
+    auto load_weight = [&](int head) __attribute__((always_inline)) {
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const bool in = head < s.heads && g + c * 64 < chunks;
+                const int64_t o = head * s.weight_stride + off[c][i];
+                if (p.weight_f32) {
+                    const VF v = in ? *reinterpret_cast<const VF*>((const float*)s.weight + o) : VF{};
+#pragma unroll
+                    for (int e = 0; e < V; ++e) w[c][i][e] = at<float, V>(v, e);
+                } else {
+                    const VT v = in ? *reinterpret_cast<const VT*>((const T*)s.weight + o) : VT{};
+#pragma unroll
+                    for (int e = 0; e < V; ++e) w[c][i][e] = E::up(at<T, V>(v, e));
+                }
+            }
+    };
+    if (s.weight && s.weight_stride == 0) load_weight(0);
+
+#pragma unroll
+    for (int h = 0; h < HEADS; ++h) {
+        if (unit * rows * HEADS + h * rows >= s.heads) break;  // the wave's last rows
+        const int head = head0 + h * rows;
+        float y[NC][2][V];
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int e = 0; e < V; ++e) y[c][i][e] = E::up(at<T, V>(raw[h][c][i], e));
+        if (s.weight) {
+            if (s.weight_stride != 0) load_weight(head);
+            float ss = 0.0f;
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int e = 0; e < V; ++e) ss = __builtin_fmaf(y[c][i][e], y[c][i][e], ss);
+            ss = row_sum(ss, p.lanes);
+            const float rs = 1.0f / __builtin_sqrtf(ss / (float)p.d + p.eps);
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int e = 0; e < V; ++e) y[c][i][e] = y[c][i][e] * rs * w[c][i][e];
+        }
+        if (s.rotate) {
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                const bool turn = g + c * 64 < turned;
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    // interleaved: pair e of the 2 V neighbours is (2 e, 2 e + 1)
+                    float& a = INTER ? y[c][2 * e / V][2 * e % V] : y[c][0][e];
+                    float& b = INTER ? y[c][(2 * e + 1) / V][(2 * e + 1) % V] : y[c][1][e];
+                    const float co = at<float, V>(cs[c], e), si = at<float, V>(sn[c], e);
+                    const float ra = __builtin_fmaf(a, co, -(b * si)), rb = __builtin_fmaf(a, si, b * co);
+                    a = turn ? ra : a;
+                    b = turn ? rb : b;
+                }
+            }
+        }
+        float r = 1.0f;
+        if (s.dest == kDestStatic) {
+            r = 1.0f / s.cache.scale[head < s.heads ? head * s.cache.scale_head_stride : 0];
+        } else if (s.dest == kDestRowScale) {
+            float m = 0.0f;
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int e = 0; e < V; ++e) m = mag_max(m, __builtin_fabsf(y[c][i][e]));
+            const float scale = amax_scale(row_max(m, p.lanes), kE4M3Recip);
+            r = 1.0f / scale;
+            if (g == 0 && head < s.heads)
+                s.cache.scale[page * s.cache.scale_page_stride + place * s.cache.scale_slot_stride +
+                              head * s.cache.scale_head_stride] = scale;
+        }
+        if (head >= s.heads) continue;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            if (g + c * 64 >= chunks) continue;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                if (s.dest >= kDestStatic) {
+                    float q[V];
+#pragma unroll
+                    for (int e = 0; e < V; ++e) q[e] = clamp_e4m3(y[c][i][e] * r);
+                    uint8_t* const to = (uint8_t*)s.cache.pages + page * s.cache.page_stride +
+                                        place * s.cache.slot_stride + head * s.cache.head_stride;
+                    store_codes<V>(to + off[c][i], q);
+                } else {
+                    VT v;
+#pragma unroll
+                    for (int e = 0; e < V; ++e) {
+                        if constexpr (V == 1) v = E::down(y[c][i][e]);
+                        else v[e] = E::down(y[c][i][e]);
+                    }
+                    T* const to = s.dest == kDestRows
+                                      ? (T*)s.out + token * s.out_token_stride + head * s.out_head_stride
+                                      : (T*)s.cache.pages + page * s.cache.page_stride + place * s.cache.slot_stride +
+                                            head * s.cache.head_stride;
+                    *reinterpret_cast<VT*>(to + off[c][i]) = v;
+                }
+            }
+        }
+    }
+}
+
+// cos and sin of position * frequency, times magnitude.  The angle is a binary64 product (positions of
+// millions lose 1e-10 of a turn), taken to turns and reduced to half a turn there; the rest is binary32.
+// V values a thread.
+template <typename P, int V>
+__global__ __launch_bounds__(256) void rotary_tables_kernel(const P* positions, const double* frequencies, int64_t n,
+                                                            int half, double magnitude, float* cos_out,
+                                                            float* sin_out) {
+    using VF = typename Vec<float, V>::type;
+    const uint32_t i = blockIdx.x * 256u + threadIdx.x;
+    const uint32_t per = (uint32_t)half / V;
+    if (i >= (uint32_t)n * per) return;
+    const uint32_t row = i / per, col = (i - row * per) * V;
+    const double position = (double)positions[row];
+    VF c, s;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+        const double turns = position * frequencies[col + e] * 0.15915494309189533577;
+        const float part = 2.0f * (float)(turns - __builtin_rint(turns));
+        float si, co;
+        sincospif(part, &si, &co);
+        if constexpr (V == 1) {
+            c = co * (float)magnitude;
+            s = si * (float)magnitude;
+        } else {
+            c[e] = co * (float)magnitude;
+            s[e] = si * (float)magnitude;
+        }
+    }
+    *reinterpret_cast<VF*>(cos_out + (int64_t)row * half + col) = c;
+    *reinterpret_cast<VF*>(sin_out + (int64_t)row * half + col) = s;
+}
+
+// Position and slot of each token of a step, one thread a token: the last sequence whose first token is
+// not behind it (sequences without tokens share their bound with the next), by bisection.
+__global__ __launch_bounds__(256) void plan_append_kernel(PlanAppendArgs p) {
+    const int64_t token = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (token >= p.tokens) return;
+    int position = -1, slot = -1;
+    if (token >= p.cu[0] && token < p.cu[p.seqs]) {
+        int64_t lo = 0, hi = p.seqs;  // cu[lo] <= token < cu[hi]
+        while (hi - lo > 1) {
+            const int64_t mid = (lo + hi) >> 1;
+            if (p.cu[mid] <= token) lo = mid;
+            else hi = mid;
+        }
+        const int64_t at = (int64_t)p.lengths[lo] + token - p.cu[lo];
+        if (at >= 0 && at <= 0x7FFFFFFF) {
+            position = (int)at;
+            const int column = position / p.page_size;
+            if (column < p.columns) {
+                const int page = p.table[lo * p.table_stride + column];
+                const int64_t to = (int64_t)page * p.page_size + position % p.page_size;
+                if (page >= 0 && to <= 0x7FFFFFFF) slot = (int)to;
+            }
+        }
+    }
+    p.positions[token] = position;
+    p.slots[token] = slot;
+}
+
+template <int DT, int V, int NC, int HEADS>
+hipError_t launch_heads_cfg(const HeadArgs& a, int units, hipStream_t st) {
+    const dim3 grid((unsigned)((a.tokens + 3) / 4), (unsigned)units);
+    if (a.interleaved) hipLaunchKernelGGL((head_rotary_kernel<DT, V, NC, HEADS, true>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((head_rotary_kernel<DT, V, NC, HEADS, false>), grid, dim3(256), 0, st, a);
+    return hipGetLastError();
+}
+
+template <int DT, int V, int NC>
+hipError_t launch_heads_vec(HeadArgs a, hipStream_t st) {
+    a.lanes = 1;
+    while (a.lanes < 64 && a.lanes * 2 * V < a.d) a.lanes *= 2;
+    const int rows = 64 / a.lanes;
+    // Four rows a lane group where that still leaves the chip enough waves; one for a few tokens.
+    auto units = [&](int heads) {
+        int sum = 0;
+        for (int i = 0; i < a.segments; ++i) sum += a.seg[i].units = (a.seg[i].heads + rows * heads - 1) / (rows * heads);
+        return sum;
+    };
+    if (a.tokens * units(4) >= 4096) return launch_heads_cfg<DT, V, NC, 4>(a, units(4), st);
+    return launch_heads_cfg<DT, V, NC, 1>(a, units(1), st);
+}
+
+template <int DT>
+hipError_t launch_heads_type(const HeadArgs& a, int vec, hipStream_t st) {
+    if constexpr (DT != kInF32) {
+        if (vec == 8) return launch_heads_vec<DT, 8, 1>(a, st);
+    }
+    if (vec >= 4) return launch_heads_vec<DT, 4, 1>(a, st);
+    return launch_heads_vec<DT, 1, 4>(a, st);
+}
+
+// Whether every vector of V channels of the call is whole and aligned.
+bool vectors_fit(const HeadArgs& a, int size, int v) {
+    const auto fits = [&](const void* p, int64_t bytes) { return (uintptr_t)p % bytes == 0; };
+    if (a.d % (2 * v) || a.half % v) return false;
+    if (a.cos && (!fits(a.cos, v >= 4 ? 16 : 4) || !fits(a.sin, v >= 4 ? 16 : 4))) return false;
+    for (int i = 0; i < a.segments; ++i) {
+        const HeadSegment& s = a.seg[i];
+        if (!fits(s.x, v * size) || s.token_stride % v || s.head_stride % v) return false;
+        const int wsize = a.weight_f32 ? 4 : size;
+        if (s.weight && (!fits(s.weight, v * wsize < 16 ? v * wsize : 16) || s.weight_stride % v)) return false;
+        if (s.dest == kDestRows) {
+            if (!fits(s.out, v * size) || s.out_token_stride % v || s.out_head_stride % v) return false;
+        } else if (!fits(s.cache.pages, v * (s.dest >= kDestStatic ? 1 : size)) || s.cache.page_stride % v ||
+                   s.cache.slot_stride % v || s.cache.head_stride % v) {
+            return false;
+        }
+    }
+    return true;
+}
+
+}  // namespace
+
+hipError_t launch_head_rotary(int dtype, const HeadArgs& a, hipStream_t st) {
+    const int size = dtype == kInF32 ? 4 : 2;
+    const int vec = dtype != kInF32 && vectors_fit(a, size, 8) ? 8 : vectors_fit(a, size, 4) ? 4 : 1;
+    if (dtype == kInBF16) return launch_heads_type<kInBF16>(a, vec, st);
+    if (dtype == kInF16) return launch_heads_type<kInF16>(a, vec, st);
+    return launch_heads_type<kInF32>(a, vec, st);
+}
+
+hipError_t launch_rotary_tables(const void* positions, int type, int64_t n, const double* frequencies, int half,
+                                double magnitude, float* cos_out, float* sin_out, hipStream_t st) {
+    const int v = half % 4 == 0 && ((uintptr_t)cos_out | (uintptr_t)sin_out) % 16 == 0 ? 4 : 1;
+    const unsigned blocks = (unsigned)((n * (half / v) + 255) / 256);
+    auto go = [&](auto* at) {
+        using P = std::remove_pointer_t<decltype(at)>;
+        if (v == 4)
+            hipLaunchKernelGGL((rotary_tables_kernel<P, 4>), dim3(blocks), dim3(256), 0, st, (const P*)positions,
+                               frequencies, n, half, magnitude, cos_out, sin_out);
+        else
+            hipLaunchKernelGGL((rotary_tables_kernel<P, 1>), dim3(blocks), dim3(256), 0, st, (const P*)positions,
+                               frequencies, n, half, magnitude, cos_out, sin_out);
+    };
+    if (type == kPositionsI32) go((int32_t*)nullptr);
+    else if (type == kPositionsI64) go((int64_t*)nullptr);
+    else if (type == kPositionsF32) go((float*)nullptr);
+    else go((double*)nullptr);
+    return hipGetLastError();
+}
+
+hipError_t launch_plan_append(const PlanAppendArgs& a, hipStream_t st) {
+    hipLaunchKernelGGL(plan_append_kernel, dim3((unsigned)((a.tokens + 255) / 256)), dim3(256), 0, st, a);
+    return hipGetLastError();
+}
+
+}  // namespace h3q

@@ -368,6 +368,223 @@ Opt expert_ffn(const Tensor& x, const Tensor& experts, const Tensor& weights, co
     return out;
 }
 
+// ---- rotary positions, head norms, paged cache
+
+bool head_rows(const Tensor& t, const Tensor& first, at::ScalarType type) {
+    return on(t, first) && t.scalar_type() == type && t.dim() == 3 && (t.size(2) <= 1 || t.stride(2) == 1);
+}
+
+// Whether no two elements share memory.
+bool apart(const Tensor& t) {
+    int64_t stride[4], size[4], n = 0;
+    if (t.dim() > 4) return false;
+    for (int64_t i = 0; i < t.dim(); ++i) {
+        if (t.size(i) <= 1) continue;
+        int64_t at = n++;
+        for (; at > 0 && stride[at - 1] > t.stride(i); --at) stride[at] = stride[at - 1], size[at] = size[at - 1];
+        stride[at] = t.stride(i), size[at] = t.size(i);
+    }
+    int64_t reach = 0;
+    for (int64_t i = 0; i < n; ++i) {
+        if (stride[i] <= reach) return false;
+        reach += stride[i] * (size[i] - 1);
+    }
+    return true;
+}
+
+// The rows, their norm's weights and where they go; false: something is out of the ordinary.
+bool heads_of(h3q_heads& h, const Tensor& x, const Opt& weight, const Tensor* out, int& weight_dtype) {
+    const int64_t heads = x.size(1), d = x.size(2);
+    h = {};
+    h.x = x.data_ptr();
+    h.token_stride = x.stride(0);
+    h.head_stride = x.stride(1);
+    h.heads = heads;
+    if (weight) {
+        const at::ScalarType type = weight->scalar_type();
+        if (!on(*weight, x) || (type != x.scalar_type() && type != at::kFloat)) return false;
+        const int kind = logit_type(type);
+        if (weight_dtype >= 0 && weight_dtype != kind) return false;
+        weight_dtype = kind;
+        const bool each = weight->dim() == 2 && weight->size(0) == heads && weight->size(1) == d;
+        if (!each && !(weight->dim() == 1 && weight->size(0) == d)) return false;
+        if (d > 1 && weight->stride(-1) != 1) return false;
+        h.weight = weight->data_ptr();
+        h.weight_stride = each ? weight->stride(0) : 0;
+    }
+    if (out) {
+        h.out = out->data_ptr();
+        h.out_token_stride = out->stride(0);
+        h.out_head_stride = out->stride(1);
+    }
+    return true;
+}
+
+bool rotation_of(h3q_rotation& r, const Tensor& x, const Tensor& cos, const Tensor& sin, const Opt& positions,
+                 bool interleaved, bool inverse) {
+    if (!dense(cos, x, at::kFloat) || !dense(sin, x, at::kFloat) || cos.dim() != 2 || sin.sizes() != cos.sizes())
+        return false;
+    r = {};
+    r.cos = floats(cos);
+    r.sin = floats(sin);
+    r.rows = cos.size(0);
+    r.rot_dim = 2 * cos.size(1);
+    r.interleaved = interleaved;
+    r.inverse = inverse;
+    if (positions) {
+        const at::ScalarType type = positions->scalar_type();
+        if ((type != at::kInt && type != at::kLong) || !dense(*positions, x, type) || positions->dim() != 1 ||
+            positions->size(0) != x.size(0))
+            return false;
+        r.positions = positions->data_ptr();
+        r.positions_i64 = type == at::kLong;
+    }
+    return true;
+}
+
+// out as given, or a new tensor; false: it does not fit.
+bool rows_like(const Tensor& x, Opt& out) {
+    if (!out) {
+        out = empty(x, x.sizes(), x.scalar_type());
+        return true;
+    }
+    return head_rows(*out, x, x.scalar_type()) && out->sizes() == x.sizes() && apart(*out);
+}
+
+std::optional<Pair> rotary_tables(const Tensor& positions, const Tensor& frequencies, double magnitude, int64_t stream) {
+    const at::ScalarType type = positions.scalar_type();
+    const int kind = type == at::kInt     ? H3Q_POSITIONS_I32
+                     : type == at::kLong  ? H3Q_POSITIONS_I64
+                     : type == at::kFloat ? H3Q_POSITIONS_F32
+                     : type == at::kDouble ? H3Q_POSITIONS_F64
+                                           : -1;
+    if (!positions.is_cuda() || kind < 0 || !positions.is_contiguous() || positions.dim() != 1 ||
+        !dense(frequencies, positions, at::kDouble) || frequencies.dim() != 1 || positions.size(0) == 0)
+        return std::nullopt;
+    const int64_t n = positions.size(0), half = frequencies.size(0);
+    if (half < 1 || half > 256 || n >= (int64_t(1) << 31) / half) return std::nullopt;
+    const c10::DeviceGuard guard(positions.device());
+    const Tensor cos = empty(positions, {n, half}, at::kFloat), sin = empty(positions, {n, half}, at::kFloat);
+    if (h3q_rotary_tables(positions.data_ptr(), kind, n, static_cast<const double*>(frequencies.data_ptr()), half,
+                          magnitude, floats(cos), floats(sin), stream_of(stream)))
+        return std::nullopt;
+    return Pair(cos, sin);
+}
+
+Opt rotary(const Tensor& x, const Tensor& cos, const Tensor& sin, const Opt& positions, bool interleaved, bool inverse,
+           Opt out, int64_t stream) {
+    const int dtype = logit_type(x.scalar_type());
+    if (!x.is_cuda() || dtype < 0 || !head_rows(x, x, x.scalar_type()) || x.numel() == 0) return std::nullopt;
+    h3q_rotation r;
+    h3q_heads h;
+    int weight_dtype = -1;
+    if (!rotation_of(r, x, cos, sin, positions, interleaved, inverse)) return std::nullopt;
+    const c10::DeviceGuard guard(x.device());
+    if (!rows_like(x, out) || !heads_of(h, x, std::nullopt, &*out, weight_dtype)) return std::nullopt;
+    if (h3q_rotary(dtype, &h, x.size(0), x.size(2), &r, stream_of(stream))) return std::nullopt;
+    return out;
+}
+
+std::optional<Pair> qk_norm_rotary(const Tensor& q, const Tensor& k, const Opt& q_weight, const Opt& k_weight,
+                                   const Tensor& cos, const Tensor& sin, const Opt& positions, double eps,
+                                   bool interleaved, Opt q_out, Opt k_out, int64_t stream) {
+    const int dtype = logit_type(q.scalar_type());
+    if (!q.is_cuda() || dtype < 0 || !head_rows(q, q, q.scalar_type()) || q.numel() == 0 ||
+        !head_rows(k, q, q.scalar_type()) || k.size(0) != q.size(0) || k.size(2) != q.size(2))
+        return std::nullopt;
+    h3q_rotation r;
+    h3q_heads qh, kh;
+    int weight_dtype = -1;
+    if (!rotation_of(r, q, cos, sin, positions, interleaved, false)) return std::nullopt;
+    const c10::DeviceGuard guard(q.device());
+    if (!rows_like(q, q_out) || !rows_like(k, k_out) || !heads_of(qh, q, q_weight, &*q_out, weight_dtype) ||
+        !heads_of(kh, k, k_weight, &*k_out, weight_dtype))
+        return std::nullopt;
+    if (h3q_qk_norm_rotary(dtype, weight_dtype < 0 ? dtype : weight_dtype, &qh, &kh, q.size(0), q.size(2), (float)eps, &r,
+                           stream_of(stream)))
+        return std::nullopt;
+    return Pair(*q_out, *k_out);
+}
+
+std::optional<Pair> plan_append(const Tensor& table, const Tensor& lengths, const Tensor& cu, int64_t tokens,
+                                int64_t page_size, int64_t stream) {
+    if (!table.is_cuda() || !rows_2d(table, at::kInt) || !dense(lengths, table, at::kInt) || !dense(cu, table, at::kInt))
+        return std::nullopt;
+    const int64_t seqs = table.size(0), columns = table.size(1);
+    if (lengths.dim() != 1 || lengths.size(0) != seqs || cu.dim() != 1 || cu.size(0) != seqs + 1 || tokens < 1 ||
+        tokens >= (int64_t(1) << 31))
+        return std::nullopt;
+    const c10::DeviceGuard guard(table.device());
+    const Tensor positions = empty(table, {tokens}, at::kInt), slots = empty(table, {tokens}, at::kInt);
+    if (h3q_plan_append(ints(table), seqs > 1 ? table.stride(0) : columns, seqs, columns, ints(lengths), ints(cu), tokens,
+                        page_size, ints(positions), ints(slots), stream_of(stream)))
+        return std::nullopt;
+    return Pair(positions, slots);
+}
+
+bool pages_of(h3q_pages& p, const Tensor& x, const Tensor& pages, const Opt& scale) {
+    const int64_t heads = x.size(1), d = x.size(2);
+    const at::ScalarType type = pages.scalar_type();
+    if (!on(pages, x) || (type != x.scalar_type() && type != at::kFloat8_e4m3fn) || pages.dim() != 4 ||
+        pages.size(2) != heads || pages.size(3) != d || pages.stride(3) != 1 || !apart(pages))
+        return false;
+    p = {};
+    p.pages = pages.data_ptr();
+    p.n_pages = pages.size(0);
+    p.page_size = pages.size(1);
+    p.page_stride = pages.stride(0);
+    p.slot_stride = pages.stride(1);
+    p.head_stride = pages.stride(2);
+    p.kind = H3Q_PAGES_ROWS;
+    if ((type == at::kFloat8_e4m3fn) != scale.has_value()) return false;
+    if (!scale) return true;
+    if (!on(*scale, x) || scale->scalar_type() != at::kFloat) return false;
+    p.scale = floats(*scale);
+    if (scale->dim() == 1 && (scale->size(0) == 1 || scale->size(0) == heads)) {
+        p.kind = H3Q_PAGES_STATIC;
+        p.scale_head_stride = scale->size(0) > 1 ? scale->stride(0) : 0;
+        return true;
+    }
+    if (scale->dim() != 3 || scale->size(0) != p.n_pages || scale->size(1) != p.page_size || scale->size(2) != heads ||
+        !apart(*scale))
+        return false;
+    p.kind = H3Q_PAGES_BY_ROW;
+    p.scale_page_stride = scale->stride(0);
+    p.scale_slot_stride = scale->stride(1);
+    p.scale_head_stride = scale->stride(2);
+    return true;
+}
+
+// q's output (k where there is no q), or nothing.
+Opt append_kv(const Tensor& k, const Tensor& v, const Tensor& k_pages, const Tensor& v_pages, const Tensor& slots,
+              const Opt& k_scale, const Opt& v_scale, const Opt& k_weight, double eps, const Opt& cos, const Opt& sin,
+              const Opt& positions, bool interleaved, const Opt& q, const Opt& q_weight, Opt q_out, int64_t stream) {
+    const at::ScalarType type = k.scalar_type();
+    const int dtype = logit_type(type);
+    if (!k.is_cuda() || dtype < 0 || !head_rows(k, k, type) || k.numel() == 0 || !head_rows(v, k, type) ||
+        v.sizes() != k.sizes() || !dense(slots, k, at::kInt) || slots.dim() != 1 || slots.size(0) != k.size(0))
+        return std::nullopt;
+    if (cos.has_value() != sin.has_value() || (positions && !cos) || (!q && (q_weight || q_out))) return std::nullopt;
+    h3q_rotation r;
+    if (cos && !rotation_of(r, k, *cos, *sin, positions, interleaved, false)) return std::nullopt;
+    h3q_heads qh, kh, vh;
+    h3q_pages kp, vp;
+    int weight_dtype = -1;
+    const c10::DeviceGuard guard(k.device());
+    if (q) {
+        if (!head_rows(*q, k, type) || q->size(0) != k.size(0) || q->size(2) != k.size(2) || !rows_like(*q, q_out) ||
+            !heads_of(qh, *q, q_weight, &*q_out, weight_dtype))
+            return std::nullopt;
+    }
+    if (!heads_of(kh, k, k_weight, nullptr, weight_dtype) || !heads_of(vh, v, std::nullopt, nullptr, weight_dtype) ||
+        !pages_of(kp, k, k_pages, k_scale) || !pages_of(vp, v, v_pages, v_scale))
+        return std::nullopt;
+    if (h3q_append_kv(dtype, weight_dtype < 0 ? dtype : weight_dtype, q ? &qh : nullptr, &kh, &vh, &kp, &vp, ints(slots),
+                      k.size(0), k.size(2), (float)eps, cos ? &r : nullptr, stream_of(stream)))
+        return std::nullopt;
+    return q ? q_out : Opt(k);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -383,5 +600,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("plan_experts", torch::wrap_pybind_function_no_gil(&plan_experts));
     m.def("grouped_scaled_mm", torch::wrap_pybind_function_no_gil(&grouped_scaled_mm));
     m.def("combine_experts", torch::wrap_pybind_function_no_gil(&combine_experts));
+    m.def("rotary_tables", torch::wrap_pybind_function_no_gil(&rotary_tables));
+    m.def("rotary", torch::wrap_pybind_function_no_gil(&rotary));
+    m.def("qk_norm_rotary", torch::wrap_pybind_function_no_gil(&qk_norm_rotary));
+    m.def("plan_append", torch::wrap_pybind_function_no_gil(&plan_append));
+    m.def("append_kv", torch::wrap_pybind_function_no_gil(&append_kv));
     m.def("expert_ffn", torch::wrap_pybind_function_no_gil(&expert_ffn));
 }

@@ -9,6 +9,7 @@ current HIP stream of the input's device.  Output tensors may be supplied
 from __future__ import annotations
 
 import ctypes
+import math
 import weakref
 from typing import NamedTuple
 
@@ -30,6 +31,10 @@ QUOTIENT_TRITON = 1
 SKINNY_MAX_M = 128   # rows up to which the weight-streaming GEMM runs
 MAX_EXPERTS = 1024   # experts of one routing / plan
 MAX_TOP_K = 64       # slots of a token
+MAX_HEAD_DIM = 512
+PAGES_ROWS = 0       # kinds of a cache's pages: rows of the call's dtype,
+PAGES_STATIC = 1     # e4m3fn codes with a scale for each head,
+PAGES_BY_ROW = 2     # e4m3fn codes with a scale for each row
 SCORE_SOFTMAX = 0
 SCORE_SIGMOID = 1
 
@@ -834,3 +839,290 @@ def expert_ffn(x: torch.Tensor, experts: torch.Tensor, weights: torch.Tensor, w1
               _ptr(w13_scale), _ptr(w2), LAYOUT_TILED if w2_tiled else LAYOUT_ROWS, _ptr(w2_scale), _ptr(out),
               _row_stride(out), _ptr(ws), size)
     return out
+
+
+# --------------------------------- rotary positions, head norms, paged cache
+
+_POSITION_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2, torch.float64: 3}
+
+
+class AppendPlan(NamedTuple):
+    """Where the tokens of a step go in a paged cache."""
+
+    positions: torch.Tensor  # int32 [tokens]: place in its sequence, -1 for a token of none (padding)
+    slots: torch.Tensor      # int32 [tokens]: page * page_size + place in the page, -1 where no page holds it
+
+
+def rotary_frequencies(rot_dim: int, base: float = 10000.0, *, scaling: str = "none", factor: float = 1.0,
+                       original_length: int = 0, fast: float = 32.0, slow: float = 1.0, low: float = 1.0,
+                       high: float = 4.0, device: torch.device | str = "cuda") -> tuple[torch.Tensor, float]:
+    """Radians a position of each rotated pair, float64 [rot_dim / 2], and the factor of cos and sin.
+
+    f_i = base^(-2 i / rot_dim); for contexts longer than the ``original_length`` a model learned:
+    "linear"  f / factor
+    "base"    the base times factor^(rot_dim / (rot_dim - 2)): the slowest pair as "linear", the fastest as it is
+    "yarn"    f where a pair turns more than ``fast`` times in original_length, f / factor where fewer than
+              ``slow`` times, a linear blend over the pairs between; cos and sin times 0.1 ln(factor) + 1
+    "bands"   f for wavelengths below original_length / high, f / factor for those above
+              original_length / low, a blend by the wavelength between"""
+    if rot_dim < 2 or rot_dim % 2 or rot_dim > MAX_HEAD_DIM:
+        raise ValueError(f"rotary_frequencies: rot_dim={rot_dim} must be even, 2 to {MAX_HEAD_DIM}")
+    if base <= 0.0 or factor <= 0.0:
+        raise ValueError("rotary_frequencies: base and factor must be positive")
+    if scaling in ("yarn", "bands") and original_length < 1:
+        raise ValueError(f"rotary_frequencies: {scaling} needs the original_length")
+    if scaling == "base":
+        if rot_dim == 2:
+            raise ValueError("rotary_frequencies: one pair has no other base")
+        base = base * factor ** (rot_dim / (rot_dim - 2))
+    f = base ** (-torch.arange(0, rot_dim, 2, dtype=torch.float64) / rot_dim)
+    magnitude = 1.0
+    if scaling == "linear":
+        f = f / factor
+    elif scaling == "yarn":
+        pair = lambda turns: rot_dim * math.log(original_length / (turns * 2.0 * math.pi)) / (2.0 * math.log(base))
+        first, last = max(math.floor(pair(fast)), 0), min(math.ceil(pair(slow)), rot_dim - 1)
+        ramp = ((torch.arange(rot_dim // 2, dtype=torch.float64) - first) / max(last - first, 0.001)).clamp(0.0, 1.0)
+        f = f * (1.0 - ramp) + f / factor * ramp
+        magnitude = 0.1 * math.log(factor) + 1.0 if factor > 1.0 else 1.0
+    elif scaling == "bands":
+        if high <= low:
+            raise ValueError("rotary_frequencies: high must be above low")
+        share = ((original_length * f / (2.0 * math.pi) - low) / (high - low)).clamp(0.0, 1.0)
+        f = f * share + f / factor * (1.0 - share)
+    elif scaling not in ("none", "base"):
+        raise ValueError(f"rotary_frequencies: unknown scaling {scaling!r}")
+    return f.to(device), magnitude
+
+
+def rotary_tables(positions: torch.Tensor, frequencies: torch.Tensor,
+                  magnitude: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
+    """cos and sin, fp32 [n, pairs], of ``positions`` (int32, int64, float32 or float64 [n]) times
+    ``frequencies`` (float64 [pairs], radians), both times ``magnitude``.  Angles are binary64."""
+    got = _native_call("rotary_tables", positions, frequencies, float(magnitude))
+    if got is not None:
+        return got
+    name = "rotary_tables"
+    _require_gpu(name, positions, frequencies)
+    if positions.dtype not in _POSITION_TYPES:
+        raise TypeError(f"{name}: positions must be int32, int64, float32 or float64, got {positions.dtype}")
+    _contiguous(f"{name} positions", positions, positions.dtype)
+    _contiguous(f"{name} frequencies", frequencies, torch.float64)
+    if positions.ndim != 1 or frequencies.ndim != 1:
+        raise ValueError(f"{name}: positions and frequencies must be vectors")
+    n, half = int(positions.shape[0]), int(frequencies.shape[0])
+    cos, sin = (torch.empty((n, half), device=positions.device, dtype=torch.float32) for _ in range(2))
+    _call_on(positions, "h3q_rotary_tables", _ptr(positions), _POSITION_TYPES[positions.dtype], n, _ptr(frequencies),
+             half, float(magnitude), _ptr(cos), _ptr(sin))
+    return cos, sin
+
+
+def _apart(name: str, t: torch.Tensor) -> None:
+    """Raise where two elements of an output share memory."""
+    reach = 0
+    for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz > 1):
+        if stride <= reach:
+            raise ValueError(f"{name}: elements of an output share memory")
+        reach += stride * (size - 1)
+
+
+def _head_rows(name: str, t: torch.Tensor, dtype: torch.dtype | None = None,
+               shape: tuple[int, ...] | None = None) -> None:
+    if t.dtype not in _TENSOR_DTYPES or (dtype is not None and t.dtype != dtype):
+        raise TypeError(f"{name}: expected {dtype or 'bfloat16, float16 or float32'}, got {t.dtype}")
+    if t.ndim != 3 or (t.shape[2] > 1 and t.stride(2) != 1):
+        raise ValueError(f"{name}: expected [tokens, heads, head_dim] with unit stride along head_dim, got "
+                         f"{tuple(t.shape)}")
+    if shape is not None and tuple(t.shape) != shape:
+        raise ValueError(f"{name}: expected shape {shape}, got {tuple(t.shape)}")
+
+
+def _heads(name: str, x: torch.Tensor, weight: torch.Tensor | None, out: torch.Tensor | None) -> _lib.Heads:
+    heads, d = int(x.shape[1]), int(x.shape[2])
+    if weight is not None:
+        if weight.dtype not in (x.dtype, torch.float32):
+            raise TypeError(f"{name}: weights must be {x.dtype} or float32, got {weight.dtype}")
+        if tuple(weight.shape) not in ((d,), (heads, d)) or (d > 1 and weight.stride(-1) != 1):
+            raise ValueError(f"{name}: weights must be [{d}] or [{heads}, {d}] with unit stride, got "
+                             f"{tuple(weight.shape)}")
+    ptr = lambda t: None if t is None else t.data_ptr()
+    return _lib.Heads(ptr(x), x.stride(0), x.stride(1), heads, ptr(weight),
+                      weight.stride(0) if weight is not None and weight.ndim == 2 else 0, ptr(out),
+                      0 if out is None else out.stride(0), 0 if out is None else out.stride(1))
+
+
+def _rotation(name: str, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor | None, tokens: int, d: int,
+              interleaved: bool, inverse: bool = False) -> _lib.Rotation:
+    _contiguous(f"{name} cos", cos, torch.float32)
+    _contiguous(f"{name} sin", sin, torch.float32, tuple(cos.shape))
+    if cos.ndim != 2 or not 0 < 2 * cos.shape[1] <= d:
+        raise ValueError(f"{name}: tables must be [rows, pairs] of at most {d // 2} pairs, got {tuple(cos.shape)}")
+    if positions is not None:
+        if positions.dtype not in (torch.int32, torch.int64):
+            raise TypeError(f"{name}: positions must be int32 or int64, got {positions.dtype}")
+        _contiguous(f"{name} positions", positions, positions.dtype, (tokens,))
+    elif cos.shape[0] < tokens:
+        raise ValueError(f"{name}: tables of {cos.shape[0]} rows for {tokens} tokens without positions")
+    return _lib.Rotation(cos.data_ptr(), sin.data_ptr(), cos.shape[0], 2 * cos.shape[1],
+                         None if positions is None else positions.data_ptr(),
+                         int(positions is not None and positions.dtype == torch.int64), int(bool(interleaved)),
+                         int(bool(inverse)))
+
+
+def _like_heads(name: str, x: torch.Tensor, out: torch.Tensor | None) -> torch.Tensor:
+    if out is None:
+        return torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    _head_rows(name, out, x.dtype, tuple(x.shape))
+    _apart(name, out)
+    return out
+
+
+def rotary(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor | None = None, *,
+           interleaved: bool = False, inverse: bool = False, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Rotates the first 2 * pairs channels of ``x [tokens, heads, head_dim]`` (bf16, fp16 or fp32, any
+    strides but the last) by the angles of the tables' rows ``positions`` (int32 or int64 [tokens]; None: row
+    t for token t): (a, b) -> (a cos - b sin, a sin + b cos), rounded once; further channels go through.
+
+    ``cos``, ``sin``: fp32 [rows, pairs] (rotary_tables).  Pairs are (i, pairs + i), or (2 i, 2 i + 1)
+    (``interleaved``).  ``inverse``: by the negative angle, which is also the rotation's gradient.  ``out`` may be
+    x itself and otherwise holds no element of it.  A position below 0 is padding, its rows of out are left as
+    they were (allocated here: undefined); one past the tables gives NaN."""
+    got = _native_call("rotary", x, cos, sin, positions, interleaved, inverse, out)
+    if got is not None:
+        return got
+    name = "rotary"
+    _require_gpu(name, x, cos, sin, positions, out)
+    _head_rows(f"{name} x", x)
+    tokens, _, d = x.shape
+    rotation = _rotation(name, cos, sin, positions, tokens, d, interleaved, inverse)
+    out = _like_heads(f"{name} out", x, out)
+    _call_on(x, "h3q_rotary", _TENSOR_DTYPES[x.dtype], _heads(name, x, None, out), tokens, d, rotation)
+    return out
+
+
+def _weight_dtype(name: str, x: torch.Tensor, *weights: torch.Tensor | None) -> int:
+    given = {w.dtype for w in weights if w is not None}
+    if len(given) > 1:
+        raise TypeError(f"{name}: the weights of one call have one dtype, got {given}")
+    return _TENSOR_DTYPES.get(given.pop() if given else x.dtype, -1)
+
+
+def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | None, k_weight: torch.Tensor | None,
+                   cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor | None = None, *, eps: float = 1e-6,
+                   interleaved: bool = False, q_out: torch.Tensor | None = None,
+                   k_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """RMS norm of every query and key head and their rotation, in one launch and one rounding:
+    x / sqrt(mean(x * x) + eps) * weight, then ``rotary``.
+
+    ``q [tokens, q_heads, head_dim]`` and ``k [tokens, k_heads, head_dim]`` may be views of the packed rows of a
+    qkv product.  Weights [head_dim], or one for each head [heads, head_dim], in q's dtype or fp32; None leaves
+    out the norm.  The outputs may be the inputs themselves."""
+    got = _native_call("qk_norm_rotary", q, k, q_weight, k_weight, cos, sin, positions, float(eps), interleaved, q_out,
+                       k_out)
+    if got is not None:
+        return got
+    name = "qk_norm_rotary"
+    _require_gpu(name, q, k, q_weight, k_weight, cos, sin, positions, q_out, k_out)
+    _head_rows(f"{name} q", q)
+    tokens, _, d = q.shape
+    _head_rows(f"{name} k", k, q.dtype, (tokens, k.shape[1] if k.ndim == 3 else 0, d))
+    rotation = _rotation(name, cos, sin, positions, tokens, d, interleaved)
+    q_out, k_out = _like_heads(f"{name} q_out", q, q_out), _like_heads(f"{name} k_out", k, k_out)
+    _call_on(q, "h3q_qk_norm_rotary", _TENSOR_DTYPES[q.dtype], _weight_dtype(name, q, q_weight, k_weight),
+             _heads(f"{name} q", q, q_weight, q_out), _heads(f"{name} k", k, k_weight, k_out), tokens, d, float(eps),
+             rotation)
+    return q_out, k_out
+
+
+def plan_append(table: torch.Tensor, lengths: torch.Tensor, cu_tokens: torch.Tensor, tokens: int,
+                page_size: int) -> AppendPlan:
+    """Positions and cache slots of a step's ``tokens`` packed tokens, once for all layers.
+
+    ``table`` int32 [seqs, columns]: the page of each page_size positions of a sequence (below 0: none);
+    ``lengths`` int32 [seqs]: tokens that the cache holds already; ``cu_tokens`` int32 [seqs + 1]: first token of
+    each sequence in the step (a decode step's are 0, 1, 2, ...), the rest up to ``tokens`` is padding."""
+    got = _native_call("plan_append", table, lengths, cu_tokens, tokens, page_size)
+    if got is not None:
+        return AppendPlan(*got)
+    name = "plan_append"
+    _require_gpu(name, table, lengths, cu_tokens)
+    _rows_2d(f"{name} table", table, torch.int32)
+    seqs, columns = table.shape
+    _contiguous(f"{name} lengths", lengths, torch.int32, (seqs,))
+    _contiguous(f"{name} cu_tokens", cu_tokens, torch.int32, (seqs + 1,))
+    if not 0 <= tokens < 2 ** 31:
+        raise ValueError(f"{name}: {tokens} tokens")
+    positions, slots = (torch.empty(tokens, device=table.device, dtype=torch.int32) for _ in range(2))
+    _call_on(table, "h3q_plan_append", _ptr(table), table.stride(0) if seqs > 1 else columns, seqs, columns,
+             _ptr(lengths), _ptr(cu_tokens), int(tokens), int(page_size), _ptr(positions), _ptr(slots))
+    return AppendPlan(positions, slots)
+
+
+def _pages(name: str, x: torch.Tensor, pages: torch.Tensor, scale: torch.Tensor | None) -> _lib.Pages:
+    heads, d = int(x.shape[1]), int(x.shape[2])
+    if pages.dtype not in (x.dtype, torch.float8_e4m3fn):
+        raise TypeError(f"{name}: pages must be {x.dtype} or float8_e4m3fn, got {pages.dtype}")
+    if pages.ndim != 4 or tuple(pages.shape[2:]) != (heads, d) or pages.stride(3) != 1:
+        raise ValueError(f"{name}: pages must be [pages, page_size, {heads}, {d}] with unit stride along head_dim, got "
+                         f"{tuple(pages.shape)}")
+    _apart(name, pages)
+    kind, strides = PAGES_ROWS, (0, 0, 0)
+    if pages.dtype == torch.float8_e4m3fn:
+        if scale is None or scale.dtype != torch.float32:
+            raise TypeError(f"{name}: e4m3fn pages need fp32 scales")
+        if tuple(scale.shape) in ((1,), (heads,)):
+            kind, strides = PAGES_STATIC, (0, 0, scale.stride(0) if scale.shape[0] > 1 else 0)
+        elif tuple(scale.shape) == tuple(pages.shape[:3]):
+            _apart(f"{name} scale", scale)
+            kind, strides = PAGES_BY_ROW, scale.stride()
+        else:
+            raise ValueError(f"{name}: scales must be [1], [{heads}] or {tuple(pages.shape[:3])}, got "
+                             f"{tuple(scale.shape)}")
+    elif scale is not None:
+        raise ValueError(f"{name}: {pages.dtype} pages have no scales")
+    return _lib.Pages(pages.data_ptr(), pages.shape[0], pages.shape[1], *pages.stride()[:3], kind,
+                      None if scale is None else scale.data_ptr(), *strides)
+
+
+def append_kv(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, slots: torch.Tensor, *,
+              k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None,
+              k_weight: torch.Tensor | None = None, eps: float = 1e-6, cos: torch.Tensor | None = None,
+              sin: torch.Tensor | None = None, positions: torch.Tensor | None = None, interleaved: bool = False,
+              q: torch.Tensor | None = None, q_weight: torch.Tensor | None = None,
+              q_out: torch.Tensor | None = None) -> torch.Tensor | None:
+    """One layer's append to a paged cache, one launch: keys normed (``k_weight``) and rotated (``cos``, ``sin``,
+    ``positions``) as qk_norm_rotary does and values as they are, ``k``, ``v [tokens, kv_heads, head_dim]``, into
+    the slots (int32 [tokens]: page * page_size + place; see plan_append) of ``k_pages`` and ``v_pages [pages,
+    page_size, kv_heads, head_dim]`` (any strides but the last, so heads may lie outside a page's tokens).
+    ``q`` is normed and rotated beside them into ``q_out`` (returned; allocated here when None).
+
+    Pages hold k's dtype, or float8_e4m3fn codes e4m3(clamp(y / s, +-448)): with ``k_scale``, ``v_scale`` fp32 [1]
+    or [kv_heads] those are the scales; with [pages, page_size, kv_heads] each row's scale max|y| / 448 is stored
+    there.  Slots below 0 or past the pages are not stored, and a token with a position below 0 (padding) has
+    no q either: those rows are left as they were.  The slots of a call that are stored are distinct."""
+    got = _native_call("append_kv", k, v, k_pages, v_pages, slots, k_scale, v_scale, k_weight, float(eps), cos, sin,
+                       positions, interleaved, q, q_weight, q_out)
+    if got is not None:
+        return got if q is not None else None
+    name = "append_kv"
+    _require_gpu(name, k, v, k_pages, v_pages, slots, k_scale, v_scale, k_weight, cos, sin, positions, q, q_weight,
+                 q_out)
+    _head_rows(f"{name} k", k)
+    tokens, _, d = k.shape
+    _head_rows(f"{name} v", v, k.dtype, tuple(k.shape))
+    _contiguous(f"{name} slots", slots, torch.int32, (tokens,))
+    if (cos is None) != (sin is None) or (cos is None and positions is not None):
+        raise ValueError(f"{name}: cos and sin go together, and positions with them")
+    rotation = None if cos is None else _rotation(name, cos, sin, positions, tokens, d, interleaved)
+    q_heads = None
+    if q is not None:
+        _head_rows(f"{name} q", q, k.dtype, (tokens, q.shape[1] if q.ndim == 3 else 0, d))
+        q_out = _like_heads(f"{name} q_out", q, q_out)
+        q_heads = _heads(f"{name} q", q, q_weight, q_out)
+    elif q_weight is not None or q_out is not None:
+        raise ValueError(f"{name}: q_weight and q_out go with q")
+    _call_on(k, "h3q_append_kv", _TENSOR_DTYPES[k.dtype], _weight_dtype(name, k, q_weight, k_weight), q_heads,
+             _heads(f"{name} k", k, k_weight, None), _heads(f"{name} v", v, None, None),
+             _pages(f"{name} k_pages", k, k_pages, k_scale), _pages(f"{name} v_pages", v, v_pages, v_scale),
+             _ptr(slots), tokens, d, float(eps), rotation)
+    return q_out
