@@ -502,6 +502,43 @@ int h3q_append_kv(int dtype, int weight_dtype, const h3q_heads* q, const h3q_hea
                   const h3q_pages* k_pages, const h3q_pages* v_pages, const int32_t* slots, int64_t tokens,
                   int64_t head_dim, float eps, const h3q_rotation* rotation, void* stream);
 
+/*
+ * Products with 4-bit weights and group scales, for models whose decode is bound by their
+ * weights' bytes.  No counterpart in the reference.
+ *   y[m, n] = sum_g s[n, g] * sum_{k in g} x[m, k] * (u[n, k] - z[n, g])  [+ bias[n]]
+ * u, z: integers 0 .. 15 (no zero points: z = 8); a group is 32, 64 or a multiple of 128
+ * columns, the last of a row may be shorter; s is bf16 or binary16.  Rows of a checkpoint:
+ * codes two a byte [n, k / 2], the low nibble first, scales and zeros (bytes) [n, groups].
+ *
+ * The products read the layout that h3q_w4_pack writes (once, when a model is loaded):
+ * blocks of 16 rows x 128 columns, 1 KiB each, [ceil(n / 16)][ceil(k / 128)]; scales and zeros
+ * [ceil(n / 16)][groups][16].  k % 16 == 0, 16 <= k <= 2^22.
+ */
+int64_t h3q_w4_code_bytes(int64_t n, int64_t k);
+int h3q_w4_pack(const void* codes, int64_t ldc, const void* scales, int64_t lds, const void* zeros, int64_t ldz,
+                int64_t n, int64_t k, int64_t group, void* codes_out, void* scales_out, void* zeros_out, void* stream);
+
+/*
+ * The quantizer of weights [n, k] (dtype: H3Q_DTYPE_*; scales binary16 for binary16 weights, else
+ * bf16) into contiguous rows: s = max|w| / 7 and u = clamp(rne(w / s), -8, 7) + 8, or with zeros (not
+ * NULL) s = (max(w, 0) - min(w, 0)) / 15, z = clamp(rne(-min / s), 0, 15) and u = clamp(rne(w / s) + z, 0, 15).
+ * s is rounded to its type before it is used; a group of zeros has s = 0.
+ */
+int h3q_w4_quantize(const void* w, int dtype, int64_t ldw, int64_t n, int64_t k, int64_t group, void* codes,
+                    void* scales, void* zeros, void* stream);
+
+/*
+ * The product, x [m, k] and out [m, n] bf16 or binary16 (dtype; ldx and ldo elements), binary32
+ * sums rounded once; codes, scales (scale_dtype bf16 or binary16) and zeros (or NULL) as packed,
+ * bias [n] of x's type or NULL.  x 16-byte aligned with ldx % 8 == 0, ldx < 2^23.  workspace:
+ * h3q_w4_mm_workspace_bytes(...) bytes of the caller's (0: none), free to use again when the call's
+ * work on the stream is done.  A row of x with an infinity or a NaN gives NaN or infinities.
+ */
+int64_t h3q_w4_mm_workspace_bytes(int64_t m, int64_t n, int64_t k, int64_t group);
+int h3q_w4_mm(int dtype, const void* x, int64_t ldx, const void* codes, const void* scales, int scale_dtype,
+              const void* zeros, int64_t group, const void* bias, void* out, int64_t ldo, int64_t m, int64_t n,
+              int64_t k, void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -81,6 +81,11 @@ SIGNATURES: dict[str, tuple[type | None, list]] = {
     "h3q_rotary": (_I, [_I, _HEADS, _I64, _I64, _ROTATION, _P]),
     "h3q_qk_norm_rotary": (_I, [_I, _I, _HEADS, _HEADS, _I64, _I64, _F, _ROTATION, _P]),
     "h3q_plan_append": (_I, [_P, _I64, _I64, _I64, _P, _P, _I64, _I64, _P, _P, _P]),
+    "h3q_w4_code_bytes": (_I64, [_I64, _I64]),
+    "h3q_w4_pack": (_I, [_P, _I64, _P, _I64, _P, _I64, _I64, _I64, _I64, _P, _P, _P, _P]),
+    "h3q_w4_quantize": (_I, [_P, _I, _I64, _I64, _I64, _I64, _P, _P, _P, _P]),
+    "h3q_w4_mm_workspace_bytes": (_I64, [_I64, _I64, _I64, _I64]),
+    "h3q_w4_mm": (_I, [_I, _P, _I64, _P, _P, _I, _P, _I64, _P, _P, _I64, _I64, _I64, _I64, _P, _I64, _P]),
     "h3q_append_kv": (_I, [_I, _I, _HEADS, _HEADS, _HEADS, _PAGES, _PAGES, _P, _I64, _I64, _F, _ROTATION, _P]),
 }
 

@@ -1002,4 +1002,135 @@ __attribute__((visibility("default"))) int h3q_append_kv(int dtype, int weight_d
     return check_launch(h3q::launch_head_rotary(dtype, a, (hipStream_t)stream), who);
 }
 
+static int check_w4(const char* who, int64_t n, int64_t k, int64_t group) {
+    if (n < 0 || n >= (int64_t(1) << 31)) return fail(H3Q_ERR_INVALID, "%s: n=%lld", who, (long long)n);
+    if (k < 16 || k % 16 || k > (int64_t(1) << 22))
+        return fail(H3Q_ERR_INVALID, "%s: k=%lld must be a multiple of 16, 16 to 2^22", who, (long long)k);
+    if (group != 32 && group != 64 && (group < 128 || group % 128 || group > (int64_t(1) << 22)))
+        return fail(H3Q_ERR_INVALID, "%s: group=%lld must be 32, 64 or a multiple of 128", who, (long long)group);
+    return H3Q_OK;
+}
+
+static int64_t w4_groups(int64_t k, int64_t group) { return (k + group - 1) / group; }
+
+__attribute__((visibility("default"))) int64_t h3q_w4_code_bytes(int64_t n, int64_t k) {
+    return n <= 0 || k <= 0 ? 0 : (n + 15) / 16 * ((k + 127) / 128) * 1024;
+}
+
+__attribute__((visibility("default"))) int h3q_w4_pack(const void* codes, int64_t ldc, const void* scales, int64_t lds,
+                                                       const void* zeros, int64_t ldz, int64_t n, int64_t k,
+                                                       int64_t group, void* codes_out, void* scales_out,
+                                                       void* zeros_out, void* stream) {
+    const char* who = "h3q_w4_pack";
+    const int rc = check_w4(who, n, k, group);
+    if (rc != H3Q_OK) return rc;
+    const int64_t groups = w4_groups(k, group);
+    if (ldc < k / 2 || lds < groups || (zeros && ldz < groups))
+        return fail(H3Q_ERR_INVALID, "%s: row strides %lld, %lld, %lld are below the rows", who, (long long)ldc,
+                    (long long)lds, (long long)ldz);
+    if ((zeros != nullptr) != (zeros_out != nullptr)) return fail(H3Q_ERR_INVALID, "%s: zeros on one side only", who);
+    if (n == 0) return ok();
+    if (!codes || !scales || !codes_out || !scales_out) return fail(H3Q_ERR_INVALID, "%s: null pointer", who);
+    if (!aligned(codes_out, 16) || !aligned(scales_out, 16) || !aligned(zeros_out, 16) || !aligned(scales, 2))
+        return fail(H3Q_ERR_INVALID, "%s: the packed buffers must be 16-byte aligned", who);
+    h3q::W4PackArgs a{};
+    a.codes = (const uint8_t*)codes;
+    a.scales = (const uint16_t*)scales;
+    a.zeros = (const uint8_t*)zeros;
+    a.ldc = ldc;
+    a.lds = lds;
+    a.ldz = ldz;
+    a.n = n;
+    a.k = k;
+    a.groups = groups;
+    a.codes_out = (uint8_t*)codes_out;
+    a.scales_out = (uint16_t*)scales_out;
+    a.zeros_out = (uint8_t*)zeros_out;
+    return check_launch(h3q::launch_w4_pack(a, (hipStream_t)stream), who);
+}
+
+__attribute__((visibility("default"))) int h3q_w4_quantize(const void* w, int dtype, int64_t ldw, int64_t n, int64_t k,
+                                                           int64_t group, void* codes, void* scales, void* zeros,
+                                                           void* stream) {
+    const char* who = "h3q_w4_quantize";
+    if (dtype != H3Q_DTYPE_BF16 && dtype != H3Q_DTYPE_F16 && dtype != H3Q_DTYPE_F32)
+        return fail(H3Q_ERR_INVALID, "%s: unknown dtype %d", who, dtype);
+    const int rc = check_w4(who, n, k, group);
+    if (rc != H3Q_OK) return rc;
+    if (ldw < k) return fail(H3Q_ERR_INVALID, "%s: row stride %lld below k", who, (long long)ldw);
+    if (n * w4_groups(k, group) >= (int64_t(1) << 34))
+        return fail(H3Q_ERR_UNSUPPORTED, "%s: %lld rows of %lld groups", who, (long long)n, (long long)w4_groups(k, group));
+    if (n == 0) return ok();
+    if (!w || !codes || !scales) return fail(H3Q_ERR_INVALID, "%s: null pointer", who);
+    if (!aligned(w, dtype == H3Q_DTYPE_F32 ? 4 : 2) || !aligned(scales, 2))
+        return fail(H3Q_ERR_INVALID, "%s: misaligned pointer", who);
+    h3q::W4QuantArgs a{};
+    a.w = w;
+    a.ldw = ldw;
+    a.n = n;
+    a.k = k;
+    a.dtype = dtype;
+    a.group = (int)group;
+    a.codes = (uint8_t*)codes;
+    a.scales = (uint16_t*)scales;
+    a.zeros = (uint8_t*)zeros;
+    return check_launch(h3q::launch_w4_quant(a, (hipStream_t)stream), who);
+}
+
+__attribute__((visibility("default"))) int64_t h3q_w4_mm_workspace_bytes(int64_t m, int64_t n, int64_t k, int64_t group) {
+    if (m <= h3q::kW4StreamRows || n <= 0 || k <= 0 || k > (int64_t(1) << 22) || group <= 0 ||
+        !h3q::w4_tile_fits(m, n, k, (int)group))
+        return 0;
+    return h3q::w4_tile_workspace_bytes(m, n, k, (int)group);
+}
+
+__attribute__((visibility("default"))) int h3q_w4_mm(int dtype, const void* x, int64_t ldx, const void* codes,
+                                                     const void* scales, int scale_dtype, const void* zeros,
+                                                     int64_t group, const void* bias, void* out, int64_t ldo,
+                                                     int64_t m, int64_t n, int64_t k, void* workspace,
+                                                     int64_t workspace_bytes, void* stream) {
+    const char* who = "h3q_w4_mm";
+    if ((dtype != H3Q_DTYPE_BF16 && dtype != H3Q_DTYPE_F16) ||
+        (scale_dtype != H3Q_DTYPE_BF16 && scale_dtype != H3Q_DTYPE_F16))
+        return fail(H3Q_ERR_INVALID, "%s: activations and scales are bf16 or binary16", who);
+    const int rc = check_w4(who, n, k, group);
+    if (rc != H3Q_OK) return rc;
+    if (m < 0 || m >= (int64_t(1) << 31)) return fail(H3Q_ERR_INVALID, "%s: m=%lld", who, (long long)m);
+    if (ldx < k || ldx % 8 || ldx >= (int64_t(1) << 23))
+        return fail(H3Q_ERR_INVALID, "%s: ldx=%lld must be a multiple of 8, k to 2^23", who, (long long)ldx);
+    if (ldo < n) return fail(H3Q_ERR_INVALID, "%s: ldo=%lld below n", who, (long long)ldo);
+    if (m == 0 || n == 0) return ok();
+    if (!x || !codes || !scales || !out) return fail(H3Q_ERR_INVALID, "%s: null pointer", who);
+    if (!aligned(x, 16) || !aligned(codes, 16) || !aligned(scales, 16) || !aligned(zeros, 16) || !aligned(bias, 2) ||
+        !aligned(out, 2))
+        return fail(H3Q_ERR_INVALID, "%s: x and the packed weights must be 16-byte aligned", who);
+    h3q::W4Args a{};
+    a.x = (const uint16_t*)x;
+    a.ldx = ldx;
+    a.m = m;
+    a.n = n;
+    a.k = k;
+    a.group = (int)group;
+    a.groups = (int)w4_groups(k, group);
+    a.blocks_per_group = group >= 128 ? (int)(group / 128) : 1;
+    a.codes = (const uint8_t*)codes;
+    a.scales = (const uint16_t*)scales;
+    a.zeros = (const uint8_t*)zeros;
+    a.bias = (const uint16_t*)bias;
+    a.out = (uint16_t*)out;
+    a.ldo = ldo;
+    a.f16 = dtype == H3Q_DTYPE_F16;
+    a.scales_f16 = scale_dtype == H3Q_DTYPE_F16;
+    a.out_vec = aligned(out, 8) && ldo % 4 == 0;
+    if (m <= h3q::kW4StreamRows) return check_launch(h3q::launch_w4_stream(a, (hipStream_t)stream), who);
+    if (!h3q::w4_tile_fits(m, n, k, (int)group))
+        return fail(H3Q_ERR_UNSUPPORTED, "%s: %lld rows of %lld x %lld are too many for one launch", who, (long long)m,
+                    (long long)n, (long long)k);
+    const int64_t need = h3q::w4_tile_workspace_bytes(m, n, k, (int)group);
+    if (!workspace || !aligned(workspace, 16) || workspace_bytes < need)
+        return fail(H3Q_ERR_INVALID, "%s: workspace of %lld bytes, %lld needed (16-byte aligned)", who,
+                    (long long)workspace_bytes, (long long)need);
+    return check_launch(h3q::launch_w4_tile(a, workspace, (hipStream_t)stream), who);
+}
+
 }  // extern "C"

@@ -322,4 +322,44 @@ struct PlanAppendArgs {
 };
 hipError_t launch_plan_append(const PlanAppendArgs& a, hipStream_t st);
 
+// Products with 4-bit weights and group scales (w4.hpp: the layout; w4_stream.hip: few rows, w4_tile.hip: many).
+struct W4Args {
+    const uint16_t* x;  // bf16 or binary16 [m, k], ldx elements
+    int64_t ldx, m, n, k;
+    int group, groups, blocks_per_group;  // blocks of 128 columns in a group of 128 or more
+    const uint8_t* codes;
+    const uint16_t* scales;  // bf16, or binary16 (scales_f16)
+    const uint8_t* zeros;    // null: 8 everywhere
+    const uint16_t* bias;    // of x's type, or null
+    uint16_t* out;           // of x's type [m, n], ldo elements
+    int64_t ldo;
+    int f16, scales_f16, out_vec;  // out_vec: four columns at once are aligned
+};
+constexpr int kW4StreamRows = 32;
+hipError_t launch_w4_stream(const W4Args& a, hipStream_t st);
+bool w4_tile_fits(int64_t m, int64_t n, int64_t k, int group);  // a launch's grid and the sums' 32-bit offsets
+int64_t w4_tile_workspace_bytes(int64_t m, int64_t n, int64_t k, int group);
+hipError_t launch_w4_tile(const W4Args& a, void* workspace, hipStream_t st);
+// Codes two a byte [n, k / 2] (the low nibble first), scales and zeros [n, groups] -> the layout.
+struct W4PackArgs {
+    const uint8_t* codes;
+    const uint16_t* scales;
+    const uint8_t* zeros;
+    int64_t ldc, lds, ldz, n, k, groups;
+    uint8_t* codes_out;
+    uint16_t* scales_out;
+    uint8_t* zeros_out;
+};
+hipError_t launch_w4_pack(const W4PackArgs& a, hipStream_t st);
+// Weights [n, k] -> codes, scales and (zeros given) zero points as rows.
+struct W4QuantArgs {
+    const void* w;
+    int64_t ldw, n, k;
+    int dtype, group;  // kInBF16, kInF16, kInF32 (bf16 scales)
+    uint8_t* codes;    // [n, k / 2]
+    uint16_t* scales;  // [n, groups]
+    uint8_t* zeros;
+};
+hipError_t launch_w4_quant(const W4QuantArgs& a, hipStream_t st);
+
 }  // namespace h3q

@@ -585,6 +585,34 @@ Opt append_kv(const Tensor& k, const Tensor& v, const Tensor& k_pages, const Ten
     return q ? q_out : Opt(k);
 }
 
+Opt w4_mm(const Tensor& x, const Tensor& codes, const Tensor& scales, const Opt& zeros, int64_t n, int64_t k,
+          int64_t group, const Opt& bias, Opt out, int64_t stream) {
+    const at::ScalarType type = x.scalar_type(), scale_type = scales.scalar_type();
+    if (!x.is_cuda() || (type != at::kBFloat16 && type != at::kHalf) || !rows_2d(x, type) || x.size(1) != k ||
+        x.size(0) == 0 || n < 1 || k < 16 || group < 32)
+        return std::nullopt;
+    const int64_t m = x.size(0), blocks = (n + 15) / 16, groups = (k + group - 1) / group;
+    const auto packed = [&](const Tensor& t, at::ScalarType of, int64_t b, int64_t c) {
+        return dense(t, x, of) && t.dim() == 3 && t.size(0) == blocks && t.size(1) == b && t.size(2) == c;
+    };
+    if ((scale_type != at::kBFloat16 && scale_type != at::kHalf) || !packed(codes, at::kByte, (k + 127) / 128, 1024) ||
+        !packed(scales, scale_type, groups, 16) || (zeros && !packed(*zeros, at::kByte, groups, 16)))
+        return std::nullopt;
+    if (bias && !(dense(*bias, x, type) && bias->dim() == 1 && bias->size(0) == n)) return std::nullopt;
+    if (out && !(on(*out, x) && rows_2d(*out, type) && out->size(0) == m && out->size(1) == n && apart(*out)))
+        return std::nullopt;
+    const c10::DeviceGuard guard(x.device());
+    if (!out) out = empty(x, {m, n}, type);
+    const int64_t bytes = h3q_w4_mm_workspace_bytes(m, n, k, group);
+    Opt ws;
+    if (bytes > 0) ws = empty(x, {bytes}, at::kByte);
+    if (h3q_w4_mm(logit_type(type), x.data_ptr(), m > 1 ? x.stride(0) : (k + 7) / 8 * 8, codes.data_ptr(),
+                  scales.data_ptr(), logit_type(scale_type), ptr(zeros), group, ptr(bias), out->data_ptr(),
+                  m > 1 ? out->stride(0) : n, m, n, k, ws ? ws->data_ptr() : nullptr, bytes, stream_of(stream)))
+        return std::nullopt;
+    return out;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -605,5 +633,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("qk_norm_rotary", torch::wrap_pybind_function_no_gil(&qk_norm_rotary));
     m.def("plan_append", torch::wrap_pybind_function_no_gil(&plan_append));
     m.def("append_kv", torch::wrap_pybind_function_no_gil(&append_kv));
+    m.def("w4_mm", torch::wrap_pybind_function_no_gil(&w4_mm));
     m.def("expert_ffn", torch::wrap_pybind_function_no_gil(&expert_ffn));
 }

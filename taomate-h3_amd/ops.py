@@ -1126,3 +1126,121 @@ def append_kv(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: 
              _pages(f"{name} k_pages", k, k_pages, k_scale), _pages(f"{name} v_pages", v, v_pages, v_scale),
              _ptr(slots), tokens, d, float(eps), rotation)
     return q_out
+
+
+# ------------------------------------------- 4-bit weights with group scales
+
+class W4Weight(NamedTuple):
+    """4-bit weights [n, k] as w4_mm reads them (pack_w4)."""
+
+    codes: torch.Tensor         # uint8 [ceil(n / 16), ceil(k / 128), 1024]
+    scales: torch.Tensor        # bf16 or fp16 [ceil(n / 16), groups, 16]
+    zeros: torch.Tensor | None  # uint8 [ceil(n / 16), groups, 16]; None: 8 everywhere
+    n: int
+    k: int
+    group: int
+
+
+def _w4_groups(name: str, k: int, group: int) -> int:
+    if k < 16 or k % 16 or k > 1 << 22:
+        raise ValueError(f"{name}: k={k} must be a multiple of 16, 16 to 2^22")
+    if group not in (32, 64) and (group < 128 or group % 128 or group > 1 << 22):
+        raise ValueError(f"{name}: group={group} must be 32, 64 or a multiple of 128")
+    return (k + group - 1) // group
+
+
+def quantize_w4(w: torch.Tensor, group: int = 128, *,
+                zeros: bool = False) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None]:
+    """4-bit codes, scales and zero points of weights ``w [n, k]`` (bf16, fp16 or fp32), as rows: uint8 [n, k / 2]
+    (two codes a byte, the low nibble first), [n, groups] in fp16 for fp16 weights and else bf16, and uint8
+    [n, groups] or None.
+
+    Without ``zeros``: s = max|w| / 7 of the group, u = clamp(rne(w / s), -8, 7) + 8.  With: s = (max(w, 0) -
+    min(w, 0)) / 15, z = rne(-min / s), u = clamp(rne(w / s) + z, 0, 15).  s is rounded before it is used."""
+    name = "quantize_w4"
+    _require_gpu(name, w)
+    if w.dtype not in _TENSOR_DTYPES:
+        raise TypeError(f"{name}: expected bfloat16, float16 or float32 weights, got {w.dtype}")
+    _rows_2d(name, w, w.dtype)
+    n, k = w.shape
+    groups = _w4_groups(name, k, group)
+    codes = torch.empty((n, k // 2), device=w.device, dtype=torch.uint8)
+    scales = torch.empty((n, groups), device=w.device, dtype=torch.float16 if w.dtype == torch.float16 else torch.bfloat16)
+    points = torch.empty((n, groups), device=w.device, dtype=torch.uint8) if zeros else None
+    _call_on(w, "h3q_w4_quantize", _ptr(w), _TENSOR_DTYPES[w.dtype], w.stride(0) if n > 1 else k, n, k, int(group),
+             _ptr(codes), _ptr(scales), _ptr(points))
+    return codes, scales, points
+
+
+def pack_w4(codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None = None, *,
+            group: int = 128) -> W4Weight:
+    """The layout of w4_mm from the rows of a checkpoint (or of quantize_w4): ``codes`` uint8 [n, k / 2], the low
+    nibble first, ``scales`` bf16 or fp16 [n, groups], ``zeros`` uint8 [n, groups] of values 0 to 15 (None: 8).
+    A group is 32, 64 or a multiple of 128 columns; the last of a row may be shorter."""
+    name = "pack_w4"
+    _require_gpu(name, codes, scales, zeros)
+    _rows_2d(f"{name} codes", codes, torch.uint8)
+    n, k = int(codes.shape[0]), 2 * int(codes.shape[1])
+    groups = _w4_groups(name, k, group)
+    if scales.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"{name}: scales must be bfloat16 or float16, got {scales.dtype}")
+    _rows_2d(f"{name} scales", scales, scales.dtype)
+    if zeros is not None:
+        _rows_2d(f"{name} zeros", zeros, torch.uint8)
+    for label, t in (("scales", scales), ("zeros", zeros)):
+        if t is not None and tuple(t.shape) != (n, groups):
+            raise ValueError(f"{name}: {label} must be {(n, groups)}, got {tuple(t.shape)}")
+    blocks = (n + 15) // 16
+    out = W4Weight(torch.empty((blocks, (k + 127) // 128, 1024), device=codes.device, dtype=torch.uint8),
+                   torch.empty((blocks, groups, 16), device=codes.device, dtype=scales.dtype),
+                   None if zeros is None else torch.empty((blocks, groups, 16), device=codes.device, dtype=torch.uint8),
+                   n, k, int(group))
+    row = lambda t: 0 if t is None else t.stride(0) if n > 1 else t.shape[1]
+    _call_on(codes, "h3q_w4_pack", _ptr(codes), row(codes), _ptr(scales), row(scales), _ptr(zeros), row(zeros), n, k,
+             int(group), _ptr(out.codes), _ptr(out.scales), _ptr(out.zeros))
+    return out
+
+
+def _check_w4(name: str, w: W4Weight) -> None:
+    groups = _w4_groups(name, w.k, w.group)
+    blocks = (w.n + 15) // 16
+    _contiguous(f"{name} codes", w.codes, torch.uint8, (blocks, (w.k + 127) // 128, 1024))
+    if w.scales.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"{name}: scales must be bfloat16 or float16, got {w.scales.dtype}")
+    _contiguous(f"{name} scales", w.scales, w.scales.dtype, (blocks, groups, 16))
+    if w.zeros is not None:
+        _contiguous(f"{name} zeros", w.zeros, torch.uint8, (blocks, groups, 16))
+
+
+def w4_mm(x: torch.Tensor, weight: W4Weight, *, bias: torch.Tensor | None = None,
+          out: torch.Tensor | None = None) -> torch.Tensor:
+    """x @ w^T [+ bias] of 4-bit weights (pack_w4), ``x [m, k]`` bf16 or fp16 -> [m, n] in x's dtype:
+    out[m, n] = sum_g s[n, g] * sum_{k in g} x[m, k] (u[n, k] - z[n, g]), binary32 sums rounded once.
+
+    x has 16-byte aligned rows (a row stride that is a multiple of 8); ``bias [n]`` and ``out`` are of its dtype."""
+    got = _native_call("w4_mm", x, weight.codes, weight.scales, weight.zeros, weight.n, weight.k, weight.group, bias, out)
+    if got is not None:
+        return got
+    name = "w4_mm"
+    _require_gpu(name, x, weight.codes, weight.scales, weight.zeros, bias, out)
+    if x.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"{name}: expected bfloat16 or float16 activations, got {x.dtype}")
+    _rows_2d(f"{name} x", x, x.dtype)
+    _check_w4(name, weight)
+    m, n, k = int(x.shape[0]), weight.n, weight.k
+    if x.shape[1] != k:
+        raise ValueError(f"{name}: inner dimensions differ ({x.shape[1]} vs {k})")
+    if bias is not None:
+        _contiguous(f"{name} bias", bias, x.dtype, (n,))
+    if out is None:
+        out = torch.empty((m, n), device=x.device, dtype=x.dtype)
+    _rows_2d(f"{name} out", out, x.dtype)
+    if tuple(out.shape) != (m, n):
+        raise ValueError(f"{name}: out shape {tuple(out.shape)} != {(m, n)}")
+    _apart(f"{name} out", out)
+    size = int(_lib.lib().h3q_w4_mm_workspace_bytes(m, n, k, weight.group))
+    ws = torch.empty(size, device=x.device, dtype=torch.uint8) if size else None
+    _call_on(x, "h3q_w4_mm", _TENSOR_DTYPES[x.dtype], _ptr(x), x.stride(0) if m > 1 else (k + 7) // 8 * 8,
+             _ptr(weight.codes), _ptr(weight.scales), _TENSOR_DTYPES[weight.scales.dtype], _ptr(weight.zeros),
+             weight.group, _ptr(bias), _ptr(out), out.stride(0) if m > 1 else n, m, n, k, _ptr(ws), size)
+    return out

@@ -1,0 +1,93 @@
+"""Plain 64-bit form of the products with 4-bit weights, the quantizer, the packed layout and the bound of results
+that are summed in binary32 and rounded once."""
+
+from __future__ import annotations
+
+import numpy as np
+import torch
+
+
+def unpack_rows(codes: torch.Tensor) -> torch.Tensor:
+    """uint8 [n, k / 2] -> integers [n, k], the low nibble first."""
+    c = codes.cpu()
+    return torch.stack((c & 15, c >> 4), dim=2).flatten(1)
+
+
+def dequantized(codes, scales, zeros, group: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """Weights s (u - z) and scales by column, float64 [n, k]."""
+    u = unpack_rows(codes).double()
+    by = torch.arange(u.shape[1]) // group
+    s = scales.cpu().double()[:, by]
+    z = 8.0 if zeros is None else zeros.cpu().double()[:, by]
+    return s * (u - z), s
+
+
+def product(x, codes, scales, zeros, group: int, bias=None) -> tuple[torch.Tensor, torch.Tensor]:
+    """(value, bound of its binary32 error), float64 [m, n].
+
+    A group of g <= 128 columns is summed as x (16 + u): at most g + 4 roundings (of 2^-23, a matrix
+    instruction may cut off) of a sum of at most 31 |x|; 16 + z times the sum of x (as many) is taken off,
+    at most 31 |x| again; the scale and the sum over the groups add one rounding each for every group (a
+    wider group counts as its blocks of 128), and the parts of a split sum or of a workgroup's waves a
+    few: (g + 4 + groups + 16) 2^-23 * 62 sum |s x| covers it."""
+    w, s = dequantized(codes, scales, zeros, group)
+    a = x.cpu().double()
+    y = a @ w.T
+    rounds = min(group, 128) + 4 + (a.shape[1] + min(group, 128) - 1) // min(group, 128) + 16
+    bound = rounds * 2.0 ** -23 * 62.0 * (a.abs() @ s.abs().T)
+    if bias is not None:
+        y = y + bias.cpu().double()
+        bound = bound + 2.0 ** -23 * y.abs()
+    return y, bound
+
+
+def assert_product(got: torch.Tensor, want: torch.Tensor, bound: torch.Tensor, what: str = "") -> None:
+    info = torch.finfo(got.dtype)
+    g = got.detach().cpu().double()
+    bound = bound + info.eps / 2 * (want.abs() + bound) + info.smallest_normal * info.eps / 2
+    bad = ~((g - want).abs() <= bound)
+    assert not bad.any(), (f"{what}: {int(bad.sum())} of {bad.numel()}, first at {bad.nonzero()[0].tolist()}: "
+                           f"{g[bad][0].item()!r} for {want[bad][0].item()!r} +- {bound[bad][0].item():.3g}")
+
+
+def quantize(w: torch.Tensor, group: int, zeros: bool):
+    """The quantizer in binary32, operation by operation (numpy: IEEE, no reciprocal of a constant divisor)."""
+    kind = torch.float16 if w.dtype == torch.float16 else torch.bfloat16
+    a = w.float().cpu().numpy()
+    n, k = a.shape
+    groups = (k + group - 1) // group
+    codes = np.zeros((n, k), np.uint8)
+    scales = torch.zeros(n, groups, dtype=kind)
+    points = np.full((n, groups), 8, np.uint8)
+    for g in range(groups):
+        part = a[:, g * group:(g + 1) * group]
+        low, high = np.minimum(part.min(1), np.float32(0)), np.maximum(part.max(1), np.float32(0))
+        reach = (high - low) / np.float32(15) if zeros else np.maximum(high, -low) / np.float32(7)
+        scales[:, g] = torch.from_numpy(reach).to(kind)
+        s = scales[:, g].float().numpy()
+        live = s > 0
+        safe = np.where(live, s, np.float32(1))
+        z = np.where(live, np.clip(np.rint(-low / safe), 0, 15), 0) if zeros else np.full(n, 8.0)
+        q = np.where(live[:, None], np.rint(part / safe[:, None]), 0)
+        codes[:, g * group:(g + 1) * group] = np.clip(q + z[:, None], 0, 15).astype(np.uint8)
+        points[:, g] = z.astype(np.uint8)
+    packed = codes[:, 0::2] | (codes[:, 1::2] << 4)
+    return torch.from_numpy(packed), scales, torch.from_numpy(points) if zeros else None
+
+
+def packed_codes(codes: torch.Tensor) -> torch.Tensor:
+    """The layout, word by word: word s of lane L of block (r, b) holds the codes 128 b + 32 s + 8 (L / 16) .. + 7 of
+    row 16 r + L % 16, k0 k2 k4 k6 k1 k3 k5 k7 from the low nibble, rotated left by 3."""
+    u = unpack_rows(codes).numpy().astype(np.uint64)
+    n, k = u.shape
+    rows, cols = -(-n // 16), -(-k // 128)
+    full = np.zeros((rows * 16, cols * 128), np.uint64)
+    full[:n, :k] = u
+    out = np.zeros((rows, cols, 64, 4), np.uint32)
+    for lane in range(64):
+        for s in range(4):
+            base = 32 * s + 8 * (lane // 16)
+            e = [full[lane % 16::16, base + i::128] for i in (0, 2, 4, 6, 1, 3, 5, 7)]
+            w = sum(v << np.uint64(4 * i) for i, v in enumerate(e))
+            out[:, :, lane, s] = ((w << np.uint64(3)) | (w >> np.uint64(29))) & np.uint64(0xFFFFFFFF)
+    return torch.from_numpy(out.view(np.uint8).reshape(rows, cols, 1024))

@@ -1,0 +1,232 @@
+"""Products with 4-bit weights on the GPU against the plain 64-bit form of _w4.py: every kernel, row count around its
+tiles, group size, type, ragged widths, strides, splits, graphs."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from _util import activations
+from _w4 import assert_product, packed_codes, product, quantize
+
+pytestmark = pytest.mark.gpu
+
+TYPES = {"bf16": torch.bfloat16, "f16": torch.float16}
+
+
+def _weights(n, k, group, zeros, dtype, device, seed=0):
+    """Codes over their whole range, scales of either sign, zero points: rows on the host and the packed form."""
+    gen = torch.Generator().manual_seed(seed + n + k)
+    groups = -(-k // group)
+    codes = torch.randint(0, 256, (n, k // 2), generator=gen, dtype=torch.uint8)
+    scales = (torch.randn(n, groups, generator=gen) * k ** -0.5 * 0.25).to(dtype)
+    points = torch.randint(0, 16, (n, groups), generator=gen, dtype=torch.uint8) if zeros else None
+    return codes, scales, points
+
+
+def _pack(ops, device, codes, scales, points, group):
+    up = lambda t: None if t is None else t.to(device)
+    return ops.pack_w4(up(codes), up(scales), up(points), group=group)
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("group", [32, 64, 128, 256])
+@pytest.mark.parametrize("m", [1, 13, 16, 17, 32, 33, 64, 65, 130, 200])
+@pytest.mark.parametrize("n,k", [(48, 64), (201, 528), (1000, 1040)])
+def test_w4_mm(ops, device, m, n, k, group, dtype, zeros):
+    kind = TYPES[dtype]
+    rows = _weights(n, k, group, zeros, kind, device)
+    w = _pack(ops, device, *rows, group)
+    x = activations(m, k, seed=m, outlier_channels=3).to(kind).to(device)
+    bias = torch.randn(n, generator=torch.Generator().manual_seed(n)).to(kind).to(device) if m % 2 else None
+    got = ops.w4_mm(x, w, bias=bias)
+    assert got.shape == (m, n) and got.dtype == kind
+    assert_product(got, *product(x, *rows, group, bias))
+
+
+@pytest.mark.parametrize("m,n,k,group", [(1, 5376, 7168, 128), (5, 16, 14336, 128), (48, 256, 14336, 64),
+                                         (100, 5376, 7168, 32), (700, 2048, 2048, 128), (2500, 1000, 512, 128),
+                                         (1111, 5376, 1040, 64), (1, 1, 16, 32), (64, 1, 16, 32), (300, 17, 16, 128),
+                                         (2048, 4096, 256, 32)])
+def test_w4_mm_sizes(ops, device, m, n, k, group):
+    rows = _weights(n, k, group, True, torch.bfloat16, device)
+    w = _pack(ops, device, *rows, group)
+    x = activations(m, k, seed=m).to(device)
+    got = ops.w4_mm(x, w)
+    assert_product(got, *product(x, *rows, group))
+    again = ops.w4_mm(x, w)
+    assert torch.equal(got, again)  # sums in a fixed order
+
+
+@pytest.mark.parametrize("group", [32, 128, 384])
+@pytest.mark.parametrize("m", [1, 20, 100, 1000])
+def test_w4_mm_single_columns(ops, device, m, group):
+    """x picks one column a row: every product is s (u - z), exact in both types."""
+    n, k = 333, 464
+    rows = _weights(n, k, group, True, torch.bfloat16, device)
+    scales = torch.exp2(torch.randint(-8, 3, rows[1].shape, generator=torch.Generator().manual_seed(1)).float())
+    rows = rows[0], scales.to(torch.bfloat16), rows[2]
+    w = _pack(ops, device, *rows, group)
+    x = torch.zeros(m, k, dtype=torch.bfloat16)
+    at = torch.randperm(k, generator=torch.Generator().manual_seed(2)).repeat(3)[:m]
+    x[torch.arange(m), at] = 1.0
+    want, _ = product(x, *rows, group)
+    assert torch.equal(ops.w4_mm(x.to(device), w).cpu().double(), want)
+
+
+@pytest.mark.parametrize("m", [7, 40, 900])
+def test_w4_mm_strides_and_scale_types(ops, device, m):
+    """Rows of wider x and out, an unaligned out and bias, scales of the other type; the rest of out is left."""
+    n, k, group = 99, 272, 64
+    rows = _weights(n, k, group, True, torch.float16, device)
+    w = _pack(ops, device, *rows, group)
+    wide = activations(m, k + 24, seed=m).to(device)
+    x = wide[:, 8:8 + k]
+    bias = torch.randn(n + 1, generator=torch.Generator().manual_seed(3)).to(torch.bfloat16).to(device)[1:]
+    whole = torch.full((m + 1, n + 7), 5.0, device=device, dtype=torch.bfloat16)
+    out = whole[:m, 3:3 + n]
+    assert ops.w4_mm(x, w, bias=bias, out=out).data_ptr() == out.data_ptr()
+    assert_product(out, *product(x, *rows, group, bias))
+    assert (whole[:, :3] == 5.0).all() and (whole[:, 3 + n:] == 5.0).all() and (whole[m] == 5.0).all()
+
+
+@pytest.mark.parametrize("m", [3, 150])
+def test_w4_mm_other_rows_of_x_do_not_reach_a_row(ops, device, m):
+    """Infinities and NaN in one row of x, and in the columns behind k of a wider x, stay there."""
+    n, k, group = 64, 208, 32
+    rows = _weights(n, k, group, False, torch.bfloat16, device)
+    w = _pack(ops, device, *rows, group)
+    wide = activations(m, k + 16, seed=m).to(device)
+    clean = ops.w4_mm(wide[:, :k], w)
+    wide[:, k:] = float("nan")
+    wide[1, 5], wide[1, 100] = float("inf"), float("nan")
+    got = ops.w4_mm(wide[:, :k], w)
+    others = [i for i in range(m) if i != 1]
+    assert torch.equal(got[others], clean[others]) and not torch.isfinite(got[1]).any()
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("n,k,group", [(1, 16, 32), (37, 208, 32), (16, 1024, 128), (70, 400, 256), (5, 96, 64)])
+def test_pack_and_quantize(ops, device, n, k, group, zeros):
+    for dtype in (torch.bfloat16, torch.float16, torch.float32):
+        w = torch.randn(n, k, generator=torch.Generator().manual_seed(n + k)).to(dtype)
+        w[n // 2, :16] = 0.0
+        want = quantize(w, group, zeros)
+        got = ops.quantize_w4(w.to(device), group, zeros=zeros)
+        assert torch.equal(got[0].cpu(), want[0]) and torch.equal(got[1].cpu(), want[1]) and got[1].dtype == want[1].dtype
+        assert (got[2] is None) == (not zeros) and (not zeros or torch.equal(got[2].cpu(), want[2]))
+        packed = ops.pack_w4(*got, group=group)
+        assert torch.equal(packed.codes.cpu(), packed_codes(want[0]))
+        blocks, groups = -(-n // 16), -(-k // group)
+        for label, rows in (("scales", want[1]), ("zeros", want[2])):
+            if rows is None:
+                continue
+            full = torch.zeros(blocks * 16, groups, dtype=rows.dtype)
+            full[:n] = rows
+            assert torch.equal(getattr(packed, label).cpu(), full.view(blocks, 16, groups).transpose(1, 2))
+
+
+def test_quantize_and_pack_of_strided_rows(ops, device):
+    w = torch.randn(20, 200, generator=torch.Generator().manual_seed(5)).to(torch.bfloat16).to(device)
+    want = ops.quantize_w4(w[:, 3:163].contiguous(), 32, zeros=True)
+    got = ops.quantize_w4(w[:, 3:163], 32, zeros=True)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    wide = [torch.cat((t, t), dim=1) for t in want]
+    sliced = [t[:, :t.shape[1] // 2] for t in wide]
+    for a, b in zip(ops.pack_w4(*sliced, group=32)[:3], ops.pack_w4(*want, group=32)[:3]):
+        assert torch.equal(a, b)
+
+
+def test_w4_refuses(ops, device):
+    rows = _weights(32, 64, 32, True, torch.bfloat16, device)
+    w = _pack(ops, device, *rows, 32)
+    x = activations(4, 64).to(device)
+    with pytest.raises(TypeError):
+        ops.w4_mm(x.float(), w)
+    with pytest.raises(ValueError):
+        ops.w4_mm(x[:, :48], w)
+    with pytest.raises(ValueError):
+        ops.w4_mm(x[0], w)
+    with pytest.raises(RuntimeError, match="ldx"):
+        ops.w4_mm(torch.zeros(4, 68, device=device, dtype=x.dtype)[:, :64], w)
+    with pytest.raises(RuntimeError, match="aligned"):
+        ops.w4_mm(torch.zeros(4, 72, device=device, dtype=x.dtype)[:, 4:68], w)
+    with pytest.raises(TypeError):
+        ops.w4_mm(x, w, bias=torch.zeros(32, device=device))
+    with pytest.raises(ValueError):
+        ops.w4_mm(x, w, bias=torch.zeros(31, device=device, dtype=x.dtype))
+    with pytest.raises(ValueError):
+        ops.w4_mm(x, w, out=torch.zeros(4, 31, device=device, dtype=x.dtype))
+    with pytest.raises(ValueError):
+        ops.w4_mm(x, w, out=torch.zeros(1, 32, device=device, dtype=x.dtype).expand(4, 32))
+    with pytest.raises(ValueError):
+        ops.w4_mm(x, w._replace(group=64))
+    with pytest.raises(ValueError):
+        ops.w4_mm(x, w._replace(n=33))
+    with pytest.raises(TypeError):
+        ops.w4_mm(x, w._replace(scales=w.scales.float()))
+    with pytest.raises(RuntimeError):
+        ops.w4_mm(x, w._replace(codes=w.codes.cpu()))
+    codes, scales, points = (t.to(device) for t in rows)
+    with pytest.raises(ValueError):
+        ops.pack_w4(codes, scales, points, group=64)
+    with pytest.raises(ValueError):
+        ops.pack_w4(codes, scales, points, group=48)
+    with pytest.raises(TypeError):
+        ops.pack_w4(codes, scales.float(), points, group=32)
+    with pytest.raises(TypeError):
+        ops.pack_w4(codes.int(), scales, points, group=32)
+    with pytest.raises(ValueError):
+        ops.quantize_w4(x[:, :40])
+    with pytest.raises(TypeError):
+        ops.quantize_w4(x.double())
+    assert ops.w4_mm(x[:0], w).shape == (0, 32)
+
+
+def test_w4_mm_in_a_graph_and_on_a_stream(ops, device):
+    """Captured once over the three kinds of call (their workspaces are the graph's own), replayed with new
+    inputs and eager work between; and eager on another stream."""
+    rows = _weights(1000, 1040, 64, True, torch.bfloat16, device)
+    w = _pack(ops, device, *rows, 64)
+    xs = [activations(m, 1040, seed=m).to(device) for m in (3, 90, 1500)]
+    outs = [torch.empty(x.shape[0], 1000, device=device, dtype=x.dtype) for x in xs]
+
+    def run():
+        for x, out in zip(xs, outs):
+            ops.w4_mm(x, w, out=out)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    for x, out in zip(xs, outs):
+        assert torch.equal(out, ops.w4_mm(x, w))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    for replay in range(3):
+        for x in xs:
+            x.copy_(activations(x.shape[0], 1040, seed=50 + replay).to(device))
+        want = [ops.w4_mm(x, w) for x in xs]
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for out, y in zip(outs, want):
+            assert torch.equal(out, y)
+
+
+def test_w4_python_body_equals_native(ops, device, monkeypatch):
+    rows = _weights(200, 528, 32, True, torch.float16, device)
+    w = _pack(ops, device, *rows, 32)
+    xs = [activations(m, 528, seed=m).half().to(device) for m in (1, 70)]
+    bias = torch.ones(200, device=device, dtype=torch.float16)
+    want = [ops.w4_mm(x, w, bias=bias) for x in xs]
+    taken = []
+    monkeypatch.setattr(ops, "_native_call", lambda name, *a: taken.append(name))
+    for x, y in zip(xs, want):
+        assert torch.equal(ops.w4_mm(x, w, bias=bias), y)
+    assert taken == ["w4_mm", "w4_mm"]
