@@ -1079,9 +1079,9 @@ __attribute__((visibility("default"))) int h3q_w4_quantize(const void* w, int dt
 
 __attribute__((visibility("default"))) int64_t h3q_w4_mm_workspace_bytes(int64_t m, int64_t n, int64_t k, int64_t group) {
     if (m <= h3q::kW4StreamRows || n <= 0 || k <= 0 || k > (int64_t(1) << 22) || group <= 0 ||
-        !h3q::w4_tile_fits(m, n, k, (int)group))
+        !h3q::w4_tile_fits(m, n))
         return 0;
-    return h3q::w4_tile_workspace_bytes(m, n, k, (int)group);
+    return h3q::w4_tile_workspace_bytes(m, n, k);
 }
 
 __attribute__((visibility("default"))) int h3q_w4_mm(int dtype, const void* x, int64_t ldx, const void* codes,
@@ -1113,6 +1113,8 @@ __attribute__((visibility("default"))) int h3q_w4_mm(int dtype, const void* x, i
     a.group = (int)group;
     a.groups = (int)w4_groups(k, group);
     a.blocks_per_group = group >= 128 ? (int)(group / 128) : 1;
+    const int64_t span = group / 32;  // blocks of four groups
+    a.group_shift = (span & (span - 1)) == 0 ? __builtin_ctzll((unsigned long long)span) : -1;
     a.codes = (const uint8_t*)codes;
     a.scales = (const uint16_t*)scales;
     a.zeros = (const uint8_t*)zeros;
@@ -1123,11 +1125,11 @@ __attribute__((visibility("default"))) int h3q_w4_mm(int dtype, const void* x, i
     a.scales_f16 = scale_dtype == H3Q_DTYPE_F16;
     a.out_vec = aligned(out, 8) && ldo % 4 == 0;
     if (m <= h3q::kW4StreamRows) return check_launch(h3q::launch_w4_stream(a, (hipStream_t)stream), who);
-    if (!h3q::w4_tile_fits(m, n, k, (int)group))
+    if (!h3q::w4_tile_fits(m, n))
         return fail(H3Q_ERR_UNSUPPORTED, "%s: %lld rows of %lld x %lld are too many for one launch", who, (long long)m,
                     (long long)n, (long long)k);
-    const int64_t need = h3q::w4_tile_workspace_bytes(m, n, k, (int)group);
-    if (!workspace || !aligned(workspace, 16) || workspace_bytes < need)
+    const int64_t need = h3q::w4_tile_workspace_bytes(m, n, k);
+    if (need > 0 && (!workspace || !aligned(workspace, 16) || workspace_bytes < need))
         return fail(H3Q_ERR_INVALID, "%s: workspace of %lld bytes, %lld needed (16-byte aligned)", who,
                     (long long)workspace_bytes, (long long)need);
     return check_launch(h3q::launch_w4_tile(a, workspace, (hipStream_t)stream), who);

@@ -326,7 +326,9 @@ hipError_t launch_plan_append(const PlanAppendArgs& a, hipStream_t st);
 struct W4Args {
     const uint16_t* x;  // bf16 or binary16 [m, k], ldx elements
     int64_t ldx, m, n, k;
-    int group, groups, blocks_per_group;  // blocks of 128 columns in a group of 128 or more
+    int group, groups;
+    int blocks_per_group;  // 128-column blocks of a group (1 below 128 columns)
+    int group_shift;       // log2 of the blocks that four groups span, -1: no power of two
     const uint8_t* codes;
     const uint16_t* scales;  // bf16, or binary16 (scales_f16)
     const uint8_t* zeros;    // null: 8 everywhere
@@ -337,8 +339,8 @@ struct W4Args {
 };
 constexpr int kW4StreamRows = 32;
 hipError_t launch_w4_stream(const W4Args& a, hipStream_t st);
-bool w4_tile_fits(int64_t m, int64_t n, int64_t k, int group);  // a launch's grid and the sums' 32-bit offsets
-int64_t w4_tile_workspace_bytes(int64_t m, int64_t n, int64_t k, int group);
+bool w4_tile_fits(int64_t m, int64_t n);  // a launch's grid
+int64_t w4_tile_workspace_bytes(int64_t m, int64_t n, int64_t k);
 hipError_t launch_w4_tile(const W4Args& a, void* workspace, hipStream_t st);
 // Codes two a byte [n, k / 2] (the low nibble first), scales and zeros [n, groups] -> the layout.
 struct W4PackArgs {

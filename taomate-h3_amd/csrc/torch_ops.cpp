@@ -591,12 +591,14 @@ Opt w4_mm(const Tensor& x, const Tensor& codes, const Tensor& scales, const Opt&
     if (!x.is_cuda() || (type != at::kBFloat16 && type != at::kHalf) || !rows_2d(x, type) || x.size(1) != k ||
         x.size(0) == 0 || n < 1 || k < 16 || group < 32)
         return std::nullopt;
-    const int64_t m = x.size(0), blocks = (n + 15) / 16, groups = (k + group - 1) / group;
-    const auto packed = [&](const Tensor& t, at::ScalarType of, int64_t b, int64_t c) {
-        return dense(t, x, of) && t.dim() == 3 && t.size(0) == blocks && t.size(1) == b && t.size(2) == c;
+    const int64_t m = x.size(0), blocks = (n + 15) / 16, quads = ((k + group - 1) / group + 3) / 4;
+    const auto packed = [&](const Tensor& t, at::ScalarType of) {
+        return dense(t, x, of) && t.dim() == 4 && t.size(0) == blocks && t.size(1) == quads && t.size(2) == 16 &&
+               t.size(3) == 4;
     };
-    if ((scale_type != at::kBFloat16 && scale_type != at::kHalf) || !packed(codes, at::kByte, (k + 127) / 128, 1024) ||
-        !packed(scales, scale_type, groups, 16) || (zeros && !packed(*zeros, at::kByte, groups, 16)))
+    if ((scale_type != at::kBFloat16 && scale_type != at::kHalf) || !dense(codes, x, at::kByte) || codes.dim() != 3 ||
+        codes.size(0) != blocks || codes.size(1) != (k + 127) / 128 || codes.size(2) != 1024 ||
+        !packed(scales, scale_type) || (zeros && !packed(*zeros, at::kByte)))
         return std::nullopt;
     if (bias && !(dense(*bias, x, type) && bias->dim() == 1 && bias->size(0) == n)) return std::nullopt;
     if (out && !(on(*out, x) && rows_2d(*out, type) && out->size(0) == m && out->size(1) == n && apart(*out)))

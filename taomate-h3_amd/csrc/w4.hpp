@@ -1,18 +1,23 @@
-// 4-bit weights with group scales: layout, unpacking and the arguments that the kernels share.
+// 4-bit weights with group scales: layout, unpacking and what the kernels share.
 //
-//   y[m, n] = sum_g s[n, g] * sum_{k in g} x[m, k] (u[n, k] - z[n, g])  [+ bias[n]]
+//   y[m, n] = sum_k x[m, k] * w[n, k]  [+ bias[n]],   w[n, k] = rn(s[n, g] * (u[n, k] - z[n, g])), g = k / group
+//
+// The weight is rounded once, to x's 16-bit type, because the matrix instructions multiply that type; the product
+// before it is exact in binary32 (an 11-bit scale times a 5-bit integer), so w is one definite matrix, the same
+// for every kernel and row count.  It costs 1.1 times the rounding error of the output alone.  The other way, the
+// integers in the matrix instructions and the scale on every group's sum, was built and measured first: 4096 rows of
+// 14336 x 5376 took 600 us at groups of 128 without zero points, but 1330 us at groups of 32 with them, because
+// each group costs an fma and an offset for every output, where rounding costs the same for all groups.
 //
 // Layout.  Codes lie in blocks of 16 rows x 128 columns, 1 KiB, [row blocks][column blocks]: lane L's 16 bytes
-// are four words, word s the eight codes k = 128 b + 32 s + 8 (L / 16) .. + 7 of row L % 16, which is the
-// operand of one v_mfma_f32_16x16x32 (a wave's load of a block is one contiguous KiB).  Scales (bf16 or binary16)
-// and zero points (bytes) lie as [row blocks][groups][16].
+// are four words, word s the eight codes k = 128 b + 32 s + 8 (L / 16) .. + 7 of row L % 16, from the low nibble
+// k0 k2 k4 k6 k1 k3 k5 k7: the operand of one v_mfma_f32_16x16x32, and with the lanes' 16 bytes taken as row L % 32
+// and k quarter L / 32 (+ 2) of two blocks, of two v_mfma_f32_32x32x16.  Scales (bf16 or binary16) and zero
+// points (bytes) lie as [row blocks][groups / 4][16][4]: a lane's row has four groups in one load.
 //
-// Unpacking.  A code in the middle of a 16-bit float's mantissa is a number: with the exponent of 16 and the
-// nibble in the top mantissa bits the float is 16 + u exactly.  The word holds the pairs (k0, k1), (k2, k3),
-// (k4, k5), (k6, k7) at bits {3, 19}, {7, 23}, {11, 27}, {15, 31 wrapped}, so a pair takes one shift or rotation
-// and one and-or: 7 operations for 8 codes (bf16; 8 in binary16, whose mantissa is longer).  Each group's
-// product then carries (16 + z) sum(x) too much, which is taken off in binary32 before the group's scale; an
-// offset of 16 costs the sum under 3 bits of binary32's 24, where the 128 of a whole bf16 mantissa would cost 5.
+// Unpacking.  A byte 0 .. 15 is the e4m3 number of 2^-9 times its value (subnormals up to 7, then the first
+// binade, of the same step), so v_cvt_pk_f32_fp8 turns two masked nibbles into binary32 at once: three mask
+// operations, four conversions, eight fmas with 2^9 s and -z s, four roundings to pairs for eight codes.
 #pragma once
 
 #include "h3q_common.hpp"
@@ -21,45 +26,50 @@
 namespace h3q {
 
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 
 constexpr uint32_t kW4Oob = 0x80000000u;  // beyond every descriptor's range: loads return 0
-constexpr int kW4Stream = 2;              // cache policy of loads that are read once: non-temporal
 
 template <bool F16>
-__device__ __forceinline__ v4u w4_unpack(uint32_t w) {
-    constexpr uint32_t mask = F16 ? 0x03C003C0u : 0x00780078u, one = F16 ? 0x4C004C00u : 0x41804180u;
-    v4u d;
-    d[0] = ((F16 ? w << 3 : w) & mask) | one;
-    d[1] = ((F16 ? w >> 1 : w >> 4) & mask) | one;
-    d[2] = ((F16 ? w >> 5 : w >> 8) & mask) | one;
-    d[3] = (__builtin_amdgcn_alignbit(w, w, F16 ? 9 : 12) & mask) | one;
-    return d;
+__device__ __forceinline__ uint32_t w4_pair(float lo, float hi) {
+    if constexpr (F16) return __builtin_bit_cast(uint32_t, __builtin_convertvector(v2f{lo, hi}, v2h));
+    else return pack_bf16x2(lo, hi);
 }
 
+// Eight codes of a row -> its weights: scale = 2^9 s, shift = -z s.
 template <bool F16>
-__device__ __forceinline__ v4f w4_mfma(v4u a, v4u b, v4f c) {
-    if constexpr (F16)
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
-    else
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0,
-                                                       0);
+__device__ __forceinline__ v4u w4_weights(uint32_t w, float scale, float shift) {
+    const int even = (int)(w & 0x0F0F0F0Fu), odd = (int)(w >> 4 & 0x0F0F0F0Fu);
+    const v2f a = __builtin_amdgcn_cvt_pk_f32_fp8(even, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(even, true);
+    const v2f c = __builtin_amdgcn_cvt_pk_f32_fp8(odd, false), d = __builtin_amdgcn_cvt_pk_f32_fp8(odd, true);
+    const auto f = [&](float v) { return __builtin_fmaf(v, scale, shift); };
+    return v4u{w4_pair<F16>(f(a[0]), f(b[0])), w4_pair<F16>(f(c[0]), f(d[0])), w4_pair<F16>(f(a[1]), f(b[1])),
+               w4_pair<F16>(f(c[1]), f(d[1]))};
 }
 
-__device__ __forceinline__ v4u w4_load16(__amdgpu_buffer_rsrc_t r, uint32_t off, int policy) {
-    return policy == kW4Stream ? __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, kW4Stream)
-                               : __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0);
+// Scale and shift of a row for its group `e` of the four in `s` and `z` (e wave-uniform).
+__device__ __forceinline__ void w4_group(v2u s, uint32_t z, int e, bool f16, float& scale, float& shift) {
+    const uint32_t pair = e & 2 ? s[1] : s[0], bits = e & 1 ? pair >> 16 : pair;
+    const float v = f16 ? f16_lo(bits) : bf16_lo(bits);
+    scale = v * 512.0f;
+    shift = -v * (float)(z >> (8 * e) & 255u);
 }
 
-// A lane's four scales (one of four consecutive rows each) and zero points of a group.
-__device__ __forceinline__ v4f w4_scales(v2u w, bool f16) {
-    return f16 ? v4f{f16_lo(w[0]), f16_hi(w[0]), f16_lo(w[1]), f16_hi(w[1])}
-               : v4f{bf16_lo(w[0]), bf16_hi(w[0]), bf16_lo(w[1]), bf16_hi(w[1])};
+// A descriptor whose words are in scalar registers for sure: where the compiler loses sight of that, every load
+// through it becomes a loop over the lanes' values.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t w4_rsrc(const void* base, int64_t bytes) {
+    const uint64_t b = (uint64_t)base;
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)b), hi = __builtin_amdgcn_readfirstlane((uint32_t)(b >> 32));
+    return make_rsrc((const void*)((uint64_t)hi << 32 | lo), __builtin_amdgcn_readfirstlane((uint32_t)bytes));
 }
-template <bool ZEROS>
-__device__ __forceinline__ v4f w4_offsets(uint32_t z) {
-    if constexpr (!ZEROS) return v4f{24.0f, 24.0f, 24.0f, 24.0f};  // 16 and a zero point of 8
-    return v4f{16.0f + (float)(z & 255), 16.0f + (float)(z >> 8 & 255), 16.0f + (float)(z >> 16 & 255),
-               16.0f + (float)(z >> 24)};
+
+// The four-group entry of block b's first group, and the group of its 32-column step s in that entry.
+__device__ __forceinline__ int w4_quad(const W4Args& p, int b) {
+    return p.group_shift >= 0 ? b >> p.group_shift : b / (4 * p.blocks_per_group);
+}
+__device__ __forceinline__ int w4_element(const W4Args& p, int b, int s) {
+    if (p.group < 128) return p.group == 32 ? s : 2 * (b & 1) + (s >> 1);
+    return (p.group_shift >= 0 ? b >> (p.group_shift - 2) : b / p.blocks_per_group) & 3;
 }
 
 // out[m, n .. n + 3] = y + bias, rounded once; rows and columns past the end are dropped.

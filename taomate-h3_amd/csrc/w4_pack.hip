@@ -18,15 +18,17 @@ __global__ __launch_bounds__(256) void w4_pack_kernel(W4PackArgs p, int64_t word
 #pragma unroll
             for (int j = 0; j < 4; ++j) w |= (uint32_t)(c[j] & 15) << (4 * j) | (uint32_t)(c[j] >> 4) << (16 + 4 * j);
         }
-        ((uint32_t*)p.codes_out)[i] = w << 3 | w >> 29;
+        ((uint32_t*)p.codes_out)[i] = w;
     }
 }
 
 __global__ __launch_bounds__(256) void w4_pack_scales_kernel(W4PackArgs p, int64_t count) {
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256) {
-        const int64_t panel = i >> 4, g = panel % p.groups, row = panel / p.groups * 16 + (i & 15);
-        p.scales_out[i] = row < p.n ? p.scales[row * p.lds + g] : 0;
-        if (p.zeros) p.zeros_out[i] = row < p.n ? p.zeros[row * p.ldz + g] & 15 : 0;
+        const int64_t quads = (p.groups + 3) / 4, panel = i >> 6;
+        const int64_t g = panel % quads * 4 + (i & 3), row = panel / quads * 16 + (i >> 2 & 15);
+        const bool in = row < p.n && g < p.groups;
+        p.scales_out[i] = in ? p.scales[row * p.lds + g] : 0;
+        if (p.zeros) p.zeros_out[i] = in ? p.zeros[row * p.ldz + g] & 15 : 0;
     }
 }
 
@@ -84,7 +86,7 @@ unsigned blocks_for(int64_t threads) {
 
 hipError_t launch_w4_pack(const W4PackArgs& a, hipStream_t st) {
     const int64_t blocks = (a.n + 15) / 16, steps = (a.k + 127) / 128;
-    const int64_t words = blocks * steps * 256, count = blocks * a.groups * 16;
+    const int64_t words = blocks * steps * 256, count = blocks * ((a.groups + 3) / 4) * 64;
     hipLaunchKernelGGL(w4_pack_kernel, dim3(blocks_for(words)), dim3(256), 0, st, a, words, (int)steps);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;

@@ -1,14 +1,11 @@
-// Product with 4-bit weights for many rows, gfx950: bound by the matrix instructions.
+// Product with 4-bit weights for many rows, gfx950: bound by the matrix instructions (and, below 128 rows to a
+// tile, by the unpacking: 19 operations for 8 codes, once for every row tile).
 //
-// A workgroup of four waves owns a tile of 16 TB rows x 64 JB columns, each wave all rows and 16 JB of the
-// columns, so every code is unpacked once in a workgroup.  Per 128 columns of k the x tile is copied into LDS in
-// operand order (double-buffered, buffer_load ... lds, no registers), the codes go straight into registers one
-// block ahead, and one barrier a block closes both.  A group's product is accumulated apart from zero (rather:
-// from -(16 + z) sum(x), the offset of the unpacked codes, so no subtraction follows), then added to the tile's
-// sums with the group's scale: one binary32 fma for 128 (or 64, 32) multiply-adds.
-//
-// sum(x) of every group and row comes from a small kernel in front (x is read once more); a wave's own sums
-// would cost it as many matrix instructions as one column block.
+// A workgroup of four waves owns a tile of 32 MT rows x 128 NT columns, each wave all rows and 32 NT of the
+// columns, so every code is unpacked once in a workgroup, straight into operand registers.  Per 128 columns of k the
+// x tile is copied into an LDS ring of D stages (buffer_load ... lds, no registers; a row is 256 contiguous bytes,
+// its 16-byte chunk c in slot c ^ (row % 16), so that 16 rows' reads of one chunk meet no bank twice), and the
+// codes, scales and zero points into registers as many blocks ahead.  One barrier a block.
 //
 // Few tiles: k is split over several workgroups, whose binary32 sums a last kernel adds in order.
 #include "w4.hpp"
@@ -19,20 +16,27 @@ namespace {
 
 struct TileArgs {
     W4Args w;
-    const float* sums;  // [steps * GPB][mpad]
-    float* parts;       // [splits][m][npad], null: not split
-    int mpad, npad, mtiles, ntiles, splits, per_split, steps;
+    float* parts;  // [splits][m][npad], null: not split
+    int npad, mtiles, ntiles, splits, per_split, steps;
 };
 
-template <bool F16, bool ZEROS, int GPB, int JB, int TB>
+template <bool F16>
+__device__ __forceinline__ v16f mfma32(v4u a, v4u b, v16f c) {
+    if constexpr (F16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0,
+                                                       0);
+}
+
+template <bool F16, int NT, int MT, int D>
 __global__ __launch_bounds__(256, 2) void w4_tile_kernel(TileArgs p) {
-    constexpr int SPG = 4 / GPB;
-    constexpr int XBYTES = TB * 4 * 1024, SBYTES = GPB * 1024;
-    __shared__ __attribute__((aligned(1024))) uint8_t lds_raw[2 * (XBYTES + SBYTES)];
+    constexpr int STAGE = MT * 32 * 256;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds_raw[D * STAGE];
     H3Q_LDS uint8_t* const lds = (H3Q_LDS uint8_t*)lds_raw;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int r16 = lane & 15, kq = lane >> 4;
+    const int r32 = lane & 31, half = lane >> 5;
 
     // Workgroups b, b + 8, ... share an XCD: each gets a contiguous run of tiles, in bands of 8 row tiles
     // with the row tile fastest.
@@ -42,150 +46,128 @@ __global__ __launch_bounds__(256, 2) void w4_tile_kernel(TileArgs p) {
         const int q = total / 8, r = total % 8, x = id % 8;
         id = x * q + (x < r ? x : r) + id / 8;
     }
-    const int z = id % p.splits;
+    const int z = __builtin_amdgcn_readfirstlane(id % p.splits);  // a division leaves the scalar registers
     id /= p.splits;
     const int band = id / (8 * p.ntiles), in = id % (8 * p.ntiles);
     const int high = p.mtiles - band * 8 < 8 ? p.mtiles - band * 8 : 8;
-    const int mt = band * 8 + in % high, nt = in / high;
+    const int mt = __builtin_amdgcn_readfirstlane(band * 8 + in % high);
+    const int nt = __builtin_amdgcn_readfirstlane(in / high);
 
-    const int64_t m0 = (int64_t)mt * 16 * TB;
-    const int blk0 = nt * 4 * JB + wave * JB, blocks = (int)((p.w.n + 15) / 16);
-    const int nblk = blocks - blk0 < 0 ? 0 : blocks - blk0 < JB ? blocks - blk0 : JB;
-    const int groups = p.w.groups, steps = p.steps;
-    const int64_t rows = p.w.m - m0 < 16 * TB ? p.w.m - m0 : 16 * TB;
+    const int64_t m0 = (int64_t)mt * 32 * MT;
+    const int blk0 = nt * 8 * NT + wave * 2 * NT, blocks = (int)((p.w.n + 15) / 16);
+    const int nblk = blocks - blk0 < 0 ? 0 : blocks - blk0 < 2 * NT ? blocks - blk0 : 2 * NT;
+    const int steps = p.steps, quads = (p.w.groups + 3) / 4;
+    const int64_t rows = p.w.m - m0 < 32 * MT ? p.w.m - m0 : 32 * MT;
     const CopySrc rx(p.w.x + m0 * p.w.ldx, (uint32_t)(((rows - 1) * p.w.ldx + p.w.k) * 2));
-    const CopySrc rsum(p.sums, (uint32_t)((int64_t)steps * GPB * p.mpad * 4));
     const int64_t first = nblk > 0 ? blk0 : 0;
-    const __amdgpu_buffer_rsrc_t rw = make_rsrc(p.w.codes + first * steps * 1024, (uint32_t)(nblk * steps * 1024));
-    const __amdgpu_buffer_rsrc_t rs = make_rsrc(p.w.scales + first * groups * 16, (uint32_t)(nblk * groups * 32));
+    const __amdgpu_buffer_rsrc_t rw = w4_rsrc(p.w.codes + first * steps * 1024, (int64_t)nblk * steps * 1024);
+    const __amdgpu_buffer_rsrc_t rs = w4_rsrc(p.w.scales + first * quads * 64, (int64_t)nblk * quads * 128);
     const __amdgpu_buffer_rsrc_t rz =
-        make_rsrc(p.w.zeros + (ZEROS ? first * groups * 16 : 0), ZEROS ? (uint32_t)(nblk * groups * 16) : 0);
+        w4_rsrc(p.w.zeros + (p.w.zeros ? first * quads * 64 : 0), p.w.zeros ? (int64_t)nblk * quads * 64 : 0);
     const uint32_t row_bytes = (uint32_t)(p.w.ldx * 2);
 
-    // Wave w copies the 32 columns 32 w .. + 31 of each 16-row block, and the sums of group w of the block.
-    auto copy = [&](int b, int buf) __attribute__((always_inline)) {
-        const uint32_t base = (uint32_t)(uintptr_t)(lds + buf * (XBYTES + SBYTES));
-        const uint32_t off = 128 * b + 32 * wave + 8 * kq < p.w.k
-                                 ? r16 * row_bytes + 256u * b + 64u * wave + 16u * kq : kW4Oob;
+    // A copy instruction takes four rows; wave w the rows 4 w .. + 3 of every 16.
+    const int crow = 4 * wave + (lane >> 4), chunk = (lane & 15) ^ crow;
+    constexpr int COPIES = 2 * MT;
+    auto copy = [&](int b, int stage) __attribute__((always_inline)) {
+        const uint32_t base = (uint32_t)(uintptr_t)(lds + stage * STAGE);
+        const uint32_t off =
+            128 * b + 8 * chunk < p.w.k ? crow * row_bytes + 256u * b + 16u * chunk : kW4Oob;
 #pragma unroll
-        for (int t = 0; t < TB; ++t)
-            copy16(rx, base + (4 * t + wave) * 1024, off == kW4Oob ? kW4Oob : off + 16u * t * row_bytes);
-        if (wave < GPB)
-            copy16(rsum, base + XBYTES + wave * 1024,
-                   lane < 4 * TB ? (uint32_t)(((b * GPB + wave) * p.mpad + m0) * 4 + 16 * lane) : kW4Oob);
+        for (int i = 0; i < COPIES; ++i)
+            copy16(rx, base + (wave + 4 * i) * 1024, off == kW4Oob ? kW4Oob : off + 16u * i * row_bytes);
     };
-    v4u codes[JB];
-    v2u scales[JB][GPB];
-    uint32_t zeros[JB][GPB];
-    auto load = [&](int b) __attribute__((always_inline)) {
+    // Row r32 of 32-column tile j: its block and place there; k quarters half and half + 2.
+    uint32_t code_off[NT], scale_off[NT];
 #pragma unroll
-        for (int j = 0; j < JB; ++j) {
-            codes[j] = w4_load16(rw, (uint32_t)((j * steps + b) * 1024 + 16 * lane), 0);
+    for (int j = 0; j < NT; ++j) {
+        const int blk = 2 * j + (r32 >> 4);
+        code_off[j] = (uint32_t)(blk * steps * 1024 + ((r32 & 15) + 16 * half) * 16);
+        scale_off[j] = (uint32_t)(blk * quads * 16 + (r32 & 15));
+    }
+    v4u codes[D][NT][2];
+    v2u scales[D][NT];
+    uint32_t zeros[D][NT];
+    auto load = [&](int i, int b) __attribute__((always_inline)) {
+        const int q = w4_quad(p.w, b);
 #pragma unroll
-            for (int q = 0; q < GPB; ++q) {
-                const int g = GPB == 1 ? b / p.w.blocks_per_group : b * GPB + q;
-                scales[j][q] = __builtin_amdgcn_raw_buffer_load_b64(
-                    rs, g < groups ? (uint32_t)((j * groups + g) * 32 + 8 * kq) : kW4Oob, 0, 0);
-                zeros[j][q] = 0;
-                if constexpr (ZEROS)
-                    zeros[j][q] = __builtin_amdgcn_raw_buffer_load_b32(
-                        rz, g < groups ? (uint32_t)((j * groups + g) * 16 + 4 * kq) : kW4Oob, 0, 0);
-            }
+        for (int j = 0; j < NT; ++j) {
+            codes[i][j][0] = __builtin_amdgcn_raw_buffer_load_b128(rw, code_off[j] + 1024u * b, 0, 0);
+            codes[i][j][1] = __builtin_amdgcn_raw_buffer_load_b128(rw, code_off[j] + 1024u * b + 512u, 0, 0);
+            scales[i][j] = __builtin_amdgcn_raw_buffer_load_b64(rs, (scale_off[j] + 16u * q) * 8, 0, 0);
+            zeros[i][j] = 0x08080808u;
+            if (p.w.zeros) zeros[i][j] = __builtin_amdgcn_raw_buffer_load_b32(rz, (scale_off[j] + 16u * q) * 4, 0, 0);
         }
     };
 
-    v4f acc[JB][TB];
+    v16f acc[NT][MT];
 #pragma unroll
-    for (int j = 0; j < JB; ++j)
+    for (int j = 0; j < NT; ++j)
 #pragma unroll
-        for (int t = 0; t < TB; ++t) acc[j][t] = v4f{};
+        for (int t = 0; t < MT; ++t) acc[j][t] = v16f{};
+    // This lane's chunk of step (s, h) in a row: 4 s + 2 h + half.
+    uint32_t xoff[8];
+#pragma unroll
+    for (int c = 0; c < 8; ++c) xoff[c] = r32 * 256 + 16 * ((2 * c + half) ^ (r32 & 15));
 
     const int b0 = z * p.per_split, b1 = b0 + p.per_split < steps ? b0 + p.per_split : steps;
-    if (b0 < b1) {
-        copy(b0, 0);
-        load(b0);
-    }
-    for (int b = b0; b < b1; ++b) {
-        const int buf = (b - b0) & 1;
-        wait_vmcnt0();
-        __syncthreads();  // block b is in LDS, and every wave is done with the other buffer
-        v4u held[JB];
-        v4f scale[JB][GPB], off[JB][GPB];
+    // Blocks past b1 are copied nowhere (out of range), but counted: every stage has as many copies in flight.
+    auto ask = [&](int i, int b) __attribute__((always_inline)) {
+        load(i, b < b1 ? b : b1 - 1);
+        __builtin_amdgcn_sched_barrier(0);
+        copy(b < b1 ? b : steps, i);
+    };
 #pragma unroll
-        for (int j = 0; j < JB; ++j) {
-            held[j] = codes[j];
+    for (int i = 0; i < D - 1; ++i) ask(i, b0 + i);
+    for (int b = b0; b < b1; b += D) {
 #pragma unroll
-            for (int q = 0; q < GPB; ++q) {
-                scale[j][q] = w4_scales(scales[j][q], p.w.scales_f16);
-                off[j][q] = w4_offsets<ZEROS>(zeros[j][q]);
+        for (int i = 0; i < D; ++i) {
+            if (b + i >= b1) break;
+            // Stage i has landed: the D - 2 stages behind it may be under way (the loads among them are not
+            // counted, which makes the wait stricter than it has to be).
+            wait_vmcnt<(D - 2) * COPIES>();
+            __syncthreads();  // and every wave is done with the stage before it
+            ask((i + D - 1) % D, b + i + D - 1);
+            __builtin_amdgcn_sched_barrier(0);
+            const H3Q_LDS uint8_t* const tile = lds + i * STAGE;
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                const int e = w4_element(p.w, b + i, s);
+                v4u w[NT][2];
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    float scale, shift;
+                    w4_group(scales[i][j], zeros[i][j], e, p.w.scales_f16, scale, shift);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) w[j][h] = w4_weights<F16>(codes[i][j][h][s], scale, shift);
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int t = 0; t < MT; ++t) {
+                        const v4u x = *(const H3Q_LDS v4u*)(tile + xoff[2 * s + h] + t * 32 * 256);
+#pragma unroll
+                        for (int j = 0; j < NT; ++j) acc[j][t] = mfma32<F16>(w[j][h], x, acc[j][t]);
+                    }
             }
         }
-        if (b + 1 < b1) {
-            copy(b + 1, buf ^ 1);
-            load(b + 1);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        const H3Q_LDS uint8_t* const tile = lds + buf * (XBYTES + SBYTES);
-        const H3Q_LDS float* const sums = (const H3Q_LDS float*)(tile + XBYTES);
+    }
+    wait_vmcnt0();  // the last copies
+
 #pragma unroll
-        for (int q = 0; q < GPB; ++q) {
-            v4u w[JB][SPG];
+    for (int j = 0; j < NT; ++j)
 #pragma unroll
-            for (int j = 0; j < JB; ++j)
+        for (int t = 0; t < MT; ++t)
 #pragma unroll
-                for (int i = 0; i < SPG; ++i) w[j][i] = w4_unpack<F16>(held[j][q * SPG + i]);
-#pragma unroll
-            for (int t = 0; t < TB; ++t) {
-                v4u x[SPG];
-#pragma unroll
-                for (int i = 0; i < SPG; ++i)
-                    x[i] = *(const H3Q_LDS v4u*)(tile + (4 * t + q * SPG + i) * 1024 + 16 * lane);
-                const float sum = -sums[q * 256 + 16 * t + r16];
-                const float plain = 24.0f * sum;
-#pragma unroll
-                for (int j = 0; j < JB; ++j) {
-                    v4f part;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) part[e] = ZEROS ? off[j][q][e] * sum : plain;
-#pragma unroll
-                    for (int i = 0; i < SPG; ++i) part = w4_mfma<F16>(w[j][i], x[i], part);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[j][t][e] = __builtin_fmaf(scale[j][q][e], part[e], acc[j][t][e]);
+            for (int v = 0; v < 4; ++v) {
+                const v4f y = {acc[j][t][4 * v], acc[j][t][4 * v + 1], acc[j][t][4 * v + 2], acc[j][t][4 * v + 3]};
+                const int64_t m = m0 + 32 * t + r32, n = 16 * (int64_t)blk0 + 32 * j + 8 * v + 4 * half;
+                if (p.parts) {
+                    if (m < p.w.m && n < p.npad) *reinterpret_cast<v4f*>(p.parts + (z * p.w.m + m) * p.npad + n) = y;
+                } else {
+                    w4_store<F16>(p.w, m, n, y);
                 }
             }
-        }
-    }
-
-#pragma unroll
-    for (int j = 0; j < JB; ++j)
-#pragma unroll
-        for (int t = 0; t < TB; ++t) {
-            const int64_t m = m0 + 16 * t + r16, n = 16 * (int64_t)(blk0 + j) + 4 * kq;
-            if (p.parts) {
-                if (m < p.w.m && j < nblk) *reinterpret_cast<v4f*>(p.parts + (z * p.w.m + m) * p.npad + n) = acc[j][t];
-            } else {
-                w4_store<F16>(p.w, m, n, acc[j][t]);
-            }
-        }
-}
-
-// sums[i][m] = sum of x[m, size i .. size i + size - 1] (zeros past k), size 32, 64 or 128: a wave takes 512
-// columns of a row, 8 a lane.
-template <bool F16>
-__global__ __launch_bounds__(256) void w4_sums_kernel(W4Args p, float* sums, int mpad, int count, int lanes) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t m = (int64_t)blockIdx.x * 4 + wave;
-    if (m >= p.m) return;
-    const int64_t k = (int64_t)blockIdx.y * 512 + 8 * lane;
-    float s = 0.0f;
-    if (k < p.k) {
-        const uint4 v = *reinterpret_cast<const uint4*>(p.x + m * p.ldx + k);
-        s = ((out_lo(v.x, F16) + out_hi(v.x, F16)) + (out_lo(v.y, F16) + out_hi(v.y, F16))) +
-            ((out_lo(v.z, F16) + out_hi(v.z, F16)) + (out_lo(v.w, F16) + out_hi(v.w, F16)));
-    }
-    for (int off = lanes >> 1; off >= 1; off >>= 1) s += __shfl_xor(s, off, 64);
-    const int i = (int)(k / (8 * lanes));
-    if (lane % lanes == 0 && i < count) sums[(int64_t)i * mpad + m] = s;
 }
 
 template <bool F16>
@@ -199,78 +181,55 @@ __global__ __launch_bounds__(256) void w4_join_kernel(TileArgs p) {
 }
 
 struct Plan {
-    int jb, tb, splits, per_split, mtiles, ntiles, steps, mpad, npad, gpb;
-    int64_t sums_bytes, parts_bytes;
+    int nt, mt, splits, per_split, mtiles, ntiles, steps, npad;
+    int64_t parts_bytes;
 };
 
-Plan plan_tiles(int64_t m, int64_t n, int64_t k, int group) {
+Plan plan_tiles(int64_t m, int64_t n, int64_t k) {
     Plan p{};
     p.steps = (int)((k + 127) / 128);
-    p.gpb = group == 32 ? 4 : group == 64 ? 2 : 1;
-    const auto tiles = [&](int jb, int tb) { return ((m + 16 * tb - 1) / (16 * tb)) * ((n + 64 * jb - 1) / (64 * jb)); };
-    p.jb = 2;
-    p.tb = tiles(2, 8) < 256 ? 4 : 8;
-    p.mtiles = (int)((m + 16 * p.tb - 1) / (16 * p.tb));
-    p.ntiles = (int)((n + 64 * p.jb - 1) / (64 * p.jb));
-    const int64_t count = tiles(p.jb, p.tb);
+    const auto tiles = [&](int nt, int mt) { return ((m + 32 * mt - 1) / (32 * mt)) * ((n + 128 * nt - 1) / (128 * nt)); };
+    p.nt = 2;
+    p.mt = 4;
+    if (tiles(2, 4) < 256) p.nt = 1, p.mt = 2;
+    p.mtiles = (int)((m + 32 * p.mt - 1) / (32 * p.mt));
+    p.ntiles = (int)((n + 128 * p.nt - 1) / (128 * p.nt));
+    const int64_t count = tiles(p.nt, p.mt);
     int64_t splits = count >= 512 ? 1 : 512 / count;
     if (splits > 8) splits = 8;
     if (splits > p.steps / 4) splits = p.steps / 4 > 0 ? p.steps / 4 : 1;
     p.per_split = (int)((p.steps + splits - 1) / splits);
     p.splits = (p.steps + p.per_split - 1) / p.per_split;
-    p.mpad = p.mtiles * 16 * p.tb;
     p.npad = (int)((n + 15) / 16 * 16);
-    p.sums_bytes = ((int64_t)p.steps * p.gpb * p.mpad * 4 + 255) / 256 * 256;
     p.parts_bytes = p.splits > 1 ? (int64_t)p.splits * m * p.npad * 4 : 0;
     return p;
 }
 
-template <bool F16, bool ZEROS, int GPB>
-hipError_t launch_cfg(const TileArgs& a, const Plan& p, hipStream_t st) {
-    const dim3 grid((unsigned)(p.mtiles * p.ntiles * p.splits));
-    if (p.tb == 8) hipLaunchKernelGGL((w4_tile_kernel<F16, ZEROS, GPB, 2, 8>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((w4_tile_kernel<F16, ZEROS, GPB, 2, 4>), grid, dim3(256), 0, st, a);
-    return hipGetLastError();
-}
-
 template <bool F16>
 hipError_t launch_type(const TileArgs& a, const Plan& p, hipStream_t st) {
-    const W4Args& w = a.w;
-    hipLaunchKernelGGL((w4_sums_kernel<F16>), dim3((unsigned)((w.m + 3) / 4), (unsigned)((p.steps * 128 + 511) / 512)),
-                       dim3(256), 0, st, w, const_cast<float*>(a.sums), p.mpad, p.steps * p.gpb, 16 / p.gpb);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    if (w.zeros)
-        e = p.gpb == 4 ? launch_cfg<F16, true, 4>(a, p, st) : p.gpb == 2 ? launch_cfg<F16, true, 2>(a, p, st)
-                                                                         : launch_cfg<F16, true, 1>(a, p, st);
-    else
-        e = p.gpb == 4 ? launch_cfg<F16, false, 4>(a, p, st) : p.gpb == 2 ? launch_cfg<F16, false, 2>(a, p, st)
-                                                                          : launch_cfg<F16, false, 1>(a, p, st);
+    const dim3 grid((unsigned)(p.mtiles * p.ntiles * p.splits));
+    if (p.mt == 4) hipLaunchKernelGGL((w4_tile_kernel<F16, 2, 4, 2>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((w4_tile_kernel<F16, 1, 2, 4>), grid, dim3(256), 0, st, a);
+    const hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.splits == 1) return e;
-    hipLaunchKernelGGL((w4_join_kernel<F16>), dim3((unsigned)((w.m * p.npad / 4 + 255) / 256)), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((w4_join_kernel<F16>), dim3((unsigned)((a.w.m * p.npad / 4 + 255) / 256)), dim3(256), 0, st, a);
     return hipGetLastError();
 }
 
 }  // namespace
 
-bool w4_tile_fits(int64_t m, int64_t n, int64_t k, int group) {
-    const int64_t rows = (m + 127) / 128 * 128, steps = (k + 127) / 128;
-    return rows * steps * (group == 32 ? 4 : group == 64 ? 2 : 1) * 4 < (int64_t(1) << 31) &&
-           rows / 64 * ((n + 127) / 128) * 8 < (int64_t(1) << 31) && rows * ((n + 15) / 16) / 64 < (int64_t(1) << 31);
+bool w4_tile_fits(int64_t m, int64_t n) {
+    const int64_t rows = (m + 127) / 128 * 128;
+    return rows / 64 * ((n + 127) / 128) * 8 < (int64_t(1) << 31) && rows * ((n + 15) / 16) / 64 < (int64_t(1) << 31);
 }
 
-int64_t w4_tile_workspace_bytes(int64_t m, int64_t n, int64_t k, int group) {
-    const Plan p = plan_tiles(m, n, k, group);
-    return p.sums_bytes + p.parts_bytes;
-}
+int64_t w4_tile_workspace_bytes(int64_t m, int64_t n, int64_t k) { return plan_tiles(m, n, k).parts_bytes; }
 
 hipError_t launch_w4_tile(const W4Args& w, void* workspace, hipStream_t st) {
-    const Plan p = plan_tiles(w.m, w.n, w.k, w.group);
+    const Plan p = plan_tiles(w.m, w.n, w.k);
     TileArgs a{};
     a.w = w;
-    a.sums = (const float*)workspace;
-    a.parts = p.splits > 1 ? (float*)((uint8_t*)workspace + p.sums_bytes) : nullptr;
-    a.mpad = p.mpad;
+    a.parts = p.splits > 1 ? (float*)workspace : nullptr;
     a.npad = p.npad;
     a.mtiles = p.mtiles;
     a.ntiles = p.ntiles;

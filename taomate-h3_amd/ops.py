@@ -1134,8 +1134,8 @@ class W4Weight(NamedTuple):
     """4-bit weights [n, k] as w4_mm reads them (pack_w4)."""
 
     codes: torch.Tensor         # uint8 [ceil(n / 16), ceil(k / 128), 1024]
-    scales: torch.Tensor        # bf16 or fp16 [ceil(n / 16), groups, 16]
-    zeros: torch.Tensor | None  # uint8 [ceil(n / 16), groups, 16]; None: 8 everywhere
+    scales: torch.Tensor        # bf16 or fp16 [ceil(n / 16), ceil(groups / 4), 16, 4]
+    zeros: torch.Tensor | None  # uint8, as the scales; None: 8 everywhere
     n: int
     k: int
     group: int
@@ -1190,10 +1190,10 @@ def pack_w4(codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | Non
     for label, t in (("scales", scales), ("zeros", zeros)):
         if t is not None and tuple(t.shape) != (n, groups):
             raise ValueError(f"{name}: {label} must be {(n, groups)}, got {tuple(t.shape)}")
-    blocks = (n + 15) // 16
+    blocks, quads = (n + 15) // 16, (groups + 3) // 4
     out = W4Weight(torch.empty((blocks, (k + 127) // 128, 1024), device=codes.device, dtype=torch.uint8),
-                   torch.empty((blocks, groups, 16), device=codes.device, dtype=scales.dtype),
-                   None if zeros is None else torch.empty((blocks, groups, 16), device=codes.device, dtype=torch.uint8),
+                   torch.empty((blocks, quads, 16, 4), device=codes.device, dtype=scales.dtype),
+                   None if zeros is None else torch.empty((blocks, quads, 16, 4), device=codes.device, dtype=torch.uint8),
                    n, k, int(group))
     row = lambda t: 0 if t is None else t.stride(0) if n > 1 else t.shape[1]
     _call_on(codes, "h3q_w4_pack", _ptr(codes), row(codes), _ptr(scales), row(scales), _ptr(zeros), row(zeros), n, k,
@@ -1202,20 +1202,19 @@ def pack_w4(codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | Non
 
 
 def _check_w4(name: str, w: W4Weight) -> None:
-    groups = _w4_groups(name, w.k, w.group)
-    blocks = (w.n + 15) // 16
+    blocks, quads = (w.n + 15) // 16, (_w4_groups(name, w.k, w.group) + 3) // 4
     _contiguous(f"{name} codes", w.codes, torch.uint8, (blocks, (w.k + 127) // 128, 1024))
     if w.scales.dtype not in (torch.bfloat16, torch.float16):
         raise TypeError(f"{name}: scales must be bfloat16 or float16, got {w.scales.dtype}")
-    _contiguous(f"{name} scales", w.scales, w.scales.dtype, (blocks, groups, 16))
+    _contiguous(f"{name} scales", w.scales, w.scales.dtype, (blocks, quads, 16, 4))
     if w.zeros is not None:
-        _contiguous(f"{name} zeros", w.zeros, torch.uint8, (blocks, groups, 16))
+        _contiguous(f"{name} zeros", w.zeros, torch.uint8, (blocks, quads, 16, 4))
 
 
 def w4_mm(x: torch.Tensor, weight: W4Weight, *, bias: torch.Tensor | None = None,
           out: torch.Tensor | None = None) -> torch.Tensor:
     """x @ w^T [+ bias] of 4-bit weights (pack_w4), ``x [m, k]`` bf16 or fp16 -> [m, n] in x's dtype:
-    out[m, n] = sum_g s[n, g] * sum_{k in g} x[m, k] (u[n, k] - z[n, g]), binary32 sums rounded once.
+    out[m, n] = sum_k x[m, k] * w[n, k] with w = s (u - z) rounded once to x's dtype, binary32 sums, rounded once.
 
     x has 16-byte aligned rows (a row stride that is a multiple of 8); ``bias [n]`` and ``out`` are of its dtype."""
     got = _native_call("w4_mm", x, weight.codes, weight.scales, weight.zeros, weight.n, weight.k, weight.group, bias, out)

@@ -23,18 +23,17 @@ def dequantized(codes, scales, zeros, group: int) -> tuple[torch.Tensor, torch.T
 
 
 def product(x, codes, scales, zeros, group: int, bias=None) -> tuple[torch.Tensor, torch.Tensor]:
-    """(value, bound of its binary32 error), float64 [m, n].
+    """(value, bound of its binary32 error), float64 [m, n], of the weights rounded once to x's type.
 
-    A group of g <= 128 columns is summed as x (16 + u): at most g + 4 roundings (of 2^-23, a matrix
-    instruction may cut off) of a sum of at most 31 |x|; 16 + z times the sum of x (as many) is taken off,
-    at most 31 |x| again; the scale and the sum over the groups add one rounding each for every group (a
-    wider group counts as its blocks of 128), and the parts of a split sum or of a workgroup's waves a
-    few: (g + 4 + groups + 16) 2^-23 * 62 sum |s x| covers it."""
-    w, s = dequantized(codes, scales, zeros, group)
+    s (u - z) has at most 11 + 5 bits, so binary32 holds it, and the rounding of its weight is a definite one.  A
+    matrix instruction takes 16 or 32 products: its own sum has at most 32 roundings (of 2^-23: it may cut off) of
+    its terms, and one follows onto a sum of at most sum |x w|, k / 16 times; the parts of a split k and a workgroup's
+    waves add at most 16 more: (k / 16 + 48) 2^-23 sum |x w|."""
+    w, _ = dequantized(codes, scales, zeros, group)
+    w = w.to(x.dtype).double()
     a = x.cpu().double()
     y = a @ w.T
-    rounds = min(group, 128) + 4 + (a.shape[1] + min(group, 128) - 1) // min(group, 128) + 16
-    bound = rounds * 2.0 ** -23 * 62.0 * (a.abs() @ s.abs().T)
+    bound = (a.shape[1] / 16 + 48) * 2.0 ** -23 * (a.abs() @ w.abs().T)
     if bias is not None:
         y = y + bias.cpu().double()
         bound = bound + 2.0 ** -23 * y.abs()
@@ -77,7 +76,7 @@ def quantize(w: torch.Tensor, group: int, zeros: bool):
 
 def packed_codes(codes: torch.Tensor) -> torch.Tensor:
     """The layout, word by word: word s of lane L of block (r, b) holds the codes 128 b + 32 s + 8 (L / 16) .. + 7 of
-    row 16 r + L % 16, k0 k2 k4 k6 k1 k3 k5 k7 from the low nibble, rotated left by 3."""
+    row 16 r + L % 16, k0 k2 k4 k6 k1 k3 k5 k7 from the low nibble."""
     u = unpack_rows(codes).numpy().astype(np.uint64)
     n, k = u.shape
     rows, cols = -(-n // 16), -(-k // 128)
@@ -88,6 +87,13 @@ def packed_codes(codes: torch.Tensor) -> torch.Tensor:
         for s in range(4):
             base = 32 * s + 8 * (lane // 16)
             e = [full[lane % 16::16, base + i::128] for i in (0, 2, 4, 6, 1, 3, 5, 7)]
-            w = sum(v << np.uint64(4 * i) for i, v in enumerate(e))
-            out[:, :, lane, s] = ((w << np.uint64(3)) | (w >> np.uint64(29))) & np.uint64(0xFFFFFFFF)
+            out[:, :, lane, s] = sum(v << np.uint64(4 * i) for i, v in enumerate(e))
     return torch.from_numpy(out.view(np.uint8).reshape(rows, cols, 1024))
+
+
+def packed_groups(rows: torch.Tensor) -> torch.Tensor:
+    """Scales or zero points [n, groups] -> [ceil(n / 16), ceil(groups / 4), 16, 4], zeros past the ends."""
+    n, groups = rows.shape
+    full = torch.zeros(-(-n // 16) * 16, -(-groups // 4) * 4, dtype=rows.dtype)
+    full[:n, :groups] = rows
+    return full.view(-(-n // 16), 16, -1, 4).transpose(1, 2).contiguous()

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from _util import activations
-from _w4 import assert_product, packed_codes, product, quantize
+from _w4 import assert_product, packed_codes, packed_groups, product, quantize
 
 pytestmark = pytest.mark.gpu
 
@@ -118,13 +118,9 @@ def test_pack_and_quantize(ops, device, n, k, group, zeros):
         assert (got[2] is None) == (not zeros) and (not zeros or torch.equal(got[2].cpu(), want[2]))
         packed = ops.pack_w4(*got, group=group)
         assert torch.equal(packed.codes.cpu(), packed_codes(want[0]))
-        blocks, groups = -(-n // 16), -(-k // group)
-        for label, rows in (("scales", want[1]), ("zeros", want[2])):
-            if rows is None:
-                continue
-            full = torch.zeros(blocks * 16, groups, dtype=rows.dtype)
-            full[:n] = rows
-            assert torch.equal(getattr(packed, label).cpu(), full.view(blocks, 16, groups).transpose(1, 2))
+        assert torch.equal(packed.scales.cpu(), packed_groups(want[1]))
+        assert (packed.zeros is None) == (not zeros)
+        assert not zeros or torch.equal(packed.zeros.cpu(), packed_groups(want[2]))
 
 
 def test_quantize_and_pack_of_strided_rows(ops, device):
@@ -140,9 +136,9 @@ def test_quantize_and_pack_of_strided_rows(ops, device):
 
 
 def test_w4_refuses(ops, device):
-    rows = _weights(32, 64, 32, True, torch.bfloat16, device)
+    rows = _weights(32, 256, 32, True, torch.bfloat16, device)
     w = _pack(ops, device, *rows, 32)
-    x = activations(4, 64).to(device)
+    x = activations(4, 256).to(device)
     with pytest.raises(TypeError):
         ops.w4_mm(x.float(), w)
     with pytest.raises(ValueError):
@@ -150,9 +146,9 @@ def test_w4_refuses(ops, device):
     with pytest.raises(ValueError):
         ops.w4_mm(x[0], w)
     with pytest.raises(RuntimeError, match="ldx"):
-        ops.w4_mm(torch.zeros(4, 68, device=device, dtype=x.dtype)[:, :64], w)
+        ops.w4_mm(torch.zeros(4, 260, device=device, dtype=x.dtype)[:, :256], w)
     with pytest.raises(RuntimeError, match="aligned"):
-        ops.w4_mm(torch.zeros(4, 72, device=device, dtype=x.dtype)[:, 4:68], w)
+        ops.w4_mm(torch.zeros(4, 264, device=device, dtype=x.dtype)[:, 4:260], w)
     with pytest.raises(TypeError):
         ops.w4_mm(x, w, bias=torch.zeros(32, device=device))
     with pytest.raises(ValueError):

@@ -17,7 +17,7 @@ def test_plain_forms_agree_with_a_hand_made_example():
     scales, zeros = torch.tensor([[0.5, 2.0]]), torch.tensor([[8, 1]], dtype=torch.uint8)
     w, _ = dequantized(codes, scales, zeros, 32)
     assert w[0, :4].tolist() == [-4.0, -3.5, 0.0, 3.5] and w[0, 32:36].tolist() == [-2.0, 0.0, 14.0, 28.0]
-    x = torch.ones(1, 64)
+    x = torch.ones(1, 64, dtype=torch.bfloat16)
     y, bound = product(x, codes, scales, zeros, 32)
     assert float(y) == 8 * (-4.0 + 40.0) and float(bound) < 0.5
     with pytest.raises(AssertionError):
@@ -42,13 +42,13 @@ def test_packed_layout_by_hand():
     codes[2, 65] = 0x90  # column 131: code 9 of row 2: block 1, word 0, lane 2, element 3 (odd pair 1: nibble 5)
     codes[1, 6] = 0x05   # column 12: row 1, word 0, lane 16 + 1, element 4: nibble 2
     packed = packed_codes(codes).view(torch.int32).view(1, 2, 64, 4)
-    assert packed[0, 1, 2, 0] == 9 << 23 and packed[0, 0, 17, 0] == 5 << 11
+    assert packed[0, 1, 2, 0] == 9 << 20 and packed[0, 0, 17, 0] == 5 << 8
     assert int((packed != 0).sum()) == 2
 
 
 def test_wrappers_refuse_cpu_tensors(ops):
     x = torch.zeros(2, 32, dtype=torch.bfloat16)
-    w = ops.W4Weight(torch.zeros(1, 1, 1024, dtype=torch.uint8), torch.zeros(1, 1, 16, dtype=torch.bfloat16), None, 16, 32, 32)
+    w = ops.W4Weight(torch.zeros(1, 1, 1024, dtype=torch.uint8), torch.zeros(1, 1, 16, 4, dtype=torch.bfloat16), None, 16, 32, 32)
     for call in (lambda: ops.quantize_w4(x), lambda: ops.pack_w4(torch.zeros(2, 16, dtype=torch.uint8), x[:, :1]),
                  lambda: ops.w4_mm(x, w)):
         with pytest.raises(RuntimeError, match="ROCm GPU"):
@@ -81,11 +81,11 @@ def test_c_entry_points_refuse():
     assert mm(x=odd) == 1 and "aligned" in error()
     assert mm(codes=None) == 1 and "null" in error()
     assert mm(m=0) == 0 and mm(n=0) == 0
-    need = lib.h3q_w4_mm_workspace_bytes(300, 48, 64, 32)
-    assert need > 0 and lib.h3q_w4_mm_workspace_bytes(4, 48, 64, 32) == 0
-    assert mm(m=300) == 1 and "workspace" in error()
-    assert mm(m=300, ws=p, size=need - 1) == 1 and "needed" in error()
-    assert mm(m=(1 << 31) - 1, ws=p, size=1 << 40) == 2 and "too many" in error()
+    need = lib.h3q_w4_mm_workspace_bytes(300, 48, 4096, 32)  # few tiles: a split sum
+    assert need > 0 and lib.h3q_w4_mm_workspace_bytes(4, 48, 4096, 32) == 0
+    assert mm(m=300, k=4096, ldx=4096) == 1 and "workspace" in error()
+    assert mm(m=300, k=4096, ldx=4096, ws=p, size=need - 1) == 1 and "needed" in error()
+    assert mm(m=(1 << 31) - 1, n=1 << 20, ldo=1 << 20) == 2 and "too many" in error()
     assert lib.h3q_w4_code_bytes(17, 144) == 2 * 2 * 1024 and lib.h3q_w4_code_bytes(0, 144) == 0
     pack = lambda ldc=32, lds=2, z=None, ldz=0, n=4, k=64, zo=None, out=p: lib.h3q_w4_pack(
         p, ldc, p, lds, z, ldz, n, k, 32, out, p, zo, None)
