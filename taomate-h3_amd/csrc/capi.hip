@@ -1006,8 +1006,8 @@ static int check_w4(const char* who, int64_t n, int64_t k, int64_t group) {
     if (n < 0 || n >= (int64_t(1) << 31)) return fail(H3Q_ERR_INVALID, "%s: n=%lld", who, (long long)n);
     if (k < 16 || k % 16 || k > (int64_t(1) << 22))
         return fail(H3Q_ERR_INVALID, "%s: k=%lld must be a multiple of 16, 16 to 2^22", who, (long long)k);
-    if (group != 32 && group != 64 && (group < 128 || group % 128 || group > (int64_t(1) << 22)))
-        return fail(H3Q_ERR_INVALID, "%s: group=%lld must be 32, 64 or a multiple of 128", who, (long long)group);
+    if (group != 32 && group != 64 && (group < 128 || group % 128 || group > (int64_t(1) << 18)))
+        return fail(H3Q_ERR_INVALID, "%s: group=%lld must be 32, 64 or a multiple of 128 up to 2^18", who, (long long)group);
     return H3Q_OK;
 }
 
@@ -1112,9 +1112,7 @@ __attribute__((visibility("default"))) int h3q_w4_mm(int dtype, const void* x, i
     a.k = k;
     a.group = (int)group;
     a.groups = (int)w4_groups(k, group);
-    a.blocks_per_group = group >= 128 ? (int)(group / 128) : 1;
-    const int64_t span = group / 32;  // blocks of four groups
-    a.group_shift = (span & (span - 1)) == 0 ? __builtin_ctzll((unsigned long long)span) : -1;
+    a.group_magic = (uint32_t)(((int64_t(1) << 32) + group / 16 - 1) / (group / 16));
     a.codes = (const uint8_t*)codes;
     a.scales = (const uint16_t*)scales;
     a.zeros = (const uint8_t*)zeros;

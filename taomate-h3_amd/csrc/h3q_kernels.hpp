@@ -327,8 +327,7 @@ struct W4Args {
     const uint16_t* x;  // bf16 or binary16 [m, k], ldx elements
     int64_t ldx, m, n, k;
     int group, groups;
-    int blocks_per_group;  // 128-column blocks of a group (1 below 128 columns)
-    int group_shift;       // log2 of the blocks that four groups span, -1: no power of two
+    uint32_t group_magic;  // ceil(2^32 / (group / 16))
     const uint8_t* codes;
     const uint16_t* scales;  // bf16, or binary16 (scales_f16)
     const uint8_t* zeros;    // null: 8 everywhere

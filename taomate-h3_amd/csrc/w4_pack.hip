@@ -16,7 +16,7 @@ __global__ __launch_bounds__(256) void w4_pack_kernel(W4PackArgs p, int64_t word
         if (row < p.n && k < p.k) {
             const uint8_t* const c = p.codes + row * p.ldc + k / 2;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) w |= (uint32_t)(c[j] & 15) << (4 * j) | (uint32_t)(c[j] >> 4) << (16 + 4 * j);
+            for (int e = 0; e < 8; ++e) w |= (uint32_t)(c[e / 2] >> 4 * (e & 1) & 15) << (8 * (e & 3) + (e & 4));
         }
         ((uint32_t*)p.codes_out)[i] = w;
     }

@@ -29,7 +29,7 @@ __device__ __forceinline__ v16f mfma32(v4u a, v4u b, v16f c) {
                                                        0);
 }
 
-template <bool F16, int NT, int MT, int D>
+template <bool F16, bool ZEROS, int NT, int MT, int D>
 __global__ __launch_bounds__(256, 2) void w4_tile_kernel(TileArgs p) {
     constexpr int STAGE = MT * 32 * 256;
     __shared__ __attribute__((aligned(1024))) uint8_t lds_raw[D * STAGE];
@@ -63,7 +63,7 @@ __global__ __launch_bounds__(256, 2) void w4_tile_kernel(TileArgs p) {
     const __amdgpu_buffer_rsrc_t rw = w4_rsrc(p.w.codes + first * steps * 1024, (int64_t)nblk * steps * 1024);
     const __amdgpu_buffer_rsrc_t rs = w4_rsrc(p.w.scales + first * quads * 64, (int64_t)nblk * quads * 128);
     const __amdgpu_buffer_rsrc_t rz =
-        w4_rsrc(p.w.zeros + (p.w.zeros ? first * quads * 64 : 0), p.w.zeros ? (int64_t)nblk * quads * 64 : 0);
+        w4_rsrc(p.w.zeros + (ZEROS ? first * quads * 64 : 0), ZEROS ? (int64_t)nblk * quads * 64 : 0);
     const uint32_t row_bytes = (uint32_t)(p.w.ldx * 2);
 
     // A copy instruction takes four rows; wave w the rows 4 w .. + 3 of every 16.
@@ -89,14 +89,14 @@ __global__ __launch_bounds__(256, 2) void w4_tile_kernel(TileArgs p) {
     v2u scales[D][NT];
     uint32_t zeros[D][NT];
     auto load = [&](int i, int b) __attribute__((always_inline)) {
-        const int q = w4_quad(p.w, b);
+        const int q = w4_group(p.w, b, 0) >> 2;
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
             codes[i][j][0] = __builtin_amdgcn_raw_buffer_load_b128(rw, code_off[j] + 1024u * b, 0, 0);
             codes[i][j][1] = __builtin_amdgcn_raw_buffer_load_b128(rw, code_off[j] + 1024u * b + 512u, 0, 0);
             scales[i][j] = __builtin_amdgcn_raw_buffer_load_b64(rs, (scale_off[j] + 16u * q) * 8, 0, 0);
-            zeros[i][j] = 0x08080808u;
-            if (p.w.zeros) zeros[i][j] = __builtin_amdgcn_raw_buffer_load_b32(rz, (scale_off[j] + 16u * q) * 4, 0, 0);
+            zeros[i][j] = 0;
+            if constexpr (ZEROS) zeros[i][j] = __builtin_amdgcn_raw_buffer_load_b32(rz, (scale_off[j] + 16u * q) * 4, 0, 0);
         }
     };
 
@@ -132,12 +132,14 @@ __global__ __launch_bounds__(256, 2) void w4_tile_kernel(TileArgs p) {
             const H3Q_LDS uint8_t* const tile = lds + i * STAGE;
 #pragma unroll
             for (int s = 0; s < 4; ++s) {
-                const int e = w4_element(p.w, b + i, s);
+                const int e = w4_group(p.w, b + i, s);
                 v4u w[NT][2];
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
                     float scale, shift;
-                    w4_group(scales[i][j], zeros[i][j], e, p.w.scales_f16, scale, shift);
+                    w4_scale<ZEROS>(scales[i][j], zeros[i][j], e, p.w.scales_f16, scale, shift);
+                    shift *= scale;
+                    scale *= 512.0f;
 #pragma unroll
                     for (int h = 0; h < 2; ++h) w[j][h] = w4_weights<F16>(codes[i][j][h][s], scale, shift);
                 }
@@ -185,19 +187,24 @@ struct Plan {
     int64_t parts_bytes;
 };
 
+// 128 x 256 tiles where they fill the chip (4096 rows of 14336 x 5376: 545 us, 1160 TFLOP/s; 128 x 128: 587, 64 x 256:
+// 702, three stages, which leave one workgroup to a CU: 718).  Else 128 columns, of 128 rows or, where that
+// pads the rows by over a seventh, of 64, and k in as many parts as give about two workgroups to a CU (600 rows of
+// 5376 x 7168: 64 us with 128 rows in two parts, 71 with 64 rows; 200 rows: 33 us in three parts, 47 in one, 39
+// in six, whose binary32 sums are written and read once more), each of at least four blocks.
 Plan plan_tiles(int64_t m, int64_t n, int64_t k) {
     Plan p{};
     p.steps = (int)((k + 127) / 128);
     const auto tiles = [&](int nt, int mt) { return ((m + 32 * mt - 1) / (32 * mt)) * ((n + 128 * nt - 1) / (128 * nt)); };
-    p.nt = 2;
-    p.mt = 4;
-    if (tiles(2, 4) < 256) p.nt = 1, p.mt = 2;
+    p.nt = tiles(2, 4) >= 256 ? 2 : 1;
+    p.mt = p.nt == 2 || (m + 127) / 128 * 128 * 7 <= m * 8 ? 4 : 2;
     p.mtiles = (int)((m + 32 * p.mt - 1) / (32 * p.mt));
     p.ntiles = (int)((n + 128 * p.nt - 1) / (128 * p.nt));
     const int64_t count = tiles(p.nt, p.mt);
-    int64_t splits = count >= 512 ? 1 : 512 / count;
+    int64_t splits = p.nt == 2 ? 1 : (512 + count / 2) / count;
     if (splits > 8) splits = 8;
-    if (splits > p.steps / 4) splits = p.steps / 4 > 0 ? p.steps / 4 : 1;
+    if (splits > p.steps / 4) splits = p.steps / 4;
+    if (splits < 1) splits = 1;
     p.per_split = (int)((p.steps + splits - 1) / splits);
     p.splits = (p.steps + p.per_split - 1) / p.per_split;
     p.npad = (int)((n + 15) / 16 * 16);
@@ -205,12 +212,18 @@ Plan plan_tiles(int64_t m, int64_t n, int64_t k) {
     return p;
 }
 
+template <bool F16, bool ZEROS>
+hipError_t launch_cfg(const TileArgs& a, const Plan& p, hipStream_t st) {
+    const dim3 grid((unsigned)(p.mtiles * p.ntiles * p.splits));
+    if (p.nt == 2) hipLaunchKernelGGL((w4_tile_kernel<F16, ZEROS, 2, 4, 2>), grid, dim3(256), 0, st, a);
+    else if (p.mt == 4) hipLaunchKernelGGL((w4_tile_kernel<F16, ZEROS, 1, 4, 2>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((w4_tile_kernel<F16, ZEROS, 1, 2, 3>), grid, dim3(256), 0, st, a);
+    return hipGetLastError();
+}
+
 template <bool F16>
 hipError_t launch_type(const TileArgs& a, const Plan& p, hipStream_t st) {
-    const dim3 grid((unsigned)(p.mtiles * p.ntiles * p.splits));
-    if (p.mt == 4) hipLaunchKernelGGL((w4_tile_kernel<F16, 2, 4, 2>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((w4_tile_kernel<F16, 1, 2, 4>), grid, dim3(256), 0, st, a);
-    const hipError_t e = hipGetLastError();
+    const hipError_t e = a.w.zeros ? launch_cfg<F16, true>(a, p, st) : launch_cfg<F16, false>(a, p, st);
     if (e != hipSuccess || p.splits == 1) return e;
     hipLaunchKernelGGL((w4_join_kernel<F16>), dim3((unsigned)((a.w.m * p.npad / 4 + 255) / 256)), dim3(256), 0, st, a);
     return hipGetLastError();

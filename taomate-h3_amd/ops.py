@@ -1144,8 +1144,8 @@ class W4Weight(NamedTuple):
 def _w4_groups(name: str, k: int, group: int) -> int:
     if k < 16 or k % 16 or k > 1 << 22:
         raise ValueError(f"{name}: k={k} must be a multiple of 16, 16 to 2^22")
-    if group not in (32, 64) and (group < 128 or group % 128 or group > 1 << 22):
-        raise ValueError(f"{name}: group={group} must be 32, 64 or a multiple of 128")
+    if group not in (32, 64) and (group < 128 or group % 128 or group > 1 << 18):
+        raise ValueError(f"{name}: group={group} must be 32, 64 or a multiple of 128, up to 2^18")
     return (k + group - 1) // group
 
 
@@ -1214,7 +1214,8 @@ def _check_w4(name: str, w: W4Weight) -> None:
 def w4_mm(x: torch.Tensor, weight: W4Weight, *, bias: torch.Tensor | None = None,
           out: torch.Tensor | None = None) -> torch.Tensor:
     """x @ w^T [+ bias] of 4-bit weights (pack_w4), ``x [m, k]`` bf16 or fp16 -> [m, n] in x's dtype:
-    out[m, n] = sum_k x[m, k] * w[n, k] with w = s (u - z) rounded once to x's dtype, binary32 sums, rounded once.
+    out[m, n] = sum_k x[m, k] * s (u - z), binary32 sums rounded once.  Above 32 rows the weights s (u - z) are rounded
+    to x's dtype first.
 
     x has 16-byte aligned rows (a row stride that is a multiple of 8); ``bias [n]`` and ``out`` are of its dtype."""
     got = _native_call("w4_mm", x, weight.codes, weight.scales, weight.zeros, weight.n, weight.k, weight.group, bias, out)

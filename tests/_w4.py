@@ -23,17 +23,25 @@ def dequantized(codes, scales, zeros, group: int) -> tuple[torch.Tensor, torch.T
 
 
 def product(x, codes, scales, zeros, group: int, bias=None) -> tuple[torch.Tensor, torch.Tensor]:
-    """(value, bound of its binary32 error), float64 [m, n], of the weights rounded once to x's type.
+    """(value, bound of its binary32 error), float64 [m, n].
 
-    s (u - z) has at most 11 + 5 bits, so binary32 holds it, and the rounding of its weight is a definite one.  A
-    matrix instruction takes 16 or 32 products: its own sum has at most 32 roundings (of 2^-23: it may cut off) of
-    its terms, and one follows onto a sum of at most sum |x w|, k / 16 times; the parts of a split k and a workgroup's
-    waves add at most 16 more: (k / 16 + 48) 2^-23 sum |x w|."""
-    w, _ = dequantized(codes, scales, zeros, group)
-    w = w.to(x.dtype).double()
+    Above 32 rows the weights s (u - z) are rounded once to x's type; binary32 holds them before that (11 + 5
+    bits), so the rounding is a definite one.  A matrix instruction takes 16 or 32 products: its own sum has at most
+    32 roundings (of 2^-23: it may cut off) of its terms, and one follows onto a sum of at most sum |x w|, k / 16
+    times; the parts of a split k and a workgroup's waves add at most 16 more: (k / 16 + 48) 2^-23 sum |x w|.
+
+    Up to 32 rows a group (at most 128 columns of it at a time) is summed as x u, at most 15 |x| a term, with 32 + 4
+    roundings as above, and z times the sum of x, as large, with as many, is taken off in one; the scale and the
+    sum over the groups are one more rounding each of at most 30 |s x|: (56 + k / min(group, 128)) 2^-23 * 30
+    sum |s x|."""
+    w, s = dequantized(codes, scales, zeros, group)
     a = x.cpu().double()
+    if len(x) > 32:
+        w = w.to(x.dtype).double()
+        bound = (a.shape[1] / 16 + 48) * 2.0 ** -23 * (a.abs() @ w.abs().T)
+    else:
+        bound = (56 + a.shape[1] / min(group, 128)) * 2.0 ** -23 * 30.0 * (a.abs() @ s.abs().T)
     y = a @ w.T
-    bound = (a.shape[1] / 16 + 48) * 2.0 ** -23 * (a.abs() @ w.abs().T)
     if bias is not None:
         y = y + bias.cpu().double()
         bound = bound + 2.0 ** -23 * y.abs()
@@ -76,7 +84,7 @@ def quantize(w: torch.Tensor, group: int, zeros: bool):
 
 def packed_codes(codes: torch.Tensor) -> torch.Tensor:
     """The layout, word by word: word s of lane L of block (r, b) holds the codes 128 b + 32 s + 8 (L / 16) .. + 7 of
-    row 16 r + L % 16, k0 k2 k4 k6 k1 k3 k5 k7 from the low nibble."""
+    row 16 r + L % 16, k0 .. k3 in the low nibbles of its bytes and k4 .. k7 in the high ones."""
     u = unpack_rows(codes).numpy().astype(np.uint64)
     n, k = u.shape
     rows, cols = -(-n // 16), -(-k // 128)
@@ -86,8 +94,8 @@ def packed_codes(codes: torch.Tensor) -> torch.Tensor:
     for lane in range(64):
         for s in range(4):
             base = 32 * s + 8 * (lane // 16)
-            e = [full[lane % 16::16, base + i::128] for i in (0, 2, 4, 6, 1, 3, 5, 7)]
-            out[:, :, lane, s] = sum(v << np.uint64(4 * i) for i, v in enumerate(e))
+            e = [full[lane % 16::16, base + i::128] for i in range(8)]
+            out[:, :, lane, s] = sum(v << np.uint64(8 * (i & 3) + (i & 4)) for i, v in enumerate(e))
     return torch.from_numpy(out.view(np.uint8).reshape(rows, cols, 1024))
 
 

@@ -48,7 +48,11 @@ def test_w4_mm(ops, device, m, n, k, group, dtype, zeros):
 @pytest.mark.parametrize("m,n,k,group", [(1, 5376, 7168, 128), (5, 16, 14336, 128), (48, 256, 14336, 64),
                                          (100, 5376, 7168, 32), (700, 2048, 2048, 128), (2500, 1000, 512, 128),
                                          (1111, 5376, 1040, 64), (1, 1, 16, 32), (64, 1, 16, 32), (300, 17, 16, 128),
-                                         (2048, 4096, 256, 32)])
+                                         (2048, 4096, 256, 32),
+                                         # x of few rows in several chunks of LDS; two and four column blocks a workgroup
+                                         (4, 40, 14336, 64), (1, 33, 23056, 128), (3, 4100, 9200, 32), (2, 12400, 256, 32),
+                                         (12, 4112, 400, 32), (12, 8300, 400, 64), (31, 4112, 400, 32),
+                                         (31, 8300, 400, 64), (31, 8300, 400, 32)])
 def test_w4_mm_sizes(ops, device, m, n, k, group):
     rows = _weights(n, k, group, True, torch.bfloat16, device)
     w = _pack(ops, device, *rows, group)

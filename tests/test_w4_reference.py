@@ -39,10 +39,10 @@ def test_quantizer_is_within_half_a_step(dtype, zeros):
 
 def test_packed_layout_by_hand():
     codes = torch.zeros(3, 72, dtype=torch.uint8)  # k = 144: a second block of 16 columns
-    codes[2, 65] = 0x90  # column 131: code 9 of row 2: block 1, word 0, lane 2, element 3 (odd pair 1: nibble 5)
-    codes[1, 6] = 0x05   # column 12: row 1, word 0, lane 16 + 1, element 4: nibble 2
+    codes[2, 65] = 0x90  # column 131: code 9 of row 2: block 1, word 0, lane 2, element 3: the low nibble of byte 3
+    codes[1, 6] = 0x05   # column 12: row 1, word 0, lane 16 + 1, element 4: the high nibble of byte 0
     packed = packed_codes(codes).view(torch.int32).view(1, 2, 64, 4)
-    assert packed[0, 1, 2, 0] == 9 << 20 and packed[0, 0, 17, 0] == 5 << 8
+    assert packed[0, 1, 2, 0] == 9 << 24 and packed[0, 0, 17, 0] == 5 << 4
     assert int((packed != 0).sum()) == 2
 
 
