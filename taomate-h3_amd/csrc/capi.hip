@@ -977,10 +977,16 @@ __attribute__((visibility("default"))) int h3q_append_kv(int dtype, int weight_d
     if (k->heads != v->heads)
         return fail(H3Q_ERR_INVALID, "%s: %lld k heads and %lld v heads", who, (long long)k->heads, (long long)v->heads);
     if (v->weight) return fail(H3Q_ERR_INVALID, "%s: values have no norm", who);
+    if (k_pages->n_pages != v_pages->n_pages || k_pages->page_size != v_pages->page_size)
+        return fail(H3Q_ERR_INVALID, "%s: %lld k pages of %lld tokens, but %lld v pages of %lld", who,
+                    (long long)k_pages->n_pages, (long long)k_pages->page_size, (long long)v_pages->n_pages,
+                    (long long)v_pages->page_size);
     if (tokens == 0) return ok();
     if (!slots || !aligned(slots, 4)) return fail(H3Q_ERR_INVALID, "%s: null or misaligned slots", who);
     h3q::HeadArgs a = head_args(dtype, weight_dtype, tokens, head_dim, eps, rotation);
     a.slots = slots;
+    a.cache_slots = (int)(k_pages->n_pages * k_pages->page_size);
+    a.page_size = (int)k_pages->page_size;
     if (q && q->heads > 0) a.seg[a.segments++] = head_segment(*q, h3q::kDestRows, rotation != nullptr);
     for (int i = 0; i < 2 && k->heads > 0; ++i) {
         const h3q_pages& p = i ? *v_pages : *k_pages;
@@ -990,8 +996,6 @@ __attribute__((visibility("default"))) int h3q_append_kv(int dtype, int weight_d
         s.cache.page_stride = p.page_stride;
         s.cache.slot_stride = p.slot_stride;
         s.cache.head_stride = p.head_stride;
-        s.cache.slots = (int)(p.n_pages * p.page_size);
-        s.cache.page_size = (int)p.page_size;
         s.cache.scale = p.scale;
         s.cache.scale_page_stride = p.scale_page_stride;
         s.cache.scale_slot_stride = p.scale_slot_stride;

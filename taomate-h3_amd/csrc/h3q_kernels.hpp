@@ -281,7 +281,6 @@ enum PositionType : int { kPositionsI32 = 0, kPositionsI64 = 1, kPositionsF32 = 
 struct HeadCache {
     void* pages;
     int64_t page_stride, slot_stride, head_stride;  // elements of a page's type
-    int slots, page_size;                           // pages * page_size
     float* scale;  // e4m3 pages: [heads] (kDestStatic) or [pages, page_size, heads] (kDestRowScale)
     int64_t scale_page_stride, scale_slot_stride, scale_head_stride;
 };
@@ -306,8 +305,10 @@ struct HeadArgs {
     int64_t table_rows;
     const void* positions;  // row of the tables for each token (null: its own number), below 0: padding
     int positions_i64;
-    const int* slots;
+    const int* slots;  // of the caches' pages * page_size, or null
+    int cache_slots, page_size;
     int lanes;  // of a row (set by the launch)
+    float inverse_d;
 };
 constexpr int kHeadMaxDim = 512;
 constexpr int kHeadMaxHeads = 16384;  // three segments of one row a wave stay within a grid's 65535

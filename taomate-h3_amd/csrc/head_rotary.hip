@@ -14,9 +14,9 @@
 // together, ahead of the first use.  The lanes that own a row read all of it before they store any of it,
 // so a call may run in place.
 //
-// Pairs: (i, half + i), where a lane's two vectors are those at c V and half + c V, or (2 i, 2 i + 1), where
-// they are neighbours.  Channels from 2 * half on go through as they are (a select, not a rotation by zero:
-// 0 * inf would be a NaN).
+// Pairs: (i, half + i), where a lane's two vectors at c V and half + c V hold both sides, or (2 i, 2 i + 1), where
+// each of them holds V / 2 whole pairs.  Channels from 2 * half on go through as they are (a select, not a
+// rotation by zero: 0 * inf would be a NaN).
 #include "h3q_common.hpp"
 #include "h3q_kernels.hpp"
 
@@ -59,14 +59,31 @@ __device__ __forceinline__ T at(const typename Vec<T, V>::type& v, int i) {
     else return v[i];
 }
 
-// Sum, and largest magnitude (bits; a NaN above all), over the G lanes of a row.
-__device__ __forceinline__ float row_sum(float v, int lanes) {
-    for (int off = lanes >> 1; off >= 1; off >>= 1) v += __shfl_xor(v, off, 64);
+// A value of the lane that differs in one bit of its number within a row of 16 (for the third and fourth step: of a
+// lane whose quad, or half, the other is; the steps before have made those alike).
+template <int CTRL>
+__device__ __forceinline__ float lane_dpp(float v) {
+    return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), CTRL, 0xF, 0xF, true));
+}
+constexpr int kDppXor1 = 0xB1, kDppXor2 = 0x4E, kDppHalfMirror = 0x141, kDppMirror = 0x140;
+
+// f over the `lanes` (a power of two) lanes of a row, in every one of them.
+template <typename F>
+__device__ __forceinline__ float row_fold(float v, int lanes, F f) {
+    if (lanes >= 2) v = f(v, lane_dpp<kDppXor1>(v));
+    if (lanes >= 4) v = f(v, lane_dpp<kDppXor2>(v));
+    if (lanes >= 8) v = f(v, lane_dpp<kDppHalfMirror>(v));
+    if (lanes >= 16) v = f(v, lane_dpp<kDppMirror>(v));
+    if (lanes >= 32) v = f(v, __shfl_xor(v, 16, 64));
+    if (lanes >= 64) v = f(v, __shfl_xor(v, 32, 64));
     return v;
 }
-__device__ __forceinline__ float row_max(float v, int lanes) {
-    for (int off = lanes >> 1; off >= 1; off >>= 1) v = mag_max(v, __shfl_xor(v, off, 64));
-    return v;
+
+// 1 / sqrt(v), one rounding of the hardware's reciprocal root off, where that has no subnormals either.
+__device__ __forceinline__ float inverse_root(float v) {
+    const bool tiny = v < 0x1p-100f;
+    const float r = __builtin_amdgcn_rsqf(tiny ? v * 0x1p+100f : v);
+    return tiny ? r * 0x1p+50f : r;
 }
 
 // V binary32 values -> V e4m3 codes at p.
@@ -85,13 +102,16 @@ __device__ __forceinline__ void store_codes(uint8_t* p, const float (&y)[V]) {
 }
 
 // DT: the rows' type.  V: channels a vector.  NC: chunks of 2 V channels a lane (1, or 4 at V = 1).
-// HEADS: rows a lane group takes.  INTER: interleaved pairs.
-template <int DT, int V, int NC, int HEADS, bool INTER>
+// HEADS: rows a lane group takes.  INTER: interleaved pairs.  CACHE: some rows go into pages.
+template <int DT, int V, int NC, int HEADS, bool INTER, bool CACHE>
 __global__ __launch_bounds__(256) void head_rotary_kernel(HeadArgs p) {
     using E = Elem<DT>;
     using T = typename E::T;
     using VT = typename Vec<T, V>::type;
+    constexpr int HALF = INTER && V > 1 ? V / 2 : V;  // pairs of one of a lane's vectors
+    constexpr int TABLES = V / HALF;                  // runs of cosines a lane
     using VF = typename Vec<float, V>::type;
+    using VC = typename Vec<float, HALF>::type;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t token = (int64_t)blockIdx.x * 4 + wave;
@@ -100,61 +120,80 @@ __global__ __launch_bounds__(256) void head_rotary_kernel(HeadArgs p) {
     while (which + 1 < p.segments && unit >= p.seg[which].units) unit -= p.seg[which++].units;
     const HeadSegment& s = p.seg[which];
 
-    int64_t pos = token;
-    if (p.positions) pos = p.positions_i64 ? ((const int64_t*)p.positions)[token] : ((const int32_t*)p.positions)[token];
-    if (pos < 0) return;  // padding: its rows are left as they were
-    int64_t page = 0;
-    int place = 0;
-    if (s.dest != kDestRows) {
-        const int slot = p.slots[token];
-        if (slot < 0 || slot >= s.cache.slots) return;  // no page for it
-        page = slot / s.cache.page_size;
-        place = slot - (int)page * s.cache.page_size;
-    }
-
+    // Lanes and row groups past the end load what lies at it, and store nothing: the loads of a wave are one run.
     const int g = lane & (p.lanes - 1), rows = 64 / p.lanes;  // this lane of a row; rows of a wave at a time
-    const int head0 = unit * rows * HEADS + lane / p.lanes;
+    const int first = unit * rows * HEADS, head0 = first + lane / p.lanes;
     const int turned = s.rotate ? p.half / V : 0;  // chunks that are rotated; the others lie behind 2 * half
     const int chunks = p.d / (2 * V);
+    // A lane's two vectors are as far apart as its region (the rotated channels, or those behind them) has chunks, so
+    // that every access of a wave is whole runs.
     int off[NC][2];
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-        const int chunk = g + c * 64;
-        const bool apart = !INTER && chunk < turned;
-        off[c][0] = apart ? chunk * V : chunk * 2 * V;
-        // a head without rotation is read as one run, whatever the pairs
-        off[c][1] = apart ? p.half + chunk * V : chunk * 2 * V + V;
+        const int chunk = g + c * 64 < chunks ? g + c * 64 : chunks - 1;
+        const bool turn = chunk < turned;
+        off[c][0] = turn ? chunk * V : (turned + chunk) * V;
+        off[c][1] = off[c][0] + (turn ? turned : chunks - turned) * V;
+        if (INTER && V == 1 && turn) {
+            off[c][0] = 2 * chunk;
+            off[c][1] = 2 * chunk + 1;
+        }
     }
 
     VT raw[HEADS][NC][2];
     const T* const x = (const T*)s.x + token * s.token_stride;
 #pragma unroll
     for (int h = 0; h < HEADS; ++h) {
-        const int head = head0 + h * rows;
+        if (first + h * rows >= s.heads) break;  // the wave's last rows
+        const int head = head0 + h * rows < s.heads ? head0 + h * rows : s.heads - 1;
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            const bool in = head < s.heads && g + c * 64 < chunks;
+        for (int c = 0; c < NC; ++c)
 #pragma unroll
             for (int i = 0; i < 2; ++i)
-                raw[h][c][i] = in ? *reinterpret_cast<const VT*>(x + head * s.head_stride + off[c][i]) : VT{};
-        }
+                raw[h][c][i] = *reinterpret_cast<const VT*>(x + head * s.head_stride + off[c][i]);
     }
 
-    VF cs[NC], sn[NC];
-    if (s.rotate) {
-        const bool known = pos < p.table_rows;  // a position past the table gives NaN, never another one's angle
+    // Behind the rows' loads: what a token's rows are multiplied by and where they go is one round trip further.
+    int64_t pos = token;
+    if (p.positions) pos = p.positions_i64 ? ((const int64_t*)p.positions)[token] : ((const int32_t*)p.positions)[token];
+    if (pos < 0) return;  // padding: its rows are left as they were
+    int64_t to = token * s.out_token_stride, scale_to = 0;
+    if (CACHE && s.dest != kDestRows) {
+        const int slot = p.slots[token];
+        if (slot < 0 || slot >= p.cache_slots) return;  // no page for it
+        const int page = slot / p.page_size, place = slot - page * p.page_size;
+        to = page * s.cache.page_stride + place * s.cache.slot_stride;
+        scale_to = page * s.cache.scale_page_stride + place * s.cache.scale_slot_stride;
+    }
+
+    float cs[NC][V], sn[NC][V];
+    if (turned > 0) {
+        const bool known = pos < p.table_rows;
         const int64_t row = (known ? pos : 0) * p.half;
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            const int chunk = g + c * 64;
-            cs[c] = VF{};
-            sn[c] = VF{};
-            if (chunk < turned) {
-                cs[c] = *reinterpret_cast<const VF*>(p.cos + row + chunk * V);
-                sn[c] = *reinterpret_cast<const VF*>(p.sin + row + chunk * V);
-                if (!known) cs[c] = sn[c] = VF{} + __builtin_nanf("");
-                if (p.inverse) sn[c] = -sn[c];
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int i = 0; i < TABLES; ++i) {
+                const int chunk = g + c * 64 < turned ? g + c * 64 : turned - 1;
+                const VC co = *reinterpret_cast<const VC*>(p.cos + row + (chunk + i * turned) * HALF);
+                const VC si = *reinterpret_cast<const VC*>(p.sin + row + (chunk + i * turned) * HALF);
+#pragma unroll
+                for (int e = 0; e < HALF; ++e) {
+                    cs[c][i * HALF + e] = at<float, HALF>(co, e);
+                    sn[c][i * HALF + e] = at<float, HALF>(si, e);
+                }
             }
+        if (p.inverse) {
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int e = 0; e < V; ++e) sn[c][e] = -sn[c][e];
+        }
+        if (!known) {  // a position past the table gives NaN, never another one's angle
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int e = 0; e < V; ++e) cs[c][e] = sn[c][e] = __builtin_nanf("");
         }
     }
 
@@ -164,14 +203,13 @@ __global__ __launch_bounds__(256) void head_rotary_kernel(HeadArgs p) {
         for (int c = 0; c < NC; ++c)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const bool in = head < s.heads && g + c * 64 < chunks;
                 const int64_t o = head * s.weight_stride + off[c][i];
                 if (p.weight_f32) {
-                    const VF v = in ? *reinterpret_cast<const VF*>((const float*)s.weight + o) : VF{};
+                    const VF v = *reinterpret_cast<const VF*>((const float*)s.weight + o);
 #pragma unroll
                     for (int e = 0; e < V; ++e) w[c][i][e] = at<float, V>(v, e);
                 } else {
-                    const VT v = in ? *reinterpret_cast<const VT*>((const T*)s.weight + o) : VT{};
+                    const VT v = *reinterpret_cast<const VT*>((const T*)s.weight + o);
 #pragma unroll
                     for (int e = 0; e < V; ++e) w[c][i][e] = E::up(at<T, V>(v, e));
                 }
@@ -181,7 +219,7 @@ __global__ __launch_bounds__(256) void head_rotary_kernel(HeadArgs p) {
 
 #pragma unroll
     for (int h = 0; h < HEADS; ++h) {
-        if (unit * rows * HEADS + h * rows >= s.heads) break;  // the wave's last rows
+        if (first + h * rows >= s.heads) break;
         const int head = head0 + h * rows;
         float y[NC][2][V];
 #pragma unroll
@@ -191,16 +229,19 @@ __global__ __launch_bounds__(256) void head_rotary_kernel(HeadArgs p) {
 #pragma unroll
                 for (int e = 0; e < V; ++e) y[c][i][e] = E::up(at<T, V>(raw[h][c][i], e));
         if (s.weight) {
-            if (s.weight_stride != 0) load_weight(head);
+            if (s.weight_stride != 0) load_weight(head < s.heads ? head : s.heads - 1);
             float ss = 0.0f;
 #pragma unroll
-            for (int c = 0; c < NC; ++c)
+            for (int c = 0; c < NC; ++c) {
+                float part = 0.0f;
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
-                    for (int e = 0; e < V; ++e) ss = __builtin_fmaf(y[c][i][e], y[c][i][e], ss);
-            ss = row_sum(ss, p.lanes);
-            const float rs = 1.0f / __builtin_sqrtf(ss / (float)p.d + p.eps);
+                    for (int e = 0; e < V; ++e) part = __builtin_fmaf(y[c][i][e], y[c][i][e], part);
+                ss += g + c * 64 < chunks ? part : 0.0f;
+            }
+            ss = row_fold(ss, p.lanes, [](float a, float b) { return a + b; });
+            const float rs = inverse_root(__builtin_fmaf(ss, p.inverse_d, p.eps));
 #pragma unroll
             for (int c = 0; c < NC; ++c)
 #pragma unroll
@@ -208,67 +249,66 @@ __global__ __launch_bounds__(256) void head_rotary_kernel(HeadArgs p) {
 #pragma unroll
                     for (int e = 0; e < V; ++e) y[c][i][e] = y[c][i][e] * rs * w[c][i][e];
         }
-        if (s.rotate) {
+        if (turned > 0) {
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
                 const bool turn = g + c * 64 < turned;
 #pragma unroll
                 for (int e = 0; e < V; ++e) {
-                    // interleaved: pair e of the 2 V neighbours is (2 e, 2 e + 1)
-                    float& a = INTER ? y[c][2 * e / V][2 * e % V] : y[c][0][e];
-                    float& b = INTER ? y[c][(2 * e + 1) / V][(2 * e + 1) % V] : y[c][1][e];
-                    const float co = at<float, V>(cs[c], e), si = at<float, V>(sn[c], e);
+                    // interleaved: the pairs (2 e, 2 e + 1) of one vector, then of the other
+                    float& a = INTER && V > 1 ? y[c][e / HALF][2 * (e % HALF)] : y[c][0][e];
+                    float& b = INTER && V > 1 ? y[c][e / HALF][2 * (e % HALF) + 1] : y[c][1][e];
+                    const float co = cs[c][e], si = sn[c][e];
                     const float ra = __builtin_fmaf(a, co, -(b * si)), rb = __builtin_fmaf(a, si, b * co);
                     a = turn ? ra : a;
                     b = turn ? rb : b;
                 }
             }
         }
-        float r = 1.0f;
-        if (s.dest == kDestStatic) {
-            r = 1.0f / s.cache.scale[head < s.heads ? head * s.cache.scale_head_stride : 0];
-        } else if (s.dest == kDestRowScale) {
-            float m = 0.0f;
+        if (!CACHE || s.dest <= kDestPages) {
+            T* const row = (CACHE && s.dest != kDestRows ? (T*)s.cache.pages + head * s.cache.head_stride
+                                                         : (T*)s.out + head * s.out_head_stride) + to;
 #pragma unroll
             for (int c = 0; c < NC; ++c)
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int e = 0; e < V; ++e) m = mag_max(m, __builtin_fabsf(y[c][i][e]));
-            const float scale = amax_scale(row_max(m, p.lanes), kE4M3Recip);
-            r = 1.0f / scale;
-            if (g == 0 && head < s.heads)
-                s.cache.scale[page * s.cache.scale_page_stride + place * s.cache.scale_slot_stride +
-                              head * s.cache.scale_head_stride] = scale;
-        }
-        if (head >= s.heads) continue;
-#pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            if (g + c * 64 >= chunks) continue;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                if (s.dest >= kDestStatic) {
-                    float q[V];
-#pragma unroll
-                    for (int e = 0; e < V; ++e) q[e] = clamp_e4m3(y[c][i][e] * r);
-                    uint8_t* const to = (uint8_t*)s.cache.pages + page * s.cache.page_stride +
-                                        place * s.cache.slot_stride + head * s.cache.head_stride;
-                    store_codes<V>(to + off[c][i], q);
-                } else {
+                for (int i = 0; i < 2; ++i) {
                     VT v;
 #pragma unroll
                     for (int e = 0; e < V; ++e) {
                         if constexpr (V == 1) v = E::down(y[c][i][e]);
                         else v[e] = E::down(y[c][i][e]);
                     }
-                    T* const to = s.dest == kDestRows
-                                      ? (T*)s.out + token * s.out_token_stride + head * s.out_head_stride
-                                      : (T*)s.cache.pages + page * s.cache.page_stride + place * s.cache.slot_stride +
-                                            head * s.cache.head_stride;
-                    *reinterpret_cast<VT*>(to + off[c][i]) = v;
+                    if (head < s.heads && g + c * 64 < chunks) *reinterpret_cast<VT*>(row + off[c][i]) = v;
                 }
-            }
+            continue;
         }
+        float scale;
+        if (s.dest == kDestStatic) {
+            scale = s.cache.scale[head < s.heads ? head * s.cache.scale_head_stride : 0];
+        } else {
+            float m = 0.0f;
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int e = 0; e < V; ++e)
+                        m = mag_max(m, __builtin_fabsf(y[c][i][e]));  // lanes past the row repeat its last channels
+            m = row_fold(m, p.lanes, [](float a, float b) { return mag_max(a, b); });
+            scale = amax_scale(m, kE4M3Recip);
+            if (g == 0 && head < s.heads) s.cache.scale[scale_to + head * s.cache.scale_head_stride] = scale;
+        }
+        const float r = 1.0f / scale;
+        uint8_t* const row = (uint8_t*)s.cache.pages + head * s.cache.head_stride + to;
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                float q[V];
+#pragma unroll
+                for (int e = 0; e < V; ++e) q[e] = clamp_e4m3(y[c][i][e] * r);
+                if (head < s.heads && g + c * 64 < chunks) store_codes<V>(row + off[c][i], q);
+            }
     }
 }
 
@@ -332,16 +372,23 @@ __global__ __launch_bounds__(256) void plan_append_kernel(PlanAppendArgs p) {
     p.slots[token] = slot;
 }
 
+template <int DT, int V, int NC, int HEADS, bool CACHE>
+hipError_t launch_heads_pairs(const HeadArgs& a, int units, hipStream_t st) {
+    const dim3 grid((unsigned)((a.tokens + 3) / 4), (unsigned)units);
+    if (a.interleaved) hipLaunchKernelGGL((head_rotary_kernel<DT, V, NC, HEADS, true, CACHE>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((head_rotary_kernel<DT, V, NC, HEADS, false, CACHE>), grid, dim3(256), 0, st, a);
+    return hipGetLastError();
+}
+
 template <int DT, int V, int NC, int HEADS>
 hipError_t launch_heads_cfg(const HeadArgs& a, int units, hipStream_t st) {
-    const dim3 grid((unsigned)((a.tokens + 3) / 4), (unsigned)units);
-    if (a.interleaved) hipLaunchKernelGGL((head_rotary_kernel<DT, V, NC, HEADS, true>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((head_rotary_kernel<DT, V, NC, HEADS, false>), grid, dim3(256), 0, st, a);
-    return hipGetLastError();
+    return a.slots ? launch_heads_pairs<DT, V, NC, HEADS, true>(a, units, st)
+                   : launch_heads_pairs<DT, V, NC, HEADS, false>(a, units, st);
 }
 
 template <int DT, int V, int NC>
 hipError_t launch_heads_vec(HeadArgs a, hipStream_t st) {
+    a.inverse_d = 1.0f / (float)a.d;
     a.lanes = 1;
     while (a.lanes < 64 && a.lanes * 2 * V < a.d) a.lanes *= 2;
     const int rows = 64 / a.lanes;

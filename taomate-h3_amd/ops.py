@@ -1113,6 +1113,9 @@ def append_kv(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: 
     _contiguous(f"{name} slots", slots, torch.int32, (tokens,))
     if (cos is None) != (sin is None) or (cos is None and positions is not None):
         raise ValueError(f"{name}: cos and sin go together, and positions with them")
+    if k_pages.shape[:2] != v_pages.shape[:2]:
+        raise ValueError(f"{name}: k_pages and v_pages differ in pages or page_size ({tuple(k_pages.shape[:2])}, "
+                         f"{tuple(v_pages.shape[:2])})")
     rotation = None if cos is None else _rotation(name, cos, sin, positions, tokens, d, interleaved)
     q_heads = None
     if q is not None:

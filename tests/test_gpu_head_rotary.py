@@ -409,6 +409,10 @@ def test_append_kv_refuses(ops, device):
     with pytest.raises(ValueError):
         ops.append_kv(k, k, kp[:1].expand(2, 4, 2, 16), vp, slots)  # pages that share memory
     with pytest.raises(ValueError):
+        ops.append_kv(k, k, kp, vp[:1], slots)  # not as many pages
+    with pytest.raises(ValueError):
+        ops.append_kv(k, k, kp, vp.view(4, 2, 2, 16), slots)
+    with pytest.raises(ValueError):
         ops.append_kv(k, k, kp, vp, slots, cos=cos)
     with pytest.raises(ValueError):
         ops.append_kv(k, k, kp, vp, slots, positions=slots)

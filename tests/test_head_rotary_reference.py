@@ -181,6 +181,7 @@ def test_c_entry_points_refuse(lib):
     assert append(kp=_pages(lib, kind=1)) == 1 and "need scales" in error()
     assert append(vp=_pages(lib, n_pages=1 << 27)) == 2 and "2^31" in error()
     assert append(vp=_pages(lib, page_size=0)) == 2
+    assert append(vp=_pages(lib, n_pages=5)) == 1 and "v pages" in error()
     assert append(v=_rows(lib, heads=3)) == 1 and "v heads" in error()
     assert append(v=_rows(lib, weight=256)) == 1 and "no norm" in error()
     assert append(slots=None) == 1 and "slots" in error()
