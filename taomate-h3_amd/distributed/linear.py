@@ -7,7 +7,8 @@ FL/distributed/linear.py:16-181:
   dispatches on module attributes: ``_cutlass_w8a8_weight_scale`` -> int8
   W8A8, ``_fp8_w8a8_weight_scale`` -> per-token x per-channel FP8 W8A8 (the
   BASELINE.json format; no counterpart in the reference), ``_fp8_weight_scale`` ->
-  per-tensor FP8 (FL), otherwise ``F.linear``.
+  per-tensor FP8 (FL), ``_w4_sizes`` -> 4-bit weights with group scales (no counterpart
+  either), otherwise ``F.linear``.
 * ``_linear(...)`` keeps FL's functional signature (FL/distributed/linear.py:50-101)
   including the "cannot combine" error.
 * ``_module_fp8_input_scale`` and the two context managers keep FL's
@@ -31,7 +32,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .. import ops
-from ..inference import fused_kernels, w8a8
+from ..inference import fused_kernels, w4, w8a8
 from ..inference.fused_kernels import QuantizedActivations, as_dense
 
 
@@ -77,7 +78,7 @@ def _fp8_tensor_linear(inputs: torch.Tensor, weight: torch.Tensor, weight_scale:
 
 
 def _module_linear(module: nn.Module, inputs: torch.Tensor, bias: torch.Tensor | None) -> torch.Tensor:
-    """H3/distributed/linear.py:15-33 plus the FP8 formats.  ``inputs`` may
+    """H3/distributed/linear.py:15-33 plus the FP8 and 4-bit formats.  ``inputs`` may
     also be per-token codes from a fused producer (QuantizedActivations): the
     per-token W8A8 paths consume them directly, the others use their bf16 rows."""
     if getattr(module, ops.TILED_WEIGHT_ATTR, False):
@@ -100,6 +101,9 @@ def _module_linear(module: nn.Module, inputs: torch.Tensor, bias: torch.Tensor |
     fp8_tensor = getattr(module, "_fp8_weight_scale", None)
     if fp8_tensor is not None:
         return _fp8_tensor_linear(inputs, module.weight, fp8_tensor, bias, _module_fp8_input_scale(module, inputs))
+    packed = w4.module_w4_weight(module)
+    if packed is not None:
+        return w4.w4_linear(inputs, packed, bias)
     return F.linear(inputs, module.weight, bias)
 
 
