@@ -1124,7 +1124,7 @@ __attribute__((visibility("default"))) int h3q_w4_mm(int dtype, const void* x, i
     a.out = (uint16_t*)out;
     a.ldo = ldo;
     a.f16 = dtype == H3Q_DTYPE_F16;
-    a.scales_f16 = scale_dtype == H3Q_DTYPE_F16;
+    a.scales_f16 = scale_dtype == H3Q_DTYPE_F16 ? ~0u : 0u;
     a.out_vec = aligned(out, 8) && ldo % 4 == 0;
     if (m <= h3q::kW4StreamRows) return check_launch(h3q::launch_w4_stream(a, (hipStream_t)stream), who);
     if (!h3q::w4_tile_fits(m, n))

@@ -37,15 +37,12 @@ __device__ __forceinline__ uint32_t w4_pair(float lo, float hi) {
     else return pack_bf16x2(lo, hi);
 }
 
-// Eight codes of a row -> its weights, rounded to x's type: scale = 2^9 s, shift = -z s.
+// Pair q of a word's eight codes -> weights 2 q and 2 q + 1, rounded to x's type: scale = 2^9 s, shift = -z s.
 template <bool F16>
-__device__ __forceinline__ v4u w4_weights(uint32_t w, float scale, float shift) {
-    const int even = (int)(w & 0x0F0F0F0Fu), odd = (int)(w >> 4 & 0x0F0F0F0Fu);
-    const v2f a = __builtin_amdgcn_cvt_pk_f32_fp8(even, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(even, true);
-    const v2f c = __builtin_amdgcn_cvt_pk_f32_fp8(odd, false), d = __builtin_amdgcn_cvt_pk_f32_fp8(odd, true);
-    const auto f = [&](float v) { return __builtin_fmaf(v, scale, shift); };
-    return v4u{w4_pair<F16>(f(a[0]), f(a[1])), w4_pair<F16>(f(b[0]), f(b[1])), w4_pair<F16>(f(c[0]), f(c[1])),
-               w4_pair<F16>(f(d[0]), f(d[1]))};
+__device__ __forceinline__ uint32_t w4_weight_pair(uint32_t w, int q, float scale, float shift) {
+    const int codes = (int)((q < 2 ? w : w >> 4) & 0x0F0F0F0Fu);
+    const v2f u = q & 1 ? __builtin_amdgcn_cvt_pk_f32_fp8(codes, true) : __builtin_amdgcn_cvt_pk_f32_fp8(codes, false);
+    return w4_pair<F16>(__builtin_fmaf(u[0], scale, shift), __builtin_fmaf(u[1], scale, shift));
 }
 
 // Group of the 32-column step s of block b: floor((4 b + s) / (group / 32)), by a multiplication that is exact for
@@ -55,12 +52,13 @@ __device__ __forceinline__ int w4_group(const W4Args& p, int b, int s) {
 }
 
 // Scale and -(zero point) of a row for group e & 3 of the four in `s` and `z`; e is wave-uniform, so the choice is
-// one byte permutation with a selector from a scalar register.
+// one byte permutation with a selector from a scalar register.  f16 is a mask: a condition would become a branch,
+// which keeps the compiler from mixing the unpacking of one step with the matrix instructions of another.
 template <bool ZEROS>
-__device__ __forceinline__ void w4_scale(v2u s, uint32_t z, int e, bool f16, float& scale, float& shift) {
+__device__ __forceinline__ void w4_scale(v2u s, uint32_t z, int e, uint32_t f16, float& scale, float& shift) {
     const uint32_t at = (uint32_t)(e & 3) * 0x0202u + 0x0100u;  // its two bytes
     const uint32_t bits = __builtin_amdgcn_perm(s[1], s[0], at << 16 | 0x0C0Cu);
-    scale = f16 ? f16_hi(bits) : __uint_as_float(bits);
+    scale = __uint_as_float((__float_as_uint(f16_hi(bits)) & f16) | (bits & ~f16));
     shift = ZEROS ? -(float)(z >> (8 * (e & 3)) & 255u) : -8.0f;
 }
 
@@ -70,6 +68,35 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t w4_rsrc(const void* base, int6
     const uint64_t b = (uint64_t)base;
     const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)b), hi = __builtin_amdgcn_readfirstlane((uint32_t)(b >> 32));
     return make_rsrc((const void*)((uint64_t)hi << 32 | lo), __builtin_amdgcn_readfirstlane((uint32_t)bytes));
+}
+
+template <bool F16>
+__device__ __forceinline__ v16f w4_mfma(v4u a, v4u b, v16f c) {
+    if constexpr (F16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0,
+                                                       0);
+}
+
+struct W4Tile {
+    int m, n, z;  // row tile, column tile, part of k; in scalar registers
+};
+
+// Workgroups b, b + 8, ... share an XCD: each gets a contiguous run of tiles, in bands of 8 row tiles with the row
+// tile fastest.
+__device__ __forceinline__ W4Tile w4_tile_of(int mtiles, int ntiles, int splits) {
+    const int total = mtiles * ntiles * splits;
+    int id = blockIdx.x;
+    const int q = total / 8, r = total % 8, x = id % 8;
+    id = x * q + (x < r ? x : r) + id / 8;
+    const int z = id % splits;
+    id /= splits;
+    const int band = id / (8 * ntiles), in = id % (8 * ntiles);
+    const int high = mtiles - band * 8 < 8 ? mtiles - band * 8 : 8;
+    // A division leaves the scalar registers.
+    return {__builtin_amdgcn_readfirstlane(band * 8 + in % high), __builtin_amdgcn_readfirstlane(in / high),
+            __builtin_amdgcn_readfirstlane(z)};
 }
 
 // out[m, n .. n + 3] = y + bias, rounded once; rows and columns past the end are dropped.

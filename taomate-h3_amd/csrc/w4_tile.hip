@@ -3,9 +3,12 @@
 //
 // A workgroup of four waves owns a tile of 32 MT rows x 128 NT columns, each wave all rows and 32 NT of the
 // columns, so every code is unpacked once in a workgroup, straight into operand registers.  Per 128 columns of k the
-// x tile is copied into an LDS ring of D stages (buffer_load ... lds, no registers; a row is 256 contiguous bytes,
-// its 16-byte chunk c in slot c ^ (row % 16), so that 16 rows' reads of one chunk meet no bank twice), and the
-// codes, scales and zero points into registers as many blocks ahead.  One barrier a block.
+// x tile is copied into one of two LDS stages (buffer_load ... lds, no registers; a row is 256 contiguous bytes, its
+// 16-byte chunk c in slot c ^ (row % 16), so that 16 rows' reads of one chunk meet no bank twice), and the codes,
+// scales and zero points into registers, one block ahead.  One barrier a block.  Inside a block the operands of the
+// next 16 columns are read and unpacked between the matrix instructions of these, in pieces that the scheduler
+// must not gather: 4096 rows of 14336 x 5376 524 us, 549 in the compiler's order.  At 1.9 GHz, where such a product
+// holds the clock, the matrix instructions are busy for 60 % of that; the library's bf16 product takes 505 to 517.
 //
 // Few tiles: k is split over several workgroups, whose binary32 sums a last kernel adds in order.
 #include "w4.hpp"
@@ -20,41 +23,29 @@ struct TileArgs {
     int npad, mtiles, ntiles, splits, per_split, steps;
 };
 
+// Four columns of a row: the result, or this part of k's share of it.
 template <bool F16>
-__device__ __forceinline__ v16f mfma32(v4u a, v4u b, v16f c) {
-    if constexpr (F16)
-        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
-    else
-        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0,
-                                                       0);
+__device__ __forceinline__ void store_sums(const TileArgs& p, int z, int64_t m, int64_t n, v4f y) {
+    if (p.parts) {
+        if (m < p.w.m && n < p.npad) *reinterpret_cast<v4f*>(p.parts + (z * p.w.m + m) * p.npad + n) = y;
+    } else {
+        w4_store<F16>(p.w, m, n, y);
+    }
 }
 
-template <bool F16, bool ZEROS, int NT, int MT, int D>
+template <bool F16, bool ZEROS, int NT, int MT>
 __global__ __launch_bounds__(256, 2) void w4_tile_kernel(TileArgs p) {
-    constexpr int STAGE = MT * 32 * 256;
+    constexpr int D = 2, STAGE = MT * 32 * 256;
     __shared__ __attribute__((aligned(1024))) uint8_t lds_raw[D * STAGE];
     H3Q_LDS uint8_t* const lds = (H3Q_LDS uint8_t*)lds_raw;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r32 = lane & 31, half = lane >> 5;
 
-    // Workgroups b, b + 8, ... share an XCD: each gets a contiguous run of tiles, in bands of 8 row tiles
-    // with the row tile fastest.
-    const int total = p.mtiles * p.ntiles * p.splits;
-    int id = blockIdx.x;
-    {
-        const int q = total / 8, r = total % 8, x = id % 8;
-        id = x * q + (x < r ? x : r) + id / 8;
-    }
-    const int z = __builtin_amdgcn_readfirstlane(id % p.splits);  // a division leaves the scalar registers
-    id /= p.splits;
-    const int band = id / (8 * p.ntiles), in = id % (8 * p.ntiles);
-    const int high = p.mtiles - band * 8 < 8 ? p.mtiles - band * 8 : 8;
-    const int mt = __builtin_amdgcn_readfirstlane(band * 8 + in % high);
-    const int nt = __builtin_amdgcn_readfirstlane(in / high);
+    const W4Tile at = w4_tile_of(p.mtiles, p.ntiles, p.splits);
 
-    const int64_t m0 = (int64_t)mt * 32 * MT;
-    const int blk0 = nt * 8 * NT + wave * 2 * NT, blocks = (int)((p.w.n + 15) / 16);
+    const int64_t m0 = (int64_t)at.m * 32 * MT;
+    const int blk0 = at.n * 8 * NT + wave * 2 * NT, blocks = (int)((p.w.n + 15) / 16);
     const int nblk = blocks - blk0 < 0 ? 0 : blocks - blk0 < 2 * NT ? blocks - blk0 : 2 * NT;
     const int steps = p.steps, quads = (p.w.groups + 3) / 4;
     const int64_t rows = p.w.m - m0 < 32 * MT ? p.w.m - m0 : 32 * MT;
@@ -110,7 +101,7 @@ __global__ __launch_bounds__(256, 2) void w4_tile_kernel(TileArgs p) {
 #pragma unroll
     for (int c = 0; c < 8; ++c) xoff[c] = r32 * 256 + 16 * ((2 * c + half) ^ (r32 & 15));
 
-    const int b0 = z * p.per_split, b1 = b0 + p.per_split < steps ? b0 + p.per_split : steps;
+    const int b0 = at.z * p.per_split, b1 = b0 + p.per_split < steps ? b0 + p.per_split : steps;
     // Blocks past b1 are copied nowhere (out of range), but counted: every stage has as many copies in flight.
     auto ask = [&](int i, int b) __attribute__((always_inline)) {
         load(i, b < b1 ? b : b1 - 1);
@@ -123,35 +114,40 @@ __global__ __launch_bounds__(256, 2) void w4_tile_kernel(TileArgs p) {
 #pragma unroll
         for (int i = 0; i < D; ++i) {
             if (b + i >= b1) break;
-            // Stage i has landed: the D - 2 stages behind it may be under way (the loads among them are not
-            // counted, which makes the wait stricter than it has to be).
-            wait_vmcnt<(D - 2) * COPIES>();
-            __syncthreads();  // and every wave is done with the stage before it
+            wait_vmcnt0();    // this wave's part of stage i has landed
+            __syncthreads();  // everyone's has, and every wave is done with the stage before it
             ask((i + D - 1) % D, b + i + D - 1);
             __builtin_amdgcn_sched_barrier(0);
             const H3Q_LDS uint8_t* const tile = lds + i * STAGE;
+            // Operands one step of 16 k ahead: between two matrix instructions' issues the next step's reads and a
+            // part of its unpacking.
+            v4u x[2][MT], w[2][NT];
+            float scale[NT], shift[NT];
+            auto prepare = [&](int g, int t) __attribute__((always_inline)) {  // part t of MT for step g
+                x[g & 1][t] = *(const H3Q_LDS v4u*)(tile + xoff[g] + t * 32 * 256);
 #pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                const int e = w4_group(p.w, b + i, s);
-                v4u w[NT][2];
-#pragma unroll
-                for (int j = 0; j < NT; ++j) {
-                    float scale, shift;
-                    w4_scale<ZEROS>(scales[i][j], zeros[i][j], e, p.w.scales_f16, scale, shift);
-                    shift *= scale;
-                    scale *= 512.0f;
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) w[j][h] = w4_weights<F16>(codes[i][j][h][s], scale, shift);
-                }
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int t = 0; t < MT; ++t) {
-                        const v4u x = *(const H3Q_LDS v4u*)(tile + xoff[2 * s + h] + t * 32 * 256);
-#pragma unroll
-                        for (int j = 0; j < NT; ++j) acc[j][t] = mfma32<F16>(w[j][h], x, acc[j][t]);
+                for (int q = 4 * NT / MT * t; q < 4 * NT / MT * (t + 1); ++q) {
+                    const int j = q / 4;
+                    if (q % 4 == 0 && g % 2 == 0) {
+                        w4_scale<ZEROS>(scales[i][j], zeros[i][j], w4_group(p.w, b + i, g / 2), p.w.scales_f16, scale[j],
+                                        shift[j]);
+                        shift[j] *= scale[j];
+                        scale[j] *= 512.0f;
                     }
-            }
+                    w[g & 1][j][q % 4] = w4_weight_pair<F16>(codes[i][j][g & 1][g / 2], q % 4, scale[j], shift[j]);
+                }
+            };
+#pragma unroll
+            for (int t = 0; t < MT; ++t) prepare(0, t);
+#pragma unroll
+            for (int g = 0; g < 8; ++g)
+#pragma unroll
+                for (int t = 0; t < MT; ++t) {
+                    if (g < 7) prepare(g + 1, t);
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) acc[j][t] = w4_mfma<F16>(w[g & 1][j], x[g & 1][t], acc[j][t]);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
         }
     }
     wait_vmcnt0();  // the last copies
@@ -164,11 +160,7 @@ __global__ __launch_bounds__(256, 2) void w4_tile_kernel(TileArgs p) {
             for (int v = 0; v < 4; ++v) {
                 const v4f y = {acc[j][t][4 * v], acc[j][t][4 * v + 1], acc[j][t][4 * v + 2], acc[j][t][4 * v + 3]};
                 const int64_t m = m0 + 32 * t + r32, n = 16 * (int64_t)blk0 + 32 * j + 8 * v + 4 * half;
-                if (p.parts) {
-                    if (m < p.w.m && n < p.npad) *reinterpret_cast<v4f*>(p.parts + (z * p.w.m + m) * p.npad + n) = y;
-                } else {
-                    w4_store<F16>(p.w, m, n, y);
-                }
+                store_sums<F16>(p, at.z, m, n, y);
             }
 }
 
@@ -183,15 +175,22 @@ __global__ __launch_bounds__(256) void w4_join_kernel(TileArgs p) {
 }
 
 struct Plan {
-    int nt, mt, splits, per_split, mtiles, ntiles, steps, npad;
+    int nt, mt, splits, per_split, mtiles, ntiles, steps, npad, slab;  // slab: its 32-column tiles, or 0
     int64_t parts_bytes;
 };
 
-// 128 x 256 tiles where they fill the chip (4096 rows of 14336 x 5376: 545 us, 1160 TFLOP/s; 128 x 128: 587, 64 x 256:
-// 702, three stages, which leave one workgroup to a CU: 718).  Else 128 columns, of 128 rows or, where that
+// 128 x 256 tiles where they fill the chip (4096 rows of 14336 x 5376: 524 us, 1205 TFLOP/s; 128 x 128: 605, 64 x 256:
+// 702, three stages, which leave one workgroup to a CU: 603).  Else 128 columns, of 128 rows or, where that
 // pads the rows by over a seventh, of 64, and k in as many parts as give about two workgroups to a CU (600 rows of
-// 5376 x 7168: 64 us with 128 rows in two parts, 71 with 64 rows; 200 rows: 33 us in three parts, 47 in one, 39
-// in six, whose binary32 sums are written and read once more), each of at least four blocks.
+// 5376 x 7168: 62 us with 128 rows in two parts, 73 with 64), each of at least four blocks.
+//
+// Or w4_slab.hip, whose waves split k inside a workgroup, when it is estimated to take less.  The estimate, in
+// 1/20 of 0.87 us, is a line through some sixty timings: a workgroup of it takes 20 (1 + NT) for eight
+// blocks, a tile 26 or 17 (64 rows) a block, each once for 256 workgroups, beside 80, or 220 with sums in memory and
+// their launch.  Measured, us, slab and tile, the chosen one first: 64 rows of 1024 x 4096 8.8 and 11.5, 40 of 5376 x 7168
+// 14.7 and 19.5, 200 of 4096 x 4096 15.1 and 22.9, 200 of 5376 x 7168 28.7 and 33.1, 128 of 10752 x 5376 24.2 and 29.9; tile
+// and slab: 64 of 2048 x 16384 24.6 and 31.4, 384 of 5376 x 7168 42.4 and 47.2, 600 of it 61 and 84.  Near the
+// line the other one would at times be better, by up to 19 % (200 of 2048 x 16384: slab 39, tile 33).
 Plan plan_tiles(int64_t m, int64_t n, int64_t k) {
     Plan p{};
     p.steps = (int)((k + 127) / 128);
@@ -208,16 +207,25 @@ Plan plan_tiles(int64_t m, int64_t n, int64_t k) {
     p.per_split = (int)((p.steps + splits - 1) / splits);
     p.splits = (p.steps + p.per_split - 1) / p.per_split;
     p.npad = (int)((n + 15) / 16 * 16);
-    p.parts_bytes = p.splits > 1 ? (int64_t)p.splits * m * p.npad * 4 : 0;
+    if (p.nt == 1) {
+        const auto rounds = [](int64_t workgroups) { return (workgroups + 255) / 256; };
+        int64_t best = (p.splits > 1 ? 220 : 80) + rounds(count * p.splits) * p.per_split * (p.mt == 4 ? 26 : 17);
+        for (int nt = 1; nt <= 3; ++nt) {
+            const int64_t workgroups = (m + 63) / 64 * ((n + 32 * nt - 1) / (32 * nt));
+            const int64_t cost = 80 + rounds(workgroups) * ((p.steps + 7) / 8) * 20 * (1 + nt);
+            if (cost < best) best = cost, p.slab = nt;
+        }
+    }
+    p.parts_bytes = p.splits > 1 && !p.slab ? (int64_t)p.splits * m * p.npad * 4 : 0;
     return p;
 }
 
 template <bool F16, bool ZEROS>
 hipError_t launch_cfg(const TileArgs& a, const Plan& p, hipStream_t st) {
     const dim3 grid((unsigned)(p.mtiles * p.ntiles * p.splits));
-    if (p.nt == 2) hipLaunchKernelGGL((w4_tile_kernel<F16, ZEROS, 2, 4, 2>), grid, dim3(256), 0, st, a);
-    else if (p.mt == 4) hipLaunchKernelGGL((w4_tile_kernel<F16, ZEROS, 1, 4, 2>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((w4_tile_kernel<F16, ZEROS, 1, 2, 3>), grid, dim3(256), 0, st, a);
+    if (p.nt == 2) hipLaunchKernelGGL((w4_tile_kernel<F16, ZEROS, 2, 4>), grid, dim3(256), 0, st, a);
+    else if (p.mt == 4) hipLaunchKernelGGL((w4_tile_kernel<F16, ZEROS, 1, 4>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((w4_tile_kernel<F16, ZEROS, 1, 2>), grid, dim3(256), 0, st, a);
     return hipGetLastError();
 }
 
@@ -240,6 +248,7 @@ int64_t w4_tile_workspace_bytes(int64_t m, int64_t n, int64_t k) { return plan_t
 
 hipError_t launch_w4_tile(const W4Args& w, void* workspace, hipStream_t st) {
     const Plan p = plan_tiles(w.m, w.n, w.k);
+    if (p.slab) return launch_w4_slab(w, p.slab, st);
     TileArgs a{};
     a.w = w;
     a.parts = p.splits > 1 ? (float*)workspace : nullptr;

@@ -63,6 +63,23 @@ def test_w4_mm_sizes(ops, device, m, n, k, group):
     assert torch.equal(got, again)  # sums in a fixed order
 
 
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("m,n,k,group", [(40, 8300, 1040, 32), (64, 9217, 144, 128), (70, 8300, 528, 128),
+                                         (130, 12300, 400, 64), (33, 16500, 1040, 256), (129, 2070, 2320, 32),
+                                         (600, 4096, 4096, 128)])
+def test_w4_mm_dozens_of_rows(ops, device, m, n, k, group, dtype, zeros):
+    """Where a workgroup's waves split k: one to three column tiles of 32, ragged in rows, columns and k."""
+    kind = TYPES[dtype]
+    rows = _weights(n, k, group, zeros, kind, device)
+    w = _pack(ops, device, *rows, group)
+    x = activations(m, k, seed=m).to(kind).to(device)
+    bias = torch.randn(n, generator=torch.Generator().manual_seed(n)).to(kind).to(device)
+    got = ops.w4_mm(x, w, bias=bias)
+    assert_product(got, *product(x, *rows, group, bias))
+    assert torch.equal(ops.w4_mm(x, w, bias=bias), got)
+
+
 @pytest.mark.parametrize("group", [32, 128, 384])
 @pytest.mark.parametrize("m", [1, 20, 100, 1000])
 def test_w4_mm_single_columns(ops, device, m, group):
