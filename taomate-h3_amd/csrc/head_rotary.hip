@@ -11,8 +11,13 @@
 // holds d / (2 V)), each with V pairs of one 16-byte vector per side, and a wave takes 64 / G heads of one
 // token at a time.  The token's cosines and sines (fp32: as many bytes as two bf16 rows) and the norm's
 // weights stay in registers over the HEADS * 64 / G heads of the wave; its HEADS vectors are asked for
-// together, ahead of the first use.  The lanes that own a row read all of it before they store any of it,
-// so a call may run in place.
+// together, ahead of the first use and of the position and the slot they are needed with.  The lanes that own a row
+// read all of it before they store any of it, so a call may run in place.  The folds over a row go by lane
+// permutation, two to four instructions where a shuffle takes a round trip through LDS.
+//
+// Measured: 18603 tokens of 28 + 28 heads of 128, bf16, 110 us, 4.9 TB/s (a copy reaches 5.1); 6201 tokens of 28
+// rotated 16 us, of which the caches hold a part; 8190 tokens of 32 query heads and 8 + 8 heads into e4m3 pages
+// with a scale a row 45 us, 4.1 TB/s; one token 3 us, which is a launch.
 //
 // Pairs: (i, half + i), where a lane's two vectors at c V and half + c V hold both sides, or (2 i, 2 i + 1), where
 // each of them holds V / 2 whole pairs.  Channels from 2 * half on go through as they are (a select, not a
@@ -392,13 +397,16 @@ hipError_t launch_heads_vec(HeadArgs a, hipStream_t st) {
     a.lanes = 1;
     while (a.lanes < 64 && a.lanes * 2 * V < a.d) a.lanes *= 2;
     const int rows = 64 / a.lanes;
-    // Four rows a lane group where that still leaves the chip enough waves; one for a few tokens.
+    // Four rows a lane group where that spares waves and leaves the chip 16 a CU, else one.  28 + 28 heads of 192: 512
+    // tokens 7.2 us with four and 6.7 with one, 1024 tokens 10.4 and 11.3; 32 + 8 heads of 128: 1024 tokens 6.3 and 5.7, 2048
+    // 10.1 and 10.7; 8 + 2 of 64, which one row a group holds: 4096 tokens 6.9 and 6.0.
     auto units = [&](int heads) {
         int sum = 0;
         for (int i = 0; i < a.segments; ++i) sum += a.seg[i].units = (a.seg[i].heads + rows * heads - 1) / (rows * heads);
         return sum;
     };
-    if (a.tokens * units(4) >= 4096) return launch_heads_cfg<DT, V, NC, 4>(a, units(4), st);
+    const int one = units(1), four = units(4);
+    if (four < one && a.tokens * four >= 4096) return launch_heads_cfg<DT, V, NC, 4>(a, four, st);
     return launch_heads_cfg<DT, V, NC, 1>(a, units(1), st);
 }
 

@@ -189,7 +189,7 @@ struct Plan {
 // blocks, a tile 26 or 17 (64 rows) a block, each once for 256 workgroups, beside 80, or 220 with sums in memory and
 // their launch.  Measured, us, slab and tile, the chosen one first: 64 rows of 1024 x 4096 8.8 and 11.5, 40 of 5376 x 7168
 // 14.7 and 19.5, 200 of 4096 x 4096 15.1 and 22.9, 200 of 5376 x 7168 28.7 and 33.1, 128 of 10752 x 5376 24.2 and 29.9; tile
-// and slab: 64 of 2048 x 16384 24.6 and 31.4, 384 of 5376 x 7168 42.4 and 47.2, 600 of it 61 and 84.  Near the
+// and slab: 64 of 2048 x 16384 24.6 and 31.4, 256 of 14336 x 5376 52.6 and 66.9, 600 of 5376 x 7168 61 and 84.  Near the
 // line the other one would at times be better, by up to 19 % (200 of 2048 x 16384: slab 39, tile 33).
 Plan plan_tiles(int64_t m, int64_t n, int64_t k) {
     Plan p{};

@@ -1,5 +1,5 @@
 """Linears with 4-bit weights and group scales, the sibling of the W8A8 linears for decode, where a
-linear's time is its weights' bytes.  No counterpart in the reference.
+linear's time is its weights' bytes.  Forward only.  No counterpart in the reference.
 
 * ``W4Linear``                        a linear on packed 4-bit weights, from full weights or a checkpoint's codes
 * ``set_module_w4_weight_``           the same on a module that keeps its class: a parallel linear of the
@@ -29,8 +29,9 @@ def quantize_w4_weight(weight: torch.Tensor, *, group: int = 128, zeros: bool = 
 def w4_linear(inputs: torch.Tensor, weight: ops.W4Weight, bias: torch.Tensor | None = None) -> torch.Tensor:
     """``inputs [..., k]`` times the transposed weights: [..., n] in the inputs' dtype."""
     flat = inputs.reshape(-1, int(inputs.shape[-1]))
-    if flat.stride(-1) != 1 or flat.data_ptr() % 16 or (flat.shape[0] > 1 and flat.stride(0) % 8):
-        flat = flat.contiguous()
+    if flat.stride(-1) != 1 or flat.data_ptr() % 16 or (
+            flat.shape[0] > 1 and (flat.stride(0) % 8 or flat.stride(0) < flat.shape[1])):
+        flat = flat.clone(memory_format=torch.contiguous_format)  # contiguous() keeps an unaligned start
     if bias is not None and bias.dtype != inputs.dtype:
         bias = bias.to(inputs.dtype)
     return ops.w4_mm(flat, weight, bias=bias).reshape(*inputs.shape[:-1], weight.n)

@@ -13,7 +13,7 @@ from _toy_layers import ToyColumnLinear
 from _util import activations
 from _w4 import assert_product, product
 from taomate_h3_amd.distributed.linear import _module_linear
-from taomate_h3_amd.inference import w4
+from taomate_h3_amd.inference import lora, w4
 from taomate_h3_amd.inference.fused_kernels import QuantizedActivations
 from taomate_h3_amd.inference.paged_cache import PagedKVCache, QKNormRotary
 
@@ -149,9 +149,30 @@ def test_module_dispatch(ops, device, bias):
     assert _module_linear(layer, x[:0], layer.bias).shape == (0, 40, 100)
     unaligned = torch.zeros(4, 216, device=device, dtype=torch.bfloat16)[:, 3:211]
     assert layer(unaligned).shape == (4, 100)
+    values = activations(4, 216, seed=4).to(device)
+    for view in (values[:, 3:211], values[0, 3:211], values[:1, 8:].expand(6, 208), values.t()[:208, :1].t()):
+        want, bound = product(view.reshape(-1, 208), *(r.cpu() for r in rows), 32, layer.bias)
+        assert_product(layer(view).reshape(-1, 100), want, bound)
     with pytest.raises(TypeError):  # codes of another format have no bf16 rows
         codes, s = ops.quant_rows(x.reshape(-1, 208), ops.FMT_INT8)
         layer(QuantizedActivations(codes, s, tuple(x.shape), ops.FMT_INT8))
+
+
+def test_lora_on_a_4_bit_base(ops, device):
+    """The wrapper adds its branch to such a base by the two-product formula; folding it in is refused."""
+    layer = ToyColumnLinear(128, 96, bias=False, dtype=torch.bfloat16, device=device)
+    rows = ops.quantize_w4((torch.randn(96, 128, generator=_gen(1)) * 0.1).to(torch.bfloat16).to(device), 64)
+    w4.set_module_w4_weight_(layer, ops.pack_w4(*rows, group=64))
+    a, b = ((torch.randn(shape, generator=_gen(seed)) * 0.1).to(torch.bfloat16).to(device)
+            for shape, seed in (((8, 128), 2), ((96, 8), 3)))
+    wrapped = lora.H3InferenceParallelLinearLoRA(layer, kind="column", a=a, b=b, scale=0.5)
+    x = activations(7, 128, seed=4).to(device)
+    branch = torch.nn.functional.linear(torch.nn.functional.linear(x, a), b)
+    assert torch.equal(wrapped(x), layer(x) + branch * 0.5)
+    model = torch.nn.Module()
+    model.layer = wrapped
+    with pytest.raises(lora.H3LoRACheckpointError):
+        lora.merge_h3_lora_weights_(model)
 
 
 def test_block_policy(ops, device):
