@@ -28,6 +28,7 @@ import torch.nn.functional as F
 
 from .. import ops
 from .fused_kernels import as_dense
+from .w4 import module_w4_weight
 
 FUSED_MAX_RANK = 128
 
@@ -212,7 +213,9 @@ def fuse_h3_lora_wrappers_(transformer: Any) -> Mapping[str, Any]:
         weight = getattr(base, "weight", None)
         if weight is None or lora_a.ndim != 2 or lora_b.ndim != 2 or int(lora_a.shape[0]) != int(lora_b.shape[1]):
             raise H3LoRACheckpointError(f"H3 inference LoRA local shape differs: {name}")
-        if int(lora_a.shape[1]) != int(weight.shape[1]) or int(lora_b.shape[0]) != int(weight.shape[0]):
+        packed = module_w4_weight(base)
+        rows, cols = (weight.shape[0], weight.shape[1]) if packed is None else (packed.n, packed.k)
+        if int(lora_a.shape[1]) != int(cols) or int(lora_b.shape[0]) != int(rows):
             raise H3LoRACheckpointError(f"H3 inference LoRA local shape differs: {name}")
         if kind == "row" and int(getattr(base, "tp_size", 1)) > 1:
             kept.append(name)

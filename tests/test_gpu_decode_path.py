@@ -170,7 +170,11 @@ def test_lora_on_a_4_bit_base(ops, device):
     branch = torch.nn.functional.linear(torch.nn.functional.linear(x, a), b)
     assert torch.equal(wrapped(x), layer(x) + branch * 0.5)
     model = torch.nn.Module()
-    model.layer = wrapped
+    model.layer = torch.nn.Module()  # an installed wrapper, to be swapped
+    model.layer.base, model.layer.kind, model.layer.scale = layer, "column", 0.5
+    model.layer.lora_a, model.layer.lora_b, model.layer._taomate_h3_inference_lora = a, b, True
+    assert lora.fuse_h3_lora_wrappers_(model)["replaced_count"] == 1
+    assert torch.equal(model.layer(x), wrapped(x))
     with pytest.raises(lora.H3LoRACheckpointError):
         lora.merge_h3_lora_weights_(model)
 

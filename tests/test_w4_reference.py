@@ -81,10 +81,10 @@ def test_c_entry_points_refuse():
     assert mm(x=odd) == 1 and "aligned" in error()
     assert mm(codes=None) == 1 and "null" in error()
     assert mm(m=0) == 0 and mm(n=0) == 0
-    need = lib.h3q_w4_mm_workspace_bytes(300, 48, 4096, 32)  # few tiles: a split sum
+    need = lib.h3q_w4_mm_workspace_bytes(300, 48, 16384, 32)  # few tiles, long rows: a split sum
     assert need > 0 and lib.h3q_w4_mm_workspace_bytes(4, 48, 4096, 32) == 0
-    assert mm(m=300, k=4096, ldx=4096) == 1 and "workspace" in error()
-    assert mm(m=300, k=4096, ldx=4096, ws=p, size=need - 1) == 1 and "needed" in error()
+    assert mm(m=300, k=16384, ldx=16384) == 1 and "workspace" in error()
+    assert mm(m=300, k=16384, ldx=16384, ws=p, size=need - 1) == 1 and "needed" in error()
     assert mm(m=(1 << 31) - 1, n=1 << 20, ldo=1 << 20) == 2 and "too many" in error()
     assert lib.h3q_w4_code_bytes(17, 144) == 2 * 2 * 1024 and lib.h3q_w4_code_bytes(0, 144) == 0
     pack = lambda ldc=32, lds=2, z=None, ldz=0, n=4, k=64, zo=None, out=p: lib.h3q_w4_pack(
