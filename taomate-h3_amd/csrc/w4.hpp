@@ -3,12 +3,12 @@
 //   y[m, n] = sum_k x[m, k] * s[n, g] * (u[n, k] - z[n, g])  [+ bias[n]],   g = k / group
 //
 // Up to 32 rows (w4_stream.hpp) the integers go into the matrix instructions and a group's sum is scaled in
-// binary32: bound by the weights' bytes, it has room for that.  Above (w4_tile.hip) the weight s (u - z), which
-// binary32 holds exactly, is rounded once to x's 16-bit type and summed over all of k in the matrix instructions'
-// accumulators.  The rounding costs 1.1 times the error of the output's own; what it saves is an fma and an
-// offset for every output and group: scaling the sums was built for many rows too, and took 600 us for 4096 rows of
-// 14336 x 5376 at groups of 128 without zero points, 1330 us at groups of 32 with them, where this takes 545
-// and 549.
+// binary32: bound by the weights' bytes, it has room for that.  Above (w4_slab.hip, w4_tile.hip) the weight s (u - z),
+// which binary32 holds exactly, is rounded once to x's 16-bit type and summed over all of k in the matrix instructions'
+// accumulators.  Against 64 bits the result is off by 1.3 times what the output's own rounding costs; what it saves is an
+// fma and an offset for every output and group: scaling the sums was built for many rows too, and took 600 us for 4096
+// rows of 14336 x 5376 at groups of 128 without zero points, 1330 us at groups of 32 with them, where this takes 524
+// and 541.
 //
 // Layout.  Codes lie in blocks of 16 rows x 128 columns, 1 KiB, [row blocks][column blocks]: lane L's 16 bytes
 // are four words, word s the eight codes k = 128 b + 32 s + 8 (L / 16) .. + 7 of row L % 16, the low nibbles of

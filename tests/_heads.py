@@ -4,7 +4,7 @@ that are computed in binary32 and rounded once.
 A value y = a c - b s of normed channels is off by
 * half a step of its type where it is stored: eps / 2 of its magnitude (and half of the smallest subnormal),
 * binary32 before that: the norm's factor has a sum of d squares (d / 2 V of them in a lane, each one fused
-  step, then log2 steps), a division, a sum, a root and a quotient, and two products; at most 24 + d / 8
+  step, then log2 steps), a product, a sum, the reciprocal root (a unit) and two products; at most 24 + d / 8
   roundings of 2^-24 in all, of which the sum's count half (a root), then two products and a sum: the
   roundings apply to |a c| + |b s|, which cancellation does not shrink.
 FP32 = 2^-24 (32 + d / 8) of |a c| + |b s| covers all of it."""

@@ -129,6 +129,41 @@ def test_tokens_appended_in_pieces_are_the_prompts_rows(ops, device, scales):
         assert torch.equal(k, k2) and torch.equal(v, v2)
 
 
+@pytest.mark.parametrize("scales", [None, "rows"])
+def test_decode_step_in_a_graph(ops, device, scales):
+    """A step of three sequences captured once (a product, plan, append, a product) and replayed as they grow, with
+    eager work between; every replay gives the eager step's bits, in the pages too."""
+    (qkv, _), (out, _) = _block(ops, device, False)[0]
+    norm = _block(ops, device, False)[1]
+    cache, eager = (PagedKVCache(12, PAGE, HK, D, scales=scales, device=device) for _ in range(2))
+    table = torch.randperm(12, generator=_gen(4)).int().view(3, 4).to(device)
+    lengths = torch.tensor([14, 0, 47], dtype=torch.int32, device=device)
+    cu = torch.arange(4, dtype=torch.int32, device=device)
+    x = activations(4, WIDTH, seed=0).to(device)  # the last row is padding
+
+    def step(cache):
+        rows = qkv(x)
+        return out(norm.append(rows, cache, cache.plan(table, lengths, cu, 4)).flatten(1))
+
+    q = step(cache)  # also what the graph's own first call would otherwise load
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        q = step(cache)
+    assert torch.equal(step(eager)[:3], step(cache)[:3])
+    for replay in range(4):
+        x.copy_(activations(4, WIDTH, seed=10 + replay).to(device))
+        want = step(eager)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(q[:3], want[:3])
+        assert torch.equal(cache.k.float(), eager.k.float()) and torch.equal(cache.v.float(), eager.v.float())
+        if scales:
+            assert torch.equal(cache.k_scale, eager.k_scale) and torch.equal(cache.v_scale, eager.v_scale)
+        lengths += 1
+
+
 @pytest.mark.parametrize("bias", [False, True])
 def test_module_dispatch(ops, device, bias):
     """A parallel linear with 4-bit weights through _module_linear, its deep copy, and any leading dimensions."""

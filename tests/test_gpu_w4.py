@@ -247,3 +247,31 @@ def test_w4_python_body_equals_native(ops, device, monkeypatch):
     for x, y in zip(xs, want):
         assert torch.equal(ops.w4_mm(x, w, bias=bias), y)
     assert taken == ["w4_mm", "w4_mm"]
+
+
+def test_w4_split_sums_of_two_graphs(ops, device):
+    """Long rows and few tiles: k in parts, whose sums lie in a workspace of each captured call's own."""
+    n, k = 256, 14336
+    rows = _weights(n, k, 128, True, torch.bfloat16, device)
+    w = _pack(ops, device, *rows, 128)
+    xs = [activations(m, k, seed=m).to(device) for m in (48, 100)]
+    outs = [torch.empty(x.shape[0], n, device=device, dtype=x.dtype) for x in xs]
+    graphs = []
+    for x, out in zip(xs, outs):
+        assert_product(ops.w4_mm(x, w), *product(x, *rows, 128))
+        torch.cuda.synchronize()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            ops.w4_mm(x, w, out=out)
+    side = torch.cuda.Stream()
+    for replay in range(3):
+        for x in xs:
+            x.copy_(activations(x.shape[0], k, seed=70 + replay).to(device))
+        want = [ops.w4_mm(x, w) for x in xs]
+        torch.cuda.synchronize()
+        graphs[0].replay()
+        with torch.cuda.stream(side):
+            graphs[1].replay()
+        torch.cuda.synchronize()
+        for out, y in zip(outs, want):
+            assert torch.equal(out, y)
