@@ -37,14 +37,6 @@ __device__ __forceinline__ uint32_t w4_pair(float lo, float hi) {
     else return pack_bf16x2(lo, hi);
 }
 
-// Pair q of a word's eight codes -> weights 2 q and 2 q + 1, rounded to x's type: scale = 2^9 s, shift = -z s.
-template <bool F16>
-__device__ __forceinline__ uint32_t w4_weight_pair(uint32_t w, int q, float scale, float shift) {
-    const int codes = (int)((q < 2 ? w : w >> 4) & 0x0F0F0F0Fu);
-    const v2f u = q & 1 ? __builtin_amdgcn_cvt_pk_f32_fp8(codes, true) : __builtin_amdgcn_cvt_pk_f32_fp8(codes, false);
-    return w4_pair<F16>(__builtin_fmaf(u[0], scale, shift), __builtin_fmaf(u[1], scale, shift));
-}
-
 // Group of the 32-column step s of block b: floor((4 b + s) / (group / 32)), by a multiplication that is exact for
 // k <= 2^22 and groups up to 2^18 (numerator and divisor are doubled so that a divisor of 1 has a reciprocal).
 __device__ __forceinline__ int w4_group(const W4Args& p, int b, int s) {
@@ -59,8 +51,47 @@ __device__ __forceinline__ void w4_scale(v2u s, uint32_t z, int e, uint32_t f16,
     const uint32_t at = (uint32_t)(e & 3) * 0x0202u + 0x0100u;  // its two bytes
     const uint32_t bits = __builtin_amdgcn_perm(s[1], s[0], at << 16 | 0x0C0Cu);
     scale = __uint_as_float((__float_as_uint(f16_hi(bits)) & f16) | (bits & ~f16));
-    shift = ZEROS ? -(float)(z >> (8 * (e & 3)) & 255u) : -8.0f;
+    shift = ZEROS ? -(float)(__builtin_amdgcn_perm(0u, z, (uint32_t)(e & 3)) & 255u) : -8.0f;
 }
+
+// A row's scale and zero point, and the weights that they make of its codes: s (u - z), rounded once to x's type.
+// With binary16 on both sides u - z (exact) and the product are packed binary16 (15 operations for 8 codes); else an fma
+// of u with s and -z s (exact in binary32) and a rounding (19).
+template <bool F16, bool SF16, bool ZEROS>
+struct W4Row {
+    static constexpr bool PACKED = F16 && SF16;
+    float scale, shift;  // 2^9 s and -z s
+    v2h scale2, shift2;  // s and -z, twice
+
+    __device__ __forceinline__ void set(v2u s, uint32_t z, int e) {
+        if constexpr (PACKED) {
+            const uint32_t at = (uint32_t)(e & 3) * 0x0202u + 0x0100u, place = (uint32_t)(e & 3) | 0x0C00u;
+            scale2 = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(s[1], s[0], at << 16 | at));
+            const v2h top = {(_Float16)1024.0f, (_Float16)1024.0f};  // with z in its last bits: 1024 + z
+            if (ZEROS)
+                shift2 = top - __builtin_bit_cast(v2h, __builtin_amdgcn_perm(0u, z, place << 16 | place) | 0x64006400u);
+            else
+                shift2 = v2h{(_Float16)-8.0f, (_Float16)-8.0f};
+        } else {
+            w4_scale<ZEROS>(s, z, e, SF16 ? ~0u : 0u, scale, shift);
+            shift *= scale;
+            scale *= 512.0f;
+        }
+    }
+    // Weights 2 q and 2 q + 1 of a word's eight.
+    __device__ __forceinline__ uint32_t pair(uint32_t w, int q) const {
+        const uint32_t codes = (q < 2 ? w : w >> 4) & 0x0F0F0F0Fu;
+        if constexpr (PACKED) {
+            const v2h u = q & 1 ? __builtin_bit_cast(v2h, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, 512.0f, true))
+                                : __builtin_bit_cast(v2h, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, 512.0f, false));
+            return __builtin_bit_cast(uint32_t, (u + shift2) * scale2);
+        } else {
+            const v2f u = q & 1 ? __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, true)
+                                : __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, false);
+            return w4_pair<F16>(__builtin_fmaf(u[0], scale, shift), __builtin_fmaf(u[1], scale, shift));
+        }
+    }
+};
 
 // A descriptor whose words are in scalar registers for sure: where the compiler loses sight of that, every load
 // through it becomes a loop over the lanes' values.

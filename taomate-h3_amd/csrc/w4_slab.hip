@@ -27,7 +27,7 @@ __device__ __forceinline__ void copy4(const CopySrc& src, uint32_t lds_base, uin
                  : "memory");
 }
 
-template <bool F16, bool ZEROS, int NT>
+template <bool F16, bool SF16, bool ZEROS, int NT>
 __global__ __launch_bounds__(512) void w4_slab_kernel(W4Args p, int mtiles, int ntiles) {
     constexpr int MT = 2, WAVES = 8, RING = NT == 1 ? 4 : 3, XSTAGE = 64 * 64;
     constexpr int CODES = NT * (2048 + 256 + (ZEROS ? 256 : 0)), COPIES = 4, CODE_COPIES = NT * (ZEROS ? 4 : 3);
@@ -58,23 +58,22 @@ __global__ __launch_bounds__(512) void w4_slab_kernel(W4Args p, int mtiles, int 
     const uint32_t xat = (uint32_t)(lane >> 2) * row_bytes + 16u * chunk;
     auto ask_x = [&](int b, int q, int r) __attribute__((always_inline)) {
         const bool ok = b < steps && 128 * b + 32 * q + 8 * chunk < p.k;
-        const uint32_t off = xat + 256u * b + 64u * q;
+        const uint32_t off = ok ? xat + 256u * b + 64u * q : kW4Oob;  // past the range from there on, too
 #pragma unroll
-        for (int i = 0; i < COPIES; ++i)
-            copy16(rx, base + r * XSTAGE + i * 1024, ok ? off + 16u * i * row_bytes : kW4Oob);
+        for (int i = 0; i < COPIES; ++i) copy16(rx, base + r * XSTAGE + i * 1024, off + 16u * i * row_bytes);
     };
     auto ask_codes = [&](int b) __attribute__((always_inline)) {
         const bool ok = b < steps;
         const int q = w4_group(p, b, 0) >> 2;
+        const uint32_t off = ok ? (uint32_t)b * 1024u + 16u * lane : kW4Oob;
 #pragma unroll
-        for (int j = 0; j < 2 * NT; ++j)
-            copy16(rw, codes_base + j * 1024, ok ? (uint32_t)(j * steps + b) * 1024u + 16u * lane : kW4Oob);
+        for (int j = 0; j < 2 * NT; ++j) copy16(rw, codes_base + j * 1024, off + (uint32_t)(j * steps) * 1024u);
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-            const int row = (2 * j + (lane >> 5)) * quads + q;
-            copy4(rs, codes_base + NT * 2048 + j * 256, ok ? (uint32_t)row * 128u + 4u * (lane & 31) : kW4Oob);
+            const int quad = (2 * j + (lane >> 5)) * quads + q;
+            copy4(rs, codes_base + NT * 2048 + j * 256, ok ? (uint32_t)quad * 128u + 4u * (lane & 31) : kW4Oob);
             if constexpr (ZEROS)
-                copy4(rz, codes_base + NT * 2304 + j * 256, ok && (lane & 16) == 0 ? (uint32_t)row * 64u + 4u * (lane & 15) : kW4Oob);
+                copy4(rz, codes_base + NT * 2304 + j * 256, ok && (lane & 16) == 0 ? (uint32_t)quad * 64u + 4u * (lane & 15) : kW4Oob);
         }
     };
 
@@ -86,7 +85,7 @@ __global__ __launch_bounds__(512) void w4_slab_kernel(W4Args p, int mtiles, int 
     v4u codes[NT][2], w[2][NT], x[2][MT];
     v2u scales[NT];
     uint32_t zeros[NT];
-    float scale[NT], shift[NT];
+    W4Row<F16, SF16, ZEROS> row[NT];
     auto fetch = [&]() __attribute__((always_inline)) {
         const H3Q_LDS uint8_t* const from = mine + RING * XSTAGE;
 #pragma unroll
@@ -108,12 +107,8 @@ __global__ __launch_bounds__(512) void w4_slab_kernel(W4Args p, int mtiles, int 
 #pragma unroll
         for (int q = 4 * NT / MT * t; q < 4 * NT / MT * (t + 1); ++q) {
             const int j = q / 4;
-            if (q % 4 == 0 && g % 2 == 0) {
-                w4_scale<ZEROS>(scales[j], zeros[j], w4_group(p, b, g / 2), p.scales_f16, scale[j], shift[j]);
-                shift[j] *= scale[j];
-                scale[j] *= 512.0f;
-            }
-            w[g & 1][j][q % 4] = w4_weight_pair<F16>(codes[j][g & 1][g / 2], q % 4, scale[j], shift[j]);
+            if (q % 4 == 0 && g % 2 == 0) row[j].set(scales[j], zeros[j], w4_group(p, b, g / 2));
+            w[g & 1][j][q % 4] = row[j].pair(codes[j][g & 1][g / 2], q % 4);
         }
     };
 
@@ -181,21 +176,26 @@ __global__ __launch_bounds__(512) void w4_slab_kernel(W4Args p, int mtiles, int 
     }
 }
 
-template <bool F16, bool ZEROS>
+template <bool F16, bool SF16, bool ZEROS>
 hipError_t launch_cols(const W4Args& a, int nt, hipStream_t st) {
     const int mtiles = (int)((a.m + 63) / 64), ntiles = (int)((a.n + 32 * nt - 1) / (32 * nt));
     const dim3 grid((unsigned)(mtiles * ntiles));
-    if (nt == 1) hipLaunchKernelGGL((w4_slab_kernel<F16, ZEROS, 1>), grid, dim3(512), 0, st, a, mtiles, ntiles);
-    else if (nt == 2) hipLaunchKernelGGL((w4_slab_kernel<F16, ZEROS, 2>), grid, dim3(512), 0, st, a, mtiles, ntiles);
-    else hipLaunchKernelGGL((w4_slab_kernel<F16, ZEROS, 3>), grid, dim3(512), 0, st, a, mtiles, ntiles);
+    if (nt == 1) hipLaunchKernelGGL((w4_slab_kernel<F16, SF16, ZEROS, 1>), grid, dim3(512), 0, st, a, mtiles, ntiles);
+    else if (nt == 2) hipLaunchKernelGGL((w4_slab_kernel<F16, SF16, ZEROS, 2>), grid, dim3(512), 0, st, a, mtiles, ntiles);
+    else hipLaunchKernelGGL((w4_slab_kernel<F16, SF16, ZEROS, 3>), grid, dim3(512), 0, st, a, mtiles, ntiles);
     return hipGetLastError();
+}
+
+template <bool F16, bool SF16>
+hipError_t launch_zeros(const W4Args& a, int nt, hipStream_t st) {
+    return a.zeros ? launch_cols<F16, SF16, true>(a, nt, st) : launch_cols<F16, SF16, false>(a, nt, st);
 }
 
 }  // namespace
 
 hipError_t launch_w4_slab(const W4Args& a, int nt, hipStream_t st) {
-    if (a.f16) return a.zeros ? launch_cols<true, true>(a, nt, st) : launch_cols<true, false>(a, nt, st);
-    return a.zeros ? launch_cols<false, true>(a, nt, st) : launch_cols<false, false>(a, nt, st);
+    if (a.f16) return a.scales_f16 ? launch_zeros<true, true>(a, nt, st) : launch_zeros<true, false>(a, nt, st);
+    return a.scales_f16 ? launch_zeros<false, true>(a, nt, st) : launch_zeros<false, false>(a, nt, st);
 }
 
 }  // namespace h3q

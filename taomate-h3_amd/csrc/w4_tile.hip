@@ -33,7 +33,7 @@ __device__ __forceinline__ void store_sums(const TileArgs& p, int z, int64_t m, 
     }
 }
 
-template <bool F16, bool ZEROS, int NT, int MT>
+template <bool F16, bool SF16, bool ZEROS, int NT, int MT>
 __global__ __launch_bounds__(256, 2) void w4_tile_kernel(TileArgs p) {
     constexpr int D = 2, STAGE = MT * 32 * 256;
     __shared__ __attribute__((aligned(1024))) uint8_t lds_raw[D * STAGE];
@@ -66,7 +66,7 @@ __global__ __launch_bounds__(256, 2) void w4_tile_kernel(TileArgs p) {
             128 * b + 8 * chunk < p.w.k ? crow * row_bytes + 256u * b + 16u * chunk : kW4Oob;
 #pragma unroll
         for (int i = 0; i < COPIES; ++i)
-            copy16(rx, base + (wave + 4 * i) * 1024, off == kW4Oob ? kW4Oob : off + 16u * i * row_bytes);
+            copy16(rx, base + (wave + 4 * i) * 1024, off + 16u * i * row_bytes);  // past the range from kW4Oob on, too
     };
     // Row r32 of 32-column tile j: its block and place there; k quarters half and half + 2.
     uint32_t code_off[NT], scale_off[NT];
@@ -122,19 +122,14 @@ __global__ __launch_bounds__(256, 2) void w4_tile_kernel(TileArgs p) {
             // Operands one step of 16 k ahead: between two matrix instructions' issues the next step's reads and a
             // part of its unpacking.
             v4u x[2][MT], w[2][NT];
-            float scale[NT], shift[NT];
+            W4Row<F16, SF16, ZEROS> row[NT];
             auto prepare = [&](int g, int t) __attribute__((always_inline)) {  // part t of MT for step g
                 x[g & 1][t] = *(const H3Q_LDS v4u*)(tile + xoff[g] + t * 32 * 256);
 #pragma unroll
                 for (int q = 4 * NT / MT * t; q < 4 * NT / MT * (t + 1); ++q) {
                     const int j = q / 4;
-                    if (q % 4 == 0 && g % 2 == 0) {
-                        w4_scale<ZEROS>(scales[i][j], zeros[i][j], w4_group(p.w, b + i, g / 2), p.w.scales_f16, scale[j],
-                                        shift[j]);
-                        shift[j] *= scale[j];
-                        scale[j] *= 512.0f;
-                    }
-                    w[g & 1][j][q % 4] = w4_weight_pair<F16>(codes[i][j][g & 1][g / 2], q % 4, scale[j], shift[j]);
+                    if (q % 4 == 0 && g % 2 == 0) row[j].set(scales[i][j], zeros[i][j], w4_group(p.w, b + i, g / 2));
+                    w[g & 1][j][q % 4] = row[j].pair(codes[i][j][g & 1][g / 2], q % 4);
                 }
             };
 #pragma unroll
@@ -220,18 +215,19 @@ Plan plan_tiles(int64_t m, int64_t n, int64_t k) {
     return p;
 }
 
-template <bool F16, bool ZEROS>
+template <bool F16, bool SF16, bool ZEROS>
 hipError_t launch_cfg(const TileArgs& a, const Plan& p, hipStream_t st) {
     const dim3 grid((unsigned)(p.mtiles * p.ntiles * p.splits));
-    if (p.nt == 2) hipLaunchKernelGGL((w4_tile_kernel<F16, ZEROS, 2, 4>), grid, dim3(256), 0, st, a);
-    else if (p.mt == 4) hipLaunchKernelGGL((w4_tile_kernel<F16, ZEROS, 1, 4>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((w4_tile_kernel<F16, ZEROS, 1, 2>), grid, dim3(256), 0, st, a);
+    if (p.nt == 2) hipLaunchKernelGGL((w4_tile_kernel<F16, SF16, ZEROS, 2, 4>), grid, dim3(256), 0, st, a);
+    else if (p.mt == 4) hipLaunchKernelGGL((w4_tile_kernel<F16, SF16, ZEROS, 1, 4>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((w4_tile_kernel<F16, SF16, ZEROS, 1, 2>), grid, dim3(256), 0, st, a);
     return hipGetLastError();
 }
 
 template <bool F16>
 hipError_t launch_type(const TileArgs& a, const Plan& p, hipStream_t st) {
-    const hipError_t e = a.w.zeros ? launch_cfg<F16, true>(a, p, st) : launch_cfg<F16, false>(a, p, st);
+    const hipError_t e = a.w.scales_f16 ? (a.w.zeros ? launch_cfg<F16, true, true>(a, p, st) : launch_cfg<F16, true, false>(a, p, st))
+                                        : (a.w.zeros ? launch_cfg<F16, false, true>(a, p, st) : launch_cfg<F16, false, false>(a, p, st));
     if (e != hipSuccess || p.splits == 1) return e;
     hipLaunchKernelGGL((w4_join_kernel<F16>), dim3((unsigned)((a.w.m * p.npad / 4 + 255) / 256)), dim3(256), 0, st, a);
     return hipGetLastError();
