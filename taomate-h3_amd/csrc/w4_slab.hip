@@ -4,15 +4,16 @@
 // blocks w, w + 8, ... on its own, from a ring of x and a place for a block's codes in LDS that only it fills
 // (buffer_load ... lds) and reads, so that there is no barrier before the last sums are joined there, in order.
 // Where w4_tile.hip splits k over workgroups it writes and reads binary32 sums and takes a second launch: 100 rows
-// of 4096 x 4096 12.5 us against 15.5, 48 rows of 5376 x 7168 15.9 against 18.9, 200 rows 29.4 against 32.4.
+// of 4096 x 4096 11.6 us against 18.3, 40 rows of 5376 x 7168 14.1 against 16.7, 200 rows 26.5 against 29.5.
 //
 // Everything that is fetched goes through LDS copies, whose count is known at every point; with a load into registers
 // among them the compiler's own wait for it would count the copies behind it as done too early.  x comes in
 // quarters of a block (32 columns, 64 bytes of a row; chunk c of a row lies in slot c ^ (row / 4 % 4), which
 // keeps eight rows' reads of one chunk apart).  One step of 16 k ahead the operands are read and unpacked
-// between the matrix instructions.  Eight waves and not four: a wave alone on its SIMD issues a vector instruction of 8
-// bytes every 8 cycles, two share them at one every 4.  What bounds it is a sum of three like parts, at 200 rows of
-// 5376 x 7168 each 9 to 12 us: the matrix instructions, the unpacking (once for 64 rows) and the copies.
+// between the matrix instructions, and the copies are asked for there one at a time.  Eight waves and not four: a
+// wave alone on its SIMD issues a vector instruction of 8 bytes every 8 cycles, two share them at one every 4.  What bounds
+// it at 200 rows of 5376 x 7168: the vector port (some 560 instructions a wave and block, and 16 cycles of each
+// of 48 matrix instructions) for 17 of the 26 us, without the copies 22 in all, and the copies' waits.
 #include "w4.hpp"
 
 namespace h3q {
@@ -25,6 +26,21 @@ __device__ __forceinline__ void copy4(const CopySrc& src, uint32_t lds_base, uin
                  :
                  : "s"(lds_base), "v"(voff), "s"(src.d)
                  : "memory");
+}
+
+// A block's loop has 16 steps, four to a quarter, each with one copy of x and, in the first eight, as many of the
+// next block's codes: how many of those come before step `at` of the block.
+constexpr int code_copies(int copies, int at) {
+    const int n = (copies + 7) / 8 * at;
+    return n < copies ? n : copies;
+}
+// Copies that may be under way in the middle of quarter q, when the x of quarter q + 1 has to be there: those asked
+// for behind it, which are RING - 3 quarters and a half.
+template <int RING, int CODE_COPIES>
+constexpr int asked(int q) {
+    const int from = q + 3 - RING;  // the first quarter behind it; below 0, one of the last block's, without codes
+    const int first = from < 0 ? 0 : from;
+    return 4 * (q - from) + 2 + code_copies(CODE_COPIES, 4 * q + 2) - code_copies(CODE_COPIES, 4 * first);
 }
 
 template <bool F16, bool SF16, bool ZEROS, int NT>
@@ -56,25 +72,21 @@ __global__ __launch_bounds__(512) void w4_slab_kernel(W4Args p, int mtiles, int 
     // A copy instruction takes 64 bytes of 16 rows; chunk c of a row lies in slot c ^ (row / 4 % 4).
     const int chunk = (lane & 3) ^ (lane >> 4);
     const uint32_t xat = (uint32_t)(lane >> 2) * row_bytes + 16u * chunk;
-    auto ask_x = [&](int b, int q, int r) __attribute__((always_inline)) {
+    auto ask_x = [&](int b, int q, int r, int i) __attribute__((always_inline)) {
         const bool ok = b < steps && 128 * b + 32 * q + 8 * chunk < p.k;
         const uint32_t off = ok ? xat + 256u * b + 64u * q : kW4Oob;  // past the range from there on, too
-#pragma unroll
-        for (int i = 0; i < COPIES; ++i) copy16(rx, base + r * XSTAGE + i * 1024, off + 16u * i * row_bytes);
+        copy16(rx, base + r * XSTAGE + i * 1024, off + 16u * i * row_bytes);
     };
-    auto ask_codes = [&](int b) __attribute__((always_inline)) {
+    auto ask_codes = [&](int b, int o) __attribute__((always_inline)) {  // copy o of CODE_COPIES
         const bool ok = b < steps;
-        const int q = w4_group(p, b, 0) >> 2;
-        const uint32_t off = ok ? (uint32_t)b * 1024u + 16u * lane : kW4Oob;
-#pragma unroll
-        for (int j = 0; j < 2 * NT; ++j) copy16(rw, codes_base + j * 1024, off + (uint32_t)(j * steps) * 1024u);
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            const int quad = (2 * j + (lane >> 5)) * quads + q;
+        const int j = o - 2 * NT, quad = (2 * (j % NT) + (lane >> 5)) * quads + (w4_group(p, b, 0) >> 2);
+        if (o < 2 * NT)
+            copy16(rw, codes_base + o * 1024, (ok ? (uint32_t)b * 1024u + 16u * lane : kW4Oob) + (uint32_t)(o * steps) * 1024u);
+        else if (j < NT)
             copy4(rs, codes_base + NT * 2048 + j * 256, ok ? (uint32_t)quad * 128u + 4u * (lane & 31) : kW4Oob);
-            if constexpr (ZEROS)
-                copy4(rz, codes_base + NT * 2304 + j * 256, ok && (lane & 16) == 0 ? (uint32_t)quad * 64u + 4u * (lane & 15) : kW4Oob);
-        }
+        else if (o < CODE_COPIES)
+            copy4(rz, codes_base + NT * 2304 + (j - NT) * 256,
+                  ok && (lane & 16) == 0 ? (uint32_t)quad * 64u + 4u * (lane & 15) : kW4Oob);
     };
 
     v16f acc[NT][MT];
@@ -113,9 +125,12 @@ __global__ __launch_bounds__(512) void w4_slab_kernel(W4Args p, int mtiles, int 
     };
 
     const int b0 = wave;
-    ask_codes(b0);
 #pragma unroll
-    for (int q = 0; q < RING - 1; ++q) ask_x(b0, q, q);
+    for (int o = 0; o < CODE_COPIES; ++o) ask_codes(b0, o);
+#pragma unroll
+    for (int q = 0; q < RING - 1; ++q)
+#pragma unroll
+        for (int i = 0; i < COPIES; ++i) ask_x(b0, q, q, i);
     wait_vmcnt<(RING - 2) * COPIES>();
     fetch();
 #pragma unroll
@@ -128,23 +143,24 @@ __global__ __launch_bounds__(512) void w4_slab_kernel(W4Args p, int mtiles, int 
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             const int r1 = r == RING - 1 ? 0 : r + 1, last = r == 0 ? RING - 1 : r - 1;
-            if (q == 0) {
-                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the fetch: its place is filled again
-                ask_codes(b + WAVES);
-            }
-            ask_x(q + RING - 1 < 4 ? b : b + WAVES, (q + RING - 1) & 3, last);
-            __builtin_amdgcn_sched_barrier(0);
+            if (q == 0) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the fetch: its place is filled again
 #pragma unroll
             for (int g = 2 * q; g < 2 * q + 2; ++g) {
                 if (g & 1) {
-                    if (q < RING - 2) wait_vmcnt<(RING - 2) * COPIES + CODE_COPIES>();
-                    else wait_vmcnt<(RING - 2) * COPIES>();
+                    if (q == 0) wait_vmcnt<asked<RING, CODE_COPIES>(0)>();
+                    else if (q == 1) wait_vmcnt<asked<RING, CODE_COPIES>(1)>();
+                    else if (q == 2) wait_vmcnt<asked<RING, CODE_COPIES>(2)>();
+                    else wait_vmcnt<asked<RING, CODE_COPIES>(3)>();
                     if (q == 3) fetch();
                 }
 #pragma unroll
                 for (int t = 0; t < MT; ++t) {
                     read(g + 1, t, g & 1 ? r1 : r);
                     unpack(g == 7 ? b + WAVES : b, (g + 1) & 7, t);
+                    ask_x(q + RING - 1 < 4 ? b : b + WAVES, (q + RING - 1) & 3, last, (g & 1) * MT + t);
+#pragma unroll
+                    for (int o = code_copies(CODE_COPIES, g * MT + t); o < code_copies(CODE_COPIES, g * MT + t + 1); ++o)
+                        ask_codes(b + WAVES, o);
 #pragma unroll
                     for (int j = 0; j < NT; ++j) acc[j][t] = w4_mfma<F16>(w[g & 1][j], x[g & 1][t], acc[j][t]);
                     __builtin_amdgcn_sched_barrier(0);

@@ -6,9 +6,10 @@
 // x tile is copied into one of two LDS stages (buffer_load ... lds, no registers; a row is 256 contiguous bytes, its
 // 16-byte chunk c in slot c ^ (row % 16), so that 16 rows' reads of one chunk meet no bank twice), and the codes,
 // scales and zero points into registers, one block ahead.  One barrier a block.  Inside a block the operands of the
-// next 16 columns are read and unpacked between the matrix instructions of these, in pieces that the scheduler
-// must not gather: 4096 rows of 14336 x 5376 524 us, 549 in the compiler's order.  At 1.9 GHz, where such a product
-// holds the clock, the matrix instructions are busy for 60 % of that; the library's bf16 product takes 505 to 517.
+// next 16 columns are read and unpacked between the matrix instructions of these, and the next block's copies and loads
+// issued there one at a time, in pieces that the scheduler must not gather: 4096 rows of 14336 x 5376 492 us, 511 with
+// the copies and loads together, 549 in the compiler's order; the library's bf16 product takes 505 to 517.  A matrix
+// instruction keeps the vector port for 16 of its 32 cycles, whoever wants it, so the unpacking hides behind half.
 //
 // Few tiles: k is split over several workgroups, whose binary32 sums a last kernel adds in order.
 #include "w4.hpp"
@@ -60,13 +61,11 @@ __global__ __launch_bounds__(256, 2) void w4_tile_kernel(TileArgs p) {
     // A copy instruction takes four rows; wave w the rows 4 w .. + 3 of every 16.
     const int crow = 4 * wave + (lane >> 4), chunk = (lane & 15) ^ crow;
     constexpr int COPIES = 2 * MT;
-    auto copy = [&](int b, int stage) __attribute__((always_inline)) {
+    auto copy = [&](int b, int stage, int i) __attribute__((always_inline)) {
         const uint32_t base = (uint32_t)(uintptr_t)(lds + stage * STAGE);
         const uint32_t off =
             128 * b + 8 * chunk < p.w.k ? crow * row_bytes + 256u * b + 16u * chunk : kW4Oob;
-#pragma unroll
-        for (int i = 0; i < COPIES; ++i)
-            copy16(rx, base + (wave + 4 * i) * 1024, off + 16u * i * row_bytes);  // past the range from kW4Oob on, too
+        copy16(rx, base + (wave + 4 * i) * 1024, off + 16u * i * row_bytes);  // past the range from kW4Oob on, too
     };
     // Row r32 of 32-column tile j: its block and place there; k quarters half and half + 2.
     uint32_t code_off[NT], scale_off[NT];
@@ -79,17 +78,18 @@ __global__ __launch_bounds__(256, 2) void w4_tile_kernel(TileArgs p) {
     v4u codes[D][NT][2];
     v2u scales[D][NT];
     uint32_t zeros[D][NT];
-    auto load = [&](int i, int b) __attribute__((always_inline)) {
-        const int q = w4_group(p.w, b, 0) >> 2;
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            codes[i][j][0] = __builtin_amdgcn_raw_buffer_load_b128(rw, code_off[j] + 1024u * b, 0, 0);
-            codes[i][j][1] = __builtin_amdgcn_raw_buffer_load_b128(rw, code_off[j] + 1024u * b + 512u, 0, 0);
-            scales[i][j] = __builtin_amdgcn_raw_buffer_load_b64(rs, (scale_off[j] + 16u * q) * 8, 0, 0);
-            zeros[i][j] = 0;
-            if constexpr (ZEROS) zeros[i][j] = __builtin_amdgcn_raw_buffer_load_b32(rz, (scale_off[j] + 16u * q) * 4, 0, 0);
-        }
+    constexpr int LOADS = NT * (ZEROS ? 4 : 3);
+    auto load = [&](int b, int stage, int o) __attribute__((always_inline)) {
+        const int j = o % NT, q = w4_group(p.w, b, 0) >> 2;
+        if (o < 2 * NT)
+            codes[stage][j][o / NT] = __builtin_amdgcn_raw_buffer_load_b128(rw, code_off[j] + 1024u * b + 512u * (o / NT), 0, 0);
+        else if (o < 3 * NT)
+            scales[stage][j] = __builtin_amdgcn_raw_buffer_load_b64(rs, (scale_off[j] + 16u * q) * 8, 0, 0);
+        else
+            zeros[stage][j] = __builtin_amdgcn_raw_buffer_load_b32(rz, (scale_off[j] + 16u * q) * 4, 0, 0);
     };
+#pragma unroll
+    for (int j = 0; j < NT; ++j) zeros[0][j] = zeros[1][j] = 0;
 
     v16f acc[NT][MT];
 #pragma unroll
@@ -102,25 +102,23 @@ __global__ __launch_bounds__(256, 2) void w4_tile_kernel(TileArgs p) {
     for (int c = 0; c < 8; ++c) xoff[c] = r32 * 256 + 16 * ((2 * c + half) ^ (r32 & 15));
 
     const int b0 = at.z * p.per_split, b1 = b0 + p.per_split < steps ? b0 + p.per_split : steps;
-    // Blocks past b1 are copied nowhere (out of range), but counted: every stage has as many copies in flight.
-    auto ask = [&](int i, int b) __attribute__((always_inline)) {
-        load(i, b < b1 ? b : b1 - 1);
-        __builtin_amdgcn_sched_barrier(0);
-        copy(b < b1 ? b : steps, i);
+    // A block's copies and loads, one at a time.  Past b1 the copies are out of range and the loads repeat.
+    auto ask = [&](int b, int stage, int o) __attribute__((always_inline)) {
+        if (o < COPIES) copy(b < b1 ? b : steps, stage, o);
+        else if (o < COPIES + LOADS) load(b < b1 ? b : b1 - 1, stage, o - COPIES);
     };
 #pragma unroll
-    for (int i = 0; i < D - 1; ++i) ask(i, b0 + i);
+    for (int o = 0; o < COPIES + LOADS; ++o) ask(b0, 0, o);
+    static_assert(COPIES + LOADS <= 8 * MT, "one at each step of the loop");
     for (int b = b0; b < b1; b += D) {
 #pragma unroll
         for (int i = 0; i < D; ++i) {
             if (b + i >= b1) break;
             wait_vmcnt0();    // this wave's part of stage i has landed
             __syncthreads();  // everyone's has, and every wave is done with the stage before it
-            ask((i + D - 1) % D, b + i + D - 1);
-            __builtin_amdgcn_sched_barrier(0);
             const H3Q_LDS uint8_t* const tile = lds + i * STAGE;
-            // Operands one step of 16 k ahead: between two matrix instructions' issues the next step's reads and a
-            // part of its unpacking.
+            // Operands one step of 16 k ahead, the next block's copies and loads one at a time: between two matrix
+            // instructions' issues a read, a part of the unpacking and one of those.
             v4u x[2][MT], w[2][NT];
             W4Row<F16, SF16, ZEROS> row[NT];
             auto prepare = [&](int g, int t) __attribute__((always_inline)) {  // part t of MT for step g
@@ -139,6 +137,7 @@ __global__ __launch_bounds__(256, 2) void w4_tile_kernel(TileArgs p) {
 #pragma unroll
                 for (int t = 0; t < MT; ++t) {
                     if (g < 7) prepare(g + 1, t);
+                    ask(b + i + 1, 1 - i, g * MT + t);
 #pragma unroll
                     for (int j = 0; j < NT; ++j) acc[j][t] = w4_mfma<F16>(w[g & 1][j], x[g & 1][t], acc[j][t]);
                     __builtin_amdgcn_sched_barrier(0);
@@ -174,18 +173,19 @@ struct Plan {
     int64_t parts_bytes;
 };
 
-// 128 x 256 tiles where they fill the chip (4096 rows of 14336 x 5376: 524 us, 1205 TFLOP/s; 128 x 128: 605, 64 x 256:
-// 702, three stages, which leave one workgroup to a CU: 603).  Else 128 columns, of 128 rows or, where that
-// pads the rows by over a seventh, of 64, and k in as many parts as give about two workgroups to a CU (600 rows of
-// 5376 x 7168: 62 us with 128 rows in two parts, 73 with 64), each of at least four blocks.
+// 128 x 256 tiles where they fill the chip (4096 rows of 14336 x 5376: 492 us, 1285 TFLOP/s; 128 x 128: 553, 64 x 128:
+// 642).  Else 128 columns, of 128 rows or, where that pads the rows by over a seventh, of 64, and k in as many
+// parts as give about two workgroups to a CU (600 rows of 5376 x 7168: 57 us with 128 rows in two parts, 70 with 64),
+// each of at least four blocks.
 //
 // Or w4_slab.hip, whose waves split k inside a workgroup, when it is estimated to take less.  The estimate, in
-// 1/20 of 0.87 us, is a line through some sixty timings: a workgroup of it takes 20 (1 + NT) for eight
-// blocks, a tile 26 or 17 (64 rows) a block, each once for 256 workgroups, beside 80, or 220 with sums in memory and
-// their launch.  Measured, us, slab and tile, the chosen one first: 64 rows of 1024 x 4096 8.8 and 11.5, 40 of 5376 x 7168
-// 14.7 and 19.5, 200 of 4096 x 4096 15.1 and 22.9, 200 of 5376 x 7168 28.7 and 33.1, 128 of 10752 x 5376 24.2 and 29.9; tile
-// and slab: 64 of 2048 x 16384 24.6 and 31.4, 256 of 14336 x 5376 52.6 and 66.9, 600 of 5376 x 7168 61 and 84.  Near the
-// line the other one would at times be better, by up to 19 % (200 of 2048 x 16384: slab 39, tile 33).
+// 1/20 of 0.87 us, is a line through 48 shapes (40 to 600 rows, 1024 to 14336 columns, k 4096 to 16384): a workgroup
+// of it takes 20 (1 + NT) for eight blocks, a tile 22 or 15 (64 rows) a block, each once for 256 workgroups, beside
+// 80 there, and 60 or, with sums in memory and their launch, 240 here.  Measured, us, slab and tile, the chosen one
+// first: 64 rows of 1024 x 4096 8.2 and 10.6, 40 of 5376 x 7168 14.1 and 16.7, 200 of 4096 x 4096 14.0 and 20.2, 200 of
+// 5376 x 7168 26.5 and 29.5; tile and slab: 64 of 2048 x 16384 19.3 and 32.5, 384 of 5376 x 7168 39 and 46, 600 of it
+// 57 and 81, 256 of 14336 x 5376 48 and 63.  At two of the 48 the other one is better, by 4 and 19 % (128 of 10752 x
+// 5376: tile 26.4, slab 22.2).
 Plan plan_tiles(int64_t m, int64_t n, int64_t k) {
     Plan p{};
     p.steps = (int)((k + 127) / 128);
@@ -204,7 +204,7 @@ Plan plan_tiles(int64_t m, int64_t n, int64_t k) {
     p.npad = (int)((n + 15) / 16 * 16);
     if (p.nt == 1) {
         const auto rounds = [](int64_t workgroups) { return (workgroups + 255) / 256; };
-        int64_t best = (p.splits > 1 ? 220 : 80) + rounds(count * p.splits) * p.per_split * (p.mt == 4 ? 26 : 17);
+        int64_t best = (p.splits > 1 ? 240 : 60) + rounds(count * p.splits) * p.per_split * (p.mt == 4 ? 22 : 15);
         for (int nt = 1; nt <= 3; ++nt) {
             const int64_t workgroups = (m + 63) / 64 * ((n + 32 * nt - 1) / (32 * nt));
             const int64_t cost = 80 + rounds(workgroups) * ((p.steps + 7) / 8) * 20 * (1 + nt);

@@ -96,6 +96,16 @@ def test_w4_mm_single_columns(ops, device, m, group):
     assert torch.equal(ops.w4_mm(x.to(device), w).cpu().double(), want)
 
 
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("m,n,k", [(20, 99, 272), (40, 8300, 1040), (33, 16500, 1040), (64, 64, 9232), (2048, 4096, 144)])
+def test_w4_mm_scales_of_the_other_type(ops, device, m, n, k, dtype, zeros):
+    kind = TYPES[dtype]
+    rows = _weights(n, k, 32, zeros, torch.float16 if kind == torch.bfloat16 else torch.bfloat16, device)
+    x = activations(m, k, seed=m).to(kind).to(device)
+    assert_product(ops.w4_mm(x, _pack(ops, device, *rows, 32)), *product(x, *rows, 32))
+
+
 @pytest.mark.parametrize("m", [7, 40, 900])
 def test_w4_mm_strides_and_scale_types(ops, device, m):
     """Rows of wider x and out, an unaligned out and bias, scales of the other type; the rest of out is left."""
