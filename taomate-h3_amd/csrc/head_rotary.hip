@@ -15,9 +15,9 @@
 // read all of it before they store any of it, so a call may run in place.  The folds over a row go by lane
 // permutation, two to four instructions where a shuffle takes a round trip through LDS.
 //
-// Measured: 18603 tokens of 28 + 28 heads of 128, bf16, 110 us, 4.9 TB/s (a copy reaches 5.1); 6201 tokens of 28
+// Measured: 18603 tokens of 28 + 28 heads of 128, bf16, 108 us, 5.0 TB/s (a copy reaches 5.1); 6201 tokens of 28
 // rotated 16 us, of which the caches hold a part; 8190 tokens of 32 query heads and 8 + 8 heads into e4m3 pages
-// with a scale a row 45 us, 4.1 TB/s; one token 3 us, which is a launch.
+// with a scale a row 41 us, 4.5 TB/s; one token 3 us, which is a launch.
 //
 // Pairs: (i, half + i), where a lane's two vectors at c V and half + c V hold both sides, or (2 i, 2 i + 1), where
 // each of them holds V / 2 whole pairs.  Channels from 2 * half on go through as they are (a select, not a
@@ -106,6 +106,8 @@ __device__ __forceinline__ void store_codes(uint8_t* p, const float (&y)[V]) {
     }
 }
 
+constexpr int kBlockRows = 65535;  // a grid's second extent
+
 // DT: the rows' type.  V: channels a vector.  NC: chunks of 2 V channels a lane (1, or 4 at V = 1).
 // HEADS: rows a lane group takes.  INTER: interleaved pairs.  CACHE: some rows go into pages.
 template <int DT, int V, int NC, int HEADS, bool INTER, bool CACHE>
@@ -119,9 +121,9 @@ __global__ __launch_bounds__(256) void head_rotary_kernel(HeadArgs p) {
     using VC = typename Vec<float, HALF>::type;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t token = (int64_t)blockIdx.x * 4 + wave;
+    const int64_t token = (((int64_t)blockIdx.z * kBlockRows + blockIdx.y) * 8 + (blockIdx.x & 7)) * 4 + wave;
     if (token >= p.tokens) return;
-    int unit = blockIdx.y, which = 0;
+    int unit = blockIdx.x >> 3, which = 0;
     while (which + 1 < p.segments && unit >= p.seg[which].units) unit -= p.seg[which++].units;
     const HeadSegment& s = p.seg[which];
 
@@ -379,7 +381,12 @@ __global__ __launch_bounds__(256) void plan_append_kernel(PlanAppendArgs p) {
 
 template <int DT, int V, int NC, int HEADS, bool CACHE>
 hipError_t launch_heads_pairs(const HeadArgs& a, int units, hipStream_t st) {
-    const dim3 grid((unsigned)((a.tokens + 3) / 4), (unsigned)units);
+    // The units of eight blocks of four tokens one after the other, each block's on one XCD: the few bytes of keys and
+    // values are on their way beside the queries (8190 tokens of 32 + 8 + 8 heads into pages 41 us, 45 with all queries
+    // first), and a token's cosines come out of that XCD's cache.
+    const int64_t blocks = (a.tokens + 31) / 32;
+    const dim3 grid((unsigned)(8 * units), (unsigned)(blocks < kBlockRows ? blocks : kBlockRows),
+                    (unsigned)((blocks + kBlockRows - 1) / kBlockRows));
     if (a.interleaved) hipLaunchKernelGGL((head_rotary_kernel<DT, V, NC, HEADS, true, CACHE>), grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL((head_rotary_kernel<DT, V, NC, HEADS, false, CACHE>), grid, dim3(256), 0, st, a);
     return hipGetLastError();
@@ -397,16 +404,17 @@ hipError_t launch_heads_vec(HeadArgs a, hipStream_t st) {
     a.lanes = 1;
     while (a.lanes < 64 && a.lanes * 2 * V < a.d) a.lanes *= 2;
     const int rows = 64 / a.lanes;
-    // Four rows a lane group where that spares waves and leaves the chip 16 a CU, else one.  28 + 28 heads of 192: 512
-    // tokens 7.2 us with four and 6.7 with one, 1024 tokens 10.4 and 11.3; 32 + 8 heads of 128: 1024 tokens 6.3 and 5.7, 2048
-    // 10.1 and 10.7; 8 + 2 of 64, which one row a group holds: 4096 tokens 6.9 and 6.0.
+    // Four rows a lane group where that spares waves and leaves the chip more than it holds at once (32 a CU), else one.
+    // us, four and one: 18603 tokens of 28 + 28 heads of 128 108 and 123, 8190 of 32 + 8 + 8 into pages 41 and 45; in the
+    // caches, 28 + 28 heads of 192: 512 tokens 7.3 and 6.8, 2048 19.7 and 20.3, 4096 32.5 and 34.7; 32 + 8 of 128: 1024 6.9
+    // and 5.7, 4096 18.9 and 18.2; 8 + 2 of 64, which one row a group holds: 4096 6.9 and 6.1.
     auto units = [&](int heads) {
         int sum = 0;
         for (int i = 0; i < a.segments; ++i) sum += a.seg[i].units = (a.seg[i].heads + rows * heads - 1) / (rows * heads);
         return sum;
     };
     const int one = units(1), four = units(4);
-    if (four < one && a.tokens * four >= 4096) return launch_heads_cfg<DT, V, NC, 4>(a, four, st);
+    if (four < one && a.tokens * four > 8192) return launch_heads_cfg<DT, V, NC, 4>(a, four, st);
     return launch_heads_cfg<DT, V, NC, 1>(a, units(1), st);
 }
 
