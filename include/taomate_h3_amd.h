@@ -496,7 +496,8 @@ int h3q_plan_append(const int32_t* table, int64_t table_stride, int64_t seqs, in
  * hold e4m3(clamp(y * RN(1 / s), +-448)), s of the head, or max(max|y| * RN(1/448), 1e-12) of the
  * row, which goes into the scale pages; NaN and infinities as in h3q_quant_rows.  Slots outside
  * [0, n_pages * page_size), the same for both, are not stored; padding (position below 0) stores neither k, v nor q.
- * Slots of one call that are stored are distinct.  rotation NULL: no rotation, no positions.
+ * Slots of one call that are stored are distinct, and k and v pages share no memory.  rotation NULL: no
+ * rotation, no positions.
  */
 int h3q_append_kv(int dtype, int weight_dtype, const h3q_heads* q, const h3q_heads* k, const h3q_heads* v,
                   const h3q_pages* k_pages, const h3q_pages* v_pages, const int32_t* slots, int64_t tokens,

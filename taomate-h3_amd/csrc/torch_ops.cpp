@@ -565,6 +565,9 @@ Opt append_kv(const Tensor& k, const Tensor& v, const Tensor& k_pages, const Ten
         v.sizes() != k.sizes() || !dense(slots, k, at::kInt) || slots.dim() != 1 || slots.size(0) != k.size(0))
         return std::nullopt;
     if (cos.has_value() != sin.has_value() || (positions && !cos) || (!q && (q_weight || q_out))) return std::nullopt;
+    const auto same = [](const Tensor& a, const Tensor& b) { return a.numel() > 0 && a.data_ptr() == b.data_ptr(); };
+    if (same(k_pages, v_pages) || (k_scale && v_scale && k_scale->dim() == 3 && same(*k_scale, *v_scale)))
+        return std::nullopt;
     h3q_rotation r;
     if (cos && !rotation_of(r, k, *cos, *sin, positions, interleaved, false)) return std::nullopt;
     h3q_heads qh, kh, vh;

@@ -1099,7 +1099,8 @@ def append_kv(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: 
     Pages hold k's dtype, or float8_e4m3fn codes e4m3(clamp(y / s, +-448)): with ``k_scale``, ``v_scale`` fp32 [1]
     or [kv_heads] those are the scales; with [pages, page_size, kv_heads] each row's scale max|y| / 448 is stored
     there.  Slots below 0 or past the pages are not stored, and a token with a position below 0 (padding) has
-    no q either: those rows are left as they were.  The slots of a call that are stored are distinct."""
+    no q either: those rows are left as they were.  The slots of a call that are stored are distinct, and the pages
+    of k and v share no memory."""
     got = _native_call("append_kv", k, v, k_pages, v_pages, slots, k_scale, v_scale, k_weight, float(eps), cos, sin,
                        positions, interleaved, q, q_weight, q_out)
     if got is not None:
@@ -1116,6 +1117,9 @@ def append_kv(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: 
     if k_pages.shape[:2] != v_pages.shape[:2]:
         raise ValueError(f"{name}: k_pages and v_pages differ in pages or page_size ({tuple(k_pages.shape[:2])}, "
                          f"{tuple(v_pages.shape[:2])})")
+    same = lambda a, b: a is not None and b is not None and a.numel() > 0 and a.data_ptr() == b.data_ptr()
+    if same(k_pages, v_pages) or (k_scale is not None and k_scale.ndim == 3 and same(k_scale, v_scale)):
+        raise ValueError(f"{name}: k and v have pages and stored scales of their own")
     rotation = None if cos is None else _rotation(name, cos, sin, positions, tokens, d, interleaved)
     q_heads = None
     if q is not None:

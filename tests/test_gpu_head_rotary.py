@@ -425,6 +425,22 @@ def test_append_kv_refuses(ops, device):
     assert ops.append_kv(k, k, empty, empty.clone(), slots) is None  # no pages: nothing is stored
 
 
+def test_append_kv_refuses_shared_pages(ops, device):
+    k = _rows(3, 2, 16, torch.bfloat16, device)
+    pages = torch.zeros(2, 4, 2, 16, device=device, dtype=torch.bfloat16)
+    slots = torch.arange(3, device=device, dtype=torch.int32)
+    with pytest.raises(ValueError):
+        ops.append_kv(k, k, pages, pages, slots)
+    kp, vp = (torch.zeros(2, 4, 2, 16, device=device, dtype=torch.float8_e4m3fn) for _ in range(2))
+    one, stored = torch.ones(2, device=device), torch.ones(2, 4, 2, device=device)
+    with pytest.raises(ValueError):
+        ops.append_kv(k, k, kp, vp, slots, k_scale=stored, v_scale=stored)
+    ops.append_kv(k, k, kp, vp, slots, k_scale=one, v_scale=one)  # scales that are only read may be one tensor
+    both = torch.zeros(2, 4, 4, 16, device=device, dtype=torch.bfloat16)
+    ops.append_kv(k, 2 * k, both[:, :, :2], both[:, :, 2:], slots)  # and pages may be views of one
+    assert torch.equal(both.flatten(0, 1)[:3], torch.cat((k, 2 * k), 1))
+
+
 # ------------------------------------------- streams, graphs, the Python bodies
 
 def _step(ops, device, seed=0):

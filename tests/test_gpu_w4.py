@@ -285,3 +285,38 @@ def test_w4_split_sums_of_two_graphs(ops, device):
         torch.cuda.synchronize()
         for out, y in zip(outs, want):
             assert torch.equal(out, y)
+
+
+def _picked(n, k, group, cols, x, device, seed=3):
+    """Weights with exact values and an x whose row r holds 2^-3 in column cols[r % len(cols)], and the result: the weights
+    there (exact in both kinds of kernel)."""
+    gen = torch.Generator(device=device).manual_seed(seed)
+    groups = -(-k // group)
+    codes = torch.randint(0, 256, (n, k // 2), generator=gen, device=device, dtype=torch.uint8)
+    scales = torch.exp2(torch.randint(-6, 3, (n, groups), generator=gen, device=device).float()).to(torch.bfloat16)
+    points = torch.randint(0, 16, (n, groups), generator=gen, device=device, dtype=torch.uint8)
+    at = torch.tensor(cols, device=device)[torch.arange(x.shape[0], device=device) % len(cols)]
+    x[torch.arange(x.shape[0], device=device), at] = 0.125
+    u = codes[:, at // 2].int() >> (4 * (at % 2)) & 15
+    g = at // group
+    return (codes, scales, points), ((u - points[:, g].int()).float() * scales[:, g].float() * 0.125).t().to(torch.bfloat16)
+
+
+@pytest.mark.parametrize("group", [32, 1 << 18])
+def test_w4_mm_longest_rows(ops, device, group):
+    n, k = 19, 1 << 22
+    for m in (1, 5, 20, 40):
+        x = torch.zeros(m, k, device=device, dtype=torch.bfloat16)
+        cols = [k - 1, 0, k // 2 + 77, 3 * 128 + 31, k - 4097] if m > 1 else [k - 1]
+        rows, want = _picked(n, k, group, cols, x, device)
+        assert torch.equal(ops.w4_mm(x, ops.pack_w4(*rows, group=group)), want)
+
+
+@pytest.mark.parametrize("m,ldx,n,k", [(130, (1 << 23) - 8, 48, 208), (3, (1 << 23) - 8, 48, 208), (33, (1 << 23) - 8, 48, 208),
+                                       (140001, 16400, 17, 80), (40, 4096, (1 << 20) + 5, 144), (2, 4096, (1 << 20) + 5, 144),
+                                       (70001, 64, 32771, 48)])
+def test_w4_mm_far_rows_and_columns(ops, device, m, ldx, n, k):
+    """The widest row stride, and x and out past 4 GiB."""
+    x = torch.zeros(m, ldx, device=device, dtype=torch.bfloat16)[:, :k]
+    rows, want = _picked(n, k, 32, [k - 1, 5, k // 2], x, device)
+    assert torch.equal(ops.w4_mm(x, ops.pack_w4(*rows, group=32)), want)
