@@ -507,7 +507,7 @@ int h3q_append_kv(int dtype, int weight_dtype, const h3q_heads* q, const h3q_hea
  * Products with 4-bit weights and group scales, for models whose decode is bound by their
  * weights' bytes.  No counterpart in the reference.
  *   y[m, n] = sum_k x[m, k] * s[n, k / group] * (u[n, k] - z[n, k / group])  [+ bias[n]]
- * above 32 rows with the weights s (u - z) rounded once to x's type.  u, z: integers 0 .. 15 (no zero
+ * above 16 rows with the weights s (u - z) rounded once to x's type.  u, z: integers 0 .. 15 (no zero
  * points: z = 8); a group is 32, 64 or a multiple of 128 columns up to 2^18, the last of a row may be
  * shorter; s is bf16 or binary16.  Rows of a checkpoint: codes two a byte [n, k / 2], the low nibble
  * first, scales and zeros (bytes) [n, groups].

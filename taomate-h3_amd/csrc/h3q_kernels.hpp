@@ -338,12 +338,12 @@ struct W4Args {
     uint32_t scales_f16;  // a mask, all ones or none
     int f16, out_vec;     // out_vec: four columns at once are aligned
 };
-constexpr int kW4StreamRows = 32;
+constexpr int kW4StreamRows = 16;
 hipError_t launch_w4_stream(const W4Args& a, hipStream_t st);
 bool w4_tile_fits(int64_t m, int64_t n);  // a launch's grid
 int64_t w4_tile_workspace_bytes(int64_t m, int64_t n, int64_t k);
 hipError_t launch_w4_tile(const W4Args& a, void* workspace, hipStream_t st);
-hipError_t launch_w4_slab(const W4Args& a, int nt, hipStream_t st);  // 64-row tiles of 32 nt columns (1 .. 3)
+hipError_t launch_w4_slab(const W4Args& a, int nt, hipStream_t st);  // 32 or 64 rows, 32 nt columns (1 .. 3)
 // Codes two a byte [n, k / 2] (the low nibble first), scales and zeros [n, groups] -> the layout.
 struct W4PackArgs {
     const uint8_t* codes;

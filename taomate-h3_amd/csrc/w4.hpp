@@ -2,7 +2,7 @@
 //
 //   y[m, n] = sum_k x[m, k] * s[n, g] * (u[n, k] - z[n, g])  [+ bias[n]],   g = k / group
 //
-// Up to 32 rows (w4_stream.hpp) the integers go into the matrix instructions and a group's sum is scaled in
+// Up to 16 rows (w4_stream.hpp) the integers go into the matrix instructions and a group's sum is scaled in
 // binary32: bound by the weights' bytes, it has room for that.  Above (w4_slab.hip, w4_tile.hip) the weight s (u - z),
 // which binary32 holds exactly, is rounded once to x's 16-bit type and summed over all of k in the matrix instructions'
 // accumulators.  Against 64 bits the result is off by 1.3 times what the output's own rounding costs; what it saves is an

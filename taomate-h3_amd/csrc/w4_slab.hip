@@ -1,10 +1,11 @@
 // Product with 4-bit weights for some dozens of rows, gfx950: one launch, no sums in memory.
 //
-// A workgroup owns 64 rows x 32 NT columns and all of k, which its eight waves split: wave w takes the 128-column
+// A workgroup owns 64 rows (up to 32 rows in all: 32) x 32 NT columns and all of k, which its eight waves split: wave w takes the 128-column
 // blocks w, w + 8, ... on its own, from a ring of x and a place for a block's codes in LDS that only it fills
 // (buffer_load ... lds) and reads, so that there is no barrier before the last sums are joined there, in order.
 // Where w4_tile.hip splits k over workgroups it writes and reads binary32 sums and takes a second launch: 100 rows
-// of 4096 x 4096 11.6 us against 18.3, 40 rows of 5376 x 7168 14.1 against 16.7, 200 rows 26.5 against 29.5.
+// of 4096 x 4096 11.6 us against 18.3, 40 rows of 5376 x 7168 14.1 against 16.7, 200 rows 26.5 against 29.5.  Up to 16 rows w4_stream.hpp keeps the weights
+// exact; two of its row tiles took 32 rows of 5376 x 7168 in 18.3 us where this takes 12.4, 17 rows in 13.2 and 10.0.
 //
 // Everything that is fetched goes through LDS copies, whose count is known at every point; with a load into registers
 // among them the compiler's own wait for it would count the copies behind it as done too early.  x comes in
@@ -28,25 +29,27 @@ __device__ __forceinline__ void copy4(const CopySrc& src, uint32_t lds_base, uin
                  : "memory");
 }
 
-// A block's loop has 16 steps, four to a quarter, each with one copy of x and, in the first eight, as many of the
+// A block's loop has 8 MT steps, 2 MT to a quarter, each with one copy of x and, in the first half, as many of the
 // next block's codes: how many of those come before step `at` of the block.
-constexpr int code_copies(int copies, int at) {
-    const int n = (copies + 7) / 8 * at;
-    return n < copies ? n : copies;
+template <int MT, int CODE_COPIES>
+constexpr int code_copies(int at) {
+    const int n = (CODE_COPIES + 4 * MT - 1) / (4 * MT) * at;
+    return n < CODE_COPIES ? n : CODE_COPIES;
 }
 // Copies that may be under way in the middle of quarter q, when the x of quarter q + 1 has to be there: those asked
-// for behind it, which are RING - 3 quarters and a half.
-template <int RING, int CODE_COPIES>
+// for behind it, which are RING - 3 quarters and a half.  (The codes, of quarters 0 and 1, are there in the third.)
+template <int MT, int RING, int CODE_COPIES>
 constexpr int asked(int q) {
-    const int from = q + 3 - RING;  // the first quarter behind it; below 0, one of the last block's, without codes
-    const int first = from < 0 ? 0 : from;
-    return 4 * (q - from) + 2 + code_copies(CODE_COPIES, 4 * q + 2) - code_copies(CODE_COPIES, 4 * first);
+    static_assert(RING == 3 || RING == 4, "a quarter of the last block that could be behind it has no codes");
+    const int from = q + 3 - RING;  // the first quarter behind it; -1: the last block's last
+    return 2 * MT * (q - from) + MT + code_copies<MT, CODE_COPIES>(2 * MT * q + MT) -
+           code_copies<MT, CODE_COPIES>(2 * MT * (from < 0 ? 0 : from));
 }
 
-template <bool F16, bool SF16, bool ZEROS, int NT>
+template <bool F16, bool SF16, bool ZEROS, int NT, int MT>
 __global__ __launch_bounds__(512) void w4_slab_kernel(W4Args p, int mtiles, int ntiles) {
-    constexpr int MT = 2, WAVES = 8, RING = NT == 1 ? 4 : 3, XSTAGE = 64 * 64;
-    constexpr int CODES = NT * (2048 + 256 + (ZEROS ? 256 : 0)), COPIES = 4, CODE_COPIES = NT * (ZEROS ? 4 : 3);
+    constexpr int WAVES = 8, RING = NT == 1 || MT == 1 ? 4 : 3, XSTAGE = MT * 32 * 64;
+    constexpr int CODES = NT * (2048 + 256 + (ZEROS ? 256 : 0)), COPIES = 2 * MT, CODE_COPIES = NT * (ZEROS ? 4 : 3);
     constexpr int WAVE = RING * XSTAGE + CODES;
     static_assert(WAVES * WAVE >= NT * 4 * WAVES * 1024, "the sums of a row tile");
     __shared__ __attribute__((aligned(1024))) uint8_t lds_raw[WAVES * WAVE];
@@ -56,11 +59,11 @@ __global__ __launch_bounds__(512) void w4_slab_kernel(W4Args p, int mtiles, int 
     const int r32 = lane & 31, half = lane >> 5;
     const W4Tile at = w4_tile_of(mtiles, ntiles, 1);
 
-    const int64_t m0 = (int64_t)at.m * 64;
+    const int64_t m0 = (int64_t)at.m * 32 * MT;
     const int blk0 = at.n * 2 * NT, blocks = (int)((p.n + 15) / 16);
     const int nblk = blocks - blk0 < 2 * NT ? blocks - blk0 : 2 * NT;
     const int steps = (int)((p.k + 127) / 128), quads = (p.groups + 3) / 4;
-    const int64_t rows = p.m - m0 < 64 ? p.m - m0 : 64;
+    const int64_t rows = p.m - m0 < 32 * MT ? p.m - m0 : 32 * MT;
     const CopySrc rx(p.x + m0 * p.ldx, (uint32_t)(((rows - 1) * p.ldx + p.k) * 2));
     const CopySrc rw(p.codes + (int64_t)blk0 * steps * 1024, (uint32_t)((int64_t)nblk * steps * 1024));
     const CopySrc rs(p.scales + (int64_t)blk0 * quads * 64, (uint32_t)((int64_t)nblk * quads * 128));
@@ -147,10 +150,10 @@ __global__ __launch_bounds__(512) void w4_slab_kernel(W4Args p, int mtiles, int 
 #pragma unroll
             for (int g = 2 * q; g < 2 * q + 2; ++g) {
                 if (g & 1) {
-                    if (q == 0) wait_vmcnt<asked<RING, CODE_COPIES>(0)>();
-                    else if (q == 1) wait_vmcnt<asked<RING, CODE_COPIES>(1)>();
-                    else if (q == 2) wait_vmcnt<asked<RING, CODE_COPIES>(2)>();
-                    else wait_vmcnt<asked<RING, CODE_COPIES>(3)>();
+                    if (q == 0) wait_vmcnt<asked<MT, RING, CODE_COPIES>(0)>();
+                    else if (q == 1) wait_vmcnt<asked<MT, RING, CODE_COPIES>(1)>();
+                    else if (q == 2) wait_vmcnt<asked<MT, RING, CODE_COPIES>(2)>();
+                    else wait_vmcnt<asked<MT, RING, CODE_COPIES>(3)>();
                     if (q == 3) fetch();
                 }
 #pragma unroll
@@ -159,7 +162,7 @@ __global__ __launch_bounds__(512) void w4_slab_kernel(W4Args p, int mtiles, int 
                     unpack(g == 7 ? b + WAVES : b, (g + 1) & 7, t);
                     ask_x(q + RING - 1 < 4 ? b : b + WAVES, (q + RING - 1) & 3, last, (g & 1) * MT + t);
 #pragma unroll
-                    for (int o = code_copies(CODE_COPIES, g * MT + t); o < code_copies(CODE_COPIES, g * MT + t + 1); ++o)
+                    for (int o = code_copies<MT, CODE_COPIES>(g * MT + t); o < code_copies<MT, CODE_COPIES>(g * MT + t + 1); ++o)
                         ask_codes(b + WAVES, o);
 #pragma unroll
                     for (int j = 0; j < NT; ++j) acc[j][t] = w4_mfma<F16>(w[g & 1][j], x[g & 1][t], acc[j][t]);
@@ -192,19 +195,24 @@ __global__ __launch_bounds__(512) void w4_slab_kernel(W4Args p, int mtiles, int 
     }
 }
 
-template <bool F16, bool SF16, bool ZEROS>
+template <bool F16, bool SF16, bool ZEROS, int MT>
 hipError_t launch_cols(const W4Args& a, int nt, hipStream_t st) {
-    const int mtiles = (int)((a.m + 63) / 64), ntiles = (int)((a.n + 32 * nt - 1) / (32 * nt));
+    const int mtiles = (int)((a.m + 32 * MT - 1) / (32 * MT)), ntiles = (int)((a.n + 32 * nt - 1) / (32 * nt));
     const dim3 grid((unsigned)(mtiles * ntiles));
-    if (nt == 1) hipLaunchKernelGGL((w4_slab_kernel<F16, SF16, ZEROS, 1>), grid, dim3(512), 0, st, a, mtiles, ntiles);
-    else if (nt == 2) hipLaunchKernelGGL((w4_slab_kernel<F16, SF16, ZEROS, 2>), grid, dim3(512), 0, st, a, mtiles, ntiles);
-    else hipLaunchKernelGGL((w4_slab_kernel<F16, SF16, ZEROS, 3>), grid, dim3(512), 0, st, a, mtiles, ntiles);
+    if (nt == 1) hipLaunchKernelGGL((w4_slab_kernel<F16, SF16, ZEROS, 1, MT>), grid, dim3(512), 0, st, a, mtiles, ntiles);
+    else if (nt == 2) hipLaunchKernelGGL((w4_slab_kernel<F16, SF16, ZEROS, 2, MT>), grid, dim3(512), 0, st, a, mtiles, ntiles);
+    else hipLaunchKernelGGL((w4_slab_kernel<F16, SF16, ZEROS, 3, MT>), grid, dim3(512), 0, st, a, mtiles, ntiles);
     return hipGetLastError();
+}
+
+template <bool F16, bool SF16, bool ZEROS>
+hipError_t launch_rows(const W4Args& a, int nt, hipStream_t st) {
+    return a.m <= 32 ? launch_cols<F16, SF16, ZEROS, 1>(a, nt, st) : launch_cols<F16, SF16, ZEROS, 2>(a, nt, st);
 }
 
 template <bool F16, bool SF16>
 hipError_t launch_zeros(const W4Args& a, int nt, hipStream_t st) {
-    return a.zeros ? launch_cols<F16, SF16, true>(a, nt, st) : launch_cols<F16, SF16, false>(a, nt, st);
+    return a.zeros ? launch_rows<F16, SF16, true>(a, nt, st) : launch_rows<F16, SF16, false>(a, nt, st);
 }
 
 }  // namespace

@@ -1,18 +1,18 @@
-// Product with 4-bit weights for few rows (m <= 32), gfx950: bound by the weights' bytes, n k / 2 from HBM once, as
+// Product with 4-bit weights for few rows (m <= 16), gfx950: bound by the weights' bytes, n k / 2 from HBM once, as
 // long as the instructions that fetch them are few: a CU takes about 24 cycles for a vector load whatever it brings,
 // and a first version that asked for x and scales beside every KiB of codes ran at half the memory's rate.
 //
-// A workgroup owns 16 NB output columns and all rows (MT tiles of 16); its waves split k, wave w taking the
-// 128-column blocks w, w + WAVES, ...  A block's codes, scales and zero points go from memory into registers DEPTH
-// blocks ahead.  x is the small operand: for up to 4 rows (XLDS) it is copied into LDS once (chunk by chunk
+// A workgroup owns 16 NB output columns and all rows; its waves split k, wave w taking the 128-column blocks w, w + WAVES,
+// ...  A block's codes, scales and zero points go from memory into registers DEPTH
+// blocks ahead.  x is the small operand: for up to 3 rows (XLDS) it is copied into LDS once (chunk by chunk
 // where it is long), and the lanes of the rows behind m read row 0; above that its fragments come out of the L2, once
 // for the NB column blocks of a wave.
 //
 // Weights stay integers here (u, exact in x's type) and the scale is applied to a group's sum in binary32:
 //   y += s * (sum x u - z sum x)
 // with sum(x) from one more matrix instruction, whose other operand is ones.  This takes 28 operations to unpack
-// 32 codes and 8 (a row tile) to add a group, where rounding scaled weights takes 76: at one row of 14336 x
-// 14336 22.3 us against 26.8, at 16 rows of 10752 x 5376 the same way.  x is the first operand of the matrix
+// 32 codes and 8 to add a group, where rounding scaled weights takes 76: at one row of 14336 x 14336 22.3 us against
+// 26.8, at 16 rows of 10752 x 5376 the same way.  x is the first operand of the matrix
 // instruction, so that a lane's sums belong to one output column, whose scale it holds.
 #pragma once
 
@@ -47,16 +47,15 @@ __device__ __forceinline__ v4u integers(uint32_t w) {
                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(odd, 512.0f, true))};
 }
 
-constexpr int kFewRows = 4;
+constexpr int kFewRows = 3;
 // LDS for x of few rows: three workgroups of eight waves on a CU.  Rows are 64 bytes out of step with the banks.
 constexpr int kFewBytes = 44 * 1024;
 constexpr int few_blocks(int64_t m) { return (int)((kFewBytes / m - 64) / 256); }
 
 // GPB: groups of a 128-column block (1: the group is a multiple of 128).
-template <bool F16, bool ZEROS, int GPB, int MT, int NB, int WAVES, int DEPTH, bool XLDS>
+template <bool F16, bool ZEROS, int GPB, int NB, int WAVES, int DEPTH, bool XLDS>
 __global__ __launch_bounds__(WAVES * 64) void w4_stream_kernel(W4Args p) {
-    static_assert(!XLDS || MT == 1, "few rows");
-    __shared__ __attribute__((aligned(16))) v4f red[WAVES * NB * MT * 64];
+    __shared__ __attribute__((aligned(16))) v4f red[WAVES * NB * 64];
     extern __shared__ __attribute__((aligned(16))) uint8_t x_raw[];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -70,12 +69,9 @@ __global__ __launch_bounds__(WAVES * 64) void w4_stream_kernel(W4Args p) {
         w4_rsrc(p.zeros + (ZEROS ? blk0 * quads * 64 : 0), ZEROS ? (int64_t)nblk * quads * 64 : 0);
     const __amdgpu_buffer_rsrc_t rx = w4_rsrc(p.x, ((p.m - 1) * p.ldx + p.k) * 2);
 
-    uint32_t xoff[MT];
-#pragma unroll
-    for (int t = 0; t < MT; ++t)
-        xoff[t] = 16 * t + r16 < p.m ? (uint32_t)((16 * t + r16) * p.ldx * 2 + 16 * kq) : kW4Oob;
+    const uint32_t xoff = r16 < p.m ? (uint32_t)(r16 * p.ldx * 2 + 16 * kq) : kW4Oob;
 
-    v4u codes[DEPTH][NB], x[XLDS ? 1 : DEPTH][MT][4];
+    v4u codes[DEPTH][NB], x[XLDS ? 1 : DEPTH][4];
     v2u scales[DEPTH][NB];
     uint32_t zeros[DEPTH][NB];
     auto load = [&](int i, int b) __attribute__((always_inline)) {
@@ -90,53 +86,37 @@ __global__ __launch_bounds__(WAVES * 64) void w4_stream_kernel(W4Args p) {
         }
         if constexpr (!XLDS) {
 #pragma unroll
-            for (int t = 0; t < MT; ++t)
-#pragma unroll
-                for (int s = 0; s < 4; ++s) {
-                    const bool inside = xoff[t] != kW4Oob && 128 * b + 32 * s + 8 * kq < p.k;
-                    x[i][t][s] = __builtin_amdgcn_raw_buffer_load_b128(
-                        rx, inside ? xoff[t] + (uint32_t)(256 * b + 64 * s) : kW4Oob, 0, 0);
-                }
+            for (int s = 0; s < 4; ++s) {
+                const bool inside = xoff != kW4Oob && 128 * b + 32 * s + 8 * kq < p.k;
+                x[i][s] = __builtin_amdgcn_raw_buffer_load_b128(rx, inside ? xoff + (uint32_t)(256 * b + 64 * s) : kW4Oob,
+                                                                0, 0);
+            }
         }
         __builtin_amdgcn_sched_barrier(0);  // blocks in order: a wait for one waits for none behind it
     };
-    v4f acc[NB][MT];
+    v4f acc[NB];
 #pragma unroll
-    for (int j = 0; j < NB; ++j)
-#pragma unroll
-        for (int t = 0; t < MT; ++t) acc[j][t] = v4f{};
+    for (int j = 0; j < NB; ++j) acc[j] = v4f{};
     constexpr uint32_t one = F16 ? 0x3C003C00u : 0x3F803F80u;
     const v4u ones = {one, one, one, one};
-    auto multiply = [&](int i, int b, const v4u (&xf)[MT][4]) __attribute__((always_inline)) {
+    auto multiply = [&](int i, int b, const v4u (&xf)[4]) __attribute__((always_inline)) {
         constexpr int SPG = 4 / GPB;  // matrix steps of a group
 #pragma unroll
         for (int q = 0; q < GPB; ++q) {
             const int g = w4_group(p, b, q * SPG);
-            v4f sum[MT];
+            v4f sum = {};
 #pragma unroll
-            for (int t = 0; t < MT; ++t) {
-                sum[t] = v4f{};
-#pragma unroll
-                for (int s = q * SPG; s < (q + 1) * SPG; ++s) sum[t] = mfma16<F16>(xf[t][s], ones, sum[t]);
-            }
+            for (int s = q * SPG; s < (q + 1) * SPG; ++s) sum = mfma16<F16>(xf[s], ones, sum);
 #pragma unroll
             for (int j = 0; j < NB; ++j) {
-                v4f part[MT];
+                v4f part = {};
 #pragma unroll
-                for (int t = 0; t < MT; ++t) part[t] = v4f{};
-#pragma unroll
-                for (int s = q * SPG; s < (q + 1) * SPG; ++s) {
-                    const v4u w = integers<F16>(codes[i][j][s]);
-#pragma unroll
-                    for (int t = 0; t < MT; ++t) part[t] = mfma16<F16>(xf[t][s], w, part[t]);
-                }
+                for (int s = q * SPG; s < (q + 1) * SPG; ++s) part = mfma16<F16>(xf[s], integers<F16>(codes[i][j][s]), part);
                 float scale, shift;
                 w4_scale<ZEROS>(scales[i][j], zeros[i][j], g, p.scales_f16, scale, shift);
 #pragma unroll
-                for (int t = 0; t < MT; ++t)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        acc[j][t][e] = __builtin_fmaf(scale, __builtin_fmaf(shift, sum[t][e], part[t][e]), acc[j][t][e]);
+                for (int e = 0; e < 4; ++e)
+                    acc[j][e] = __builtin_fmaf(scale, __builtin_fmaf(shift, sum[e], part[e]), acc[j][e]);
             }
         }
     };
@@ -170,9 +150,9 @@ __global__ __launch_bounds__(WAVES * 64) void w4_stream_kernel(W4Args p) {
                 if (i + d >= count) break;
                 const int b = first + (i + d) * WAVES;
                 if constexpr (XLDS) {
-                    v4u xf[MT][4];
+                    v4u xf[4];
 #pragma unroll
-                    for (int s = 0; s < 4; ++s) xf[0][s] = *(const H3Q_LDS v4u*)(xr + (b - c0) * 256 + 64 * s);
+                    for (int s = 0; s < 4; ++s) xf[s] = *(const H3Q_LDS v4u*)(xr + (b - c0) * 256 + 64 * s);
                     multiply(d, b, xf);
                 } else {
                     multiply(d, b, x[d]);
@@ -184,28 +164,21 @@ __global__ __launch_bounds__(WAVES * 64) void w4_stream_kernel(W4Args p) {
     }
 
 #pragma unroll
-    for (int j = 0; j < NB; ++j)
-#pragma unroll
-        for (int t = 0; t < MT; ++t) red[((wave * NB + j) * MT + t) * 64 + lane] = acc[j][t];
+    for (int j = 0; j < NB; ++j) red[(wave * NB + j) * 64 + lane] = acc[j];
     __syncthreads();
+    if (wave >= NB) return;
+    v4f sum = red[wave * 64 + lane];
 #pragma unroll
-    for (int j = 0; j < NB; ++j)
+    for (int w = 1; w < WAVES; ++w) sum += red[(w * NB + wave) * 64 + lane];
+    const int64_t n = 16 * (blk0 + wave) + r16;
+    if (n >= p.n) return;
+    const float bias = p.bias ? out_lo(p.bias[n], F16) : 0.0f;
 #pragma unroll
-        for (int t = 0; t < MT; ++t) {
-            if ((j * MT + t) % WAVES != wave) continue;
-            v4f s = red[(j * MT + t) * 64 + lane];
-#pragma unroll
-            for (int w = 1; w < WAVES; ++w) s += red[((w * NB + j) * MT + t) * 64 + lane];
-            const int64_t n = 16 * (blk0 + j) + r16, m0 = 16 * t + 4 * kq;
-            if (n >= p.n) continue;
-            const float bias = p.bias ? out_lo(p.bias[n], F16) : 0.0f;
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (m0 + e < p.m) p.out[(m0 + e) * p.ldo + n] = (uint16_t)pack_out2(s[e] + bias, 0.0f, F16);
-        }
+    for (int e = 0; e < 4; ++e)
+        if (4 * kq + e < p.m) p.out[(4 * kq + e) * p.ldo + n] = (uint16_t)pack_out2(sum[e] + bias, 0.0f, F16);
 }
 
-template <bool F16, bool ZEROS, int GPB, int MT, int NB, int WAVES, int DEPTH, bool XLDS>
+template <bool F16, bool ZEROS, int GPB, int NB, int WAVES, int DEPTH, bool XLDS>
 hipError_t launch_cfg(const W4Args& a, hipStream_t st) {
     const unsigned grid = (unsigned)(((a.n + 15) / 16 + NB - 1) / NB);
     size_t lds = 0;
@@ -213,7 +186,7 @@ hipError_t launch_cfg(const W4Args& a, hipStream_t st) {
         const int64_t steps = (a.k + 127) / 128, held = few_blocks(a.m);
         lds = (size_t)(a.m * ((steps < held ? steps : held) * 256 + 64));
     }
-    hipLaunchKernelGGL((w4_stream_kernel<F16, ZEROS, GPB, MT, NB, WAVES, DEPTH, XLDS>), dim3(grid), dim3(WAVES * 64), lds,
+    hipLaunchKernelGGL((w4_stream_kernel<F16, ZEROS, GPB, NB, WAVES, DEPTH, XLDS>), dim3(grid), dim3(WAVES * 64), lds,
                        st, a);
     return hipGetLastError();
 }
@@ -222,24 +195,19 @@ hipError_t launch_cfg(const W4Args& a, hipStream_t st) {
 // all of x (measured at 13 rows of 7003 x 4096, 438 blocks: 7.9 us with two, 10.4 with one, 10.9 with four; at 16
 // rows of 10752 x 5376, 672 blocks: 11.1 us with four, 15.3 with two).  With x in LDS there is less to
 // bring: one block, two from three workgroups a CU on (14336 x 14336: 21.1 us against 23.6), and sixteen waves where there
-// are fewer workgroups than CUs (1024 x 14336: 8.0 us against 9.7).  32-column groups of two row tiles stay at two:
-// four do not fit the registers.
+// are fewer workgroups than CUs (1024 x 14336: 8.0 us against 9.7).  x goes there for up to 3 rows: 3 rows of 5376 x
+// 7168 8.6 us against 8.9, of 10752 x 5376 at groups of 32 11.1 against 11.6; 4 rows 9.9 against 9.1, and 11.3 against 11.6.
 template <bool F16, bool ZEROS, int GPB>
 hipError_t launch_w4_stream_rows(const W4Args& a, hipStream_t st) {
     const int64_t blocks = (a.n + 15) / 16;
     if (a.m <= kFewRows) {
-        if (blocks <= 256) return launch_cfg<F16, ZEROS, GPB, 1, 1, 16, 2, true>(a, st);
-        if (blocks < 768) return launch_cfg<F16, ZEROS, GPB, 1, 1, 8, 2, true>(a, st);
-        return launch_cfg<F16, ZEROS, GPB, 1, 2, 8, 2, true>(a, st);
+        if (blocks <= 256) return launch_cfg<F16, ZEROS, GPB, 1, 16, 2, true>(a, st);
+        if (blocks < 768) return launch_cfg<F16, ZEROS, GPB, 1, 8, 2, true>(a, st);
+        return launch_cfg<F16, ZEROS, GPB, 2, 8, 2, true>(a, st);
     }
-    if (a.m <= 16) {
-        if (blocks <= 256) return launch_cfg<F16, ZEROS, GPB, 1, 1, 8, 2, false>(a, st);
-        if (blocks <= 512) return launch_cfg<F16, ZEROS, GPB, 1, 2, 8, 1, false>(a, st);
-        return launch_cfg<F16, ZEROS, GPB, 1, 4, 8, 1, false>(a, st);
-    }
-    if (blocks <= 256) return launch_cfg<F16, ZEROS, GPB, 2, 1, 8, 2, false>(a, st);
-    if (blocks <= 512 || GPB == 4) return launch_cfg<F16, ZEROS, GPB, 2, 2, 8, 1, false>(a, st);
-    return launch_cfg<F16, ZEROS, GPB, 2, GPB == 4 ? 2 : 4, 8, 1, false>(a, st);
+    if (blocks <= 256) return launch_cfg<F16, ZEROS, GPB, 1, 8, 2, false>(a, st);
+    if (blocks <= 512) return launch_cfg<F16, ZEROS, GPB, 2, 8, 1, false>(a, st);
+    return launch_cfg<F16, ZEROS, GPB, 4, 8, 1, false>(a, st);
 }
 
 template <bool F16, bool ZEROS>

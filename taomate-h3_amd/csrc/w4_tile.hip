@@ -180,7 +180,7 @@ struct Plan {
 //
 // Or w4_slab.hip, whose waves split k inside a workgroup, when it is estimated to take less.  The estimate, in
 // 1/20 of 0.87 us, is a line through 48 shapes (40 to 600 rows, 1024 to 14336 columns, k 4096 to 16384): a workgroup
-// of it takes 20 (1 + NT) for eight blocks, a tile 22 or 15 (64 rows) a block, each once for 256 workgroups, beside
+// of it takes 20 (1 + NT) for eight blocks (13 up to 32 rows), a tile 22 or 15 (64 rows) a block, each once for 256 workgroups, beside
 // 80 there, and 60 or, with sums in memory and their launch, 240 here.  Measured, us, slab and tile, the chosen one
 // first: 64 rows of 1024 x 4096 8.2 and 10.6, 40 of 5376 x 7168 14.1 and 16.7, 200 of 4096 x 4096 14.0 and 20.2, 200 of
 // 5376 x 7168 26.5 and 29.5; tile and slab: 64 of 2048 x 16384 19.3 and 32.5, 384 of 5376 x 7168 39 and 46, 600 of it
@@ -207,7 +207,7 @@ Plan plan_tiles(int64_t m, int64_t n, int64_t k) {
         int64_t best = (p.splits > 1 ? 240 : 60) + rounds(count * p.splits) * p.per_split * (p.mt == 4 ? 22 : 15);
         for (int nt = 1; nt <= 3; ++nt) {
             const int64_t workgroups = (m + 63) / 64 * ((n + 32 * nt - 1) / (32 * nt));
-            const int64_t cost = 80 + rounds(workgroups) * ((p.steps + 7) / 8) * 20 * (1 + nt);
+            const int64_t cost = 80 + rounds(workgroups) * ((p.steps + 7) / 8) * (m <= 32 ? 13 : 20) * (1 + nt);
             if (cost < best) best = cost, p.slab = nt;
         }
     }

@@ -1221,10 +1221,11 @@ def _check_w4(name: str, w: W4Weight) -> None:
 def w4_mm(x: torch.Tensor, weight: W4Weight, *, bias: torch.Tensor | None = None,
           out: torch.Tensor | None = None) -> torch.Tensor:
     """x @ w^T [+ bias] of 4-bit weights (pack_w4), ``x [m, k]`` bf16 or fp16 -> [m, n] in x's dtype:
-    out[m, n] = sum_k x[m, k] * s (u - z), binary32 sums rounded once.  Above 32 rows the weights s (u - z) are rounded
+    out[m, n] = sum_k x[m, k] * s (u - z), binary32 sums rounded once.  Above 16 rows the weights s (u - z) are rounded
     to x's dtype first.
 
-    x has 16-byte aligned rows (a row stride that is a multiple of 8); ``bias [n]`` and ``out`` are of its dtype."""
+    x has 16-byte aligned rows (a row stride that is a multiple of 8); ``bias [n]`` and ``out``, which holds no element of x,
+    are of its dtype."""
     got = _native_call("w4_mm", x, weight.codes, weight.scales, weight.zeros, weight.n, weight.k, weight.group, bias, out)
     if got is not None:
         return got

@@ -25,18 +25,18 @@ def dequantized(codes, scales, zeros, group: int) -> tuple[torch.Tensor, torch.T
 def product(x, codes, scales, zeros, group: int, bias=None) -> tuple[torch.Tensor, torch.Tensor]:
     """(value, bound of its binary32 error), float64 [m, n].
 
-    Above 32 rows the weights s (u - z) are rounded once to x's type; binary32 holds them before that (11 + 5
+    Above 16 rows the weights s (u - z) are rounded once to x's type; binary32 holds them before that (11 + 5
     bits), so the rounding is a definite one.  A matrix instruction takes 16 or 32 products: its own sum has at most
     32 roundings (of 2^-23: it may cut off) of its terms, and one follows onto a sum of at most sum |x w|, k / 16
     times; the parts of a split k and a workgroup's waves add at most 16 more: (k / 16 + 48) 2^-23 sum |x w|.
 
-    Up to 32 rows a group (at most 128 columns of it at a time) is summed as x u, at most 15 |x| a term, with 32 + 4
+    Up to 16 rows a group (at most 128 columns of it at a time) is summed as x u, at most 15 |x| a term, with 32 + 4
     roundings as above, and z times the sum of x, as large, with as many, is taken off in one; the scale and the
     sum over the groups are one more rounding each of at most 30 |s x|: (56 + k / min(group, 128)) 2^-23 * 30
     sum |s x|."""
     w, s = dequantized(codes, scales, zeros, group)
     a = x.cpu().double()
-    if len(x) > 32:
+    if len(x) > 16:
         w = w.to(x.dtype).double()
         bound = (a.shape[1] / 16 + 48) * 2.0 ** -23 * (a.abs() @ w.abs().T)
     else:

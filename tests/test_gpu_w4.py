@@ -67,7 +67,8 @@ def test_w4_mm_sizes(ops, device, m, n, k, group):
 @pytest.mark.parametrize("dtype", list(TYPES))
 @pytest.mark.parametrize("m,n,k,group", [(40, 8300, 1040, 32), (64, 9217, 144, 128), (70, 8300, 528, 128),
                                          (130, 12300, 400, 64), (33, 16500, 1040, 256), (129, 2070, 2320, 32),
-                                         (600, 4096, 4096, 128)])
+                                         (600, 4096, 4096, 128), (17, 5000, 1040, 128), (18, 9000, 1040, 64),
+                                         (32, 16500, 1040, 32), (25, 300, 9008, 128)])
 def test_w4_mm_dozens_of_rows(ops, device, m, n, k, group, dtype, zeros):
     """Where a workgroup's waves split k: one to three column tiles of 32, ragged in rows, columns and k."""
     kind = TYPES[dtype]
