@@ -12,8 +12,8 @@
 //
 // Layout.  Codes lie in blocks of 16 rows x 128 columns, 1 KiB, [row blocks][column blocks]: lane L's 16 bytes
 // are four words, word s the eight codes k = 128 b + 32 s + 8 (L / 16) .. + 7 of row L % 16, the low nibbles of
-// its bytes k0 .. k3 and the high ones k4 .. k7: the operand of one v_mfma_f32_16x16x32, and with the lanes' 16 bytes taken as row L % 32
-// and k quarter L / 32 (+ 2) of two blocks, of two v_mfma_f32_32x32x16.  Scales (bf16 or binary16) and zero
+// its bytes k0 .. k3 and the high ones k4 .. k7: the operand of one v_mfma_f32_16x16x32, and with the lanes' 16 bytes
+// taken as row L % 32 and k quarter L / 32 (+ 2) of two blocks, of two v_mfma_f32_32x32x16.  Scales (bf16 or binary16) and zero
 // points (bytes) lie as [row blocks][groups / 4][16][4]: a lane's row has four groups in one load.
 //
 // Unpacking.  A byte 0 .. 15 is the e4m3 number of 2^-9 times its value (subnormals up to 7, then the first

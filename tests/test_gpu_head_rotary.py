@@ -248,6 +248,18 @@ def test_plan_append(ops, device, seqs, page, pad, seed):
     assert torch.equal(got.positions.cpu().long(), want[0]) and torch.equal(got.slots.cpu().long(), want[1])
 
 
+@pytest.mark.parametrize("seqs", [255, 256, 1023, 1024, 1025, 3000])
+def test_plan_append_of_many_sequences(ops, device, seqs):
+    new = torch.randint(0, 3, (seqs,), generator=_gen(seqs))
+    lengths = torch.randint(0, 60, (seqs,), generator=_gen(1)).int()
+    cu = torch.cat((torch.tensor([2]), 2 + new.cumsum(0))).int()  # two tokens of no sequence before them
+    tokens = int(cu[-1]) + 5
+    table = torch.randperm(8 * seqs, generator=_gen(2)).int().view(seqs, 8)
+    got = ops.plan_append(table.to(device), lengths.to(device), cu.to(device), tokens, 8)
+    want = plan(table, lengths, cu, tokens, 8)
+    assert torch.equal(got.positions.cpu().long(), want[0]) and torch.equal(got.slots.cpu().long(), want[1])
+
+
 def test_plan_append_edges(ops, device):
     i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=device)
     # slots of 2^31 and more, negative lengths, a first token that is padding
