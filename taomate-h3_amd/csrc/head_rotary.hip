@@ -135,10 +135,11 @@ __global__ __launch_bounds__(256) void head_rotary_kernel(HeadArgs p) {
     // A lane's two vectors are as far apart as its region (the rotated channels, or those behind them) has chunks, so
     // that every access of a wave is whole runs.
     int off[NC][2];
+    bool turns[NC];  // of the chunk that is loaded: past the row's end the last one again, values and angles
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
         const int chunk = g + c * 64 < chunks ? g + c * 64 : chunks - 1;
-        const bool turn = chunk < turned;
+        const bool turn = turns[c] = chunk < turned;
         off[c][0] = turn ? chunk * V : (turned + chunk) * V;
         off[c][1] = off[c][0] + (turn ? turned : chunks - turned) * V;
         if (INTER && V == 1 && turn) {
@@ -259,7 +260,7 @@ __global__ __launch_bounds__(256) void head_rotary_kernel(HeadArgs p) {
         if (turned > 0) {
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
-                const bool turn = g + c * 64 < turned;
+                const bool turn = turns[c];
 #pragma unroll
                 for (int e = 0; e < V; ++e) {
                     // interleaved: the pairs (2 e, 2 e + 1) of one vector, then of the other
@@ -300,7 +301,7 @@ __global__ __launch_bounds__(256) void head_rotary_kernel(HeadArgs p) {
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
                     for (int e = 0; e < V; ++e)
-                        m = mag_max(m, __builtin_fabsf(y[c][i][e]));  // lanes past the row repeat its last channels
+                        m = mag_max(m, __builtin_fabsf(y[c][i][e]));  // lanes past the row have its last chunk's
             m = row_fold(m, p.lanes, [](float a, float b) { return mag_max(a, b); });
             scale = amax_scale(m, kE4M3Recip);
             if (g == 0 && head < s.heads) s.cache.scale[scale_to + head * s.cache.scale_head_stride] = scale;

@@ -541,3 +541,59 @@ def test_python_bodies_equal_native(ops, device, monkeypatch):
     assert set(taken) == {"plan_append", "append_kv", "rotary", "qk_norm_rotary", "rotary_tables"}
     for name in _OUT:
         assert torch.equal(s[name].float(), other[name].float()), name
+
+
+# ------------------------------------- e4m3 pages: scales of rows, quotients
+
+def _at(start, tokens, heads, d, dtype, device, seed):
+    """[tokens, heads, d] whose first element lies ``start`` elements behind an aligned one."""
+    wide = torch.empty(tokens * heads * d + start, device=device, dtype=dtype)
+    rows = wide[start:].view(tokens, heads, d)
+    return rows.copy_(torch.randn(tokens, heads, d, generator=_gen(seed)).to(dtype))
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("start", [0, 1])
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("d,rot", [(80, 80), (96, 96), (192, 192), (10, 10), (36, 36), (510, 510), (128, 128), (192, 64)])
+def test_append_kv_row_scales(ops, device, d, rot, dtype, start, interleaved):
+    """Scales and codes of rows whose largest channel is one of the last pair's (or of a further pair), at an angle that
+    makes it smaller; norms with a weight for each head.  Also the same keys in pages of their own type and with static
+    scales, and the queries beside them."""
+    tokens, hq, hk, page = 37, 3, 5, 8
+    kind, half = TYPES[dtype], rot // 2
+    q, k, v = (_at(start, tokens, h, d, kind, device, seed) for h, seed in ((hq, 1), (hk, 2), (hk, 3)))
+    angle = torch.rand(50, half, generator=_gen(4), dtype=torch.float64) * 6.3
+    rows = torch.randint(0, 50, (tokens,), generator=_gen(5))
+    for t in range(tokens):
+        pair = half - 1 if t % 3 else int(torch.randint(0, half, (1,), generator=_gen(t)))
+        big, small = (2 * pair, 2 * pair + 1) if interleaved else (pair, half + pair)
+        k[t, :, small], k[t, :, big] = 0.0, 30.0 if t % 2 else -30.0
+        angle[rows[t], pair] = 0.7853981633974483  # the pair becomes (21, 21)
+    cos, sin = angle.cos().float().to(device), angle.sin().float().to(device)
+    weights = [(1.0 + 0.3 * torch.randn(h, d, generator=_gen(6))).to(kind).to(device) for h in (hq, hk)]
+    pages = tokens // page + 2
+    slots = torch.randperm(pages * page, generator=_gen(7))[:tokens]
+    where = (slots // page).to(device), (slots % page).to(device)
+    wanted = [norm_rotate(k, weights[1], cos, sin, rows, eps=1e-5, interleaved=interleaved), norm_rotate(v)]
+    for form in ("by_row", "static", "rows"):
+        caches = [_cache(pages, page, hk, d, kind if form == "rows" else torch.float8_e4m3fn, "nhd", device, s) for s in (8, 9)]
+        scales = [None, None]
+        if form == "static":
+            scales = [torch.rand(hk, generator=_gen(10)).add(0.2).mul(0.05).to(device) for _ in range(2)]
+        elif form == "by_row":
+            scales = [torch.zeros(pages, page, hk, device=device) for _ in range(2)]
+        got = ops.append_kv(k, v, *caches, slots.int().to(device), k_scale=scales[0], v_scale=scales[1], k_weight=weights[1],
+                            eps=1e-5, cos=cos, sin=sin, positions=rows.to(device), interleaved=interleaved, q=q,
+                            q_weight=weights[0])
+        want, size = norm_rotate(q, weights[0], cos, sin, rows, eps=1e-5, interleaved=interleaved)
+        assert_close(got, want, size, d, "q")
+        for i, (want, size) in enumerate(wanted):
+            if form == "rows":
+                assert_close(caches[i][where], want, size, d, "kv"[i])
+                continue
+            by = scales[i][where] if form == "by_row" else scales[i].expand(tokens, hk)
+            if form == "by_row":  # the product with RN(1 / 448): two roundings and the row's bound
+                bound = ((32 + d / 8) * 2.0 ** -24) * size.amax(2) / 448.0 + 2e-24
+                assert ((by.cpu().double() - want.abs().amax(2) / 448.0).abs() <= bound).all(), "kv"[i]
+            assert_codes(caches[i][where], by.cpu()[:, :, None], want, size, d, "kv"[i])
