@@ -493,7 +493,7 @@ int h3q_plan_append(const int32_t* table, int64_t table_stride, int64_t seqs, in
 /*
  * One layer's append: k (norm and rotation as above, each if asked for) and v (as it is) of token t into slot
  * slots[t] of k_pages and v_pages, and q (may be NULL) normed and rotated into its out.  e4m3fn pages
- * hold e4m3(clamp(y * RN(1 / s), +-448)), s of the head, or max(max|y| * RN(1/448), 1e-12) of the
+ * hold e4m3(clamp(RN(y / s), +-448)), s of the head, or max(max|y| * RN(1/448), 1e-12) of the
  * row, which goes into the scale pages; NaN and infinities as in h3q_quant_rows.  Slots outside
  * [0, n_pages * page_size), the same for both, are not stored; padding (position below 0) stores neither k, v nor q.
  * Slots of one call that are stored are distinct, and k and v pages share no memory.  rotation NULL: no

@@ -3,7 +3,7 @@
 //
 //   n  = x * (1 / sqrt(sum(x * x) / d + eps)) * weight            (rows with a norm)
 //   (a, b) -> (a cos - b sin, a sin + b cos)                      (the first 2 * half channels, pair by pair)
-//   q  = e4m3(clamp(y * (1 / s), +-448)), s a head's own or max(max|y| / 448, 1e-12) of the row   (e4m3 pages)
+//   q  = e4m3(clamp(RN(y / s), +-448)), s a head's own or max(max|y| / 448, 1e-12) of the row   (e4m3 pages)
 //
 // All of it in binary32 on the values as they are, rounded once where the row is stored.
 //
@@ -312,9 +312,20 @@ __global__ __launch_bounds__(256) void head_rotary_kernel(HeadArgs p) {
         for (int c = 0; c < NC; ++c)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
+                // The quotient from r and one residual; where that leaves no finite value (s or r is 0, infinite or
+                // NaN, or y is), IEEE division.
                 float q[V];
+                bool odd = false;
 #pragma unroll
-                for (int e = 0; e < V; ++e) q[e] = clamp_e4m3(y[c][i][e] * r);
+                for (int e = 0; e < V; ++e) {
+                    const float v = div_rn_signed(y[c][i][e], scale, r);
+                    odd |= !(__builtin_fabsf(v) < __builtin_inff());
+                    q[e] = clamp_e4m3(v);
+                }
+                if (odd) {
+#pragma unroll
+                    for (int e = 0; e < V; ++e) q[e] = clamp_e4m3(y[c][i][e] / scale);
+                }
                 if (head < s.heads && g + c * 64 < chunks) store_codes<V>(row + off[c][i], q);
             }
     }

@@ -597,3 +597,58 @@ def test_append_kv_row_scales(ops, device, d, rot, dtype, start, interleaved):
                 bound = ((32 + d / 8) * 2.0 ** -24) * size.amax(2) / 448.0 + 2e-24
                 assert ((by.cpu().double() - want.abs().amax(2) / 448.0).abs() <= bound).all(), "kv"[i]
             assert_codes(caches[i][where], by.cpu()[:, :, None], want, size, d, "kv"[i])
+
+
+@pytest.mark.parametrize("by_row", [False, True])
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_append_kv_codes_are_of_the_quotient(ops, device, dtype, by_row):
+    """Codes are e4m3(clamp(RN(y / s))), as the other quantizers', bit for bit: rows without norm and rotation, many of
+    their quotients halfway between two codes, where the product with RN(1 / s) is on either side."""
+    kind, tokens, heads, d = TYPES[dtype], 64, 8, 128
+    gen = _gen(11)
+    odd = 2 * torch.randint(1, 16, (tokens if by_row else 1, heads, 1), generator=gen) + 1
+    s = odd.float() * 2.0 ** -6
+    # halfway between two codes: 17, 19 .. 31 sixteenths, times 2^0 .. 2^3, and (of few bits) 1, 3, 5, 7 times 2^-10;
+    # a row's first channel is 448 s
+    y = (2 * torch.randint(8, 16, (tokens, heads, d), generator=gen) + 1) / 16.0
+    y = y * torch.exp2(torch.randint(0, 4, (tokens, heads, d), generator=gen).float())
+    y[:, :, ::2] = (2 * torch.randint(0, 4, (tokens, heads, d // 2), generator=gen) + 1) * 2.0 ** -10
+    y = y * s
+    y = y * torch.where(torch.rand(tokens, heads, d, generator=gen) < 0.5, -1.0, 1.0)
+    y[:, :, ::7] = 30.0 * torch.randn(y[:, :, ::7].shape, generator=gen) * s
+    y[:, :, 1] = -0.0
+    y[:, :, 0] = 448.0 * s[:, :, 0]
+    rows = y.to(kind)
+    value = rows.float()
+    if by_row:
+        s = (value.abs().amax(2, keepdim=True) * torch.tensor(1.0 / 448.0)).clamp(min=1e-12)
+    quotient = (value / s).clamp(-448.0, 448.0).to(torch.float8_e4m3fn)
+    product = (value * (1.0 / s)).clamp(-448.0, 448.0).to(torch.float8_e4m3fn)
+    assert (quotient.view(torch.uint8) != product.view(torch.uint8)).any()  # the inputs tell them apart
+    caches = [torch.zeros(tokens // 16, 16, heads, d, device=device, dtype=torch.float8_e4m3fn) for _ in range(2)]
+    scales = [torch.zeros(tokens // 16, 16, heads, device=device) if by_row else s.view(heads).to(device) for _ in range(2)]
+    slots = torch.arange(tokens, dtype=torch.int32, device=device)
+    x = rows.to(device)
+    ops.append_kv(x, x, *caches, slots, k_scale=scales[0], v_scale=scales[1])
+    for cache, scale in zip(caches, scales):
+        if by_row:
+            assert torch.equal(scale.view(tokens, heads, 1).cpu(), s)
+        assert torch.equal(cache.view(tokens, heads, d).cpu().view(torch.uint8), quotient.view(torch.uint8))
+
+
+def test_append_kv_static_scales_out_of_the_ordinary(ops, device):
+    """Scales that have no binary32 reciprocal, 0, infinity and NaN: clamp(y / s) of IEEE division, NaN where that is."""
+    s = torch.tensor([2.0 ** -140, 2.0 ** -149, 0.0, float("inf"), float("nan"), 2.0 ** 127, 1.0], dtype=torch.float32)
+    heads, d = len(s), 16
+    row = torch.tensor([0.0, -0.0, 1.0, -2.0, 2.0 ** -139, -(2.0 ** -140), 2.0 ** -133, 3e38, -1e38, float("inf"), -float("inf"),
+                        float("nan"), 2.0 ** -149, 448.0, -449.0, 1e-12])
+    x = row.expand(2, heads, d)
+    want = (x / s[:, None]).clamp(-448.0, 448.0)
+    caches = [torch.zeros(1, 2, heads, d, device=device, dtype=torch.float8_e4m3fn) for _ in range(2)]
+    x, by = x.to(device), s.to(device)
+    ops.append_kv(x, x, *caches, torch.arange(2, dtype=torch.int32, device=device), k_scale=by, v_scale=by)
+    for cache in caches:
+        got = cache[0].float().cpu()
+        want_codes = want.to(torch.float8_e4m3fn).float()
+        assert torch.equal(torch.isnan(got), torch.isnan(want))
+        assert torch.equal(got.nan_to_num(7.0), want_codes.nan_to_num(7.0))
