@@ -524,7 +524,8 @@ int h3q_w4_pack(const void* codes, int64_t ldc, const void* scales, int64_t lds,
  * The quantizer of weights [n, k] (dtype: H3Q_DTYPE_*; scales binary16 for binary16 weights, else
  * bf16) into contiguous rows: s = max|w| / 7 and u = clamp(rne(w / s), -8, 7) + 8, or with zeros (not
  * NULL) s = (max(w, 0) - min(w, 0)) / 15, z = clamp(rne(-min / s), 0, 15) and u = clamp(rne(w / s) + z, 0, 15).
- * s is rounded to its type before it is used; a group of zeros has s = 0.
+ * s is rounded to its type before it is used; a group of zeros has s = 0.  A group with a NaN has s = NaN, one
+ * with an infinity an s that is not finite: its products are NaN or infinite.
  */
 int h3q_w4_quantize(const void* w, int dtype, int64_t ldw, int64_t n, int64_t k, int64_t group, void* codes,
                     void* scales, void* zeros, void* stream);

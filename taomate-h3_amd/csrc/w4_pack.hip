@@ -37,7 +37,8 @@ __device__ __forceinline__ float weight_at(const W4QuantArgs& p, int64_t i) {
     return out_lo(((const uint16_t*)p.w)[i], p.dtype == kInF16);
 }
 
-// Sixteen lanes a group.  s is rounded to its 16-bit type before the codes are made with it.
+// Sixteen lanes a group.  s is rounded to its 16-bit type before the codes are made with it.  A NaN among a group's
+// weights makes s a NaN (an infinity makes it one that is not finite by itself), so that no product hides it.
 __global__ __launch_bounds__(256) void w4_quant_kernel(W4QuantArgs p, int groups) {
     const int64_t team = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
     const int l = threadIdx.x & 15;
@@ -46,8 +47,10 @@ __global__ __launch_bounds__(256) void w4_quant_kernel(W4QuantArgs p, int groups
     const int g = (int)(team - row * groups);
     const int64_t k0 = (int64_t)g * p.group, k1 = k0 + p.group < p.k ? k0 + p.group : p.k;
     float low = 0.0f, high = 0.0f;
+    int nan = 0;
     for (int64_t k = k0 + l; k < k1; k += 16) {
         const float v = weight_at(p, row * p.ldw + k);
+        nan |= v != v;
         low = v < low ? v : low;
         high = v > high ? v : high;
     }
@@ -55,8 +58,9 @@ __global__ __launch_bounds__(256) void w4_quant_kernel(W4QuantArgs p, int groups
         const float a = __shfl_xor(low, off, 16), b = __shfl_xor(high, off, 16);
         low = a < low ? a : low;
         high = b > high ? b : high;
+        nan |= __shfl_xor(nan, off, 16);
     }
-    const float reach = p.zeros ? (high - low) / 15.0f : (high > -low ? high : -low) / 7.0f;
+    const float reach = nan ? __builtin_nanf("") : p.zeros ? (high - low) / 15.0f : (high > -low ? high : -low) / 7.0f;
     const bool f16 = p.dtype == kInF16;
     const uint16_t bits = (uint16_t)pack_out2(reach, 0.0f, f16);
     const float s = out_lo(bits, f16);

@@ -1163,7 +1163,8 @@ def quantize_w4(w: torch.Tensor, group: int = 128, *,
     [n, groups] or None.
 
     Without ``zeros``: s = max|w| / 7 of the group, u = clamp(rne(w / s), -8, 7) + 8.  With: s = (max(w, 0) -
-    min(w, 0)) / 15, z = rne(-min / s), u = clamp(rne(w / s) + z, 0, 15).  s is rounded before it is used."""
+    min(w, 0)) / 15, z = rne(-min / s), u = clamp(rne(w / s) + z, 0, 15).  s is rounded before it is used; a group
+    with a NaN or an infinity has one that is not finite."""
     name = "quantize_w4"
     _require_gpu(name, w)
     if w.dtype not in _TENSOR_DTYPES:

@@ -321,3 +321,30 @@ def test_w4_mm_far_rows_and_columns(ops, device, m, ldx, n, k):
     x = torch.zeros(m, ldx, device=device, dtype=torch.bfloat16)[:, :k]
     rows, want = _picked(n, k, 32, [k - 1, 5, k // 2], x, device)
     assert torch.equal(ops.w4_mm(x, ops.pack_w4(*rows, group=32)), want)
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_quantize_keeps_nan_and_infinities(ops, device, dtype, zeros):
+    """A NaN weight makes its group's scale NaN, an infinity one that is not finite: such a group's products are not
+    finite either, and every other group is what it was."""
+    n, k, group = 21, 208, 32
+    w = torch.randn(n, k, generator=torch.Generator().manual_seed(1)).to(dtype)
+    clean = quantize(w, group, zeros)
+    for place, value in (((0, 0), float("nan")), ((5, 63), float("nan")), ((20, 207), float("nan")), ((7, 100), float("inf")),
+                         ((8, 100), -float("inf"))):
+        w[place] = value
+    got = [None if t is None else t.cpu() for t in ops.quantize_w4(w.to(device), group, zeros=zeros)]
+    odd = torch.zeros(n, 7, dtype=torch.bool)
+    for r, g in ((0, 0), (5, 1), (20, 6), (7, 3), (8, 3)):
+        odd[r, g] = True
+    assert torch.equal(~torch.isfinite(got[1]), odd)
+    assert torch.isnan(got[1][0, 0]) and torch.isnan(got[1][5, 1]) and torch.isnan(got[1][20, 6])
+    columns = ~odd.repeat_interleave(group // 2, dim=1)[:, :k // 2]
+    assert torch.equal(got[0][columns], clean[0][columns]) and torch.equal(got[1][~odd], clean[1][~odd])
+    assert not zeros or torch.equal(got[2][~odd], clean[2][~odd])
+    packed = ops.pack_w4(*(None if t is None else t.to(device) for t in got), group=group)
+    for m in (1, 9, 30, 300):
+        x = activations(m, k, seed=m).to(torch.float16 if dtype == torch.float16 else torch.bfloat16).to(device)
+        finite = torch.isfinite(ops.w4_mm(x, packed).cpu())
+        assert torch.equal(finite, (~odd.any(1)).expand(m, n))
