@@ -348,3 +348,15 @@ def test_quantize_keeps_nan_and_infinities(ops, device, dtype, zeros):
         x = activations(m, k, seed=m).to(torch.float16 if dtype == torch.float16 else torch.bfloat16).to(device)
         finite = torch.isfinite(ops.w4_mm(x, packed).cpu())
         assert torch.equal(finite, (~odd.any(1)).expand(m, n))
+
+
+def test_quantize_more_groups_than_a_launch_has_threads(ops, device):
+    """2^28 and some groups, 16 lanes each: past 2^32 threads."""
+    n, k, group = (1 << 16) + 1, 1 << 17, 32
+    w = torch.zeros(n, k, device=device, dtype=torch.bfloat16)
+    at = [0, 1, 777, n // 2, n - 2, n - 1]
+    w[at] = torch.randn(len(at), k, generator=torch.Generator(device=device).manual_seed(1), device=device).to(w.dtype)
+    codes, scales, _ = ops.quantize_w4(w, group)
+    want = quantize(w[at].cpu(), group, False)
+    assert torch.equal(codes[at].cpu(), want[0]) and torch.equal(scales[at].cpu(), want[1])
+    assert (codes[2:700] == 0x88).all() and (scales[n - 1000:n - 2] == 0).all()
