@@ -533,7 +533,7 @@ int h3q_w4_quantize(const void* w, int dtype, int64_t ldw, int64_t n, int64_t k,
 /*
  * The product, x [m, k] and out [m, n] bf16 or binary16 (dtype; ldx and ldo elements), binary32
  * sums rounded once; codes, scales (scale_dtype bf16 or binary16) and zeros (or NULL) as packed,
- * bias [n] of x's type or NULL.  x 16-byte aligned with ldx % 8 == 0, ldx < 2^23.  workspace:
+ * bias [n] of x's type or NULL.  x 16-byte aligned with ldx % 8 == 0, ldx < 2^23; n < 2^28.  workspace:
  * h3q_w4_mm_workspace_bytes(...) bytes of the caller's (0: none), free to use again when the call's
  * work on the stream is done.  A row of x with an infinity or a NaN gives NaN or infinities.
  */

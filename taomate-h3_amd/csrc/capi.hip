@@ -1126,8 +1126,9 @@ __attribute__((visibility("default"))) int h3q_w4_mm(int dtype, const void* x, i
     a.f16 = dtype == H3Q_DTYPE_F16;
     a.scales_f16 = scale_dtype == H3Q_DTYPE_F16 ? ~0u : 0u;
     a.out_vec = aligned(out, 8) && ldo % 4 == 0;
-    if (m <= h3q::kW4StreamRows) return check_launch(h3q::launch_w4_stream(a, (hipStream_t)stream), who);
-    if (!h3q::w4_tile_fits(m, n))
+    if (m <= h3q::kW4StreamRows && n < h3q::kW4StreamCols)
+        return check_launch(h3q::launch_w4_stream(a, (hipStream_t)stream), who);
+    if (m <= h3q::kW4StreamRows || !h3q::w4_tile_fits(m, n))
         return fail(H3Q_ERR_UNSUPPORTED, "%s: %lld rows of %lld x %lld are too many for one launch", who, (long long)m,
                     (long long)n, (long long)k);
     const int64_t need = h3q::w4_tile_workspace_bytes(m, n, k);

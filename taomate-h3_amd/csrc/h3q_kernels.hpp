@@ -339,8 +339,9 @@ struct W4Args {
     int f16, out_vec;     // out_vec: four columns at once are aligned
 };
 constexpr int kW4StreamRows = 16;
+constexpr int64_t kW4StreamCols = int64_t(1) << 28;  // 16 threads a column stay below a grid's 2^32
 hipError_t launch_w4_stream(const W4Args& a, hipStream_t st);
-bool w4_tile_fits(int64_t m, int64_t n);  // a launch's grid
+bool w4_tile_fits(int64_t m, int64_t n);  // a grid of less than 2^32 threads, past which it is cut off
 int64_t w4_tile_workspace_bytes(int64_t m, int64_t n, int64_t k);
 hipError_t launch_w4_tile(const W4Args& a, void* workspace, hipStream_t st);
 hipError_t launch_w4_slab(const W4Args& a, int nt, hipStream_t st);  // 32 or 64 rows, 32 nt columns (1 .. 3)

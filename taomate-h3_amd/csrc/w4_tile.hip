@@ -235,10 +235,8 @@ hipError_t launch_type(const TileArgs& a, const Plan& p, hipStream_t st) {
 
 }  // namespace
 
-bool w4_tile_fits(int64_t m, int64_t n) {
-    const int64_t rows = (m + 127) / 128 * 128;
-    return rows / 64 * ((n + 127) / 128) * 8 < (int64_t(1) << 31) && rows * ((n + 15) / 16) / 64 < (int64_t(1) << 31);
-}
+// Of 256 and more tiles of 128 x 256 none is split and none goes to the slab; with fewer the other grids are small.
+bool w4_tile_fits(int64_t m, int64_t n) { return (m + 127) / 128 * ((n + 255) / 256) < (int64_t(1) << 24); }
 
 int64_t w4_tile_workspace_bytes(int64_t m, int64_t n, int64_t k) { return plan_tiles(m, n, k).parts_bytes; }
 

@@ -98,3 +98,16 @@ def test_c_entry_points_refuse():
     assert lib.h3q_w4_quantize(p, 0, 63, 4, 64, 32, p, p, None, None) == 1 and "stride" in error()
     assert lib.h3q_w4_quantize(None, 0, 64, 4, 64, 32, p, p, None, None) == 1 and "null" in error()
     assert lib.h3q_w4_quantize(p, 0, 64, 0, 64, 32, p, p, None, None) == 0
+
+
+def test_c_entry_points_refuse_grids_past_32_bits():
+    """A launch of 2^32 threads or more is cut off without an error: products that would need one are refused."""
+    from taomate_h3_amd import _lib
+
+    if not _lib.LIB_PATH.exists():
+        pytest.skip("library not built")
+    lib = _lib.lib()
+    p = ctypes.c_void_p(256)
+    mm = lambda m, n: lib.h3q_w4_mm(0, p, 64, p, p, 0, None, 32, None, p, n, m, n, 64, None, 0, None)
+    for m, n in ((1, 1 << 28), (16, 1 << 30), (1 << 20, 1 << 20)):
+        assert mm(m, n) == 2 and "too many" in lib.h3q_last_error().decode()
