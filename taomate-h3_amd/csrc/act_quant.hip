@@ -368,9 +368,16 @@ static hipError_t dispatch_rows(const uint16_t* x, int64_t ldx, int64_t rows, in
             if (nv <= 32) return launch_rows_vec<FMT, ROUND, 32, true>(x, ldx, rows, k, q, ldq, row0, scales, st);
         }
     }
-    hipLaunchKernelGGL((quant_rows_any_kernel<FMT, ROUND, TILED>), dim3((unsigned)rows), dim3(256), 0, st, x, ldx,
-                       rows, k, q, ldq, row0, scales);
-    return hipGetLastError();
+    // A grid of 2^32 threads or more is cut off without an error.
+    constexpr int64_t kMostRows = int64_t(1) << 23;
+    for (int64_t r = 0; r < rows; r += kMostRows) {
+        const int64_t n = rows - r < kMostRows ? rows - r : kMostRows;
+        hipLaunchKernelGGL((quant_rows_any_kernel<FMT, ROUND, TILED>), dim3((unsigned)n), dim3(256), 0, st, x + r * ldx,
+                           ldx, n, k, q, ldq, row0 + r, scales + r);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 template <bool TILED>

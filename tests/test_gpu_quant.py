@@ -385,3 +385,30 @@ def test_rows_of_one_wave(ops, oracle, device, rows, k, fmt, rounding):
 def test_tiled_codes_of_short_rows(ops, oracle, device, rows, k):
     """Both sides of the widths and row counts between the tiled kernels, nothing past the rows written."""
     test_tiled_ragged_rows_write_only_their_own(ops, oracle, device, rows, k)
+
+
+@pytest.mark.parametrize("fmt,tiled", [(0, False), (1, False), (0, True)])
+def test_more_unaligned_rows_than_a_launch_has_threads(ops, device, fmt, tiled):
+    """2^24 and some rows off the vectors' alignment, a workgroup each: past 2^32 threads."""
+    rows, k = (1 << 24) + 21, 128 if tiled else 9
+    x = torch.empty(rows, k + 1, device=device, dtype=torch.bfloat16)[:, 1:]
+    x.copy_(torch.arange(rows, device=device)[:, None] % 509 + torch.arange(k, device=device)[None] % 7)
+    first = (1 << 24) - 16 * 3  # a tiled block's own start
+    if tiled:
+        codes, scales = ops.quant_rows_tiled(x, fmt)
+        want, by = ops.quant_rows_tiled(x[first:], fmt)
+    else:
+        codes, scales = ops.quant_rows(x, fmt)
+        want, by = ops.quant_rows(x[first:], fmt)
+    at = slice(first, rows)
+    tail = codes[first:first + want.shape[0]].view(torch.uint8).flatten(), want.view(torch.uint8).flatten()
+    if tiled:  # rows past the last are not written
+        live = [t.view(-1, 16, 128)[:-1].flatten() for t in tail]
+        assert torch.equal(*live)
+    else:
+        assert torch.equal(*tail)
+    assert torch.equal(scales[at], by) and (by > 0).all()
+    middle = slice(1 << 20, (1 << 20) + 64)
+    if not tiled:
+        want, by = ops.quant_rows(x[middle], fmt)
+        assert torch.equal(codes[middle].view(torch.uint8), want.view(torch.uint8)) and torch.equal(scales[middle], by)
