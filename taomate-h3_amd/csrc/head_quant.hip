@@ -31,6 +31,8 @@
 // bytes (pass 1) + 2 + 1 bytes (pass 3); algorithmic 3 bytes.  Up to 256 token
 // chunks and 32 heads per column group the fold of pass 2 runs inside pass 3 instead
 // (two launches).
+#include <algorithm>
+
 #include "h3q_common.hpp"
 #include "h3q_kernels.hpp"
 #include "row_quant.hpp"  // pk_abs_max, amax_from_packed
@@ -389,10 +391,23 @@ hipError_t launch_quant_per_head_e4m3(const uint16_t* x, int64_t batch, int64_t 
                                       hipStream_t st) {
     // The shape (and the workspace size) depends on head_dim % 8 only; a
     // misaligned x or q keeps the 8-element positions with scalar accesses.
-    const HeadQuantShape sh = head_quant_shape(batch, seq, heads, head_dim);
-    if (head_dim % 8) return launch_head_quant<IoElem>(x, sh, partial, q, scales, st);
-    if ((uintptr_t)x % 16 == 0 && (uintptr_t)q % 8 == 0) return launch_head_quant<IoVec>(x, sh, partial, q, scales, st);
-    return launch_head_quant<IoVecUnaligned>(x, sh, partial, q, scales, st);
+    // A grid of 2^32 threads or more is cut off without an error: as many batches at once as keep the passes (a
+    // workgroup for each column group, with so many batches) and the fold (a wave for each head) below that.
+    const int64_t groups = head_quant_shape(1, seq, heads, head_dim).groups;
+    const int64_t most = std::min((int64_t(1) << 23) / groups, (int64_t(1) << 25) / heads);
+    for (int64_t b = 0; b < batch; b += most) {
+        const HeadQuantShape sh = head_quant_shape(std::min(most, batch - b), seq, heads, head_dim);
+        const int64_t at = b * seq * heads * head_dim;
+        const uint16_t* const xb = x + at;
+        uint8_t* const qb = q + at;
+        float* const sb = scales + b * heads;
+        const hipError_t e = head_dim % 8 ? launch_head_quant<IoElem>(xb, sh, partial, qb, sb, st)
+                             : (uintptr_t)xb % 16 == 0 && (uintptr_t)qb % 8 == 0
+                                 ? launch_head_quant<IoVec>(xb, sh, partial, qb, sb, st)
+                                 : launch_head_quant<IoVecUnaligned>(xb, sh, partial, qb, sb, st);
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 }  // namespace h3q

@@ -225,3 +225,16 @@ def test_scales_of_many_or_wide_heads(ops, oracle, device, shape):
     """Both sides of the heads per column group and of the column groups per head
     up to which the quantize pass folds the partial maxima."""
     test_scales_folded_by_the_quantize_pass(ops, oracle, device, shape)
+
+
+@pytest.mark.parametrize("batch,heads,head_dim", [((1 << 24) + 3, 1, 8), ((1 << 21) + 5, 40, 2)])
+def test_more_batches_than_a_launch_has_threads(ops, device, batch, heads, head_dim):
+    """Workgroups of the passes, or of the fold of the maxima, past 2^32 threads."""
+    x = torch.empty(batch, 1, heads, head_dim, device=device, dtype=torch.bfloat16)
+    x.copy_(torch.arange(batch, device=device)[:, None, None, None] % 251 + 1)
+    x[..., 1] = -0.5
+    codes, scales = ops.quant_per_head_e4m3(x)
+    for part in (slice(0, 70), slice(1 << 20, (1 << 20) + 70), slice(batch - 70, batch)):
+        want, by = ops.quant_per_head_e4m3(x[part])
+        assert torch.equal(codes[part].view(torch.uint8), want.view(torch.uint8)) and torch.equal(scales[part], by)
+    assert (scales > 0).all()
