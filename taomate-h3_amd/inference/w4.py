@@ -7,7 +7,8 @@ linear's time is its weights' bytes.  Forward only.  No counterpart in the refer
 * ``quantize_h3_block_linears_w4_``   the DiT block linears that a policy selects, in place
 
 Activations stay bf16 or fp16, whatever their number: one token's products and a prefill's run on
-the same packed weights (``ops.w4_mm``).
+the same packed weights (``ops.w4_mm``).  The scales keep their dtype when a model is converted to another:
+the codes were made for them.
 """
 
 from __future__ import annotations
@@ -18,6 +19,7 @@ import torch
 import torch.nn as nn
 
 from .. import ops
+from .buffers import FixedDtypeModule
 from .fp8 import _block_candidates, resolve_h3_dynamic_fp8_policy
 
 
@@ -37,8 +39,10 @@ def w4_linear(inputs: torch.Tensor, weight: ops.W4Weight, bias: torch.Tensor | N
     return ops.w4_mm(flat, weight, bias=bias).reshape(*inputs.shape[:-1], weight.n)
 
 
-class W4Linear(nn.Module):
+class W4Linear(FixedDtypeModule):
     """A linear on packed 4-bit weights (``ops.W4Weight``)."""
+
+    FIXED = ("scales",)
 
     def __init__(self, weight: ops.W4Weight, bias: torch.Tensor | None = None) -> None:
         super().__init__()
@@ -68,19 +72,29 @@ class W4Linear(nn.Module):
         return w4_linear(x, self.weight, self.bias)
 
 
+class _W4Groups(FixedDtypeModule):
+    """Scales and zero points beside the codes of a module that is not a W4Linear."""
+
+    FIXED = ("scales",)
+
+    def __init__(self, scales: torch.Tensor, zeros: torch.Tensor | None) -> None:
+        super().__init__()
+        self.register_buffer("scales", scales)
+        self.register_buffer("zeros", zeros)
+
+
 def set_module_w4_weight_(module: nn.Module, weight: ops.W4Weight) -> None:
-    """Gives a linear-like module packed 4-bit weights: ``weight`` becomes their codes, with the scales,
-    zero points and sizes beside it."""
+    """Gives a linear-like module packed 4-bit weights: ``weight`` becomes their codes, with the scales and
+    zero points (a submodule, ``_w4_groups``) and sizes beside it."""
     module.weight = nn.Parameter(weight.codes, requires_grad=False)
-    module.register_buffer("_w4_scales", weight.scales)
-    module.register_buffer("_w4_zeros", weight.zeros)
+    module._w4_groups = _W4Groups(weight.scales, weight.zeros)
     module._w4_sizes = (weight.n, weight.k, weight.group)
 
 
 def module_w4_weight(module: nn.Module) -> ops.W4Weight | None:
     """The packed weights that ``set_module_w4_weight_`` gave the module, or None."""
     sizes = getattr(module, "_w4_sizes", None)
-    return None if sizes is None else ops.W4Weight(module.weight, module._w4_scales, module._w4_zeros, *sizes)
+    return None if sizes is None else ops.W4Weight(module.weight, module._w4_groups.scales, module._w4_groups.zeros, *sizes)
 
 
 def quantize_h3_block_linears_w4_(transformer: Any, *, policy: str | None = None, group: int = 128,

@@ -253,3 +253,31 @@ def test_cache_refuses():
         PagedKVCache(2, 16, 1, 64, scales="static", device="cpu")
     with pytest.raises(ValueError):
         PagedKVCache(2, 16, 1, 64, k_scale=torch.ones(1), v_scale=torch.ones(1), device="cpu")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_4_bit_linears_keep_their_scales(ops, device, dtype):
+    """``Module.to(dtype)`` of a model does not convert the group scales, which the codes were made for: results stay bit
+    for bit; and so they do after a move to the host and back, in a deep copy and from a state dict."""
+    (qkv, _), _ = _block(ops, device, True)[0]
+    half = w4.W4Linear(w4.quantize_w4_weight((torch.randn(96, WIDTH, generator=_gen(1)) * 1e-3).half().to(device), group=32))
+    layer = ToyColumnLinear(WIDTH, 100, bias=False, dtype=torch.float16, device=device)
+    with torch.no_grad():
+        layer.weight.copy_(torch.randn(100, WIDTH, generator=_gen(2)) * 0.02)
+    w4.set_module_w4_weight_(layer, w4.quantize_w4_weight(layer.weight, group=32, zeros=True))
+    model = torch.nn.ModuleList([qkv, half, layer])
+    x = activations(20, WIDTH, seed=1).to(device)
+    run = lambda m: [m[0](x), m[1](x.half()), m[2](x.half())]
+    want = run(model)
+    model.to(dtype)
+    for a, b in zip(run(model), want):
+        assert torch.equal(a, b)
+    again = copy.deepcopy(model.cpu()).to(device)
+    model.to(device)
+    other = copy.deepcopy(model)
+    for t in other.state_dict().values():
+        t.zero_()
+    other.load_state_dict(model.state_dict())
+    for m in (model, again, other):
+        for a, b in zip(run(m), want):
+            assert torch.equal(a, b)

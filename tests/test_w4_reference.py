@@ -111,3 +111,21 @@ def test_c_entry_points_refuse_grids_past_32_bits():
     mm = lambda m, n: lib.h3q_w4_mm(0, p, 64, p, p, 0, None, 32, None, p, n, m, n, 64, None, 0, None)
     for m, n in ((1, 1 << 28), (16, 1 << 30), (1 << 20, 1 << 20)):
         assert mm(m, n) == 2 and "too many" in lib.h3q_last_error().decode()
+
+
+def test_scales_keep_their_dtype(ops):
+    """Conversions of a model convert neither a W4Linear's scales nor those beside a module of another class."""
+    import torch
+    from taomate_h3_amd.inference import w4
+
+    scales = torch.tensor([1.0009765625, 3e-6] * 32).to(torch.float16).view(1, 1, 16, 4)
+    weight = ops.W4Weight(torch.zeros(1, 1, 1024, dtype=torch.uint8), scales, None, 16, 64, 32)
+    linear, other = w4.W4Linear(weight, torch.zeros(16)), torch.nn.Linear(64, 16)
+    w4.set_module_w4_weight_(other, weight)
+    model = torch.nn.Sequential(linear, other).to(torch.bfloat16).float().half().bfloat16()
+    assert linear.bias.dtype == torch.bfloat16 and other.bias.dtype == torch.bfloat16
+    for held in (linear.weight, w4.module_w4_weight(other)):
+        assert held.scales.dtype == torch.float16 and torch.equal(held.scales, scales) and held.zeros is None
+        assert held.codes.dtype == torch.uint8
+    model.to("meta")
+    assert linear.scales.device.type == "meta" and linear.scales.dtype == torch.float16
