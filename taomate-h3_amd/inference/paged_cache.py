@@ -12,9 +12,9 @@ for the device, and every call can be captured into a graph.
 from __future__ import annotations
 
 import torch
-import torch.nn as nn
 
 from .. import ops
+from .buffers import FixedDtypeModule
 
 SCALES = (None, "static", "rows")
 
@@ -65,9 +65,12 @@ class PagedKVCache:
         return out[0], out[1]
 
 
-class QKNormRotary(nn.Module):
+class QKNormRotary(FixedDtypeModule):
     """RMS norms of the query and key heads and rotary positions, on packed qkv rows [tokens, (q_heads +
-    2 * kv_heads) * head_dim].  Weights [head_dim] or [heads, head_dim]; None leaves out that norm."""
+    2 * kv_heads) * head_dim].  Weights [head_dim] or [heads, head_dim]; None leaves out that norm.  The angle tables
+    stay fp32 when a model is converted to another dtype."""
+
+    FIXED = ("cos", "sin")
 
     def __init__(self, q_heads: int, kv_heads: int, head_dim: int, *, positions: int, q_weight: torch.Tensor | None = None,
                  k_weight: torch.Tensor | None = None, eps: float = 1e-6, rot_dim: int | None = None,

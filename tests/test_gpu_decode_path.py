@@ -281,3 +281,15 @@ def test_4_bit_linears_keep_their_scales(ops, device, dtype):
     for m in (model, again, other):
         for a, b in zip(run(m), want):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_angle_tables_keep_their_type(ops, device, dtype):
+    """``Module.to(dtype)`` of a model leaves cos and sin in fp32, also on the way to the host and back."""
+    norm = QKNormRotary(HQ, HK, D, positions=64, device=device)
+    rows = activations(20, (HQ + 2 * HK) * D, seed=1).to(device)
+    want = norm(rows)
+    model = torch.nn.ModuleList([norm]).to(dtype)
+    for m in (model, copy.deepcopy(model.to("cpu")).to(device), model.to(device)):
+        for a, b in zip(m[0](rows), want):
+            assert torch.equal(a, b)
