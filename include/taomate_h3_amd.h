@@ -421,7 +421,7 @@ int h3q_expert_ffn(int format, const void* x, int64_t ldx, int64_t tokens, int64
  * Rows [tokens, heads, head_dim] in bf16, binary16 or binary32 (dtype: H3Q_DTYPE_*)
  * with unit stride along head_dim and any other strides, in elements: the packed rows
  * of a product can be used as they are.  head_dim even, at most 512; at most 16384 heads.  A row is read
- * whole before it is stored, so out may be x; otherwise they may not overlap.
+ * whole before it is stored, so out may be its own x; otherwise no rows of a call may overlap an out.
  * Sums and rotations are binary32.
  */
 typedef struct {

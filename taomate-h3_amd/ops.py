@@ -926,6 +926,10 @@ def _apart(name: str, t: torch.Tensor) -> None:
         reach += stride * (size - 1)
 
 
+def _same_start(a: torch.Tensor | None, b: torch.Tensor | None) -> bool:
+    return a is not None and b is not None and a.numel() > 0 and b.numel() > 0 and a.data_ptr() == b.data_ptr()
+
+
 def _head_rows(name: str, t: torch.Tensor, dtype: torch.dtype | None = None,
                shape: tuple[int, ...] | None = None) -> None:
     if t.dtype not in _TENSOR_DTYPES or (dtype is not None and t.dtype != dtype):
@@ -1016,7 +1020,7 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | No
 
     ``q [tokens, q_heads, head_dim]`` and ``k [tokens, k_heads, head_dim]`` may be views of the packed rows of a
     qkv product.  Weights [head_dim], or one for each head [heads, head_dim], in q's dtype or fp32; None leaves
-    out the norm.  The outputs may be the inputs themselves."""
+    out the norm.  ``q_out`` may be q itself and ``k_out`` k; otherwise no output holds an element of q, k or the other."""
     got = _native_call("qk_norm_rotary", q, k, q_weight, k_weight, cos, sin, positions, float(eps), interleaved, q_out,
                        k_out)
     if got is not None:
@@ -1028,6 +1032,8 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | No
     _head_rows(f"{name} k", k, q.dtype, (tokens, k.shape[1] if k.ndim == 3 else 0, d))
     rotation = _rotation(name, cos, sin, positions, tokens, d, interleaved)
     q_out, k_out = _like_heads(f"{name} q_out", q, q_out), _like_heads(f"{name} k_out", k, k_out)
+    if _same_start(q_out, k_out) or _same_start(q_out, k) or _same_start(k_out, q):
+        raise ValueError(f"{name}: an output is the other rows' input or output")
     _call_on(q, "h3q_qk_norm_rotary", _TENSOR_DTYPES[q.dtype], _weight_dtype(name, q, q_weight, k_weight),
              _heads(f"{name} q", q, q_weight, q_out), _heads(f"{name} k", k, k_weight, k_out), tokens, d, float(eps),
              rotation)
@@ -1094,7 +1100,8 @@ def append_kv(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: 
     ``positions``) as qk_norm_rotary does and values as they are, ``k``, ``v [tokens, kv_heads, head_dim]``, into
     the slots (int32 [tokens]: page * page_size + place; see plan_append) of ``k_pages`` and ``v_pages [pages,
     page_size, kv_heads, head_dim]`` (any strides but the last, so heads may lie outside a page's tokens).
-    ``q`` is normed and rotated beside them into ``q_out`` (returned; allocated here when None).
+    ``q`` is normed and rotated beside them into ``q_out`` (returned; allocated here when None; q itself, or rows that
+    hold no element of q, k and v).
 
     Pages hold k's dtype, or float8_e4m3fn codes e4m3(clamp(y / s, +-448)): with ``k_scale``, ``v_scale`` fp32 [1]
     or [kv_heads] those are the scales; with [pages, page_size, kv_heads] each row's scale max|y| / 448 is stored
@@ -1117,14 +1124,15 @@ def append_kv(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: 
     if k_pages.shape[:2] != v_pages.shape[:2]:
         raise ValueError(f"{name}: k_pages and v_pages differ in pages or page_size ({tuple(k_pages.shape[:2])}, "
                          f"{tuple(v_pages.shape[:2])})")
-    same = lambda a, b: a is not None and b is not None and a.numel() > 0 and a.data_ptr() == b.data_ptr()
-    if same(k_pages, v_pages) or (k_scale is not None and k_scale.ndim == 3 and same(k_scale, v_scale)):
+    if _same_start(k_pages, v_pages) or (k_scale is not None and k_scale.ndim == 3 and _same_start(k_scale, v_scale)):
         raise ValueError(f"{name}: k and v have pages and stored scales of their own")
     rotation = None if cos is None else _rotation(name, cos, sin, positions, tokens, d, interleaved)
     q_heads = None
     if q is not None:
         _head_rows(f"{name} q", q, k.dtype, (tokens, q.shape[1] if q.ndim == 3 else 0, d))
         q_out = _like_heads(f"{name} q_out", q, q_out)
+        if _same_start(q_out, k) or _same_start(q_out, v):
+            raise ValueError(f"{name}: q_out is the input of k or v")
         q_heads = _heads(f"{name} q", q, q_weight, q_out)
     elif q_weight is not None or q_out is not None:
         raise ValueError(f"{name}: q_weight and q_out go with q")

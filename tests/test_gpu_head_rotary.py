@@ -652,3 +652,27 @@ def test_append_kv_static_scales_out_of_the_ordinary(ops, device):
         want_codes = want.to(torch.float8_e4m3fn).float()
         assert torch.equal(torch.isnan(got), torch.isnan(want))
         assert torch.equal(got.nan_to_num(7.0), want_codes.nan_to_num(7.0))
+
+
+def test_outputs_that_are_another_rows_are_refused(ops, device):
+    """An output may be its own input; one that starts where another output or the other input does is a race."""
+    q, k = _rows(4, 2, 16, torch.bfloat16, device), _rows(4, 2, 16, torch.bfloat16, device, seed=2)
+    cos, sin = _tables(4, 8, device)
+    out = torch.zeros_like(q)
+    with pytest.raises(ValueError):
+        ops.qk_norm_rotary(q, k, None, None, cos, sin, q_out=out, k_out=out)
+    with pytest.raises(ValueError):
+        ops.qk_norm_rotary(q, k, None, None, cos, sin, q_out=k)
+    with pytest.raises(ValueError):
+        ops.qk_norm_rotary(q, k, None, None, cos, sin, k_out=q)
+    with pytest.raises(ValueError):
+        ops.qk_norm_rotary(q, k, None, None, cos, sin, q_out=k, k_out=q)
+    pages = [torch.zeros(1, 4, 2, 16, device=device, dtype=torch.bfloat16) for _ in range(2)]
+    slots = torch.arange(4, device=device, dtype=torch.int32)
+    for other in (k, out):
+        with pytest.raises(ValueError):
+            ops.append_kv(k, out, *pages, slots, cos=cos, sin=sin, q=q, q_out=other)
+    want = ops.qk_norm_rotary(q, q, None, None, cos, sin)  # one input as both is read only
+    assert torch.equal(want[0], want[1])
+    got = ops.qk_norm_rotary(q.clone(), k, None, None, cos, sin, q_out=q)
+    assert torch.equal(got[0], want[0]) and got[0].data_ptr() == q.data_ptr()

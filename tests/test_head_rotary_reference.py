@@ -188,3 +188,17 @@ def test_c_entry_points_refuse(lib):
     assert append(turn=_turn(lib, rot=10)) == 1 and "rotated" in error()
     assert append(q=lib.Heads(256, 16, 8, 2, None, 0, None, 0, 0)) == 1 and "null q" in error()
     assert append(tokens=0) == 0
+
+
+def test_c_entry_points_refuse_outputs_in_other_rows(lib):
+    handle = lib.lib()
+    error = lambda: handle.h3q_last_error().decode()
+    rows = lambda x, out, heads=2: lib.Heads(x, 16, 8, heads, None, 0, out, 16, 8)
+    p, f = ctypes.c_void_p(256), ctypes.c_float(1e-6)
+    norm = lambda q, k: handle.h3q_qk_norm_rotary(0, 0, q, k, 4, 8, f, _turn(lib), None)
+    for q, k in ((rows(256, 1024), rows(512, 1024)), (rows(256, 512), rows(512, 1024)), (rows(256, 1024), rows(512, 256)),
+                 (rows(256, 512), rows(512, 256))):
+        assert norm(q, k) == 1 and "other rows" in error()
+    append = lambda q, k, v: handle.h3q_append_kv(0, 0, q, k, v, _pages(lib), _pages(lib, pages=4096), p, 4, 8, f, None, None)
+    for out in (512, 1024):
+        assert append(rows(256, out), rows(512, None), rows(1024, None)) == 1 and "k or v" in error()
