@@ -796,6 +796,10 @@ static int check_heads(const char* who, const char* what, const h3q_heads& h, in
     if (!h.x || (has_out && !h.out)) return fail(H3Q_ERR_INVALID, "%s: null %s pointer", who, what);
     if (!aligned(h.x, size) || (has_out && !aligned(h.out, size)))
         return fail(H3Q_ERR_INVALID, "%s: %s rows are not aligned to their type", who, what);
+    // In place a row goes where it came from.
+    if (has_out && h.x == h.out && ((tokens > 1 && h.token_stride != h.out_token_stride) ||
+                                    (h.heads > 1 && h.head_stride != h.out_head_stride)))
+        return fail(H3Q_ERR_INVALID, "%s: the %s rows' out is x in other strides", who, what);
     return H3Q_OK;
 }
 

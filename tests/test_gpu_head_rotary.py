@@ -676,3 +676,16 @@ def test_outputs_that_are_another_rows_are_refused(ops, device):
     assert torch.equal(want[0], want[1])
     got = ops.qk_norm_rotary(q.clone(), k, None, None, cos, sin, q_out=q)
     assert torch.equal(got[0], want[0]) and got[0].data_ptr() == q.data_ptr()
+
+
+def test_out_as_x_in_other_strides_is_refused(ops, device):
+    x = _rows(4, 4, 16, torch.bfloat16, device)
+    cos, sin = _tables(4, 8, device)
+    want = ops.rotary(x, cos, sin)
+    with pytest.raises(RuntimeError, match="strides"):
+        ops.rotary(x, cos, sin, out=x.transpose(0, 1))
+    with pytest.raises(RuntimeError, match="strides"):
+        ops.qk_norm_rotary(x, x.clone(), None, None, cos, sin, q_out=x.transpose(0, 1))
+    assert torch.equal(ops.rotary(x, cos, sin, out=x), want)
+    one, again = x[:1].clone(), ops.rotary(x[:1], cos, sin)
+    assert torch.equal(ops.rotary(one, cos, sin, out=one.as_strided((1, 4, 16), (99, 16, 1))), again)

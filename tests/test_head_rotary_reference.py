@@ -202,3 +202,22 @@ def test_c_entry_points_refuse_outputs_in_other_rows(lib):
     append = lambda q, k, v: handle.h3q_append_kv(0, 0, q, k, v, _pages(lib), _pages(lib, pages=4096), p, 4, 8, f, None, None)
     for out in (512, 1024):
         assert append(rows(256, out), rows(512, None), rows(1024, None)) == 1 and "k or v" in error()
+
+
+def test_c_entry_points_refuse_out_as_x_in_other_strides(lib):
+    """Rows that lie where others are still read; strides of one token or head do not count."""
+    handle = lib.lib()
+    p, f = ctypes.c_void_p(256), ctypes.c_float(1e-6)
+    rows = lambda token, head, out_token, out_head, heads=2: lib.Heads(256, token, head, heads, None, 0, 256, out_token, out_head)
+    good = lib.Heads(1024, 16, 8, 2, None, 0, 2048, 16, 8)
+    for bad in (rows(16, 8, 8, 32), rows(16, 8, 16, 32), rows(16, 8, 32, 8), rows(16, 8, 32, 8, heads=1)):
+        assert handle.h3q_rotary(0, bad, 4, 8, _turn(lib), None) == 1
+        assert "strides" in handle.h3q_last_error().decode()
+        for q, k in ((bad, good), (good, bad)):
+            assert handle.h3q_qk_norm_rotary(0, 0, q, k, 4, 8, f, _turn(lib), None) == 1
+        assert handle.h3q_append_kv(0, 0, bad, good, lib.Heads(4096, 16, 8, 2), _pages(lib), _pages(lib), p, 4, 8, f, None, None) == 1
+    # one token, or one head: refused further on, for another reason (a weight without a norm)
+    for fine, tokens in ((rows(16, 8, 32, 8), 1), (rows(16, 8, 16, 32, heads=1), 4), (rows(16, 8, 16, 8), 4)):
+        fine.weight = 256
+        assert handle.h3q_rotary(0, fine, tokens, 8, _turn(lib), None) == 1
+        assert "without a norm" in handle.h3q_last_error().decode()
