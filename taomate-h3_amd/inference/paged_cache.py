@@ -53,6 +53,8 @@ class PagedKVCache:
 
     def gather(self, pages: torch.Tensor, length: int) -> tuple[torch.Tensor, torch.Tensor]:
         """Keys and values [length, kv_heads, head_dim] of a sequence with the page ids ``pages``, in ``dtype``."""
+        if not 0 <= length <= pages.shape[0] * self.page_size:
+            raise ValueError(f"PagedKVCache.gather: {pages.shape[0]} pages of {self.page_size} hold no {length} tokens")
         pages = pages[:(length + self.page_size - 1) // self.page_size].long()
         out = []
         for held, scale in ((self.k, self.k_scale), (self.v, self.v_scale)):

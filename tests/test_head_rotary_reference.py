@@ -221,3 +221,15 @@ def test_c_entry_points_refuse_out_as_x_in_other_strides(lib):
         fine.weight = 256
         assert handle.h3q_rotary(0, fine, tokens, 8, _turn(lib), None) == 1
         assert "without a norm" in handle.h3q_last_error().decode()
+
+
+def test_gather_refuses_a_length_past_its_pages(ops):
+    from taomate_h3_amd.inference.paged_cache import PagedKVCache
+
+    cache = PagedKVCache(4, 16, 2, 8, device="cpu")
+    k, v = cache.gather(torch.tensor([2, 0]), 32)
+    assert k.shape == v.shape == (32, 2, 8) and cache.gather(torch.tensor([2, 0]), 0)[0].shape == (0, 2, 8)
+    with pytest.raises(ValueError):
+        cache.gather(torch.tensor([2, 0]), 33)
+    with pytest.raises(ValueError):
+        cache.gather(torch.tensor([2, 0]), -1)
