@@ -360,3 +360,46 @@ def test_quantize_more_groups_than_a_launch_has_threads(ops, device):
     want = quantize(w[at].cpu(), group, False)
     assert torch.equal(codes[at].cpu(), want[0]) and torch.equal(scales[at].cpu(), want[1])
     assert (codes[2:700] == 0x88).all() and (scales[n - 1000:n - 2] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("m", [1, 3, 4, 16])
+def test_w4_mm_of_few_rows_takes_weights_as_they_are(ops, device, m, dtype):
+    """x has +1 in one column and -1 in one of another group: s (u - z) - s' (u' - z') of weights that cancel to a few of
+    their last bits.  Every step of the kernel is exact for them (u, z and 8-bit or 11-bit scales: products below 2^24
+    steps), so the result is the exact difference, rounded once; weights rounded first miss it by whole steps."""
+    kind = TYPES[dtype]
+    n, k, group = 40, 128, 32
+    gen = torch.Generator().manual_seed(7)
+    bits = 8 if dtype == "bf16" else 11
+    codes = torch.randint(0, 16, (n, k), generator=gen)
+    points = torch.randint(0, 4, (n, 4), generator=gen)
+    codes[:, 5], codes[:, 37] = points[:, 0] + 11, points[:, 1] + 12
+    # 11 s near 12 s'
+    s = torch.randint(1 << (bits - 1), 1 << bits, (n, 4), generator=gen).float()
+    s[:, 0] = torch.randint(round(0.75 * 2 ** bits), 1 << bits, (n,), generator=gen).float()
+    s[:, 1] = (s[:, 0] * 11 / 12).round()
+    scales = (s * 2.0 ** -12).to(kind)
+    assert torch.equal(scales.float(), s * 2.0 ** -12)
+    packed = (codes[:, 0::2] | codes[:, 1::2] << 4).to(torch.uint8), scales, points.to(torch.uint8)
+    x = torch.zeros(m, k)
+    x[:, 5], x[:, 37] = 1.0, -1.0
+    got = ops.w4_mm(x.to(kind).to(device), _pack(ops, device, *packed, group)).cpu()
+    want = (11 * s[:, 0] - 12 * s[:, 1]) * 2.0 ** -12
+    rounded = (11 * s[:, 0] * 2.0 ** -12).to(kind).float() - (12 * s[:, 1] * 2.0 ** -12).to(kind).float()
+    assert (want.to(kind) != rounded.to(kind)).any()  # the inputs tell them apart
+    assert torch.equal(got, want.to(kind).expand(m, n))
+
+
+@pytest.mark.parametrize("scale_type", list(TYPES))
+@pytest.mark.parametrize("m", [2, 16, 17, 40, 300, 2048])
+def test_w4_mm_binary16_weights_below_its_normal_range(ops, device, m, scale_type):
+    """Above 16 rows weights are rounded to binary16, below 2^-14 to its subnormal steps and not to zero; up to 16 rows
+    bf16 scales stay as they are."""
+    n, k, group = 272, 208, 32
+    rows = _weights(n, k, group, True, TYPES[scale_type], device)
+    scales = (rows[1].float() * 2.0 ** -10).to(TYPES[scale_type])
+    x = (activations(m, k, seed=m).float() * 64.0).half().to(device)
+    got = ops.w4_mm(x, _pack(ops, device, rows[0], scales, rows[2], group))
+    assert_product(got, *product(x, rows[0], scales, rows[2], group))
+    assert (got != 0).float().mean() > 0.9
