@@ -689,3 +689,23 @@ def test_out_as_x_in_other_strides_is_refused(ops, device):
     assert torch.equal(ops.rotary(x, cos, sin, out=x), want)
     one, again = x[:1].clone(), ops.rotary(x[:1], cos, sin)
     assert torch.equal(ops.rotary(one, cos, sin, out=one.as_strided((1, 4, 16), (99, 16, 1))), again)
+
+
+def test_more_tokens_than_a_grids_second_extent(ops, device):
+    """65535 blocks of 32 tokens and some: the rest lies in the grid's third extent."""
+    tokens, d = 65535 * 32 + 77, 8
+    x = torch.randn(tokens, 2, d, generator=torch.Generator(device=device).manual_seed(1), device=device).to(torch.bfloat16)
+    cos, sin = _tables(100, d // 2, device)
+    rows = torch.arange(tokens, device=device) % 100
+    rows[65535 * 32 + 5] = -1
+    out = torch.zeros_like(x)
+    ops.rotary(x, cos, sin, rows, out=out)
+    pages = [torch.zeros(tokens // 16 + 1, 16, 2, d, device=device, dtype=x.dtype) for _ in range(2)]
+    slots = torch.arange(tokens, dtype=torch.int32, device=device).flip(0).contiguous()
+    ops.append_kv(x, x, *pages, slots, cos=cos, sin=sin, positions=rows)
+    for part in (slice(0, 50), slice(65535 * 32 - 40, 65535 * 32 + 4), slice(65535 * 32 + 6, tokens)):
+        want = ops.rotary(x[part], cos, sin, rows[part])
+        assert torch.equal(out[part], want)
+        at = slots[part].long()
+        assert torch.equal(pages[0].flatten(0, 1)[at], want) and torch.equal(pages[1].flatten(0, 1)[at], x[part])
+    assert (out[65535 * 32 + 5] == 0).all()
