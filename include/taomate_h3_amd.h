@@ -440,7 +440,7 @@ typedef struct {
     const void* positions;  /* row of the tables for each token (NULL: its own number, rows >= tokens) */
     int positions_i64;      /* int64, else int32 */
     int interleaved;        /* pairs (2 i, 2 i + 1), else (i, rot_dim / 2 + i) */
-    int inverse;            /* by the negative angle: the rotation's inverse, and its gradient (without the magnitude) */
+    int inverse;            /* by the negative angle: the gradient, and for tables of magnitude 1 the inverse */
 } h3q_rotation;
 
 /* Pages [pages, page_size, heads, head_dim], strides in elements, pages * page_size < 2^31. */
@@ -535,7 +535,9 @@ int h3q_w4_quantize(const void* w, int dtype, int64_t ldw, int64_t n, int64_t k,
  * sums rounded once; codes, scales (scale_dtype bf16 or binary16) and zeros (or NULL) as packed,
  * bias [n] of x's type or NULL.  x 16-byte aligned with ldx % 8 == 0, ldx < 2^23; n < 2^28.  workspace:
  * h3q_w4_mm_workspace_bytes(...) bytes of the caller's (0: none), free to use again when the call's
- * work on the stream is done.  A row of x with an infinity or a NaN gives NaN or infinities.
+ * work on the stream is done.  A row of x with an infinity or a NaN gives NaN or infinities, and so does one of up
+ * to 16 whose sums of x u over 128 columns (u up to 15) pass binary32.  Above 16 rows binary16 x takes the weights as
+ * binary16 holds them: s (u - z) of bf16 scales in steps of 2^-24 below 2^-14, infinite from 65520 on.
  */
 int64_t h3q_w4_mm_workspace_bytes(int64_t m, int64_t n, int64_t k, int64_t group);
 int h3q_w4_mm(int dtype, const void* x, int64_t ldx, const void* codes, const void* scales, int scale_dtype,

@@ -311,7 +311,7 @@ struct HeadArgs {
     float inverse_d;
 };
 constexpr int kHeadMaxDim = 512;
-constexpr int kHeadMaxHeads = 16384;  // three segments of one row a wave stay within a grid's 65535
+constexpr int kHeadMaxHeads = 16384;  // three segments of one row a wave: 2^27 threads in a grid's first extent, of 2^32
 hipError_t launch_head_rotary(int dtype, const HeadArgs& a, hipStream_t st);
 hipError_t launch_rotary_tables(const void* positions, int type, int64_t n, const double* frequencies, int half,
                                 double magnitude, float* cos_out, float* sin_out, hipStream_t st);

@@ -15,9 +15,10 @@
 // read all of it before they store any of it, so a call may run in place.  The folds over a row go by lane
 // permutation, two to four instructions where a shuffle takes a round trip through LDS.
 //
-// Measured: 18603 tokens of 28 + 28 heads of 128, bf16, 108 us, 5.0 TB/s (a copy reaches 5.1); 6201 tokens of 28
-// rotated 16 us, of which the caches hold a part; 8190 tokens of 32 query heads and 8 + 8 heads into e4m3 pages
-// with a scale a row 41 us, 4.5 TB/s; one token 3 us, which is a launch.
+// Measured, the kernel alone under the profiler: 18603 tokens of 28 + 28 heads of 128, bf16, 107 us, 5.0 TB/s (a copy
+// reaches 5.1); 6201 tokens of 28 rotated 16 us, of which the caches hold a part; 8190 tokens of 32 query heads and
+// 8 + 8 heads into e4m3 pages with a scale a row 41 us, 4.5 TB/s; one token 3.2 us, two dependent round trips (the call
+// in a replayed graph 5.0 to 5.6).
 //
 // Pairs: (i, half + i), where a lane's two vectors at c V and half + c V hold both sides, or (2 i, 2 i + 1), where
 // each of them holds V / 2 whole pairs.  Channels from 2 * half on go through as they are (a select, not a

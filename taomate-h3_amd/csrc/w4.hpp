@@ -8,7 +8,8 @@
 // accumulators.  Against 64 bits the result is off by 1.3 times what the output's own rounding costs; what it saves is an
 // fma and an offset for every output and group: scaling the sums was built for many rows too, and took 600 us for 4096
 // rows of 14336 x 5376 at groups of 128 without zero points, 1330 us at groups of 32 with them, where this takes 492
-// and 501.
+// and 501 (each a loop of one call; 503 and more with inputs that change).  binary16 holds weights from 2^-14 to 65504 in
+// full: below, where only bf16 scales reach, its subnormal steps are left of them.
 //
 // Layout.  Codes lie in blocks of 16 rows x 128 columns, 1 KiB, [row blocks][column blocks]: lane L's 16 bytes
 // are four words, word s the eight codes k = 128 b + 32 s + 8 (L / 16) .. + 7 of row L % 16, the low nibbles of

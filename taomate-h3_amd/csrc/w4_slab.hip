@@ -4,9 +4,10 @@
 // w takes the 128-column blocks w, w + 8, ... on its own, from a ring of x and a place for a block's codes in LDS that
 // only it fills (buffer_load ... lds) and reads, so that there is no barrier before the last sums are joined there, in
 // order.  Where w4_tile.hip splits k over workgroups it writes and reads binary32 sums and takes a second launch: 100
-// rows of 4096 x 4096 11.6 us against 18.3, 40 rows of 5376 x 7168 14.1 against 16.7, 200 rows 26.5 against 29.5.  Up to
-// 16 rows w4_stream.hpp keeps the weights exact; two of its row tiles took 32 rows of 5376 x 7168 in 18.3 us where this
-// takes 12.4, 17 rows in 13.2 and 10.0.
+// rows of 4096 x 4096 11.6 us against 18.3, 40 rows of 5376 x 7168 14.1 against 16.7, 200 rows 26.5 against 29.5
+// (loops of one call; the last 27.4 to 29.4 over cards and changing inputs).  Up to 16 rows w4_stream.hpp keeps the
+// weights exact; two of its row tiles took 32 rows of 5376 x 7168 in 18.3 us where this takes 12.4, 17 rows in 13.2 and
+// 10.0.
 //
 // Everything that is fetched goes through LDS copies, whose count is known at every point; with a load into registers
 // among them the compiler's own wait for it would count the copies behind it as done too early.  x comes in

@@ -1231,7 +1231,7 @@ def w4_mm(x: torch.Tensor, weight: W4Weight, *, bias: torch.Tensor | None = None
           out: torch.Tensor | None = None) -> torch.Tensor:
     """x @ w^T [+ bias] of 4-bit weights (pack_w4), ``x [m, k]`` bf16 or fp16 -> [m, n] in x's dtype:
     out[m, n] = sum_k x[m, k] * s (u - z), binary32 sums rounded once.  Above 16 rows the weights s (u - z) are rounded
-    to x's dtype first.
+    to x's dtype first (fp16: steps of 2^-24 below 2^-14, infinite from 65520 on, which bf16 scales can reach).
 
     x has 16-byte aligned rows (a row stride that is a multiple of 8); ``bias [n]`` and ``out``, which holds no element of x,
     are of its dtype."""
