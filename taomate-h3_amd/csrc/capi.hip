@@ -803,8 +803,8 @@ static int check_heads(const char* who, const char* what, const h3q_heads& h, in
     return H3Q_OK;
 }
 
-// Rows are read whole before they are stored in their own place only: q's out is not where the rows `other` start.
-static bool starts_at(const h3q_heads& q, const void* other) { return q.heads > 0 && q.out && q.out == other; }
+// A row is read whole before it is stored, which is safe in its own place only: whether q's out starts where other rows do.
+static bool starts_at(const h3q_heads& q, const void* other) { return q.heads > 0 && q.out == other; }
 
 static int check_rotation(const char* who, const h3q_rotation& r, int64_t tokens, int64_t head_dim) {
     if (r.rot_dim <= 0 || r.rot_dim % 2 || r.rot_dim > head_dim)
@@ -915,7 +915,7 @@ __attribute__((visibility("default"))) int h3q_qk_norm_rotary(int dtype, int wei
     if (rc == H3Q_OK) rc = check_heads(who, "k", *k, tokens, size, true);
     if (rc == H3Q_OK) rc = check_rotation(who, *rotation, tokens, head_dim);
     if (rc != H3Q_OK) return rc;
-    if (q->heads > 0 && k->heads > 0 && (starts_at(*q, k->out) || starts_at(*q, k->x) || starts_at(*k, q->x)))
+    if (tokens > 0 && k->heads > 0 && (starts_at(*q, k->out) || starts_at(*q, k->x) || starts_at(*k, q->x)))
         return fail(H3Q_ERR_INVALID, "%s: an output is the other rows' input or output", who);
     h3q::HeadArgs a = head_args(dtype, weight_dtype, tokens, head_dim, eps, rotation);
     for (const h3q_heads* h : {q, k})
@@ -986,7 +986,7 @@ __attribute__((visibility("default"))) int h3q_append_kv(int dtype, int weight_d
     if (k->heads != v->heads)
         return fail(H3Q_ERR_INVALID, "%s: %lld k heads and %lld v heads", who, (long long)k->heads, (long long)v->heads);
     if (v->weight) return fail(H3Q_ERR_INVALID, "%s: values have no norm", who);
-    if (q && k->heads > 0 && (starts_at(*q, k->x) || starts_at(*q, v->x)))
+    if (q && tokens > 0 && k->heads > 0 && (starts_at(*q, k->x) || starts_at(*q, v->x)))
         return fail(H3Q_ERR_INVALID, "%s: q's output is the input of k or v", who);
     if (k_pages->n_pages != v_pages->n_pages || k_pages->page_size != v_pages->page_size)
         return fail(H3Q_ERR_INVALID, "%s: %lld k pages of %lld tokens, but %lld v pages of %lld", who,

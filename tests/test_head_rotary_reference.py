@@ -195,10 +195,11 @@ def test_c_entry_points_refuse_outputs_in_other_rows(lib):
     error = lambda: handle.h3q_last_error().decode()
     rows = lambda x, out, heads=2: lib.Heads(x, 16, 8, heads, None, 0, out, 16, 8)
     p, f = ctypes.c_void_p(256), ctypes.c_float(1e-6)
-    norm = lambda q, k: handle.h3q_qk_norm_rotary(0, 0, q, k, 4, 8, f, _turn(lib), None)
+    norm = lambda q, k, tokens=4: handle.h3q_qk_norm_rotary(0, 0, q, k, tokens, 8, f, _turn(lib), None)
     for q, k in ((rows(256, 1024), rows(512, 1024)), (rows(256, 512), rows(512, 1024)), (rows(256, 1024), rows(512, 256)),
                  (rows(256, 512), rows(512, 256))):
         assert norm(q, k) == 1 and "other rows" in error()
+        assert norm(q, k, 0) == 0  # no rows
     append = lambda q, k, v: handle.h3q_append_kv(0, 0, q, k, v, _pages(lib), _pages(lib, pages=4096), p, 4, 8, f, None, None)
     for out in (512, 1024):
         assert append(rows(256, out), rows(512, None), rows(1024, None)) == 1 and "k or v" in error()
